@@ -37,7 +37,8 @@ extern "C" {
 #endif
 
 typedef enum { TG_MAXPLUS = 0, TG_MINPLUS = 1, TG_MAXMUL = 2 } tg_semiring;
-typedef enum { TG_F32 = 0, TG_F64 = 1, TG_I32 = 2, TG_I64 = 3 } tg_dtype;
+/* TG_BF16 and TG_F16 are element types of the tg_rows8_* calls only. */
+typedef enum { TG_F32 = 0, TG_F64 = 1, TG_I32 = 2, TG_I64 = 3, TG_BF16 = 4, TG_F16 = 5 } tg_dtype;
 typedef enum { TG_ROW_MAJOR = 0, TG_COL_MAJOR = 1 } tg_layout;
 
 typedef enum {
@@ -186,6 +187,91 @@ tg_status tg_gemm_i32_noalloc(tg_semiring semiring, tg_layout layout,
                               void* c, int64_t ldc,
                               int32_t* argmax,
                               void* stream);
+
+/* ------------------------------------------------------------------------
+ * Rows held in 8 bits.
+ *
+ * A (rows x cols) matrix in 8-bit rows is q (int8, row-major, leading
+ * dimension in elements) and scale (f32, one per row): element (r, c) stands
+ * for q[r*ldq + c] * scale[r].  Every call below is row-major; dtype is
+ * TG_F32, TG_F16 or TG_BF16; sizes of 0 are accepted.  Same conventions as
+ * above otherwise (device pointers, stream order, status codes).  Some calls
+ * take stream-ordered scratch from the library's own pool.
+ * No reference counterpart: these are the ordinary (+, x) layers that stand
+ * beside a tropical layer in a model.
+ * ------------------------------------------------------------------------ */
+
+/* q, scale = x in 8-bit rows: scale = max|x[r,:]| / 127, q = x / scale
+ * rounded to nearest even, in [-127, 127].  A row whose largest magnitude is
+ * below 2^-120 becomes zeros with scale 0; a row that holds a NaN or an
+ * infinity gets scale NaN, so that everything made of it is NaN. */
+tg_status tg_rows8_quantize(tg_dtype dtype, int64_t rows, int64_t cols,
+                            const void* x, int64_t ldx,
+                            int8_t* q, int64_t ldq, float* scale, void* stream);
+
+/* y = q * scale, rounded once to dtype. */
+tg_status tg_rows8_dequantize(tg_dtype dtype, int64_t rows, int64_t cols,
+                              const int8_t* q, int64_t ldq, const float* scale,
+                              void* y, int64_t ldy, void* stream);
+
+/* Root-mean-square norm with the residual's addition, out in 8-bit rows:
+ *   h = x + residual;  u[r] = 1 / sqrt(mean(h[r,:]^2) + eps);  y = h * u * weight
+ * q, scale = y in 8-bit rows (as tg_rows8_quantize).  All arithmetic and
+ * the statistics are f32 on the unrounded sum; x, residual, weight and h are
+ * of type dtype.  residual and h may be null (no addition; h not written).
+ * For training, ckpt (ldk) and ckpt_scale receive h in 8-bit rows and rstd
+ * receives u: what tg_rows8_rmsnorm_backward reads.  The three may be null. */
+tg_status tg_rows8_rmsnorm(tg_dtype dtype, int64_t rows, int64_t cols,
+                           const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                           const void* weight, float eps,
+                           void* h, int64_t ldh,
+                           int8_t* q, int64_t ldq, float* scale,
+                           int8_t* ckpt, int64_t ldk, float* ckpt_scale, float* rstd,
+                           void* stream);
+
+/* Backward of the norm from its 8-bit checkpoint.  With v = ckpt * ckpt_scale
+ * * rstd (the normalised row) and g = grad:
+ *   grad_x = rstd * (g * weight - v * mean(g * weight * v)) + grad_h
+ *   grad_weight = sum over rows of g * v
+ * grad is of type grad_dtype (dtype, or TG_F32); grad_h (null for none),
+ * weight, grad_x and grad_weight are of type dtype.  grad_x is the gradient
+ * of x and of residual alike.  The rounding to 8 bits is passed straight
+ * through.  The sum over rows has a fixed order: equal inputs give equal
+ * bits.  grad_x or grad_weight may be null. */
+tg_status tg_rows8_rmsnorm_backward(tg_dtype dtype, tg_dtype grad_dtype, int64_t rows, int64_t cols,
+                                    const void* grad, int64_t ldg, const void* grad_h, int64_t ldgh,
+                                    const void* weight, const int8_t* ckpt, int64_t ldk,
+                                    const float* ckpt_scale, const float* rstd,
+                                    void* grad_x, int64_t ldx, void* grad_weight, void* stream);
+
+/* C[i,j] = a_scale[i] * b_scale[j] * sum_k A[i,k] * B[j,k] + bias[j]
+ * A (m x k) and B (n x k) in 8-bit rows, C (m x n) of type dtype, bias (n) of
+ * type dtype or null.  The integer sums are exact: k < 131072, beyond it
+ * TG_ERR_UNSUPPORTED. */
+tg_status tg_rows8_gemm(tg_dtype dtype, int64_t m, int64_t n, int64_t k,
+                        const int8_t* a, int64_t lda, const float* a_scale,
+                        const int8_t* b, int64_t ldb, const float* b_scale,
+                        const void* bias, void* c, int64_t ldc, void* stream);
+
+/* Gradient of tg_rows8_gemm with respect to one operand, from the other in
+ * 8-bit rows (r x cols: the weights, or the activations' checkpoint):
+ *   out[p, c] = sum_i g(p, i) * scale[i] * q[i, c]
+ * transposed == 0: g is (p x r), g(p, i) = g[p*ldg + i]  (grad_A = grad B)
+ * transposed != 0: g is (r x p), g(p, i) = g[i*ldg + p]  (grad_B = grad^T A)
+ * g is of type grad_dtype, out (p x cols) of type out_dtype.  Sums are f32.
+ * Rounding of the factors: a TG_BF16 gradient meets the 8-bit operand's
+ * values rounded once to bf16; TG_F16 and TG_F32 gradients are carried with
+ * 16 and 24 significant bits. */
+tg_status tg_rows8_gemm_backward(tg_dtype grad_dtype, tg_dtype out_dtype, int transposed,
+                                 int64_t p, int64_t cols, int64_t r,
+                                 const void* g, int64_t ldg,
+                                 const int8_t* q, int64_t ldq, const float* scale,
+                                 void* out, int64_t ldo, void* stream);
+
+/* out[c] = sum over rows of x[r, c] (f32 sums, fixed order): the gradient of
+ * tg_rows8_gemm's bias.  out is of type out_dtype. */
+tg_status tg_rows8_column_sum(tg_dtype dtype, tg_dtype out_dtype, int64_t rows, int64_t cols,
+                              const void* x, int64_t ldx, void* out, void* stream);
 
 #ifdef __cplusplus
 }

@@ -166,8 +166,8 @@ size_t dtype_size(tg_dtype t) {
   switch (t) {
     case TG_F32: case TG_I32: return 4;
     case TG_F64: case TG_I64: return 8;
+    default: return 0;   // not a tropical element type
   }
-  return 0;
 }
 
 tg_status gemm_impl(tg_semiring semiring, tg_dtype dtype, tg_layout layout, int64_t batch,

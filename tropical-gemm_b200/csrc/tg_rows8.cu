@@ -1,0 +1,686 @@
+// Row kernels of the 8-bit row operators: quantisation, the root-mean-square
+// norm with the residual's addition, its backward, and column sums.
+//
+// All are bound by memory: each reads its inputs once, keeps the row in
+// registers between the statistics and the output, and writes once.
+#include <algorithm>
+#include "tg_rows8.cuh"
+
+namespace tg8 {
+
+struct RowArgs {
+  int64_t rows, cols;
+  const void *x, *residual, *weight;
+  void* h;
+  int8_t *q, *ckpt;
+  float *scale, *ckpt_scale, *rstd;
+  int64_t ldx, ldr, ldh, ldq, ldk;
+  float eps;
+  int tpr;   // threads per row: 32 .. 1024
+};
+
+struct RowStats {
+  float sum;        // of h^2
+  uint32_t top_y;   // bit patterns of the largest |h * weight| ...
+  uint32_t top_h;   // ... and |h|
+};
+
+__device__ __forceinline__ RowStats row_reduce(RowStats s, int tpr, RowStats* warp_stats) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) s.sum += __shfl_xor_sync(0xffffffffu, s.sum, d);
+  s.top_y = __reduce_max_sync(0xffffffffu, s.top_y);
+  s.top_h = __reduce_max_sync(0xffffffffu, s.top_h);
+  if (tpr > 32) {
+    const int warp = threadIdx.x >> 5, first = (threadIdx.x / tpr) * (tpr >> 5);
+    __syncthreads();   // the last use of warp_stats is over
+    if ((threadIdx.x & 31) == 0) warp_stats[warp] = s;
+    __syncthreads();
+    s = warp_stats[first];
+    for (int w = 1; w < tpr >> 5; w++) {   // the same order in every thread
+      const RowStats o = warp_stats[first + w];
+      s.sum += o.sum;
+      s.top_y = max(s.top_y, o.top_y);
+      s.top_h = max(s.top_h, o.top_h);
+    }
+  }
+  return s;
+}
+
+__device__ __forceinline__ uint32_t mag_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// One row per tpr threads, G groups of 8 elements per thread held in f32
+// registers.  VEC: 16-byte accesses; otherwise element by element, any
+// alignment.  NORM: root-mean-square norm (and the checkpoint when asked
+// for); otherwise the plain quantisation.
+template <typename T, int G, bool VEC, bool NORM>
+__global__ void __launch_bounds__(1024) rows_kernel(RowArgs p) {
+  __shared__ RowStats warp_stats[32];
+  const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, per_block = blockDim.x / p.tpr;
+  const int64_t row = int64_t(blockIdx.x) * per_block + sub;
+  const bool live = row < p.rows;
+  const T* x = static_cast<const T*>(p.x) + (live ? row : 0) * p.ldx;
+  const T* res = p.residual ? static_cast<const T*>(p.residual) + (live ? row : 0) * p.ldr : nullptr;
+  const T* wgt = static_cast<const T*>(p.weight);
+  const int cols = int(p.cols);
+  auto at = [&](int g, int e) { return VEC ? (g * p.tpr + t) * 8 + e : (g * 8 + e) * p.tpr + t; };
+
+  float v[G][8];
+  if (VEC) {
+    Vec8<T> a[G], b[G];
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      const bool in = live && at(g, 0) < cols;
+      if (in) a[g].load(x + at(g, 0)); else a[g].zero();
+      if (NORM && res && in) b[g].load(res + at(g, 0)); else b[g].zero();
+    }
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      float r[8];
+      a[g].get(v[g]);
+      b[g].get(r);
+      if (NORM && res) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[g][e] += r[e];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int c = at(g, e);
+        const bool in = live && c < cols;
+        v[g][e] = in ? to_f32(x[c]) : 0.f;
+        if (NORM && res && in) v[g][e] += to_f32(res[c]);
+      }
+  }
+
+  auto weight_of = [&](int g, float (&w)[8]) {
+    if (VEC) {
+      Vec8<T> a;
+      if (at(g, 0) < cols) a.load(wgt + at(g, 0)); else a.zero();
+      a.get(w);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) w[e] = at(g, e) < cols ? to_f32(wgt[at(g, e)]) : 0.f;
+    }
+  };
+
+  RowStats s{0.f, 0u, 0u};
+#pragma unroll
+  for (int g = 0; g < G; g++) {
+    float w[8];
+    if (NORM) weight_of(g, w);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      s.top_h = max(s.top_h, mag_bits(v[g][e]));
+      if (NORM) {
+        s.sum = fmaf(v[g][e], v[g][e], s.sum);
+        s.top_y = max(s.top_y, mag_bits(v[g][e] * w[e]));
+      }
+    }
+  }
+  s = row_reduce(s, p.tpr, warp_stats);
+
+  float u = 1.f;
+  Quant qy;
+  if (NORM) {
+    u = 1.f / sqrtf(s.sum / float(cols) + p.eps);
+    uint32_t top = mag_bits(__uint_as_float(s.top_y) * u);
+    // max|h * w| * u stands for max|(h * u) * w| unless h * w left f32's range
+    const bool redo = NORM && !(__uint_as_float(s.top_y) > 1e-25f && __uint_as_float(s.top_y) < 1e25f);
+    if (__syncthreads_or(redo)) {   // rare: zero rows, tiny or huge values
+      RowStats r{0.f, 0u, 0u};
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        float w[8];
+        weight_of(g, w);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int c = at(g, VEC ? 0 : e);
+          if (c < cols) r.top_y = max(r.top_y, mag_bits(v[g][e] * u * w[e]));
+        }
+      }
+      r = row_reduce(r, p.tpr, warp_stats);
+      if (redo) top = r.top_y;
+    }
+    qy = quant_of(top);
+  } else {
+    qy = quant_of(s.top_h);
+  }
+  if (!live) return;
+
+  const Quant qh = quant_of(s.top_h);
+  T* h = static_cast<T*>(p.h) + row * p.ldh;
+  int8_t* q = p.q + row * p.ldq;
+  int8_t* k = p.ckpt ? p.ckpt + row * p.ldk : nullptr;
+  if (t == 0) {
+    p.scale[row] = qy.scale;
+    if (NORM && k) {
+      p.ckpt_scale[row] = qh.scale;
+      p.rstd[row] = u;
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < G; g++) {
+    float w[8], y[8];
+    if (NORM) weight_of(g, w);
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] = NORM ? v[g][e] * u * w[e] : v[g][e];
+    if (VEC) {
+      const int c = at(g, 0);
+      if (c < cols) {
+        *reinterpret_cast<uint2*>(q + c) = quant_pack8(y, qy.inv);
+        if (NORM && k) *reinterpret_cast<uint2*>(k + c) = quant_pack8(v[g], qh.inv);
+        if (NORM && p.h) store8(h + c, v[g]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int c = at(g, e);
+        if (c < cols) {
+          q[c] = int8_t(quant8(y[e], qy.inv));
+          if (NORM && k) k[c] = int8_t(quant8(v[g][e], qh.inv));
+          if (NORM && p.h) h[c] = from_f32<T>(v[g][e]);
+        }
+      }
+    }
+  }
+}
+
+// Rows too long for registers: one block per row, the row read three times
+// (the second and third mostly from L2).
+template <typename T, bool NORM>
+__global__ void __launch_bounds__(1024) rows_long_kernel(RowArgs p) {
+  __shared__ RowStats warp_stats[32];
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+  const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.ldr : nullptr;
+  const T* wgt = static_cast<const T*>(p.weight);
+  auto value = [&](int64_t c) { return to_f32(x[c]) + (NORM && res ? to_f32(res[c]) : 0.f); };
+  RowStats s{0.f, 0u, 0u};
+  for (int64_t c = threadIdx.x; c < p.cols; c += blockDim.x) {
+    const float v = value(c);
+    s.sum = fmaf(v, v, s.sum);
+    s.top_h = max(s.top_h, mag_bits(v));
+  }
+  s = row_reduce(s, blockDim.x, warp_stats);
+  float u = 1.f;
+  Quant qy = quant_of(s.top_h);
+  const Quant qh = qy;
+  if (NORM) {
+    u = 1.f / sqrtf(s.sum / float(p.cols) + p.eps);
+    RowStats r{0.f, 0u, 0u};
+    for (int64_t c = threadIdx.x; c < p.cols; c += blockDim.x) r.top_y = max(r.top_y, mag_bits(value(c) * u * to_f32(wgt[c])));
+    r = row_reduce(r, blockDim.x, warp_stats);
+    qy = quant_of(r.top_y);
+  }
+  if (threadIdx.x == 0) {
+    p.scale[row] = qy.scale;
+    if (NORM && p.ckpt) {
+      p.ckpt_scale[row] = qh.scale;
+      p.rstd[row] = u;
+    }
+  }
+  for (int64_t c = threadIdx.x; c < p.cols; c += blockDim.x) {
+    const float v = value(c);
+    p.q[row * p.ldq + c] = int8_t(quant8(NORM ? v * u * to_f32(wgt[c]) : v, qy.inv));
+    if (NORM && p.ckpt) p.ckpt[row * p.ldk + c] = int8_t(quant8(v, qh.inv));
+    if (NORM && p.h) static_cast<T*>(p.h)[row * p.ldh + c] = from_f32<T>(v);
+  }
+}
+
+// y = q * scale: 8 elements per thread (VEC) or one.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) dequantize_kernel(int64_t rows, int64_t cols, const int8_t* q, int64_t ldq,
+                                                         const float* scale, T* y, int64_t ldy) {
+  const int64_t per = VEC ? cols / 8 : cols, total = rows * per;
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int64_t row = total <= 0xffffffffll ? int64_t(uint32_t(i) / uint32_t(per)) : i / per;
+  const int64_t c = i - row * per;
+  const float s = scale[row];
+  if (VEC) {
+    float v[8];
+    bytes_f32(*reinterpret_cast<const uint2*>(q + row * ldq + c * 8), v);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] *= s;
+    store8(y + row * ldy + c * 8, v);
+  } else {
+    y[row * ldy + c] = from_f32<T>(float(q[row * ldq + c]) * s);
+  }
+}
+
+// ------------------------------------------------------------------ backward
+struct BackArgs {
+  int64_t rows, cols;
+  const void *grad, *grad_h, *weight;
+  const int8_t* ckpt;
+  const float *ckpt_scale, *rstd;
+  void* grad_x;
+  float* partial;   // (slots x cols) sums of grad * v over a slot's rows, or null
+  int64_t ldg, ldgh, ldk, ldx;
+  int tpr;
+  int64_t slots;    // row groups running side by side; slot s takes rows s, s + slots, ...
+};
+
+__device__ __forceinline__ float row_sum(float s, int tpr, float* warp_sums) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  if (tpr > 32) {
+    const int warp = threadIdx.x >> 5, first = (threadIdx.x / tpr) * (tpr >> 5);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) warp_sums[warp] = s;
+    __syncthreads();
+    s = warp_sums[first];
+    for (int w = 1; w < tpr >> 5; w++) s += warp_sums[first + w];
+  }
+  return s;
+}
+
+// Each slot (tpr threads) walks its rows with a fixed set of columns per
+// thread, so the sums over rows stay in registers; they are joined by
+// column_join_kernel in a fixed order.
+template <typename T, typename GT, int G, bool VEC>
+__global__ void __launch_bounds__(1024) norm_backward_kernel(BackArgs p) {
+  __shared__ float warp_sums[32];
+  const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, per_block = blockDim.x / p.tpr;
+  const int64_t slot = int64_t(blockIdx.x) * per_block + sub;
+  const int cols = int(p.cols);
+  const T* wgt = static_cast<const T*>(p.weight);
+  auto at = [&](int g, int e) { return VEC ? (g * p.tpr + t) * 8 + e : (g * 8 + e) * p.tpr + t; };
+  float dw[G][8];
+#pragma unroll
+  for (int g = 0; g < G; g++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) dw[g][e] = 0.f;
+
+  // the same number of turns in every thread of the block: the sums synchronise
+  const int64_t first = int64_t(blockIdx.x) * per_block;
+  for (int64_t base = first; base < p.rows; base += p.slots) {
+    const int64_t row = base + sub;
+    const bool live = row < p.rows && slot < p.slots;
+    const int64_t rr = live ? row : 0;
+    const float u = p.rstd[rr], s = p.ckpt_scale[rr] * u;
+    const GT* grad = static_cast<const GT*>(p.grad) + rr * p.ldg;
+    const int8_t* k = p.ckpt + rr * p.ldk;
+    float gw[G][8], v[G][8];
+    float dot = 0.f;
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      float w[8], gr[8];
+      if (VEC) {
+        const int c = at(g, 0);
+        Vec8<T> a;
+        Vec8<GT> b;
+        uint2 kk = make_uint2(0, 0);
+        const bool in = live && c < cols;
+        if (in) { a.load(wgt + c); b.load(grad + c); kk = *reinterpret_cast<const uint2*>(k + c); } else { a.zero(); b.zero(); }
+        a.get(w);
+        b.get(gr);
+        bytes_f32(kk, v[g]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int c = at(g, e);
+          const bool in = live && c < cols;
+          w[e] = in ? to_f32(wgt[c]) : 0.f;
+          gr[e] = in ? to_f32(grad[c]) : 0.f;
+          v[g][e] = in ? float(k[c]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const bool in = live && at(g, VEC ? 0 : e) < cols;
+        v[g][e] = in ? v[g][e] * s : 0.f;
+        if (in) dw[g][e] = fmaf(gr[e], v[g][e], dw[g][e]);
+        gw[g][e] = gr[e] * w[e];
+        dot = fmaf(gw[g][e], v[g][e], dot);
+      }
+    }
+    if (!p.grad_x) continue;   // uniform over the grid
+    const float c_mean = row_sum(dot, p.tpr, warp_sums) / float(cols);
+    if (!live) continue;
+    const T* gh = p.grad_h ? static_cast<const T*>(p.grad_h) + rr * p.ldgh : nullptr;
+    T* out = static_cast<T*>(p.grad_x) + rr * p.ldx;
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) o[e] = u * (gw[g][e] - v[g][e] * c_mean);
+      if (VEC) {
+        const int c = at(g, 0);
+        if (c < cols) {
+          if (gh) {
+            Vec8<T> a;
+            float h[8];
+            a.load(gh + c);
+            a.get(h);
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] += h[e];
+          }
+          store8(out + c, o);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int c = at(g, e);
+          if (c < cols) out[c] = from_f32<T>(o[e] + (gh ? to_f32(gh[c]) : 0.f));
+        }
+      }
+    }
+  }
+  if (p.partial && slot < p.slots) {
+    float* o = p.partial + slot * p.cols;
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (at(g, e) < cols) o[at(g, e)] = dw[g][e];
+  }
+}
+
+// Rows too long for registers, grad_x: one block per row.
+template <typename T, typename GT>
+__global__ void __launch_bounds__(1024) norm_backward_long_kernel(BackArgs p) {
+  __shared__ float warp_sums[32];
+  const int64_t row = blockIdx.x;
+  const float u = p.rstd[row], s = p.ckpt_scale[row] * u;
+  const GT* grad = static_cast<const GT*>(p.grad) + row * p.ldg;
+  const int8_t* k = p.ckpt + row * p.ldk;
+  const T* wgt = static_cast<const T*>(p.weight);
+  float dot = 0.f;
+  for (int64_t c = threadIdx.x; c < p.cols; c += blockDim.x) dot = fmaf(to_f32(grad[c]) * to_f32(wgt[c]), float(k[c]) * s, dot);
+  const float c_mean = row_sum(dot, blockDim.x, warp_sums) / float(p.cols);
+  for (int64_t c = threadIdx.x; c < p.cols; c += blockDim.x) {
+    float o = u * (to_f32(grad[c]) * to_f32(wgt[c]) - float(k[c]) * s * c_mean);
+    if (p.grad_h) o += to_f32(static_cast<const T*>(p.grad_h)[row * p.ldgh + c]);
+    static_cast<T*>(p.grad_x)[row * p.ldx + c] = from_f32<T>(o);
+  }
+}
+
+// Partial column sums, one thread per column, slot blockIdx.y takes rows
+// y, y + slots, ...: sum of x (ckpt null) or of x * v (the norm's weight).
+template <typename GT>
+__global__ void __launch_bounds__(256) column_partial_kernel(int64_t rows, int64_t cols, const GT* x, int64_t ldx,
+                                                             const int8_t* ckpt, int64_t ldk, const float* ckpt_scale,
+                                                             const float* rstd, float* partial) {
+  const int64_t c = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (c >= cols) return;
+  float s = 0.f;
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    const float g = to_f32(x[r * ldx + c]);
+    s = ckpt ? fmaf(g, float(ckpt[r * ldk + c]) * (ckpt_scale[r] * rstd[r]), s) : s + g;
+  }
+  partial[int64_t(blockIdx.y) * cols + c] = s;
+}
+
+// out[c] = sum over slots of partial[slot, c]: 32 columns x 8 slot lanes per
+// block, joined in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(256) column_join_kernel(int64_t slots, int64_t cols, const float* partial, T* out) {
+  __shared__ float part[8][33];
+  const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t c = int64_t(blockIdx.x) * 32 + lane;
+  float s = 0.f;
+  if (c < cols)
+    for (int64_t r = y; r < slots; r += 8) s += partial[r * cols + c];
+  part[y][lane] = s;
+  __syncthreads();
+  if (y == 0 && c < cols) {
+#pragma unroll
+    for (int i = 1; i < 8; i++) s += part[i][lane];
+    out[c] = from_f32<T>(s);
+  }
+}
+
+}  // namespace tg8
+
+namespace tgi {
+
+using tg8::BackArgs;
+using tg8::RowArgs;
+
+constexpr int64_t kRowLimit = 1024 * 32;   // longest row that fits the registers of 1024 threads
+constexpr int64_t kGridLimit = 0x7fffffff;
+
+// Threads per row and groups of 8 elements per thread: at most 4 groups, and
+// as few as 1 while there are too few rows to fill the GPU.
+struct RowShape {
+  int tpr, groups, block;
+};
+RowShape row_shape(int64_t rows, int64_t cols) {
+  const int64_t groups = (cols + 7) / 8;
+  int g = rows >= 2 * sm_count() ? 4 : 1;
+  while (g < 4 && (groups + g - 1) / g > 1024) g *= 2;
+  int tpr = 32;
+  while (int64_t(tpr) * g < groups) tpr *= 2;
+  while (g > 1 && int64_t(tpr) * (g / 2) >= groups) g /= 2;
+  return {tpr, g, std::max(tpr, 128)};
+}
+
+template <typename T, bool NORM>
+tg_status launch_rows(RowArgs p, bool vec, cudaStream_t st) {
+  if (p.cols > kRowLimit) {
+    if (p.rows > kGridLimit) return fail(TG_ERR_UNSUPPORTED, "%lld rows", (long long)p.rows);
+    tg8::rows_long_kernel<T, NORM><<<unsigned(p.rows), 1024, 0, st>>>(p);
+    return check_launch("rows8");
+  }
+  const RowShape s = row_shape(p.rows, p.cols);
+  p.tpr = s.tpr;
+  const int per = s.block / s.tpr;
+  const int64_t grid = (p.rows + per - 1) / per;
+  if (grid > kGridLimit) return fail(TG_ERR_UNSUPPORTED, "%lld rows", (long long)p.rows);
+  auto go = [&](auto vec_c) {
+    constexpr bool V = decltype(vec_c)::value;
+    if (s.groups == 1) tg8::rows_kernel<T, 1, V, NORM><<<unsigned(grid), s.block, 0, st>>>(p);
+    else if (s.groups == 2) tg8::rows_kernel<T, 2, V, NORM><<<unsigned(grid), s.block, 0, st>>>(p);
+    else tg8::rows_kernel<T, 4, V, NORM><<<unsigned(grid), s.block, 0, st>>>(p);
+  };
+  if (vec) go(std::true_type{}); else go(std::false_type{});
+  return check_launch("rows8");
+}
+
+template <typename T, typename GT>
+tg_status launch_norm_backward(BackArgs p, T* grad_w, bool vec, cudaStream_t st) {
+  const bool lng = p.cols > kRowLimit;
+  RowShape s = lng ? RowShape{1024, 4, 1024} : row_shape(p.rows, p.cols);
+  const int per = s.block / s.tpr;
+  p.tpr = s.tpr;
+  const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((p.rows + per - 1) / per, sm_count() * int64_t(std::max(1, 1024 / s.block))));
+  p.slots = lng ? std::max<int64_t>(1, std::min<int64_t>(p.rows, 64)) : blocks * per;
+  if (lng && p.rows > kGridLimit) return fail(TG_ERR_UNSUPPORTED, "%lld rows", (long long)p.rows);
+  void* scratch = nullptr;
+  if (grad_w) {
+    const cudaError_t e = scratch_alloc(&scratch, size_t(p.slots) * size_t(p.cols) * sizeof(float), st);
+    if (e != cudaSuccess) return fail(TG_ERR_CUDA, "norm backward scratch: %s", cudaGetErrorString(e));
+    p.partial = static_cast<float*>(scratch);
+  }
+  if (lng) {
+    if (p.grad_x && p.rows) tg8::norm_backward_long_kernel<T, GT><<<unsigned(p.rows), 1024, 0, st>>>(p);
+    if (grad_w)
+      tg8::column_partial_kernel<GT><<<dim3(unsigned((p.cols + 255) / 256), unsigned(p.slots)), 256, 0, st>>>(
+          p.rows, p.cols, static_cast<const GT*>(p.grad), p.ldg, p.ckpt, p.ldk, p.ckpt_scale, p.rstd, p.partial);
+  } else {
+    auto go = [&](auto vec_c) {
+      constexpr bool V = decltype(vec_c)::value;
+      if (s.groups == 1) tg8::norm_backward_kernel<T, GT, 1, V><<<unsigned(blocks), s.block, 0, st>>>(p);
+      else if (s.groups == 2) tg8::norm_backward_kernel<T, GT, 2, V><<<unsigned(blocks), s.block, 0, st>>>(p);
+      else tg8::norm_backward_kernel<T, GT, 4, V><<<unsigned(blocks), s.block, 0, st>>>(p);
+    };
+    if (vec) go(std::true_type{}); else go(std::false_type{});
+  }
+  tg_status r = check_launch("rows8 norm backward");
+  if (grad_w) {
+    if (r == TG_OK) {
+      tg8::column_join_kernel<T><<<unsigned((p.cols + 31) / 32), 256, 0, st>>>(p.slots, p.cols, p.partial, grad_w);
+      r = check_launch("rows8 norm backward");
+    }
+    scratch_free(scratch, st);
+  }
+  return r;
+}
+
+tg_status check_rows(int64_t rows, int64_t cols) {
+  if (rows < 0 || cols < 0) return fail(TG_ERR_INVALID_ARGUMENT, "negative size (rows=%lld cols=%lld)", (long long)rows, (long long)cols);
+  if (cols > kGridLimit) return fail(TG_ERR_UNSUPPORTED, "cols=%lld", (long long)cols);
+  return TG_OK;
+}
+tg_status check_ld(const char* name, int64_t ld, int64_t cols) {
+  if (ld < cols) return fail(TG_ERR_DIMENSION_MISMATCH, "%s=%lld < %lld", name, (long long)ld, (long long)cols);
+  return TG_OK;
+}
+tg_status check_type8(tg_dtype t) {
+  if (!elem8_size(t)) return fail(TG_ERR_INVALID_ARGUMENT, "8-bit rows need f32, f16 or bf16, got dtype %d", int(t));
+  return TG_OK;
+}
+
+}  // namespace tgi
+
+using namespace tgi;
+
+#define TG8_CHECK(call)                 \
+  do {                                  \
+    const tg_status s_ = (call);        \
+    if (s_ != TG_OK) return s_;         \
+  } while (0)
+
+extern "C" {
+
+tg_status tg_rows8_quantize(tg_dtype dtype, int64_t rows, int64_t cols, const void* x, int64_t ldx, int8_t* q,
+                            int64_t ldq, float* scale, void* stream) {
+  clear_error();
+  TG8_CHECK(check_type8(dtype));
+  TG8_CHECK(check_rows(rows, cols));
+  if (rows == 0) return TG_OK;
+  if (!scale || (cols && (!x || !q))) return fail(TG_ERR_INVALID_ARGUMENT, "null operand");
+  TG8_CHECK(check_ld("ldx", ldx, cols));
+  TG8_CHECK(check_ld("ldq", ldq, cols));
+  RowArgs p{};
+  p.rows = rows; p.cols = cols; p.x = x; p.ldx = ldx; p.q = q; p.ldq = ldq; p.scale = scale;
+  const size_t e = elem8_size(dtype);
+  const bool vec = cols % 8 == 0 && rows_vec(x, ldx, e) && rows_vec(q, ldq, 1, 8);
+  return with_type8(dtype, [&](auto t) { return launch_rows<decltype(t), false>(p, vec, static_cast<cudaStream_t>(stream)); });
+}
+
+tg_status tg_rows8_dequantize(tg_dtype dtype, int64_t rows, int64_t cols, const int8_t* q, int64_t ldq,
+                              const float* scale, void* y, int64_t ldy, void* stream) {
+  clear_error();
+  TG8_CHECK(check_type8(dtype));
+  TG8_CHECK(check_rows(rows, cols));
+  if (rows == 0 || cols == 0) return TG_OK;
+  if (!q || !scale || !y) return fail(TG_ERR_INVALID_ARGUMENT, "null operand");
+  TG8_CHECK(check_ld("ldq", ldq, cols));
+  TG8_CHECK(check_ld("ldy", ldy, cols));
+  const bool vec = cols % 8 == 0 && rows_vec(y, ldy, elem8_size(dtype)) && rows_vec(q, ldq, 1, 8);
+  const int64_t per = vec ? cols / 8 : cols;
+  if (rows > (kGridLimit * 256) / per) return fail(TG_ERR_UNSUPPORTED, "%lld x %lld elements", (long long)rows, (long long)cols);
+  const unsigned grid = unsigned((rows * per + 255) / 256);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return with_type8(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (vec) tg8::dequantize_kernel<T, true><<<grid, 256, 0, st>>>(rows, cols, q, ldq, scale, static_cast<T*>(y), ldy);
+    else tg8::dequantize_kernel<T, false><<<grid, 256, 0, st>>>(rows, cols, q, ldq, scale, static_cast<T*>(y), ldy);
+    return check_launch("rows8 dequantize");
+  });
+}
+
+tg_status tg_rows8_rmsnorm(tg_dtype dtype, int64_t rows, int64_t cols, const void* x, int64_t ldx,
+                           const void* residual, int64_t ldr, const void* weight, float eps, void* h, int64_t ldh,
+                           int8_t* q, int64_t ldq, float* scale, int8_t* ckpt, int64_t ldk, float* ckpt_scale,
+                           float* rstd, void* stream) {
+  clear_error();
+  TG8_CHECK(check_type8(dtype));
+  TG8_CHECK(check_rows(rows, cols));
+  if (!(eps >= 0.f)) return fail(TG_ERR_INVALID_ARGUMENT, "eps=%g is negative", double(eps));
+  if ((ckpt != nullptr) != (ckpt_scale != nullptr) || (ckpt != nullptr) != (rstd != nullptr))
+    return fail(TG_ERR_INVALID_ARGUMENT, "ckpt, ckpt_scale and rstd are given together or not at all");
+  if (rows == 0 || cols == 0) {
+    if (rows && (!scale || ckpt)) return fail(TG_ERR_INVALID_ARGUMENT, "a row of no columns has no norm");
+    if (rows) {
+      const cudaError_t e = cudaMemsetAsync(scale, 0, size_t(rows) * sizeof(float), static_cast<cudaStream_t>(stream));
+      if (e != cudaSuccess) return fail(TG_ERR_CUDA, "memset: %s", cudaGetErrorString(e));
+    }
+    return TG_OK;
+  }
+  if (!x || !weight || !q || !scale) return fail(TG_ERR_INVALID_ARGUMENT, "null operand");
+  TG8_CHECK(check_ld("ldx", ldx, cols));
+  if (residual) TG8_CHECK(check_ld("ldr", ldr, cols));
+  if (h) TG8_CHECK(check_ld("ldh", ldh, cols));
+  TG8_CHECK(check_ld("ldq", ldq, cols));
+  if (ckpt) TG8_CHECK(check_ld("ldk", ldk, cols));
+  RowArgs p{};
+  p.rows = rows; p.cols = cols; p.x = x; p.ldx = ldx; p.residual = residual; p.ldr = ldr; p.weight = weight;
+  p.eps = eps; p.h = h; p.ldh = ldh; p.q = q; p.ldq = ldq; p.scale = scale;
+  p.ckpt = ckpt; p.ldk = ldk; p.ckpt_scale = ckpt_scale; p.rstd = rstd;
+  const size_t e = elem8_size(dtype);
+  const bool vec = cols % 8 == 0 && rows_vec(x, ldx, e) && rows_vec(residual, ldr, e) && aligned(weight, 16) &&
+                   rows_vec(h, ldh, e) && rows_vec(q, ldq, 1, 8) && rows_vec(ckpt, ldk, 1, 8);
+  return with_type8(dtype, [&](auto t) { return launch_rows<decltype(t), true>(p, vec, static_cast<cudaStream_t>(stream)); });
+}
+
+tg_status tg_rows8_rmsnorm_backward(tg_dtype dtype, tg_dtype grad_dtype, int64_t rows, int64_t cols, const void* grad,
+                                    int64_t ldg, const void* grad_h, int64_t ldgh, const void* weight,
+                                    const int8_t* ckpt, int64_t ldk, const float* ckpt_scale, const float* rstd,
+                                    void* grad_x, int64_t ldx, void* grad_weight, void* stream) {
+  clear_error();
+  TG8_CHECK(check_type8(dtype));
+  if (grad_dtype != dtype && grad_dtype != TG_F32) return fail(TG_ERR_INVALID_ARGUMENT, "grad is of type dtype or f32, got dtype %d", int(grad_dtype));
+  TG8_CHECK(check_rows(rows, cols));
+  if (cols == 0 || (!grad_x && !grad_weight)) return TG_OK;
+  if (rows && (!grad || !weight || !ckpt || !ckpt_scale || !rstd)) return fail(TG_ERR_INVALID_ARGUMENT, "null operand");
+  if (rows) {
+    TG8_CHECK(check_ld("ldg", ldg, cols));
+    if (grad_h) TG8_CHECK(check_ld("ldgh", ldgh, cols));
+    TG8_CHECK(check_ld("ldk", ldk, cols));
+    if (grad_x) TG8_CHECK(check_ld("ldx", ldx, cols));
+  }
+  BackArgs p{};
+  p.rows = rows; p.cols = cols; p.grad = grad; p.ldg = ldg; p.grad_h = grad_h; p.ldgh = ldgh; p.weight = weight;
+  p.ckpt = ckpt; p.ldk = ldk; p.ckpt_scale = ckpt_scale; p.rstd = rstd; p.grad_x = grad_x; p.ldx = ldx;
+  if (rows == 0 && !grad_weight) return TG_OK;
+  const size_t e = elem8_size(dtype);
+  const bool vec = cols % 8 == 0 && rows_vec(grad, ldg, elem8_size(grad_dtype)) && rows_vec(grad_h, ldgh, e) &&
+                   aligned(weight, 16) && rows_vec(ckpt, ldk, 1, 8) && rows_vec(grad_x, ldx, e);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return with_type8(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (grad_dtype == dtype) return launch_norm_backward<T, T>(p, static_cast<T*>(grad_weight), vec, st);
+    return launch_norm_backward<T, float>(p, static_cast<T*>(grad_weight), vec, st);
+  });
+}
+
+tg_status tg_rows8_column_sum(tg_dtype dtype, tg_dtype out_dtype, int64_t rows, int64_t cols, const void* x, int64_t ldx,
+                              void* out, void* stream) {
+  clear_error();
+  TG8_CHECK(check_type8(dtype));
+  TG8_CHECK(check_type8(out_dtype));
+  TG8_CHECK(check_rows(rows, cols));
+  if (cols == 0) return TG_OK;
+  if (!out || (rows && !x)) return fail(TG_ERR_INVALID_ARGUMENT, "null operand");
+  if (rows) TG8_CHECK(check_ld("ldx", ldx, cols));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // enough slots to fill the GPU, no more than there are rows
+  const int64_t strips = (cols + 255) / 256;
+  const int64_t slots = std::max<int64_t>(1, std::min<int64_t>({rows, 1024, (8 * int64_t(sm_count()) + strips - 1) / strips}));
+  void* scratch = nullptr;
+  const cudaError_t e = scratch_alloc(&scratch, size_t(slots) * size_t(cols) * sizeof(float), st);
+  if (e != cudaSuccess) return fail(TG_ERR_CUDA, "column sum scratch: %s", cudaGetErrorString(e));
+  float* partial = static_cast<float*>(scratch);
+  tg_status r = with_type8(dtype, [&](auto t) {
+    using T = decltype(t);
+    tg8::column_partial_kernel<T><<<dim3(unsigned(strips), unsigned(slots)), 256, 0, st>>>(
+        rows, cols, static_cast<const T*>(x), ldx, nullptr, 0, nullptr, nullptr, partial);
+    return check_launch("rows8 column sum");
+  });
+  if (r == TG_OK)
+    r = with_type8(out_dtype, [&](auto t) {
+      using T = decltype(t);
+      tg8::column_join_kernel<T><<<unsigned((cols + 31) / 32), 256, 0, st>>>(slots, cols, partial, static_cast<T*>(out));
+      return check_launch("rows8 column sum");
+    });
+  scratch_free(scratch, st);
+  return r;
+}
+
+}  // extern "C"

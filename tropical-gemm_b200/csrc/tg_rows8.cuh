@@ -1,0 +1,141 @@
+// Shared by the 8-bit row kernels: element types, 8-element vector access,
+// the quantisation rule and small host helpers.
+#pragma once
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include "tg_internal.h"
+
+namespace tg8 {
+
+using bf16 = __nv_bfloat16;
+using f16 = __half;
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(bf16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(f16 v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ bf16 from_f32<bf16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ f16 from_f32<f16>(float v) { return __float2half_rn(v); }
+
+// Eight consecutive elements as loaded (16-byte aligned), and as f32.
+template <typename T> struct Vec8;
+template <> struct Vec8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) { a = *reinterpret_cast<const float4*>(p); b = *reinterpret_cast<const float4*>(p + 4); }
+  __device__ __forceinline__ void zero() { a = b = make_float4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float (&v)[8]) const { v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w; }
+};
+template <> struct Vec8<bf16> {
+  uint4 a;
+  __device__ __forceinline__ void load(const bf16* p) { a = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void zero() { a = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  }
+};
+template <> struct Vec8<f16> {
+  uint4 a;
+  __device__ __forceinline__ void load(const f16* p) { a = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void zero() { a = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+};
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(bf16* p, const float (&v)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store8(f16* p, const float (&v)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const __half2 b = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// One row's quantisation from its largest magnitude, given as the maximum of
+// the values' bit patterns without the sign: unsigned order is magnitude
+// order, with infinities and NaN on top, so a maximum never loses a NaN.
+struct Quant {
+  float scale, inv;
+};
+__device__ __forceinline__ Quant quant_of(uint32_t top_bits) {
+  Quant s;
+  const float top = __uint_as_float(top_bits);
+  if (top_bits >= 0x7f800000u) {   // an infinity or a NaN: the row reads as NaN
+    s.scale = __uint_as_float(0x7fffffffu);
+    s.inv = 0.f;
+  } else if (top < 7.52316385e-37f) {   // 2^-120: 127 / top would overflow not far below
+    s.scale = s.inv = 0.f;
+  } else {
+    s.scale = top / 127.f;
+    s.inv = 127.f / top;
+  }
+  return s;
+}
+// y * inv rounded to nearest even, as the low byte of the result: adding
+// 1.5 * 2^23 leaves the integer in the low mantissa bits (|y * inv| < 128).
+__device__ __forceinline__ uint32_t quant8(float y, float inv) {
+  return __float_as_uint(fmaf(y, inv, 12582912.f));
+}
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+__device__ __forceinline__ uint2 quant_pack8(const float (&v)[8], float inv) {
+  return make_uint2(pack4(quant8(v[0], inv), quant8(v[1], inv), quant8(v[2], inv), quant8(v[3], inv)),
+                    pack4(quant8(v[4], inv), quant8(v[5], inv), quant8(v[6], inv), quant8(v[7], inv)));
+}
+// Byte i of w as a signed integer in f32, by way of 2^23 + (byte + 128).
+template <int I> __device__ __forceinline__ float byte_f32(uint32_t w_biased) {
+  return __uint_as_float(__byte_perm(w_biased, 0x4b000000u, 0x7650 | I)) - 8388736.f;
+}
+__device__ __forceinline__ void bytes_f32(uint2 w, float (&v)[8]) {
+  const uint32_t a = w.x ^ 0x80808080u, b = w.y ^ 0x80808080u;
+  v[0] = byte_f32<0>(a); v[1] = byte_f32<1>(a); v[2] = byte_f32<2>(a); v[3] = byte_f32<3>(a);
+  v[4] = byte_f32<0>(b); v[5] = byte_f32<1>(b); v[6] = byte_f32<2>(b); v[7] = byte_f32<3>(b);
+}
+
+}  // namespace tg8
+
+namespace tgi {
+
+inline size_t elem8_size(tg_dtype t) { return t == TG_F32 ? 4 : (t == TG_BF16 || t == TG_F16) ? 2 : 0; }
+inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+// p null, or 16-byte aligned rows of `elem`-byte elements
+inline bool rows_vec(const void* p, int64_t ld, size_t elem, size_t bytes = 16) {
+  return !p || (aligned(p, bytes) && (ld * int64_t(elem)) % int64_t(bytes) == 0);
+}
+
+// f(T{}) for the element type of a tg_rows8 call; the caller has checked dtype.
+template <typename F> tg_status with_type8(tg_dtype t, F&& f) {
+  switch (t) {
+    case TG_F32: return f(float{});
+    case TG_F16: return f(tg8::f16{});
+    case TG_BF16: return f(tg8::bf16{});
+    default: return fail(TG_ERR_INVALID_ARGUMENT, "8-bit rows need f32, f16 or bf16, got dtype %d", int(t));
+  }
+}
+
+}  // namespace tgi

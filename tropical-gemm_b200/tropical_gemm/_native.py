@@ -59,6 +59,19 @@ def lib() -> ctypes.CDLL:
             fn.argtypes = [i32, i32, i32, i64, i64, i64, i64, vp, i64, i64, i32p, vp, i64, i64, vp, i64, i64,
                            i32, vp]
             fn.restype = i32
+        f32 = ctypes.c_float
+        for name, args in {
+            "tg_rows8_quantize": [i32, i64, i64, vp, i64, vp, i64, vp, vp],
+            "tg_rows8_dequantize": [i32, i64, i64, vp, i64, vp, vp, i64, vp],
+            "tg_rows8_rmsnorm": [i32, i64, i64, vp, i64, vp, i64, vp, f32, vp, i64, vp, i64, vp, vp, i64, vp, vp, vp],
+            "tg_rows8_rmsnorm_backward": [i32, i32, i64, i64, vp, i64, vp, i64, vp, vp, i64, vp, vp, vp, i64, vp, vp],
+            "tg_rows8_gemm": [i32, i64, i64, i64, vp, i64, vp, vp, i64, vp, vp, vp, i64, vp],
+            "tg_rows8_gemm_backward": [i32, i32, i32, i64, i64, i64, vp, i64, vp, i64, vp, vp, i64, vp],
+            "tg_rows8_column_sum": [i32, i32, i64, i64, vp, i64, vp, vp],
+        }.items():
+            fn = getattr(L, name)
+            fn.argtypes = args
+            fn.restype = i32
         _lib = L
     return _lib
 
