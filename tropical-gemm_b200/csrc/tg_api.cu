@@ -78,8 +78,8 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-bool encode_tma_f32(const void* base, int64_t inner, int64_t rows, int64_t ld, int64_t batch, int64_t bstride,
-                    uint32_t box_inner, uint32_t box_rows, CUtensorMap* out, bool swizzle) {
+bool encode_tma(CUtensorMapDataType type, uint32_t elem, const void* base, int64_t inner, int64_t rows, int64_t ld,
+                int64_t batch, int64_t bstride, uint32_t box_inner, uint32_t box_rows, CUtensorMap* out, bool swizzle) {
   static std::once_flag once;
   static EncodeTiledFn fn = nullptr;
   std::call_once(once, [] {
@@ -92,12 +92,17 @@ bool encode_tma_f32(const void* base, int64_t inner, int64_t rows, int64_t ld, i
   });
   if (!fn) return false;
   const cuuint64_t dims[3] = {cuuint64_t(inner), cuuint64_t(rows), cuuint64_t(batch)};
-  const cuuint64_t strides[2] = {cuuint64_t(ld) * 4, cuuint64_t(batch > 1 ? bstride : ld * rows) * 4};
+  const cuuint64_t strides[2] = {cuuint64_t(ld) * elem, cuuint64_t(batch > 1 ? bstride : ld * rows) * elem};
   const cuuint32_t box[3] = {box_inner, box_rows, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
-  return fn(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(base), dims, strides, box, estr,
+  return fn(out, type, 3, const_cast<void*>(base), dims, strides, box, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool encode_tma_f32(const void* base, int64_t inner, int64_t rows, int64_t ld, int64_t batch, int64_t bstride,
+                    uint32_t box_inner, uint32_t box_rows, CUtensorMap* out, bool swizzle) {
+  return encode_tma(CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, inner, rows, ld, batch, bstride, box_inner, box_rows, out, swizzle);
 }
 
 int kernel_regs(const void* kern) {

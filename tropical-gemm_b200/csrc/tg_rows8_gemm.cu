@@ -2,114 +2,87 @@
 // integers and the products of its backward.
 #include <algorithm>
 #include "tg_rows8.cuh"
+#include "tg_rows8_umma.cuh"
 
-namespace tg8 {
+namespace tgi {
 
-struct GemmArgs8 {
-  int64_t m, n, k;
-  const int8_t *a, *b;
-  const float *a_scale, *b_scale;
-  const void* bias;
-  void* c;
-  int64_t lda, ldb, ldc;
+using tg8::ProductArgs;
+
+// Scratch of one call, freed in stream order when the call returns.
+class Scratch {
+ public:
+  explicit Scratch(cudaStream_t st) : st_(st) {}
+  Scratch(const Scratch&) = delete;
+  ~Scratch() {
+    if (p_) scratch_free(p_, st_);
+  }
+  cudaError_t reserve(size_t bytes) { return scratch_alloc(&p_, bytes, st_); }
+  template <typename T> T* take(size_t count) {
+    T* r = reinterpret_cast<T*>(static_cast<char*>(p_) + used_);
+    used_ += size_of<T>(count);
+    return r;
+  }
+  template <typename T> static size_t size_of(size_t count) { return (count * sizeof(T) + 255) & ~size_t(255); }
+
+ private:
+  void* p_ = nullptr;
+  size_t used_ = 0;
+  cudaStream_t st_;
 };
 
-constexpr int kST = 64;   // tile edge of the simple kernels
-constexpr int kSK = 32;   // bytes (forward) or rows (backward) of the sum per step
-
-// 64 x 64 tile, 256 threads, 4 x 4 outputs each, four products per dp4a; any
-// alignment.
-template <typename T>
-__global__ void __launch_bounds__(256) gemm8_simple_kernel(GemmArgs8 p) {
-  __shared__ __align__(16) int8_t as[kST][kSK + 4], bs[kST][kSK + 4];
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int64_t m0 = int64_t(blockIdx.y) * kST, n0 = int64_t(blockIdx.x) * kST;
-  int acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < p.k; k0 += kSK) {
-    for (int i = tid; i < kST * kSK; i += 256) {
-      const int r = i / kSK, c = i % kSK;
-      const bool in = k0 + c < p.k;
-      as[r][c] = in && m0 + r < p.m ? p.a[(m0 + r) * p.lda + k0 + c] : 0;
-      bs[r][c] = in && n0 + r < p.n ? p.b[(n0 + r) * p.ldb + k0 + c] : 0;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < kSK; c += 4) {
-      int av[4], bv[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        av[i] = *reinterpret_cast<const int*>(&as[ty * 4 + i][c]);
-        bv[i] = *reinterpret_cast<const int*>(&bs[tx + 16 * i][c]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = __dp4a(av[i], bv[j], acc[i][j]);
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int64_t r = m0 + ty * 4 + i, c = n0 + tx + 16 * j;
-      if (r < p.m && c < p.n) {
-        float z = float(acc[i][j]) * p.a_scale[r] * p.b_scale[c];
-        if (p.bias) z += to_f32(static_cast<const T*>(p.bias)[c]);
-        static_cast<T*>(p.c)[r * p.ldc + c] = from_f32<T>(z);
-      }
-    }
+int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+dim3 row_grid(int64_t cols_per_block, int64_t cols, int64_t rows) {
+  return dim3(unsigned((cols + cols_per_block - 1) / cols_per_block), unsigned(std::min<int64_t>(rows, 16384)));
 }
 
-struct BackGemmArgs {
-  int64_t p, cols, r;
-  const void* g;
+// 8-bit rows a TMA load can take: 16-byte aligned rows of at least one byte.
+bool tma_rows8(const int8_t* q, int64_t ld, int64_t rows, int64_t cols) {
+  return cols > 0 && aligned(q, 16) && (ld % 16 == 0 || rows == 1);
+}
+struct Operand8 {
   const int8_t* q;
-  const float* scale;
-  void* out;
-  int64_t ldg, ldq, ldo;
-  int transposed;
+  int64_t ld, rows, cols;
+  bool pad;
+  Operand8(const int8_t* q_, int64_t ld_, int64_t rows_, int64_t cols_)
+      : q(q_), ld(ld_), rows(rows_), cols(cols_), pad(!tma_rows8(q_, ld_, rows_, cols_)) {}
+  int64_t padded() const { return std::max<int64_t>(16, round_up(cols, 16)); }
+  size_t scratch() const { return pad ? Scratch::size_of<int8_t>(size_t(rows) * size_t(padded())) : 0; }
+  // A padded copy where the rows are not aligned; cols stays the sum's own
+  // length (at least 1: a sum of nothing is a sum over one zero).
+  void make(Scratch& s, cudaStream_t st) {
+    if (pad) {
+      int8_t* out = s.take<int8_t>(size_t(rows) * size_t(padded()));
+      tg8::pad8_kernel<<<row_grid(1024, padded(), rows), 256, 0, st>>>(rows, cols, q, ld, out, padded());
+      q = out;
+      ld = padded();
+      cols = std::max<int64_t>(cols, 1);
+    } else if (rows == 1) {
+      ld = padded();
+    }
+  }
+  bool map(uint32_t box_cols, uint32_t box_rows, CUtensorMap* m) const {
+    return encode_tma(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q, cols, rows, ld, 1, 0, box_cols, box_rows, m);
+  }
 };
 
-template <typename GT, typename T>
-__global__ void __launch_bounds__(256) gemm8_backward_simple_kernel(BackGemmArgs a) {
-  __shared__ float gs[kSK][kST + 1], qs[kSK][kST];
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int64_t p0 = int64_t(blockIdx.y) * kST, c0 = int64_t(blockIdx.x) * kST;
-  const GT* g = static_cast<const GT*>(a.g);
-  float acc[4][4] = {};
-  for (int64_t r0 = 0; r0 < a.r; r0 += kSK) {
-    for (int i = tid; i < kST * kSK; i += 256) {
-      int rr = i / kST, pp = i % kST;
-      if (!a.transposed) { rr = i % kSK; pp = i / kSK; }
-      const bool in = r0 + rr < a.r && p0 + pp < a.p;
-      gs[rr][pp] = in ? to_f32(a.transposed ? g[(r0 + rr) * a.ldg + p0 + pp] : g[(p0 + pp) * a.ldg + r0 + rr]) : 0.f;
-      const int r = i / kST, c = i % kST;
-      qs[r][c] = r0 + r < a.r && c0 + c < a.cols ? float(a.q[(r0 + r) * a.ldq + c0 + c]) * a.scale[r0 + r] : 0.f;
-    }
-    __syncthreads();
-#pragma unroll 8
-    for (int r = 0; r < kSK; r++) {
-      float gv[4], qv[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) { gv[i] = gs[r][ty * 4 + i]; qv[i] = qs[r][tx + 16 * i]; }
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = fmaf(gv[i], qv[j], acc[i][j]);
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int64_t r = p0 + ty * 4 + i, c = c0 + tx + 16 * j;
-      if (r < a.p && c < a.cols) static_cast<T*>(a.out)[r * a.ldo + c] = from_f32<T>(acc[i][j]);
-    }
+template <int MODE, typename T>
+tg_status launch_product(const CUtensorMap& a, const CUtensorMap& b, ProductArgs p, cudaStream_t st) {
+  const int64_t tm = (p.m + tg8::kTile - 1) / tg8::kTile, tn = (p.n + tg8::kTile - 1) / tg8::kTile;
+  if (tm * tn > 0x3fffffff || p.m > 0x7ffffc00 || p.n > 0x7ffffc00)
+    return fail(TG_ERR_UNSUPPORTED, "%lld x %lld outputs", (long long)p.m, (long long)p.n);
+  p.tiles_m = int(tm);
+  p.tiles_n = int(tn);
+  p.vec = aligned(p.c, 16) && (p.ldc * int64_t(sizeof(T))) % 16 == 0;
+  auto kern = tg8::product_kernel<MODE, T>;
+  using S = tg8::ProductShape<MODE>;
+  const tg_status s = ensure_smem(reinterpret_cast<const void*>(kern), S::kSmem);
+  if (s != TG_OK) return s;
+  const int pairs = int(std::min<int64_t>(tm * tn, std::max(1, sm_count() / 2)));
+  kern<<<2 * pairs, S::kThreads, S::kSmem, st>>>(a, b, p);
+  return check_launch("rows8 product");
 }
 
-}  // namespace tg8
+}  // namespace tgi
 
 using namespace tgi;
 
@@ -127,13 +100,23 @@ tg_status tg_rows8_gemm(tg_dtype dtype, int64_t m, int64_t n, int64_t k, const i
   if (lda < k) return fail(TG_ERR_DIMENSION_MISMATCH, "lda=%lld < %lld", (long long)lda, (long long)k);
   if (ldb < k) return fail(TG_ERR_DIMENSION_MISMATCH, "ldb=%lld < %lld", (long long)ldb, (long long)k);
   if (ldc < n) return fail(TG_ERR_DIMENSION_MISMATCH, "ldc=%lld < %lld", (long long)ldc, (long long)n);
-  if (m > 65535ll * tg8::kST || n > 0x7fffffff) return fail(TG_ERR_UNSUPPORTED, "m=%lld n=%lld", (long long)m, (long long)n);
-  const tg8::GemmArgs8 p{m, n, k, a, b, a_scale, b_scale, bias, c, lda, ldb, ldc};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return with_type8(dtype, [&](auto t) {
-    tg8::gemm8_simple_kernel<decltype(t)><<<dim3(unsigned((n + 63) / 64), unsigned((m + 63) / 64)), 256, 0, st>>>(p);
-    return check_launch("rows8 gemm");
-  });
+  Operand8 oa(a, lda, m, k), ob(b, ldb, n, k);
+  Scratch scratch(st);
+  if (const size_t need = oa.scratch() + ob.scratch()) {
+    const cudaError_t e = scratch.reserve(need);
+    if (e != cudaSuccess) return fail(TG_ERR_CUDA, "rows8 gemm scratch: %s", cudaGetErrorString(e));
+  }
+  oa.make(scratch, st);
+  ob.make(scratch, st);
+  ProductArgs p{};
+  p.m = m; p.n = n; p.ldc = ldc; p.c = c; p.row_scale = a_scale; p.col_scale = b_scale; p.bias = bias;
+  p.sum = int(k);
+  p.planes = 1;
+  p.blocks = std::max(1, int((k + 127) / 128));
+  CUtensorMap ma, mb;
+  if (!oa.map(128, 128, &ma) || !ob.map(128, 128, &mb)) return fail(TG_ERR_CUDA, "rows8 gemm: tensor map encoding failed");
+  return with_type8(dtype, [&](auto t) { return launch_product<tg8::kForward, decltype(t)>(ma, mb, p, st); });
 }
 
 tg_status tg_rows8_gemm_backward(tg_dtype grad_dtype, tg_dtype out_dtype, int transposed, int64_t p, int64_t cols,
@@ -149,15 +132,56 @@ tg_status tg_rows8_gemm_backward(tg_dtype grad_dtype, tg_dtype out_dtype, int tr
   if (r && ldg < need) return fail(TG_ERR_DIMENSION_MISMATCH, "ldg=%lld < %lld", (long long)ldg, (long long)need);
   if (r && ldq < cols) return fail(TG_ERR_DIMENSION_MISMATCH, "ldq=%lld < %lld", (long long)ldq, (long long)cols);
   if (ldo < cols) return fail(TG_ERR_DIMENSION_MISMATCH, "ldo=%lld < %lld", (long long)ldo, (long long)cols);
-  if (p > 65535ll * tg8::kST || cols > 0x7fffffff || r > 0x7fffffff)
+  if (p > 0x7ffffc00 || cols > 0x7ffffc00 || r > 0x3ffffc00)
     return fail(TG_ERR_UNSUPPORTED, "p=%lld cols=%lld r=%lld", (long long)p, (long long)cols, (long long)r);
-  const tg8::BackGemmArgs a{p, cols, r, g, q, scale, out, ldg, ldq, ldo, transposed};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return with_type8(grad_dtype, [&](auto gt) {
-    return with_type8(out_dtype, [&](auto t) {
-      tg8::gemm8_backward_simple_kernel<decltype(gt), decltype(t)><<<dim3(unsigned((cols + 63) / 64), unsigned((p + 63) / 64)), 256, 0, st>>>(a);
+  if (r == 0) {   // a sum of nothing
+    const size_t e = elem8_size(out_dtype);
+    const cudaError_t err = cudaMemset2DAsync(out, size_t(ldo) * e, 0, size_t(cols) * e, size_t(p), st);
+    return err == cudaSuccess ? TG_OK : fail(TG_ERR_CUDA, "memset: %s", cudaGetErrorString(err));
+  }
+  const int64_t g_rows = transposed ? r : p, g_cols = transposed ? p : r;
+  // bf16 goes to the tensor core as it is, with the scale in the 8-bit
+  // operand's expansion (one rounding to bf16); f16 and f32 as the parts of
+  // g * scale, with the 8-bit operand's integers exact.
+  const int planes = grad_dtype == TG_BF16 ? 1 : grad_dtype == TG_F16 ? 2 : 3;
+  const bool direct = grad_dtype == TG_BF16 && aligned(g, 16) && (ldg % 8 == 0 || g_rows == 1);
+  const int64_t ldp = round_up(g_cols, 8);
+  const size_t part_count = direct ? 0 : size_t(planes) * size_t(g_rows) * size_t(ldp);
+  Operand8 oq(q, ldq, r, cols);
+  Scratch scratch(st);
+  if (const size_t need = oq.scratch() + Scratch::size_of<tg8::bf16>(part_count)) {
+    const cudaError_t e = scratch.reserve(need);
+    if (e != cudaSuccess) return fail(TG_ERR_CUDA, "rows8 gemm backward scratch: %s", cudaGetErrorString(e));
+  }
+  oq.make(scratch, st);
+  if (!direct) {
+    tg8::bf16* parts = scratch.take<tg8::bf16>(part_count);
+    const tg_status s = with_type8(grad_dtype, [&](auto t) {
+      using T = decltype(t);
+      tg8::split_kernel<T><<<row_grid(256, ldp, g_rows), 256, 0, st>>>(g_rows, g_cols, static_cast<const T*>(g), ldg,
+                                                                        planes > 1 ? scale : nullptr, transposed != 0, parts, ldp, planes);
       return check_launch("rows8 gemm backward");
     });
+    if (s != TG_OK) return s;
+    g = parts;
+    ldg = ldp;
+  } else if (g_rows == 1) {
+    ldg = ldp;
+  }
+  ProductArgs a{};
+  a.m = p; a.n = cols; a.ldc = ldo; a.c = out;
+  a.sum_scale = planes == 1 ? scale : nullptr;
+  a.sum = int(r);
+  a.planes = planes;
+  a.blocks = int((r + 63) / 64);
+  CUtensorMap ma, mb;
+  if (!encode_tma(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, g, g_cols, g_rows, ldg, planes, g_rows * ldg, 64, transposed ? 64 : 128, &ma) ||
+      !oq.map(128, 64, &mb))
+    return fail(TG_ERR_CUDA, "rows8 gemm backward: tensor map encoding failed");
+  return with_type8(out_dtype, [&](auto t) {
+    using T = decltype(t);
+    return transposed ? launch_product<tg8::kBackCols, T>(ma, mb, a, st) : launch_product<tg8::kBackRows, T>(ma, mb, a, st);
   });
 }
 
