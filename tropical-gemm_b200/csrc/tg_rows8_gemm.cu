@@ -78,6 +78,9 @@ tg_status launch_product(const CUtensorMap& a, const CUtensorMap& b, ProductArgs
   const tg_status s = ensure_smem(reinterpret_cast<const void*>(kern), S::kSmem);
   if (s != TG_OK) return s;
   const int pairs = int(std::min<int64_t>(tm * tn, std::max(1, sm_count() / 2)));
+  const int64_t couples = (tm / 2) * tn;
+  p.doubles = S::kHalves == 2 ? int(couples / pairs * pairs) : 0;
+  p.singles = int(tm * tn - 2 * int64_t(p.doubles));
   kern<<<2 * pairs, S::kThreads, S::kSmem, st>>>(a, b, p);
   return check_launch("rows8 product");
 }

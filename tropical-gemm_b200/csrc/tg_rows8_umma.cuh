@@ -8,10 +8,18 @@
 //
 // Both: a pair of CTAs on two SMs computes 256 x 256 outputs (one tcgen05.mma
 // covers both), CTA r holding rows 128 r .. 128 r + 127 of the left operand
-// and half of the right one.  The sum advances by 128 bytes of each left row
-// per stage of a TMA ring; two 256-column accumulators in tensor memory let
-// the epilogue of one tile run under the products of the next.  Persistent:
-// a pair walks tiles in groups of row panels, so what it reads stays in L2.
+// and half of the right one, or two such tiles one below the other that share
+// the right operand.  The sum advances by 128 bytes of each left row per stage
+// of a TMA ring; the two accumulators in tensor memory are 256 columns each.
+// Persistent: a pair walks tiles in groups of row panels, so what it reads
+// stays in L2.
+//
+// What bounds it: shared memory.  Per 256 x 256 x (128 bytes) step an SM's
+// tensor core needs 512 cycles, and reads 32 KB (256 cycles at 128 bytes per
+// cycle); TMA writes 32 KB more (forward: 512 in all).  Backward, a step
+// writes 16 + 8 KB, and the expansion reads 8 and writes 16: 640 cycles, and
+// measured 860.  Two tiles that share the right operand need 896 (forward)
+// and 1024 (backward) cycles per 1024 of tensor work.
 #pragma once
 #include "tg_rows8.cuh"
 #include "tg_umma.cuh"
@@ -28,35 +36,97 @@ struct ProductArgs {
   const float* sum_scale;     // backward: one factor per index of the sum, or null (taken into g)
   int sum;                    // length of the sum (of one plane)
   int blocks, planes;         // stages per plane, planes of g
-  int tiles_m, tiles_n;
+  int tiles_m, tiles_n;       // 256 x 256 tiles
+  int doubles;                // two-tile items, taken first (a multiple of the pairs)
+  int singles;                // one-tile items
   int vec;                    // 16-byte stores of C's rows
 };
 
 constexpr int kTile = 256, kHalf = 128;
-constexpr int kStageA = 16384, kStageB = 16384, kStageRaw = 8192;
-constexpr int kEpiWarps = 4, kConvWarps = 4;
-constexpr int kEpiPitch = 33;
+constexpr int kOperand = 16384;                 // bytes of one operand's stage: 128 rows x 128 bytes
+constexpr int kRawBytes = 8192;                 // the 8-bit tile that is expanded to one stage
+constexpr int kEpiWarps = 4, kConvWarps = 4, kConvGroups = 2;   // a group of conv warps per 8-bit tile, in turn
+constexpr int kEpiPitch = 17;
 
+// Shared memory and barriers: a ring of both operands.  Backward the right
+// operand's stages are written by the conv warps from a ring of 8-bit tiles
+// of its own, which run ahead; a stage is full when the left operand has
+// landed and both CTAs' conv warps have arrived, so the products wait and
+// commit once per stage, as in the forward kernel (a barrier and a commit of
+// its own for the expanded operand: 0.36 -> 0.40 ms without any expansion).
 template <int MODE> struct ProductShape {
   static constexpr bool kBack = MODE != kForward;
-  static constexpr int kStages = kBack ? 5 : 6;
-  static constexpr int kStage = kStageA + kStageB + (kBack ? kStageRaw : 0);
-  static constexpr int kThreads = 32 * (4 + kEpiWarps + (kBack ? kConvWarps : 0));
-  static constexpr int kOffStaging = kStages * kStage;
+  static constexpr int kHalves = kBack ? 2 : 1;                  // tiles of an item that share the right operand
+  static constexpr int kStages = kBack ? 4 : 6;
+  static constexpr int kStage = (1 + kHalves) * kOperand;        // right operand, left operands
+  static constexpr int kRaws = kBack ? 2 : 0;
+  // a slot belongs to one conv group for good: a group that met a slot every
+  // other turn could take the parity of a turn it did not see for its own
+  static_assert(kRaws % kConvGroups == 0 && kStages % kConvGroups == 0, "rings and groups");
+  static constexpr int kThreads = 32 * (4 + kEpiWarps + (kBack ? kConvWarps * kConvGroups : 0));
+  static constexpr int kOffRaw = kStages * kStage;
+  static constexpr int kOffStaging = kOffRaw + kRaws * kRawBytes;
   static constexpr int kOffCols = kOffStaging + kEpiWarps * 32 * kEpiPitch * 4;   // b_scale, bias of the tile
   static constexpr int kOffBars = kOffCols + (kBack ? 0 : 2 * kTile * 4);
-  static constexpr int kBars = 4 * kStages + 4;
+  static constexpr int kBars = 2 * (kStages + kRaws + 2);
   static constexpr int kOffSlot = kOffBars + kBars * 8;
-  static constexpr int kSmem = kOffSlot + 16 + 1024;   // the ring starts on a 1024-byte boundary
+  static constexpr int kSmem = kOffSlot + 16 + 1024;   // the rings start on a 1024-byte boundary
 };
 
-// Tile t of the walk: groups of 8 row panels, columns outside rows in a group.
-__device__ __forceinline__ void tile_at(const ProductArgs& p, int t, int64_t& m0, int64_t& n0) {
-  constexpr int kGroup = 8;
-  const int per = kGroup * p.tiles_n, g = t / per, first = g * kGroup, rows = min(kGroup, p.tiles_m - first);
-  const int in = t - g * per;
-  m0 = int64_t(first + in % rows) * kTile;
-  n0 = int64_t(in / rows) * kTile;
+// A place in a ring: its slot and the parity of its turn.
+template <int N> struct RingAt {
+  int slot = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == N) { slot = 0; parity ^= 1; }
+  }
+};
+
+// Bytes I and I + 1 of w_biased (offset by 128) times f as a pair of bf16,
+// each rounded once: two values per f32 add and multiply.
+template <int I> __device__ __forceinline__ uint32_t bytes_scaled(uint32_t w_biased, float f) {
+  uint32_t r;
+  asm("{\n.reg .b64 v, m, s;\n.reg .f32 x, y;\n"
+      "mov.b64 v, {%1, %2};\nmov.b64 m, {%3, %3};\nmov.b64 s, {%4, %4};\n"
+      "add.rn.f32x2 v, v, m;\nmul.rn.f32x2 v, v, s;\nmov.b64 {x, y}, v;\ncvt.rn.bf16x2.f32 %0, y, x;\n}\n"
+      : "=r"(r)
+      : "r"(__byte_perm(w_biased, 0x4b000000u, 0x7650 | I)), "r"(__byte_perm(w_biased, 0x4b000000u, 0x7650 | (I + 1))),
+        "f"(-8388736.f), "f"(f));
+  return r;
+}
+
+// Item i of a pair's walk: the tile at (m0, n0) and, if halves is 2, the one
+// below it.  Double items first, in whole rounds of all pairs; then the rest
+// one tile at a time, so the last round is as even as single tiles make it.
+// Doubles go in groups of 4 (8 panels of 256 rows), columns outside rows.
+struct Item {
+  int64_t m0, n0;
+  int halves;
+};
+__device__ __forceinline__ bool item_at(const ProductArgs& p, int pair, int pairs, int i, Item& it) {
+  constexpr int kGroup = 4;
+  const int panels = p.tiles_m >> 1;
+  int d, half = 0;
+  if (i < p.doubles / pairs) {
+    d = pair + i * pairs;
+    it.halves = 2;
+  } else {
+    const int64_t s = pair + int64_t(i - p.doubles / pairs) * pairs;
+    if (s >= p.singles) return false;
+    it.halves = 1;
+    d = p.doubles + int(s >> 1);
+    half = int(s & 1);
+    if (d >= panels * p.tiles_n) {   // the last panel, when their number is odd
+      it.m0 = int64_t(p.tiles_m - 1) * kTile;
+      it.n0 = (s - 2 * int64_t(panels * p.tiles_n - p.doubles)) * kTile;
+      return true;
+    }
+  }
+  const int per = kGroup * p.tiles_n, g = d / per, first = g * kGroup, rows = min(kGroup, panels - first);
+  const int in = d - g * per;
+  it.m0 = int64_t(2 * (first + in % rows) + half) * kTile;
+  it.n0 = int64_t(in / rows) * kTile;
+  return true;
 }
 
 // One row of 32 outputs in the row's own thread, or through shared memory by
@@ -78,14 +148,18 @@ __device__ __forceinline__ void store_rows32(const ProductArgs& p, const float (
     }
     return;
   }
-  __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 32; i++) staging[lane * kEpiPitch + i] = z[i];
-  __syncwarp();
-  if (col + lane < p.n) {
-    const int rows = int(min(int64_t(32), p.m - row0));
-    T* c = static_cast<T*>(p.c) + row0 * p.ldc + col + lane;
-    for (int r = 0; r < rows; r++) c[r * p.ldc] = from_f32<T>(staging[r * kEpiPitch + lane]);
+  for (int h = 0; h < 32; h += 16) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16; i++) staging[lane * kEpiPitch + i] = z[h + i];
+    __syncwarp();
+    const int c16 = lane & 15;
+    if (col + h + c16 < p.n) {
+      const int rows = int(min(int64_t(32), p.m - row0));
+      T* c = static_cast<T*>(p.c) + row0 * p.ldc + col + h + c16;
+      for (int r = lane >> 4; r < rows; r += 2) c[r * p.ldc] = from_f32<T>(staging[r * kEpiPitch + c16]);
+    }
   }
 }
 
@@ -96,28 +170,32 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (umma::smem_u32(smem_raw) + 1023) & ~1023u;
   uint8_t* smem = smem_raw + (base - umma::smem_u32(smem_raw));
+  // barriers of the leader unless noted: a pair's products are issued there
   const uint32_t bars = base + S::kOffBars;
-  auto full = [&](int s) { return bars + 8 * s; };                       // A and B landed (leader)
-  auto empty = [&](int s) { return bars + 8 * (S::kStages + s); };       // products that read the stage are done
-  auto raw = [&](int s) { return bars + 8 * (2 * S::kStages + s); };     // 8-bit tile landed (each CTA)
-  auto conv = [&](int s) { return bars + 8 * (3 * S::kStages + s); };    // expanded in both CTAs (leader)
-  auto acc_full = [&](int b) { return bars + 8 * (4 * S::kStages + b); };
-  auto acc_empty = [&](int b) { return bars + 8 * (4 * S::kStages + 2 + b); };   // (leader)
+  auto full = [&](int s) { return bars + 8 * s; };                         // operands in place in both CTAs
+  auto empty = [&](int s) { return bars + 8 * (S::kStages + s); };         // products that read them are done (each CTA)
+  constexpr int kR = 2 * S::kStages, kAcc = kR + 2 * S::kRaws;
+  auto raw_full = [&](int s) { return bars + 8 * (kR + s); };              // 8-bit tile landed (each CTA)
+  auto raw_empty = [&](int s) { return bars + 8 * (kR + S::kRaws + s); };  // and is read (each CTA)
+  auto acc_full = [&](int b) { return bars + 8 * (kAcc + b); };            // tile summed (each CTA)
+  auto acc_empty = [&](int b) { return bars + 8 * (kAcc + 2 + b); };       // and read out in both CTAs
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + S::kOffSlot);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // warp: uniform
   const uint32_t rank = umma::cta_rank();
-  const int tiles = p.tiles_m * p.tiles_n, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int steps = p.blocks * p.planes;
 
   if (warp == 0 && lane == 0) {
     umma::tma_prefetch(&map_a);
     umma::tma_prefetch(&map_b);
     for (int s = 0; s < S::kStages; s++) {
-      umma::bar_init(full(s), 1);
+      umma::bar_init(full(s), 1 + (S::kBack ? 2 * kConvWarps : 0));
       umma::bar_init(empty(s), 1);
-      umma::bar_init(raw(s), 1);
-      umma::bar_init(conv(s), 2 * kConvWarps);
+    }
+    for (int s = 0; s < S::kRaws; s++) {
+      umma::bar_init(raw_full(s), 1);
+      umma::bar_init(raw_empty(s), kConvWarps);
     }
     for (int b = 0; b < 2; b++) {
       umma::bar_init(acc_full(b), 1);
@@ -133,80 +211,107 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   bool ok = true;   // false once a wait of this role ran out
 
   if (warp == 0) {
-    // ---- producer: this CTA's half of each operand
-    if (lane == 0) {
-      int it = 0;
-      for (int t = pair; t < tiles && ok; t += pairs) {
-        int64_t m0, n0;
-        tile_at(p, t, m0, n0);
-        const int row = int(m0) + int(rank) * kHalf, col = int(n0) + int(rank) * kHalf;
-        for (int step = 0; step < steps; step++, it++) {
-          const int s = it % S::kStages;
-          if (!umma::bar_wait(empty(s), ((it / S::kStages) & 1) ^ 1)) { ok = false; break; }
-          const uint32_t a = base + s * S::kStage, b = a + kStageA;
-          const uint32_t bar = umma::map_rank(full(s), 0);
-          if (rank == 0) umma::bar_expect(full(s), S::kBack ? 2 * kStageA : 2 * (kStageA + kStageB));
-          if (MODE == kForward) {
-            umma::tma_load_3d_pair(a, &map_a, step * 128, row, 0, bar);
-            umma::tma_load_3d_pair(b, &map_b, step * 128, col, 0, bar);
-          } else {
-            const int plane = step / p.blocks, r0 = (step - plane * p.blocks) * 64;
-            if (MODE == kBackRows) {
-              umma::tma_load_3d_pair(a, &map_a, r0, row, plane, bar);
+    // ---- producer: this CTA's half of each operand (backward: of the left one)
+    const bool issue = umma::elect_one();
+    RingAt<S::kStages> at;
+    Item item;
+    for (int i = 0; ok && item_at(p, pair, pairs, i, item); i++) {
+      const int row = int(item.m0) + int(rank) * kHalf, col = int(item.n0) + int(rank) * kHalf;
+      int plane = 0, block = 0;
+      for (int step = 0; step < steps; step++, at.next()) {
+        if (!umma::bar_wait(empty(at.slot), at.parity ^ 1)) { ok = false; break; }
+        const uint32_t b = base + at.slot * S::kStage, bar = umma::map_rank(full(at.slot), 0);
+        if (issue) {
+          if (rank == 0) umma::bar_expect(full(at.slot), 2 * kOperand * (item.halves + (S::kBack ? 0 : 1)));
+          if (MODE == kForward) umma::tma_load_3d_pair(b, &map_b, step * 128, col, 0, bar);
+#pragma unroll
+          for (int h = 0; h < S::kHalves; h++) {
+            if (h == item.halves) break;
+            const uint32_t a = b + kOperand * (1 + h);
+            const int r = row + h * kTile;
+            if (MODE == kForward) {
+              umma::tma_load_3d_pair(a, &map_a, step * 128, r, 0, bar);
+            } else if (MODE == kBackRows) {
+              umma::tma_load_3d_pair(a, &map_a, block * 64, r, plane, bar);
             } else {
-              umma::tma_load_3d_pair(a, &map_a, row, r0, plane, bar);
-              umma::tma_load_3d_pair(a + kStageA / 2, &map_a, row + 64, r0, plane, bar);
+              umma::tma_load_3d_pair(a, &map_a, r, block * 64, plane, bar);
+              umma::tma_load_3d_pair(a + kOperand / 2, &map_a, r + 64, block * 64, plane, bar);
             }
-            umma::bar_expect(raw(s), kStageRaw);
-            umma::tma_load_3d_pair(b + kStageB, &map_b, col, r0, 0, umma::map_rank(raw(s), rank));
           }
         }
+        if (++block == p.blocks) { block = 0; plane++; }
       }
-      if (!ok) umma::drain_copies();
     }
-  } else if (warp == 1) {
-    // ---- products, issued by one thread of the leader for both SMs
-    if (lane == 0 && rank == 0) {
-      constexpr uint32_t idesc = MODE == kForward ? umma::instr_desc(2, 1, false, false, kTile, kTile)
-                                                  : umma::instr_desc(1, 1, MODE == kBackCols, true, kTile, kTile);
-      // bytes from one instruction's slice of the sum to the next: 32 along a
-      // 128-byte row, or 16 rows
-      constexpr uint32_t step_a = MODE == kBackCols ? 2048 : 32, step_b = MODE == kForward ? 32 : 2048;
-      int it = 0, n = 0;
-      for (int t = pair; t < tiles && ok; t += pairs, n++) {
-        const int buf = n & 1;
-        if (!umma::bar_wait(acc_empty(buf), ((n >> 1) & 1) ^ 1)) { ok = false; break; }
-        umma::fence_after();
-        for (int step = 0; step < steps; step++, it++) {
-          const int s = it % S::kStages;
-          const uint32_t parity = (it / S::kStages) & 1;
-          if (!umma::bar_wait(full(s), parity) || (S::kBack && !umma::bar_wait(conv(s), parity))) { ok = false; break; }
-          umma::fence_after();
-          const uint32_t a = base + s * S::kStage, b = a + kStageA;
-          // contiguous along the sum: 8-row groups 1024 bytes apart; else
-          // 64-wide columns of 64 rows 8192 bytes apart
-          const uint64_t da = umma::smem_desc(a, MODE == kBackCols ? 8192 : 16, 1024);
-          const uint64_t db = umma::smem_desc(b, S::kBack ? 8192 : 16, 1024);
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            umma::mma<2, MODE == kForward>(tmem + buf * kTile, da + (i * step_a >> 4), db + (i * step_b >> 4), idesc, step | i);
-          umma::mma_commit<2>(empty(s));
+    if (!ok) umma::drain_copies();
+  } else if (S::kBack && warp == 3) {
+    // ---- producer of the 8-bit tiles
+    const bool issue = umma::elect_one();
+    RingAt<S::kBack ? S::kRaws : 1> at;
+    Item item;
+    for (int i = 0; ok && item_at(p, pair, pairs, i, item); i++) {
+      const int col = int(item.n0) + int(rank) * kHalf;
+      int block = 0;
+      for (int step = 0; step < steps; step++, at.next()) {
+        if (!umma::bar_wait(raw_empty(at.slot), at.parity ^ 1)) { ok = false; break; }
+        if (issue) {
+          umma::bar_expect(raw_full(at.slot), kRawBytes);
+          umma::tma_load_3d_pair(base + S::kOffRaw + at.slot * kRawBytes, &map_b, col, block * 64, 0, umma::map_rank(raw_full(at.slot), rank));
         }
-        if (ok) umma::mma_commit<2>(acc_full(buf));
+        if (++block == p.blocks) block = 0;
       }
-      if (!ok) umma::drain_copies();
     }
+    if (!ok) umma::drain_copies();
+  } else if (warp == 1 && rank == 0) {
+    // ---- products, issued by one thread of the leader for both SMs
+    constexpr uint32_t idesc = MODE == kForward ? umma::instr_desc(2, 1, false, false, kTile, kTile)
+                                                : umma::instr_desc(1, 1, MODE == kBackCols, true, kTile, kTile);
+    // bytes from one instruction's slice of the sum to the next: 32 along a
+    // 128-byte row, or 16 rows
+    constexpr uint32_t step_a = MODE == kBackCols ? 2048 : 32, step_b = MODE == kForward ? 32 : 2048;
+    // contiguous along the sum: 8-row groups 1024 bytes apart; else 64-wide
+    // columns of 64 rows 8192 bytes apart
+    const uint64_t db0 = umma::smem_desc(base, S::kBack ? 8192 : 16, 1024);
+    const uint64_t da0 = umma::smem_desc(base + kOperand, MODE == kBackCols ? 8192 : 16, 1024);
+    const bool issue = umma::elect_one();
+    RingAt<S::kStages> at;
+    Item item;
+    int n = 0;   // tiles so far: tile n sums into accumulator n % 2
+    for (int i = 0; ok && item_at(p, pair, pairs, i, item); n += item.halves, i++) {
+      for (int step = 0; step < steps; step++, at.next()) {
+        if (!umma::bar_wait<S::kBack>(full(at.slot), at.parity)) { ok = false; break; }
+        const uint32_t off = at.slot * (S::kStage >> 4);
+#pragma unroll
+        for (int h = 0; h < S::kHalves; h++) {
+          if (h == item.halves) break;
+          const int buf = (n + h) & 1;
+          if (step == 0 && !umma::bar_wait<true>(acc_empty(buf), (((n + h) >> 1) & 1) ^ 1)) { ok = false; break; }
+          umma::fence_after();
+          const uint32_t offa = off + h * (kOperand >> 4);
+          if (issue) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+              umma::mma<2, MODE == kForward>(tmem + buf * kTile, da0 + (offa + (j * step_a >> 4)), db0 + (off + (j * step_b >> 4)), idesc, step | j);
+          }
+        }
+        if (!ok) break;
+        if (issue) umma::mma_commit<2>(empty(at.slot));
+      }
+      if (issue && ok)
+        for (int h = 0; h < item.halves; h++) umma::mma_commit<2>(acc_full((n + h) & 1));
+      __syncwarp();
+    }
+    if (!ok) umma::drain_copies();
   } else if (warp >= 4 && warp < 4 + kEpiWarps) {
     // ---- epilogue: warp w reads lanes 32 w .. 32 w + 31 of tensor memory
     const int w = warp - 4, tid = threadIdx.x - 128;
     float* staging = reinterpret_cast<float*>(smem + S::kOffStaging) + w * 32 * kEpiPitch;
     float* cols = reinterpret_cast<float*>(smem + S::kOffCols);
+    Item item;
     int n = 0;
-    for (int t = pair; t < tiles; t += pairs, n++) {
-      int64_t m0, n0;
-      tile_at(p, t, m0, n0);
+    for (int i = 0, h = 0; item_at(p, pair, pairs, i, item); n++) {   // h: the tile within the item
+      const int64_t n0 = item.n0, row0 = item.m0 + h * kTile + rank * kHalf + w * 32, row = row0 + lane;
       const int buf = n & 1;
-      const int64_t row0 = m0 + rank * kHalf + w * 32, row = row0 + lane;
+      if (++h == item.halves) { h = 0; i++; }
       float rs = 0.f;
       if (MODE == kForward) {
         asm volatile("bar.sync 1, 128;" ::: "memory");   // the last tile's columns are no longer read
@@ -248,44 +353,60 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     // ---- 8-bit tile (64 of the sum x 128 columns) to bf16, 128-byte swizzled
     // columns of 64.  Lanes 0-7 take eight rows of one 16-byte chunk: the
     // swizzle spreads them over all banks on both sides.
-    const int w = warp - 4 - kEpiWarps, r8 = lane & 7, c4 = lane >> 3;
-    const uint32_t out0 = base + kStageA, in0 = out0 + kStageB;
-    int it = 0;
-    for (int t = pair; t < tiles && ok; t += pairs) {
-      for (int step = 0; step < steps; step++, it++) {
-        const int s = it % S::kStages;
-        const int r0 = (step % p.blocks) * 64 + w * 16 + r8;
-        float sc[2];
+    const int w = (warp - 4 - kEpiWarps) % kConvWarps, group = (warp - 4 - kEpiWarps) / kConvWarps;
+    const int r8 = lane & 7, c4 = lane >> 3;
+    int items = p.doubles / pairs;
+    if (p.singles > pair) items += (p.singles - pair + pairs - 1) / pairs;
+    const int64_t total = int64_t(items) * steps;
+    RingAt<S::kBack ? S::kRaws : 1> rw;
+    RingAt<S::kStages> cv;
+    float sc[2], next[2];
+    auto factors = [&](int block, float (&f)[2]) {
+      const int r0 = block * 64 + w * 16 + r8;
 #pragma unroll
-        for (int i = 0; i < 2; i++) sc[i] = p.sum_scale ? (r0 + 8 * i < p.sum ? p.sum_scale[r0 + 8 * i] : 0.f) : 1.f;
-        if (!umma::bar_wait(raw(s), (it / S::kStages) & 1)) { ok = false; break; }
+      for (int i = 0; i < 2; i++) f[i] = p.sum_scale ? (r0 + 8 * i < p.sum ? p.sum_scale[r0 + 8 * i] : 0.f) : 1.f;
+    };
+    int block = group % p.blocks;
+    factors(block, next);
+    for (int i = 0; i < group; i++) { rw.next(); cv.next(); }
+    for (int64_t it = group; it < total; it += kConvGroups) {
+      sc[0] = next[0];
+      sc[1] = next[1];
+      block = (block + kConvGroups) % p.blocks;
+      factors(block, next);   // a turn ahead: the load's latency stays out of the wait
+      if (!umma::bar_wait(raw_full(rw.slot), rw.parity)) { ok = false; break; }
+      const uint32_t in = base + S::kOffRaw + rw.slot * kRawBytes + (w * 16 + r8) * 128;
+      uint32_t q[4][4];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const int r = w * 16 + i * 8 + r8;
+      for (int i = 0; i < 4; i++)   // rows + 8 (i / 2), 64 columns (i % 2)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q[i][0]), "=r"(q[i][1]), "=r"(q[i][2]), "=r"(q[i][3])
+                     : "r"(in + (i >> 1) * 1024 + ((((i & 1) * 4 + c4) ^ r8) << 4)));
+      if (!umma::bar_wait(empty(cv.slot), cv.parity ^ 1)) { ok = false; break; }
+      const uint32_t out = base + cv.slot * S::kStage + (w * 16 + r8) * 128;
 #pragma unroll
-          for (int j = 0; j < 2; j++) {
-            uint32_t q[4];
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
-                         : "r"(in0 + s * S::kStage + r * 128 + (((j * 4 + c4) ^ r8) << 4)));
-            uint32_t o[8];
+      for (int i = 0; i < 4; i++) {
+        uint32_t o[8];
+        const float f = sc[i >> 1];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-              const uint32_t x = q[k] ^ 0x80808080u;
-              const __nv_bfloat162 lo = __floats2bfloat162_rn(byte_f32<0>(x) * sc[i], byte_f32<1>(x) * sc[i]);
-              const __nv_bfloat162 hi = __floats2bfloat162_rn(byte_f32<2>(x) * sc[i], byte_f32<3>(x) * sc[i]);
-              o[2 * k] = *reinterpret_cast<const uint32_t*>(&lo);
-              o[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&hi);
-            }
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(out0 + s * S::kStage + j * 8192 + r * 128 + (((2 * c4 + k) ^ r8) << 4)),
-                           "r"(o[4 * k]), "r"(o[4 * k + 1]), "r"(o[4 * k + 2]), "r"(o[4 * k + 3]) : "memory");
-          }
+        for (int k = 0; k < 4; k++) {
+          const uint32_t x = q[i][k] ^ 0x80808080u;
+          o[2 * k] = bytes_scaled<0>(x, f);
+          o[2 * k + 1] = bytes_scaled<2>(x, f);
         }
-        umma::fence_async_smem();
-        __syncwarp();
-        if (lane == 0) umma::bar_arrive_cluster(umma::map_rank(conv(s), 0));
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(out + (i >> 1) * 1024 + (i & 1) * 8192 + (((2 * c4 + k) ^ r8) << 4)),
+                       "r"(o[4 * k]), "r"(o[4 * k + 1]), "r"(o[4 * k + 2]), "r"(o[4 * k + 3]) : "memory");
       }
+      // The 8-bit tile is given back only now that its values have been used: an
+      // arrival right after the loads overtook them under load, and the next
+      // tile was read in their place.
+      __syncwarp();
+      if (lane == 0) umma::bar_arrive(raw_empty(rw.slot));
+      umma::fence_async_smem();
+      __syncwarp();
+      if (lane == 0) umma::bar_arrive_cluster(umma::map_rank(full(cv.slot), 0));
+      for (int i = 0; i < kConvGroups; i++) { rw.next(); cv.next(); }
     }
   }
 
