@@ -53,7 +53,7 @@ __device__ __forceinline__ uint32_t mag_bits(float v) { return __float_as_uint(v
 // alignment.  NORM: root-mean-square norm (and the checkpoint when asked
 // for); otherwise the plain quantisation.
 template <typename T, int G, bool VEC, bool NORM>
-__global__ void __launch_bounds__(1024) rows_kernel(RowArgs p) {
+__global__ void __launch_bounds__(G == 1 ? 1024 : 512) rows_kernel(RowArgs p) {
   __shared__ RowStats warp_stats[32];
   const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, per_block = blockDim.x / p.tpr;
   const int64_t row = int64_t(blockIdx.x) * per_block + sub;
@@ -230,22 +230,26 @@ __global__ void __launch_bounds__(1024) rows_long_kernel(RowArgs p) {
   }
 }
 
-// y = q * scale: 8 elements per thread (VEC) or one.
+// y = q * scale: 16 elements per thread (VEC) or one.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dequantize_kernel(int64_t rows, int64_t cols, const int8_t* q, int64_t ldq,
                                                          const float* scale, T* y, int64_t ldy) {
-  const int64_t per = VEC ? cols / 8 : cols, total = rows * per;
+  const int64_t per = VEC ? cols / 16 : cols, total = rows * per;
   const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (i >= total) return;
   const int64_t row = total <= 0xffffffffll ? int64_t(uint32_t(i) / uint32_t(per)) : i / per;
   const int64_t c = i - row * per;
   const float s = scale[row];
   if (VEC) {
+    const uint4 w = *reinterpret_cast<const uint4*>(q + row * ldq + c * 16);
     float v[8];
-    bytes_f32(*reinterpret_cast<const uint2*>(q + row * ldq + c * 8), v);
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] *= s;
-    store8(y + row * ldy + c * 8, v);
+    for (int h = 0; h < 2; h++) {
+      bytes_f32(h ? make_uint2(w.z, w.w) : make_uint2(w.x, w.y), v);
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] *= s;
+      store8(y + row * ldy + c * 16 + h * 8, v);
+    }
   } else {
     y[row * ldy + c] = from_f32<T>(float(q[row * ldq + c]) * s);
   }
@@ -278,105 +282,162 @@ __device__ __forceinline__ float row_sum(float s, int tpr, float* warp_sums) {
   return s;
 }
 
-// Each slot (tpr threads) walks its rows with a fixed set of columns per
-// thread, so the sums over rows stay in registers; they are joined by
-// column_join_kernel in a fixed order.
-template <typename T, typename GT, int G, bool VEC>
-__global__ void __launch_bounds__(1024) norm_backward_kernel(BackArgs p) {
-  __shared__ float warp_sums[32];
-  const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, per_block = blockDim.x / p.tpr;
-  const int64_t slot = int64_t(blockIdx.x) * per_block + sub;
-  const int cols = int(p.cols);
-  const T* wgt = static_cast<const T*>(p.weight);
-  auto at = [&](int g, int e) { return VEC ? (g * p.tpr + t) * 8 + e : (g * 8 + e) * p.tpr + t; };
-  float dw[G][8];
+// What one thread reads of a row, as loaded.
+template <typename T, typename GT, int G, bool VEC> struct BackRow;
+template <typename T, typename GT, int G> struct BackRow<T, GT, G, true> {
+  Vec8<GT> grad[G];
+  Vec8<T> gh[G];
+  uint2 q[G];
+  float u, s;
+  __device__ __forceinline__ void load(const BackArgs& p, int64_t row, int t) {
+    u = p.rstd[row];
+    s = p.ckpt_scale[row];
+    const GT* g = static_cast<const GT*>(p.grad) + row * p.ldg;
+    const T* h = p.grad_h ? static_cast<const T*>(p.grad_h) + row * p.ldgh : nullptr;
+    const int8_t* k = p.ckpt + row * p.ldk;
 #pragma unroll
-  for (int g = 0; g < G; g++)
-#pragma unroll
-    for (int e = 0; e < 8; e++) dw[g][e] = 0.f;
-
-  // the same number of turns in every thread of the block: the sums synchronise
-  const int64_t first = int64_t(blockIdx.x) * per_block;
-  for (int64_t base = first; base < p.rows; base += p.slots) {
-    const int64_t row = base + sub;
-    const bool live = row < p.rows && slot < p.slots;
-    const int64_t rr = live ? row : 0;
-    const float u = p.rstd[rr], s = p.ckpt_scale[rr] * u;
-    const GT* grad = static_cast<const GT*>(p.grad) + rr * p.ldg;
-    const int8_t* k = p.ckpt + rr * p.ldk;
-    float gw[G][8], v[G][8];
-    float dot = 0.f;
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-      float w[8], gr[8];
-      if (VEC) {
-        const int c = at(g, 0);
-        Vec8<T> a;
-        Vec8<GT> b;
-        uint2 kk = make_uint2(0, 0);
-        const bool in = live && c < cols;
-        if (in) { a.load(wgt + c); b.load(grad + c); kk = *reinterpret_cast<const uint2*>(k + c); } else { a.zero(); b.zero(); }
-        a.get(w);
-        b.get(gr);
-        bytes_f32(kk, v[g]);
+    for (int i = 0; i < G; i++) {
+      const int c = (i * p.tpr + t) * 8;
+      if (c < p.cols) {
+        grad[i].load(g + c);
+        q[i] = *reinterpret_cast<const uint2*>(k + c);
+        if (h) gh[i].load(h + c); else gh[i].zero();
       } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const int c = at(g, e);
-          const bool in = live && c < cols;
-          w[e] = in ? to_f32(wgt[c]) : 0.f;
-          gr[e] = in ? to_f32(grad[c]) : 0.f;
-          v[g][e] = in ? float(k[c]) : 0.f;
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const bool in = live && at(g, VEC ? 0 : e) < cols;
-        v[g][e] = in ? v[g][e] * s : 0.f;
-        if (in) dw[g][e] = fmaf(gr[e], v[g][e], dw[g][e]);
-        gw[g][e] = gr[e] * w[e];
-        dot = fmaf(gw[g][e], v[g][e], dot);
-      }
-    }
-    if (!p.grad_x) continue;   // uniform over the grid
-    const float c_mean = row_sum(dot, p.tpr, warp_sums) / float(cols);
-    if (!live) continue;
-    const T* gh = p.grad_h ? static_cast<const T*>(p.grad_h) + rr * p.ldgh : nullptr;
-    T* out = static_cast<T*>(p.grad_x) + rr * p.ldx;
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-      float o[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) o[e] = u * (gw[g][e] - v[g][e] * c_mean);
-      if (VEC) {
-        const int c = at(g, 0);
-        if (c < cols) {
-          if (gh) {
-            Vec8<T> a;
-            float h[8];
-            a.load(gh + c);
-            a.get(h);
-#pragma unroll
-            for (int e = 0; e < 8; e++) o[e] += h[e];
-          }
-          store8(out + c, o);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const int c = at(g, e);
-          if (c < cols) out[c] = from_f32<T>(o[e] + (gh ? to_f32(gh[c]) : 0.f));
-        }
+        grad[i].zero();
+        gh[i].zero();
+        q[i] = make_uint2(0, 0);
       }
     }
   }
+  __device__ __forceinline__ void get(int i, float (&g)[8], float (&v)[8]) const {
+    grad[i].get(g);
+    bytes_f32(q[i], v);
+  }
+  __device__ __forceinline__ void get_h(int i, float (&h)[8]) const { gh[i].get(h); }
+};
+template <typename T, typename GT, int G> struct BackRow<T, GT, G, false> {
+  GT grad[G][8];
+  T gh[G][8];
+  int8_t q[G][8];
+  float u, s;
+  __device__ __forceinline__ void load(const BackArgs& p, int64_t row, int t) {
+    u = p.rstd[row];
+    s = p.ckpt_scale[row];
+#pragma unroll
+    for (int i = 0; i < G; i++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int c = (i * 8 + e) * p.tpr + t;
+        const bool in = c < p.cols;
+        grad[i][e] = in ? static_cast<const GT*>(p.grad)[row * p.ldg + c] : from_f32<GT>(0.f);
+        q[i][e] = in ? p.ckpt[row * p.ldk + c] : int8_t(0);
+        gh[i][e] = in && p.grad_h ? static_cast<const T*>(p.grad_h)[row * p.ldgh + c] : from_f32<T>(0.f);
+      }
+  }
+  __device__ __forceinline__ void get(int i, float (&g)[8], float (&v)[8]) const {
+#pragma unroll
+    for (int e = 0; e < 8; e++) { g[e] = to_f32(grad[i][e]); v[e] = float(q[i][e]); }
+  }
+  __device__ __forceinline__ void get_h(int i, float (&h)[8]) const {
+#pragma unroll
+    for (int e = 0; e < 8; e++) h[e] = to_f32(gh[i][e]);
+  }
+};
+
+// Each slot (tpr threads) walks its rows with a fixed set of columns per
+// thread, so the sums over rows stay in registers; they are joined by
+// column_join_kernel in a fixed order.  The next row is loaded before this
+// one's sum is joined, so a row is always on its way.
+template <typename T, typename GT, int G, bool VEC>
+__global__ void __launch_bounds__(512) norm_backward_kernel(BackArgs p) {
+  __shared__ float warp_sums[2][16];
+  const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, per_block = blockDim.x / p.tpr;
+  const int cols = int(p.cols);
+  const T* wgt = static_cast<const T*>(p.weight);
+  auto at = [&](int g, int e) { return VEC ? (g * p.tpr + t) * 8 + e : (g * 8 + e) * p.tpr + t; };
+  auto weight_of = [&](int g, float (&w)[8]) {
+    if (VEC) {
+      Vec8<T> a;
+      if (at(g, 0) < cols) a.load(wgt + at(g, 0)); else a.zero();
+      a.get(w);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) w[e] = at(g, e) < cols ? to_f32(wgt[at(g, e)]) : 0.f;
+    }
+  };
+  float dw[G][8] = {};
+  const float inv_cols = 1.f / float(cols);
+  const int64_t first = int64_t(blockIdx.x) * per_block;
+  BackRow<T, GT, G, VEC> next;
+  if (first + sub < p.rows) next.load(p, first + sub, t);
+  int turn = 0;
+  // the same number of turns in every thread of the block: the sums synchronise
+  for (int64_t base = first; base < p.rows; base += p.slots, turn ^= 1) {
+    const int64_t row = base + sub;
+    const bool live = row < p.rows;
+    const BackRow<T, GT, G, VEC> cur = next;
+    if (row + p.slots < p.rows) next.load(p, row + p.slots, t);
+    const float u = cur.u, s = cur.s * u;
+    float dot = 0.f;
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < G; i++) {
+        float w[8], g[8], v[8];
+        weight_of(i, w);
+        cur.get(i, g, v);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          if (at(i, VEC ? 0 : e) < cols) {   // a NaN scale must not reach columns that are not there
+            v[e] *= s;
+            dw[i][e] = fmaf(g[e], v[e], dw[i][e]);
+            dot = fmaf(g[e] * w[e], v[e], dot);
+          }
+        }
+      }
+    }
+    if (!p.grad_x) continue;   // uniform over the grid
+#pragma unroll
+    for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+    if (p.tpr > 32) {   // two sets of sums in turn: one barrier per row
+      const int first_warp = sub * (p.tpr >> 5);
+      if ((threadIdx.x & 31) == 0) warp_sums[turn][threadIdx.x >> 5] = dot;
+      __syncthreads();
+      dot = warp_sums[turn][first_warp];
+      for (int w = 1; w < p.tpr >> 5; w++) dot += warp_sums[turn][first_warp + w];
+    }
+    const float mean = dot * inv_cols;
+    if (!live) continue;
+    T* out = static_cast<T*>(p.grad_x) + row * p.ldx;
+#pragma unroll
+    for (int i = 0; i < G; i++) {
+      float w[8], g[8], v[8], h[8], o[8];
+      weight_of(i, w);
+      cur.get(i, g, v);
+      cur.get_h(i, h);
+#pragma unroll
+      for (int e = 0; e < 8; e++) o[e] = fmaf(u, g[e] * w[e] - v[e] * s * mean, h[e]);
+      if (VEC) {
+        if (at(i, 0) < cols) store8(out + at(i, 0), o);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (at(i, e) < cols) out[at(i, e)] = from_f32<T>(o[e]);
+      }
+    }
+  }
+  const int64_t slot = first + sub;
   if (p.partial && slot < p.slots) {
     float* o = p.partial + slot * p.cols;
 #pragma unroll
-    for (int g = 0; g < G; g++)
+    for (int i = 0; i < G; i++) {
+      if (VEC) {
+        if (at(i, 0) < cols) store8(o + at(i, 0), dw[i]);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (at(g, e) < cols) o[at(g, e)] = dw[g][e];
+        for (int e = 0; e < 8; e++)
+          if (at(i, e) < cols) o[at(i, e)] = dw[i][e];
+      }
+    }
   }
 }
 
@@ -441,18 +502,20 @@ namespace tgi {
 using tg8::BackArgs;
 using tg8::RowArgs;
 
-constexpr int64_t kRowLimit = 1024 * 32;   // longest row that fits the registers of 1024 threads
+constexpr int64_t kRowLimit = 16384;   // longest row kept in registers
 constexpr int64_t kGridLimit = 0x7fffffff;
 
-// Threads per row and groups of 8 elements per thread: at most 4 groups, and
-// as few as 1 while there are too few rows to fill the GPU.
+// Threads per row and groups of 8 elements per thread (1, 2 or 4), for rows of
+// at most kRowLimit: as few threads as max_groups allows (more loads in
+// flight per thread, cheaper sums) when there are rows enough to fill the GPU;
+// one group per thread when there are not, and latency counts.
 struct RowShape {
   int tpr, groups, block;
 };
-RowShape row_shape(int64_t rows, int64_t cols) {
+RowShape row_shape(int64_t rows, int64_t cols, int max_groups, int max_threads) {
   const int64_t groups = (cols + 7) / 8;
-  int g = rows >= 2 * sm_count() ? 4 : 1;
-  while (g < 4 && (groups + g - 1) / g > 1024) g *= 2;
+  int g = rows >= 2 * sm_count() ? max_groups : 1;
+  while (groups > int64_t(g) * (g == 1 ? max_threads : 512)) g *= 2;
   int tpr = 32;
   while (int64_t(tpr) * g < groups) tpr *= 2;
   while (g > 1 && int64_t(tpr) * (g / 2) >= groups) g /= 2;
@@ -466,7 +529,7 @@ tg_status launch_rows(RowArgs p, bool vec, cudaStream_t st) {
     tg8::rows_long_kernel<T, NORM><<<unsigned(p.rows), 1024, 0, st>>>(p);
     return check_launch("rows8");
   }
-  const RowShape s = row_shape(p.rows, p.cols);
+  const RowShape s = row_shape(p.rows, p.cols, 4, 1024);
   p.tpr = s.tpr;
   const int per = s.block / s.tpr;
   const int64_t grid = (p.rows + per - 1) / per;
@@ -484,7 +547,7 @@ tg_status launch_rows(RowArgs p, bool vec, cudaStream_t st) {
 template <typename T, typename GT>
 tg_status launch_norm_backward(BackArgs p, T* grad_w, bool vec, cudaStream_t st) {
   const bool lng = p.cols > kRowLimit;
-  RowShape s = lng ? RowShape{1024, 4, 1024} : row_shape(p.rows, p.cols);
+  RowShape s = lng ? RowShape{1024, 4, 1024} : row_shape(p.rows, p.cols, 2, 512);
   const int per = s.block / s.tpr;
   p.tpr = s.tpr;
   const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((p.rows + per - 1) / per, sm_count() * int64_t(std::max(1, 1024 / s.block))));
@@ -572,8 +635,8 @@ tg_status tg_rows8_dequantize(tg_dtype dtype, int64_t rows, int64_t cols, const 
   if (!q || !scale || !y) return fail(TG_ERR_INVALID_ARGUMENT, "null operand");
   TG8_CHECK(check_ld("ldq", ldq, cols));
   TG8_CHECK(check_ld("ldy", ldy, cols));
-  const bool vec = cols % 8 == 0 && rows_vec(y, ldy, elem8_size(dtype)) && rows_vec(q, ldq, 1, 8);
-  const int64_t per = vec ? cols / 8 : cols;
+  const bool vec = cols % 16 == 0 && rows_vec(y, ldy, elem8_size(dtype)) && rows_vec(q, ldq, 1);
+  const int64_t per = vec ? cols / 16 : cols;
   if (rows > (kGridLimit * 256) / per) return fail(TG_ERR_UNSUPPORTED, "%lld x %lld elements", (long long)rows, (long long)cols);
   const unsigned grid = unsigned((rows * per + 255) / 256);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -91,7 +91,9 @@ __device__ __forceinline__ Quant quant_of(uint32_t top_bits) {
     s.scale = s.inv = 0.f;
   } else {
     s.scale = top / 127.f;
-    s.inv = 127.f / top;
+    // rounded up: a value of exactly half the largest one is a tie at 63.5,
+    // which goes to the even 64, and 16-bit inputs hit it often
+    s.inv = __fdiv_ru(127.f, top);
   }
   return s;
 }
