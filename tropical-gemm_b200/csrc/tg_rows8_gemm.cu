@@ -77,11 +77,29 @@ tg_status launch_product(const CUtensorMap& a, const CUtensorMap& b, ProductArgs
   using S = tg8::ProductShape<MODE>;
   const tg_status s = ensure_smem(reinterpret_cast<const void*>(kern), S::kSmem);
   if (s != TG_OK) return s;
-  const int pairs = int(std::min<int64_t>(tm * tn, std::max(1, sm_count() / 2)));
+  const int most = std::max(1, sm_count() / 2), steps = p.blocks * p.planes;
+  p.splits = 1;
+  // Few tiles and a long sum: several pairs share a tile's sum and a second
+  // kernel joins the parts (~3 us).  4096 x 4096 weights, one token: 16.4 us
+  // whole, JOINED in four parts.
+  if (tm * tn * 2 <= most && steps >= 16) {
+    p.split_steps = std::max<int>(4, int((steps * tm * tn + most - 1) / most));
+    p.splits = (steps + p.split_steps - 1) / p.split_steps;
+  }
+  const int pairs = p.splits > 1 ? int(tm * tn) * p.splits : int(std::min<int64_t>(tm * tn, most));
   const int64_t couples = (tm / 2) * tn;
-  p.doubles = S::kHalves == 2 ? int(couples / pairs * pairs) : 0;
+  p.doubles = S::kHalves == 2 && p.splits == 1 ? int(couples / pairs * pairs) : 0;
   p.singles = int(tm * tn - 2 * int64_t(p.doubles));
+  Scratch scratch(st);
+  if (p.splits > 1) {
+    p.ldp = round_up(p.n, 4);
+    const size_t count = size_t(p.splits) * size_t(p.m) * size_t(p.ldp);
+    const cudaError_t e = scratch.reserve(count * sizeof(uint32_t));
+    if (e != cudaSuccess) return fail(TG_ERR_CUDA, "rows8 product scratch: %s", cudaGetErrorString(e));
+    p.part = scratch.take<uint32_t>(count);
+  }
   kern<<<2 * pairs, S::kThreads, S::kSmem, st>>>(a, b, p);
+  if (p.splits > 1) tg8::join_kernel<MODE == tg8::kForward, T><<<row_grid(1024, p.n, p.m), 256, 0, st>>>(p);
   return check_launch("rows8 product");
 }
 

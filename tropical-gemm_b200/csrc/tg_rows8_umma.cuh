@@ -37,6 +37,9 @@ struct ProductArgs {
   int sum;                    // length of the sum (of one plane)
   int blocks, planes;         // stages per plane, planes of g
   int tiles_m, tiles_n;       // 256 x 256 tiles
+  int splits, split_steps;    // the sum in parts, one pair each (1: whole); stages per part
+  uint32_t* part;             // raw sums of the parts, (splits x m x ldp), joined by join_kernel
+  int64_t ldp;
   int doubles;                // two-tile items, taken first (a multiple of the pairs)
   int singles;                // one-tile items
   int vec;                    // 16-byte stores of C's rows
@@ -104,6 +107,13 @@ struct Item {
   int halves;
 };
 __device__ __forceinline__ bool item_at(const ProductArgs& p, int pair, int pairs, int i, Item& it) {
+  if (p.splits > 1) {   // one part of one tile per pair
+    const int tile = pair / p.splits;
+    it.m0 = int64_t(tile % p.tiles_m) * kTile;
+    it.n0 = int64_t(tile / p.tiles_m) * kTile;
+    it.halves = 1;
+    return i == 0;
+  }
   constexpr int kGroup = 4;
   const int panels = p.tiles_m >> 1;
   int d, half = 0;
@@ -163,6 +173,15 @@ __device__ __forceinline__ void store_rows32(const ProductArgs& p, const float (
   }
 }
 
+// 32 raw sums of one row of a part.
+__device__ __forceinline__ void store_part32(const ProductArgs& p, const uint32_t (&z)[32], int64_t row, int64_t col) {
+  if (row >= p.m) return;
+  uint32_t* c = p.part + (int64_t((blockIdx.x >> 1) % p.splits) * p.m + row) * p.ldp + col;
+#pragma unroll
+  for (int i = 0; i < 32; i += 4)
+    if (col + i < p.ldp) *reinterpret_cast<uint4*>(c + i) = make_uint4(z[i], z[i + 1], z[i + 2], z[i + 3]);
+}
+
 template <int MODE, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ProductShape<MODE>::kThreads, 1)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs p) {
@@ -184,7 +203,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // warp: uniform
   const uint32_t rank = umma::cta_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int steps = p.blocks * p.planes;
+  const int step0 = p.splits > 1 ? pair % p.splits * p.split_steps : 0;   // this pair's part of the sum
+  const int steps = min(p.blocks * p.planes - step0, p.splits > 1 ? p.split_steps : p.blocks * p.planes);
 
   if (warp == 0 && lane == 0) {
     umma::tma_prefetch(&map_a);
@@ -217,20 +237,20 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     Item item;
     for (int i = 0; ok && item_at(p, pair, pairs, i, item); i++) {
       const int row = int(item.m0) + int(rank) * kHalf, col = int(item.n0) + int(rank) * kHalf;
-      int plane = 0, block = 0;
+      int plane = step0 / p.blocks, block = step0 - plane * p.blocks;
       for (int step = 0; step < steps; step++, at.next()) {
         if (!umma::bar_wait(empty(at.slot), at.parity ^ 1)) { ok = false; break; }
         const uint32_t b = base + at.slot * S::kStage, bar = umma::map_rank(full(at.slot), 0);
         if (issue) {
           if (rank == 0) umma::bar_expect(full(at.slot), 2 * kOperand * (item.halves + (S::kBack ? 0 : 1)));
-          if (MODE == kForward) umma::tma_load_3d_pair(b, &map_b, step * 128, col, 0, bar);
+          if (MODE == kForward) umma::tma_load_3d_pair(b, &map_b, block * 128, col, 0, bar);
 #pragma unroll
           for (int h = 0; h < S::kHalves; h++) {
             if (h == item.halves) break;
             const uint32_t a = b + kOperand * (1 + h);
             const int r = row + h * kTile;
             if (MODE == kForward) {
-              umma::tma_load_3d_pair(a, &map_a, step * 128, r, 0, bar);
+              umma::tma_load_3d_pair(a, &map_a, block * 128, r, 0, bar);
             } else if (MODE == kBackRows) {
               umma::tma_load_3d_pair(a, &map_a, block * 64, r, plane, bar);
             } else {
@@ -250,7 +270,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     Item item;
     for (int i = 0; ok && item_at(p, pair, pairs, i, item); i++) {
       const int col = int(item.n0) + int(rank) * kHalf;
-      int block = 0;
+      int block = step0 % p.blocks;
       for (int step = 0; step < steps; step++, at.next()) {
         if (!umma::bar_wait(raw_empty(at.slot), at.parity ^ 1)) { ok = false; break; }
         if (issue) {
@@ -336,6 +356,14 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           if (lane == 0) umma::bar_arrive_cluster(umma::map_rank(acc_empty(buf), 0));
         }
         if (n0 + c >= p.n) continue;
+        if (p.splits > 1) {
+          if (!ok) {   // NaN, or a value no integer sum takes
+#pragma unroll
+            for (int i = 0; i < 32; i++) acc[i] = MODE == kForward ? 0x80000000u : 0x7fffffffu;
+          }
+          store_part32(p, acc, row, n0 + c);
+          continue;
+        }
 #pragma unroll
         for (int i = 0; i < 32; i++) {
           if (MODE == kForward) {
@@ -355,8 +383,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     // swizzle spreads them over all banks on both sides.
     const int w = (warp - 4 - kEpiWarps) % kConvWarps, group = (warp - 4 - kEpiWarps) / kConvWarps;
     const int r8 = lane & 7, c4 = lane >> 3;
-    int items = p.doubles / pairs;
-    if (p.singles > pair) items += (p.singles - pair + pairs - 1) / pairs;
+    int items = p.splits > 1 ? 1 : p.doubles / pairs;
+    if (p.splits == 1 && p.singles > pair) items += (p.singles - pair + pairs - 1) / pairs;
     const int64_t total = int64_t(items) * steps;
     RingAt<S::kBack ? S::kRaws : 1> rw;
     RingAt<S::kStages> cv;
@@ -366,7 +394,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
       for (int i = 0; i < 2; i++) f[i] = p.sum_scale ? (r0 + 8 * i < p.sum ? p.sum_scale[r0 + 8 * i] : 0.f) : 1.f;
     };
-    int block = group % p.blocks;
+    int block = (step0 + group) % p.blocks;
     factors(block, next);
     for (int i = 0; i < group; i++) { rw.next(); cv.next(); }
     for (int64_t it = group; it < total; it += kConvGroups) {
@@ -416,6 +444,39 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   if (warp == 2) {
     umma::fence_after();
     umma::tmem_free<2>(tmem, 512);
+  }
+}
+
+// Joins the parts of a sum, in order: forward integer sums with their scales
+// and bias, backward f32 sums.  Four columns per thread.
+template <bool FORWARD, typename T>
+__global__ void __launch_bounds__(256) join_kernel(const ProductArgs p) {
+  const int64_t c0 = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (c0 >= p.n) return;
+  for (int64_t row = blockIdx.y; row < p.m; row += gridDim.y) {
+    int si[4] = {};
+    float sf[4] = {};
+    bool bad = false;
+    for (int s = 0; s < p.splits; s++) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p.part + (int64_t(s) * p.m + row) * p.ldp + c0);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        if (FORWARD) { si[e] += int(w[e]); bad |= w[e] == 0x80000000u; } else sf[e] += __uint_as_float(w[e]);
+      }
+    }
+    T* c = static_cast<T*>(p.c) + row * p.ldc + c0;
+    const float rs = FORWARD ? p.row_scale[row] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if (c0 + e >= p.n) break;
+      float z = sf[e];
+      if (FORWARD) {
+        z = float(si[e]) * rs * p.col_scale[c0 + e] + (p.bias ? to_f32(static_cast<const T*>(p.bias)[c0 + e]) : 0.f);
+        if (bad) z = __uint_as_float(0x7fffffffu);
+      }
+      c[e] = from_f32<T>(z);
+    }
   }
 }
 

@@ -57,11 +57,8 @@ def _on(dev: torch.device, *ts) -> None:
 def _flat(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """`t` as (rows, columns) and its row stride; a copy only where rows are
     not contiguous or cannot be flattened."""
-    if t.dim() == 0:
-        raise ValueError("expected a tensor with at least one dimension")
     if t.is_contiguous():
-        k = t.shape[-1]
-        return t, k
+        return t, t.size(-1)
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1]) if t.numel() else t.reshape(_rows_of(t), t.shape[-1])
     t = N._rows(t)
@@ -69,6 +66,8 @@ def _flat(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
 
 
 def _rows_of(t: torch.Tensor) -> int:
+    if t.dim() == 2:
+        return t.size(0)
     n = 1
     for s in t.shape[:-1]:
         n *= s
@@ -83,12 +82,18 @@ def _check_rows8(r: Rows8, what: str) -> None:
         raise ValueError(f"{what} needs one scale per row: q is {tuple(q.shape)}, scale is {tuple(s.shape)}")
 
 
+# the handle of torch's current stream, without the Stream object around it
+# where this torch has that (2 us less per call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 def _call(dev: torch.device, fn, *args) -> None:
-    if dev.index == torch.cuda.current_device():
-        status = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    i = dev.index
+    if i == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(i))
     else:
         with torch.cuda.device(dev):
-            status = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            status = fn(*args, _raw_stream(i))
     if status:
         N.check(status)
 
@@ -99,10 +104,13 @@ def quantize(x: torch.Tensor) -> Rows8:
     holds a NaN or an infinity has scale NaN."""
     code = _type(x, "x")
     _on(x.device)
+    if x.dim() == 0:
+        raise ValueError("expected a tensor with at least one dimension")
     xf, ldx = _flat(x)
-    k = x.shape[-1]
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    shape = x.shape
+    k = shape[-1]
+    q = x.new_empty(shape, dtype=torch.int8)
+    scale = x.new_empty(shape[:-1], dtype=torch.float32)
     _call(x.device, N.lib().tg_rows8_quantize, code, _rows_of(x), k, xf.data_ptr(), ldx, q.data_ptr(), k, scale.data_ptr())
     return Rows8(q, scale)
 
@@ -116,7 +124,7 @@ def dequantize(r: Rows8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
     qf, ldq = _flat(q)
     k = q.shape[-1]
-    y = torch.empty(q.shape, dtype=dtype, device=q.device)
+    y = q.new_empty(q.shape, dtype=dtype)
     _call(q.device, N.lib().tg_rows8_dequantize, TYPES[dtype], _rows_of(q), k, qf.data_ptr(), ldq,
           scale.contiguous().data_ptr(), y.data_ptr(), k)
     return y
@@ -131,30 +139,31 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tens
     code = _type(x, "x")
     dev = x.device
     _on(dev, weight, residual)
-    k = x.shape[-1] if x.dim() else 0
-    if x.dim() == 0 or k == 0:
+    shape = x.shape
+    k = shape[-1] if shape else 0
+    if k == 0:
         raise ValueError("x needs at least one column")
     if weight.dtype != x.dtype or weight.shape != (k,):
         raise ValueError(f"weight must be {x.dtype} of shape ({k},), got {weight.dtype} {tuple(weight.shape)}")
-    if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape):
+    if residual is not None and (residual.dtype != x.dtype or residual.shape != shape):
         raise ValueError(f"residual must be like x ({x.dtype} {tuple(x.shape)}), got {residual.dtype} {tuple(residual.shape)}")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    rows, lead = _rows_of(x), x.shape[:-1]
+    rows, lead = _rows_of(x), shape[:-1]
     xf, ldx = _flat(x)
     weight = weight.contiguous()
-    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
-    scale = torch.empty(lead, dtype=torch.float32, device=dev)
+    q = x.new_empty(shape, dtype=torch.int8)
+    scale = x.new_empty(lead, dtype=torch.float32)
     rf, ldr, h, hp = None, 0, x, None
     if residual is not None:
         rf, ldr = _flat(residual)
-        h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        h = x.new_empty(shape)
         hp = h.data_ptr()
     ckpt = ckpt_scale = rstd = None
     if checkpoint:
-        ckpt = torch.empty(x.shape, dtype=torch.int8, device=dev)
-        ckpt_scale = torch.empty(lead, dtype=torch.float32, device=dev)
-        rstd = torch.empty(lead, dtype=torch.float32, device=dev)
+        ckpt = x.new_empty(shape, dtype=torch.int8)
+        ckpt_scale = x.new_empty(lead, dtype=torch.float32)
+        rstd = x.new_empty(lead, dtype=torch.float32)
     _call(dev, N.lib().tg_rows8_rmsnorm, code, rows, k, xf.data_ptr(), ldx, None if rf is None else rf.data_ptr(), ldr,
           weight.data_ptr(), eps, hp, k, q.data_ptr(), k, scale.data_ptr(),
           None if ckpt is None else ckpt.data_ptr(), k, None if ckpt is None else ckpt_scale.data_ptr(),
@@ -190,8 +199,8 @@ def rmsnorm_backward(grad: torch.Tensor, checkpoint: Rows8, rstd: torch.Tensor, 
     kf, ldk = _flat(ck)
     hf, ldh = (None, 0) if grad_h is None else _flat(grad_h)
     weight, cs, rstd = weight.contiguous(), cs.contiguous(), rstd.contiguous()
-    grad_x = torch.empty(grad.shape, dtype=weight.dtype, device=dev)
-    grad_w = torch.empty(k, dtype=weight.dtype, device=dev)
+    grad_x = weight.new_empty(grad.shape)
+    grad_w = weight.new_empty(k)
     _call(dev, N.lib().tg_rows8_rmsnorm_backward, code, gcode, _rows_of(ck), k, gf.data_ptr(), ldg,
           None if hf is None else hf.data_ptr(), ldh, weight.data_ptr(), kf.data_ptr(), ldk, cs.data_ptr(),
           rstd.data_ptr(), grad_x.data_ptr(), k, grad_w.data_ptr())
@@ -222,7 +231,7 @@ def matmul(a: Rows8, b: Rows8, bias: Optional[torch.Tensor] = None, dtype: torch
     asc, bsc = asc.contiguous(), bsc.contiguous()
     if bias is not None:
         bias = bias.contiguous()
-    c = torch.empty(aq.shape[:-1] + (n,), dtype=dtype, device=dev)
+    c = aq.new_empty(aq.shape[:-1] + (n,), dtype=dtype)
     _call(dev, N.lib().tg_rows8_gemm, code, _rows_of(aq), n, k, af.data_ptr(), lda, asc.data_ptr(), bf.data_ptr(), ldb,
           bsc.data_ptr(), None if bias is None else bias.data_ptr(), c.data_ptr(), n)
     return c
@@ -255,7 +264,7 @@ def matmul_backward(grad: torch.Tensor, a: Optional[Rows8], b: Optional[Rows8], 
         k = b.q.shape[1]
         bf, ldb = _flat(b.q)
         scale = b.scale.contiguous()
-        grad_a = torch.empty(grad.shape[:-1] + (k,), dtype=dtype_a or grad.dtype, device=dev)
+        grad_a = grad.new_empty(grad.shape[:-1] + (k,), dtype=dtype_a or grad.dtype)
         _call(dev, N.lib().tg_rows8_gemm_backward, code, TYPES[grad_a.dtype], 0, rows, k, n, gf.data_ptr(), ldg,
               bf.data_ptr(), ldb, scale.data_ptr(), grad_a.data_ptr(), k)
     if a is not None:
@@ -266,7 +275,7 @@ def matmul_backward(grad: torch.Tensor, a: Optional[Rows8], b: Optional[Rows8], 
         k = a.q.shape[-1]
         af, lda = _flat(a.q)
         scale = a.scale.contiguous()
-        grad_b = torch.empty((n, k), dtype=dtype_b or grad.dtype, device=dev)
+        grad_b = grad.new_empty((n, k), dtype=dtype_b or grad.dtype)
         _call(dev, N.lib().tg_rows8_gemm_backward, code, TYPES[grad_b.dtype], 1, n, k, rows, gf.data_ptr(), ldg,
               af.data_ptr(), lda, scale.data_ptr(), grad_b.data_ptr(), k)
     return grad_a, grad_b
@@ -279,8 +288,10 @@ def column_sum(x: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Te
     _on(x.device)
     if dtype is not None and dtype not in TYPES:
         raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
+    if x.dim() == 0:
+        raise ValueError("expected a tensor with at least one dimension")
     xf, ldx = _flat(x)
-    out = torch.empty(x.shape[-1], dtype=dtype or x.dtype, device=x.device)
+    out = x.new_empty(x.shape[-1], dtype=dtype or x.dtype)
     _call(x.device, N.lib().tg_rows8_column_sum, code, TYPES[out.dtype], _rows_of(x), x.shape[-1], xf.data_ptr(), ldx,
           out.data_ptr())
     return out
