@@ -103,6 +103,44 @@ tg_status launch_product(const CUtensorMap& a, const CUtensorMap& b, ProductArgs
   return check_launch("rows8 product");
 }
 
+// Tokens per tile of the few-token kernel, or 0 for the paired one.
+int token_tile(int64_t m) {
+  return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 256 ? 128 : 0;
+}
+
+template <int NT, typename T>
+tg_status launch_tokens(const CUtensorMap& tokens, const CUtensorMap& weights, ProductArgs p, cudaStream_t st) {
+  using S = tg8::TokensShape<NT>;
+  const int64_t tiles = (p.n + 127) / 128, tt = (p.m + NT - 1) / NT;
+  if (tiles > 0x0fffffff) return fail(TG_ERR_UNSUPPORTED, "n=%lld", (long long)p.n);
+  // as many CTAs of a cluster per tile as give every SM one, each with at
+  // least two stages of the sum
+  int split = 1;
+  while (split < 8 && tiles * tt * split * 2 <= sm_count() && p.blocks >= 4 * split) split *= 2;
+  p.split_steps = (p.blocks + split - 1) / split;
+  const int stages = std::min(S::kMost, p.split_steps);
+  const size_t smem = size_t(stages) * S::kStage + (split > 1 ? S::kExchange : 0) + 1024;
+  auto kern = tg8::tokens_kernel<NT, T>;
+  const tg_status s = ensure_smem(reinterpret_cast<const void*>(kern), size_t(S::kMost) * S::kStage + S::kExchange + 1024);
+  if (s != TG_OK) return s;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(tiles * split), unsigned(tt));
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {unsigned(split), 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tokens, weights, p, split, stages);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(TG_ERR_CUDA, "rows8 gemm: %s", cudaGetErrorString(e));
+  }
+  return TG_OK;
+}
+
 }  // namespace tgi
 
 using namespace tgi;
@@ -136,8 +174,18 @@ tg_status tg_rows8_gemm(tg_dtype dtype, int64_t m, int64_t n, int64_t k, const i
   p.planes = 1;
   p.blocks = std::max(1, int((k + 127) / 128));
   CUtensorMap ma, mb;
-  if (!oa.map(128, 128, &ma) || !ob.map(128, 128, &mb)) return fail(TG_ERR_CUDA, "rows8 gemm: tensor map encoding failed");
-  return with_type8(dtype, [&](auto t) { return launch_product<tg8::kForward, decltype(t)>(ma, mb, p, st); });
+  const int nt = token_tile(m);
+  if (!oa.map(128, nt ? nt : 128, &ma) || !ob.map(128, 128, &mb)) return fail(TG_ERR_CUDA, "rows8 gemm: tensor map encoding failed");
+  return with_type8(dtype, [&](auto t) {
+    using T = decltype(t);
+    switch (nt) {
+      case 16: return launch_tokens<16, T>(ma, mb, p, st);
+      case 32: return launch_tokens<32, T>(ma, mb, p, st);
+      case 64: return launch_tokens<64, T>(ma, mb, p, st);
+      case 128: return launch_tokens<128, T>(ma, mb, p, st);
+      default: return launch_product<tg8::kForward, T>(ma, mb, p, st);
+    }
+  });
 }
 
 tg_status tg_rows8_gemm_backward(tg_dtype grad_dtype, tg_dtype out_dtype, int transposed, int64_t p, int64_t cols,

@@ -447,6 +447,170 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   }
 }
 
+// The forward product for few tokens (decoding): what it has to do is read the
+// weights once, so the roles are swapped.  128 weight rows are the tensor
+// core's rows and up to NT tokens its columns; the sum is split over the S
+// CTAs of a cluster (S from 1 to 8, so that all SMs read).  Each CTA finishes a
+// share of the tokens: the others write their integer parts into its shared
+// memory (stores need no answer; fetching the parts took 860 cycles a round).
+// A CTA's whole share of the weights is in flight at once where it fits its
+// shared memory.
+//
+// A CTA that waits for its cluster must not wait for tensor memory held by
+// one that waits for another cluster: with split > 1 a CTA has at least 37 KB
+// of shared memory (NT = 128: 65 KB), so the CTAs that fit an SM together ask
+// for at most 416 of its 512 columns, and none fits beside a paired CTA.
+template <int NT> struct TokensShape {
+  static constexpr int kStage = kOperand + NT * 128;
+  static constexpr int kExchange = (NT < 32 ? 32 : NT) * 512;   // parts of this CTA's tokens (shares of 4) from the whole cluster
+  static constexpr int kMost = (200 * 1024 - kExchange) / kStage;   // stages
+  static constexpr int kBars = 2 * kMost + 1;
+  static constexpr int kColumns = NT < 32 ? 32 : NT;
+};
+
+template <int NT, typename T>
+__global__ void __launch_bounds__(128) tokens_kernel(const __grid_constant__ CUtensorMap map_tokens,
+                                                     const __grid_constant__ CUtensorMap map_weights, const ProductArgs p,
+                                                     int split, int stages) {
+  using S = TokensShape<NT>;
+  __shared__ __align__(8) uint64_t bar_store[S::kBars];
+  __shared__ uint32_t slot;
+  __shared__ float scales[NT];
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (umma::smem_u32(smem_raw) + 1023) & ~1023u, bars = umma::smem_u32(bar_store);
+  const uint32_t exchange = base + stages * S::kStage;
+  auto full = [&](int s) { return bars + 8 * s; };
+  auto empty = [&](int s) { return bars + 8 * (S::kMost + s); };
+  const uint32_t done = bars + 8 * (2 * S::kMost);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % split;
+  const int n0 = int(blockIdx.x / split) * 128, t0 = int(blockIdx.y) * NT, tokens = min(NT, int(p.m) - t0);
+  const int first = rank * p.split_steps, steps = max(0, min(p.split_steps, p.blocks - first));   // the last CTAs may have no share
+
+  if (warp == 0 && lane == 0) {
+    umma::tma_prefetch(&map_weights);
+    umma::tma_prefetch(&map_tokens);
+    for (int s = 0; s < stages; s++) {
+      umma::bar_init(full(s), 1);
+      umma::bar_init(empty(s), 1);
+    }
+    umma::bar_init(done, 1);
+    umma::bar_init_fence();
+  }
+  if (warp == 2) umma::tmem_alloc<1>(umma::smem_u32(&slot), S::kColumns);
+  umma::fence_before();
+  __syncthreads();
+  umma::fence_after();
+  if (split > 1) umma::cluster_arrive();   // all of the cluster has started: waited for before the first store
+  const uint32_t tmem = slot;
+  bool ok = true;
+  const int64_t col = int64_t(n0) + threadIdx.x;
+  float cs = 0.f, bias = 0.f;
+  if (col < p.n) {
+    cs = p.col_scale[col];
+    if (p.bias) bias = to_f32(static_cast<const T*>(p.bias)[col]);
+  }
+  if (warp >= 2)
+    for (int t = threadIdx.x - 64; t < tokens; t += 64) scales[t] = p.row_scale[t0 + t];
+
+  if (warp == 0) {
+    const bool issue = umma::elect_one();
+    int s = 0;
+    uint32_t parity = 0;
+    for (int i = 0; i < steps; i++) {
+      if (!umma::bar_wait(empty(s), parity ^ 1)) { ok = false; break; }
+      const uint32_t a = base + s * S::kStage;
+      if (issue) {
+        umma::bar_expect(full(s), S::kStage);
+        umma::tma_load_3d(a, &map_weights, (first + i) * 128, n0, 0, full(s));
+        umma::tma_load_3d(a + kOperand, &map_tokens, (first + i) * 128, t0, 0, full(s));
+      }
+      if (++s == stages) { s = 0; parity ^= 1; }
+    }
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = umma::instr_desc(2, 1, false, false, 128, NT);
+    const uint64_t da0 = umma::smem_desc(base, 16, 1024), db0 = umma::smem_desc(base + kOperand, 16, 1024);
+    const bool issue = umma::elect_one();
+    int s = 0;
+    uint32_t parity = 0;
+    for (int i = 0; i < steps; i++) {
+      if (!umma::bar_wait(full(s), parity)) { ok = false; break; }
+      umma::fence_after();
+      const uint32_t off = s * (S::kStage >> 4);
+      if (issue) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) umma::mma<1, true>(tmem, da0 + (off + j * 2), db0 + (off + j * 2), idesc, i | j);
+        umma::mma_commit<1>(empty(s));
+      }
+      if (++s == stages) { s = 0; parity ^= 1; }
+    }
+    if (issue && ok) umma::mma_commit<1>(done);
+  }
+  __syncwarp();
+  if (!umma::bar_wait(done, 0)) ok = false;
+  umma::fence_after();
+  if (!ok) umma::drain_copies();
+  __syncthreads();   // the tokens' scales
+
+  // four tokens of this thread's weight row
+  T* c = static_cast<T*>(p.c) + int64_t(t0) * p.ldc + col;
+  auto emit4 = [&](int t, const int (&sum)[4], bool bad) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      float z = float(sum[i]) * scales[t + i] * cs + bias;   // scales: NT of them, a multiple of 4
+      if (bad) z = __uint_as_float(0x7fffffffu);
+      if (t + i < tokens && col < p.n) c[int64_t(t + i) * p.ldc] = from_f32<T>(z);
+    }
+  };
+  if (split > 1) umma::cluster_wait();
+  const int share = ((tokens + split - 1) / split + 3) & ~3;   // tokens a CTA of the cluster finishes, by fours
+  const uint32_t mine = exchange + threadIdx.x * 16, row4 = 128 * 16;   // (source x share / 4 x 128 weight rows x 4 tokens)
+#pragma unroll 1
+  for (int t = 0; t < tokens; t += 16) {
+    uint32_t acc[16];
+    umma::tmem_load16(tmem + t + (uint32_t(warp * 32) << 16), acc);
+    umma::tmem_load_wait();
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      if (split == 1) {
+        emit4(t + i, {int(acc[i]), int(acc[i + 1]), int(acc[i + 2]), int(acc[i + 3])}, !ok);
+      } else if (t + i < tokens) {
+        if (!ok || !steps) acc[i] = acc[i + 1] = acc[i + 2] = acc[i + 3] = ok ? 0u : 0x80000000u;
+        const int owner = (t + i) / share, local = t + i - owner * share;
+        umma::store_cluster(umma::map_rank(mine + uint32_t(rank * share + local) / 4 * row4, owner), acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+      }
+    }
+  }
+  if (split > 1) {
+    umma::cluster_sync();
+    const int last = min(tokens - rank * share, share);
+#pragma unroll 2
+    for (int t = 0; t < last; t += 4) {
+      int sum[4] = {};
+      bool bad = false;
+#pragma unroll
+      for (int r = 0; r < 8; r++) {
+        if (r >= split) break;
+        uint32_t v[4];
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                     : "r"(mine + uint32_t(r * share + t) / 4 * row4));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          sum[i] += int(v[i]);
+          bad |= v[i] == 0x80000000u;   // no sum takes this value
+        }
+      }
+      emit4(rank * share + t, sum, bad);
+    }
+  }
+  umma::fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    umma::fence_after();
+    umma::tmem_free<1>(tmem, S::kColumns);
+  }
+}
+
 // Joins the parts of a sum, in order: forward integer sums with their scales
 // and bias, backward f32 sums.  Four columns per thread.
 template <bool FORWARD, typename T>
