@@ -105,7 +105,7 @@ tg_status launch_product(const CUtensorMap& a, const CUtensorMap& b, ProductArgs
 
 // Tokens per tile of the few-token kernel, or 0 for the paired one.
 int token_tile(int64_t m) {
-  return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 256 ? 128 : 0;
+  return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 512 ? 128 : 0;
 }
 
 template <int NT, typename T>

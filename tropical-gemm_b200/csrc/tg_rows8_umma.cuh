@@ -48,8 +48,8 @@ struct ProductArgs {
 constexpr int kTile = 256, kHalf = 128;
 constexpr int kOperand = 16384;                 // bytes of one operand's stage: 128 rows x 128 bytes
 constexpr int kRawBytes = 8192;                 // the 8-bit tile that is expanded to one stage
-constexpr int kEpiWarps = 4, kConvWarps = 4, kConvGroups = 2;   // a group of conv warps per 8-bit tile, in turn
-constexpr int kEpiPitch = 17;
+constexpr int kEpiWarps = 8, kConvWarps = 4, kConvGroups = 2;   // a group of conv warps per 8-bit tile, in turn
+constexpr int kStagingBytes = 2048;             // per epilogue warp: 64 bytes of 32 rows
 
 // Shared memory and barriers: a ring of both operands.  Backward the right
 // operand's stages are written by the conv warps from a ring of 8-bit tiles
@@ -62,14 +62,17 @@ template <int MODE> struct ProductShape {
   static constexpr int kHalves = kBack ? 2 : 1;                  // tiles of an item that share the right operand
   static constexpr int kStages = kBack ? 4 : 6;
   static constexpr int kStage = (1 + kHalves) * kOperand;        // right operand, left operands
-  static constexpr int kRaws = kBack ? 2 : 0;
+  // 8-bit tiles on their way: two of their own, and while no item has two
+  // tiles, two in each stage's unused half of the left operands: a short
+  // product is bound by the way from memory (1000 cycles a stage with two)
+  static constexpr int kOwnRaws = kBack ? 2 : 0, kRaws = kBack ? 2 + 2 * kStages : 0;
   // a slot belongs to one conv group for good: a group that met a slot every
   // other turn could take the parity of a turn it did not see for its own
-  static_assert(kRaws % kConvGroups == 0 && kStages % kConvGroups == 0, "rings and groups");
+  static_assert(kOwnRaws % kConvGroups == 0 && kRaws % kConvGroups == 0 && kStages % kConvGroups == 0, "rings and groups");
   static constexpr int kThreads = 32 * (4 + kEpiWarps + (kBack ? kConvWarps * kConvGroups : 0));
   static constexpr int kOffRaw = kStages * kStage;
-  static constexpr int kOffStaging = kOffRaw + kRaws * kRawBytes;
-  static constexpr int kOffCols = kOffStaging + kEpiWarps * 32 * kEpiPitch * 4;   // b_scale, bias of the tile
+  static constexpr int kOffStaging = kOffRaw + kOwnRaws * kRawBytes;
+  static constexpr int kOffCols = kOffStaging + kEpiWarps * kStagingBytes;   // b_scale, bias of the tile
   static constexpr int kOffBars = kOffCols + (kBack ? 0 : 2 * kTile * 4);
   static constexpr int kBars = 2 * (kStages + kRaws + 2);
   static constexpr int kOffSlot = kOffBars + kBars * 8;
@@ -97,6 +100,15 @@ template <int I> __device__ __forceinline__ uint32_t bytes_scaled(uint32_t w_bia
         "f"(-8388736.f), "f"(f));
   return r;
 }
+
+// The same for a ring whose size is known when the kernel runs.
+struct RingOf {
+  int n, slot = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == n) { slot = 0; parity ^= 1; }
+  }
+};
 
 // Item i of a pair's walk: the tile at (m0, n0) and, if halves is 2, the one
 // below it.  Double items first, in whole rounds of all pairs; then the rest
@@ -139,47 +151,52 @@ __device__ __forceinline__ bool item_at(const ProductArgs& p, int pair, int pair
   return true;
 }
 
-// One row of 32 outputs in the row's own thread, or through shared memory by
-// rows when C's rows are not 16-byte aligned or end inside.
+// 64 bytes of each of 32 rows, one row per lane, to global memory through
+// shared memory, so that a warp's store covers 8 rows' 64 bytes (a store of 32
+// lanes' own rows touches 32 lines: 900 cycles for 32 columns instead of 250).  c: the
+// first row's first element; rows, cols: how many exist; vec: 16-byte aligned
+// rows.  Two rows share 128 bytes of shared memory; the chunks are swizzled so
+// that eight lanes meet all banks either way.
 template <typename T>
-__device__ __forceinline__ void store_rows32(const ProductArgs& p, const float (&z)[32], float* staging, int lane,
-                                             int64_t row0, int64_t col) {
-  if (p.vec && col + 32 <= p.n) {
-    const int64_t row = row0 + lane;
-    if (row < p.m) {
-      T* c = static_cast<T*>(p.c) + row * p.ldc + col;
+__device__ __forceinline__ void store_rows64(T* c, int64_t ld, int rows, int64_t cols, bool vec, const uint32_t (&w)[16],
+                                             uint32_t staging, int lane) {
+  constexpr int kPer = 16 / int(sizeof(T));   // elements of a 16-byte chunk
+  __syncwarp();                               // the last chunk is read
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        float v[8];
+  for (int j = 0; j < 4; j++)
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(staging + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)),
+                 "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3]) : "memory");
+  __syncwarp();
+  const int j = lane & 3;
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = z[8 * i + e];
-        store8(c + 8 * i, v);
+  for (int k = 0; k < 4; k++) {
+    const int r = k * 8 + (lane >> 2);
+    uint32_t v[4];
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "r"(staging + r * 64 + ((j ^ ((r >> 1) & 3)) << 4)));
+    if (r < rows) {
+      T* to = c + r * ld + j * kPer;
+      if (vec && (j + 1) * kPer <= cols) {
+        *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
+      } else {
+        T e[kPer];
+        __builtin_memcpy(e, v, 16);
+#pragma unroll
+        for (int i = 0; i < kPer; i++)
+          if (j * kPer + i < cols) to[i] = e[i];
       }
-    }
-    return;
-  }
-#pragma unroll
-  for (int h = 0; h < 32; h += 16) {
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 16; i++) staging[lane * kEpiPitch + i] = z[h + i];
-    __syncwarp();
-    const int c16 = lane & 15;
-    if (col + h + c16 < p.n) {
-      const int rows = int(min(int64_t(32), p.m - row0));
-      T* c = static_cast<T*>(p.c) + row0 * p.ldc + col + h + c16;
-      for (int r = lane >> 4; r < rows; r += 2) c[r * p.ldc] = from_f32<T>(staging[r * kEpiPitch + c16]);
     }
   }
 }
 
-// 32 raw sums of one row of a part.
-__device__ __forceinline__ void store_part32(const ProductArgs& p, const uint32_t (&z)[32], int64_t row, int64_t col) {
-  if (row >= p.m) return;
-  uint32_t* c = p.part + (int64_t((blockIdx.x >> 1) % p.splits) * p.m + row) * p.ldp + col;
-#pragma unroll
-  for (int i = 0; i < 32; i += 4)
-    if (col + i < p.ldp) *reinterpret_cast<uint4*>(c + i) = make_uint4(z[i], z[i + 1], z[i + 2], z[i + 3]);
+template <typename T> __device__ __forceinline__ uint32_t pack_pair(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack_pair<bf16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack_pair<f16>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 template <int MODE, typename T>
@@ -198,6 +215,11 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   auto raw_empty = [&](int s) { return bars + 8 * (kR + S::kRaws + s); };  // and is read (each CTA)
   auto acc_full = [&](int b) { return bars + 8 * (kAcc + b); };            // tile summed (each CTA)
   auto acc_empty = [&](int b) { return bars + 8 * (kAcc + 2 + b); };       // and read out in both CTAs
+  const int raws = p.doubles ? S::kOwnRaws : S::kRaws;
+  auto raw_tile = [&](int s) {
+    return s < S::kOwnRaws ? base + S::kOffRaw + s * kRawBytes
+                           : base + ((s - S::kOwnRaws) >> 1) * S::kStage + 2 * kOperand + ((s - S::kOwnRaws) & 1) * kRawBytes;
+  };
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + S::kOffSlot);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // warp: uniform
@@ -266,7 +288,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   } else if (S::kBack && warp == 3) {
     // ---- producer of the 8-bit tiles
     const bool issue = umma::elect_one();
-    RingAt<S::kBack ? S::kRaws : 1> at;
+    RingOf at{raws};
     Item item;
     for (int i = 0; ok && item_at(p, pair, pairs, i, item); i++) {
       const int col = int(item.n0) + int(rank) * kHalf;
@@ -275,7 +297,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         if (!umma::bar_wait(raw_empty(at.slot), at.parity ^ 1)) { ok = false; break; }
         if (issue) {
           umma::bar_expect(raw_full(at.slot), kRawBytes);
-          umma::tma_load_3d_pair(base + S::kOffRaw + at.slot * kRawBytes, &map_b, col, block * 64, 0, umma::map_rank(raw_full(at.slot), rank));
+          umma::tma_load_3d_pair(raw_tile(at.slot), &map_b, col, block * 64, 0, umma::map_rank(raw_full(at.slot), rank));
         }
         if (++block == p.blocks) block = 0;
       }
@@ -322,58 +344,73 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     }
     if (!ok) umma::drain_copies();
   } else if (warp >= 4 && warp < 4 + kEpiWarps) {
-    // ---- epilogue: warp w reads lanes 32 w .. 32 w + 31 of tensor memory
-    const int w = warp - 4, tid = threadIdx.x - 128;
-    float* staging = reinterpret_cast<float*>(smem + S::kOffStaging) + w * 32 * kEpiPitch;
+    // ---- epilogue: warp w reads lanes 32 (w % 4) .. of tensor memory and one
+    // half of the columns, 64 bytes of output at a time
+    const int w = (warp - 4) & 3, half = (warp - 4) >> 2, tid = threadIdx.x - 128;
+    const uint32_t staging = base + S::kOffStaging + (warp - 4) * kStagingBytes;
     float* cols = reinterpret_cast<float*>(smem + S::kOffCols);
     Item item;
     int n = 0;
     for (int i = 0, h = 0; item_at(p, pair, pairs, i, item); n++) {   // h: the tile within the item
       const int64_t n0 = item.n0, row0 = item.m0 + h * kTile + rank * kHalf + w * 32, row = row0 + lane;
+      const int rows = int(max(int64_t(0), min(int64_t(32), p.m - row0)));
       const int buf = n & 1;
       if (++h == item.halves) { h = 0; i++; }
       float rs = 0.f;
-      if (MODE == kForward) {
-        asm volatile("bar.sync 1, 128;" ::: "memory");   // the last tile's columns are no longer read
-        for (int i = tid; i < kTile; i += 128) {
-          const bool in = n0 + i < p.n;
-          cols[i] = in ? p.col_scale[n0 + i] : 0.f;
-          cols[kTile + i] = in && p.bias ? to_f32(static_cast<const T*>(p.bias)[n0 + i]) : 0.f;
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (MODE == kForward && p.splits == 1) {
+        asm volatile("bar.sync 1, 256;" ::: "memory");   // the last tile's columns are no longer read
+        const bool in = n0 + tid < p.n;
+        cols[tid] = in ? p.col_scale[n0 + tid] : 0.f;
+        cols[kTile + tid] = in && p.bias ? to_f32(static_cast<const T*>(p.bias)[n0 + tid]) : 0.f;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
         if (row < p.m) rs = p.row_scale[row];
       }
       if (ok && !umma::bar_wait(acc_full(buf), (n >> 1) & 1)) ok = false;
       umma::fence_after();
-      for (int c = 0; c < kTile; c += 32) {
-        uint32_t acc[32];
-        float z[32];
-        umma::tmem_load32(tmem + buf * kTile + c + (uint32_t(w * 32) << 16), acc);
-        umma::tmem_load_wait();
-        if (c + 32 == kTile) {   // read out: the next tile's products may have the accumulator
-          umma::fence_before();
-          __syncwarp();
-          if (lane == 0) umma::bar_arrive_cluster(umma::map_rank(acc_empty(buf), 0));
-        }
-        if (n0 + c >= p.n) continue;
-        if (p.splits > 1) {
-          if (!ok) {   // NaN, or a value no integer sum takes
+      const uint32_t from = tmem + buf * kTile + half * 128 + (uint32_t(w * 32) << 16);
+      const int64_t col0 = n0 + half * 128;
+      auto read_out = [&] {   // the next tile's products may have the accumulator
+        umma::fence_before();
+        __syncwarp();
+        if (lane == 0) umma::bar_arrive_cluster(umma::map_rank(acc_empty(buf), 0));
+      };
+      auto value = [&](uint32_t acc, int c) {
+        float z = __uint_as_float(acc);
+        if (MODE == kForward) z = float(int(acc)) * rs * cols[half * 128 + c] + cols[kTile + half * 128 + c];
+        return ok ? z : __uint_as_float(0x7fffffffu);   // a wait ran out: the outputs say so
+      };
+      if (p.splits > 1 || sizeof(T) == 4) {
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 16) {
+          uint32_t acc[16];
+          umma::tmem_load16(from + c, acc);
+          umma::tmem_load_wait();
+          if (c == 112) read_out();
+          if (col0 + c >= p.n) continue;
+          if (p.splits > 1) {
+            if (!ok) {   // NaN, or a value no integer sum takes
 #pragma unroll
-            for (int i = 0; i < 32; i++) acc[i] = MODE == kForward ? 0x80000000u : 0x7fffffffu;
-          }
-          store_part32(p, acc, row, n0 + c);
-          continue;
-        }
+              for (int e = 0; e < 16; e++) acc[e] = MODE == kForward ? 0x80000000u : 0x7fffffffu;
+            }
+            store_rows64(p.part + (int64_t(pair % p.splits) * p.m + row0) * p.ldp + col0 + c, p.ldp, rows, p.ldp - col0 - c, true, acc, staging, lane);
+          } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 32; i++) {
-          if (MODE == kForward) {
-            z[i] = float(int(acc[i])) * rs * cols[c + i] + (p.bias ? cols[kTile + c + i] : 0.f);
-          } else {
-            z[i] = __uint_as_float(acc[i]);
+            for (int e = 0; e < 16; e++) acc[e] = __float_as_uint(value(acc[e], c + e));
+            store_rows64(static_cast<T*>(p.c) + row0 * p.ldc + col0 + c, p.ldc, rows, p.n - col0 - c, p.vec, acc, staging, lane);
           }
-          if (!ok) z[i] = __uint_as_float(0x7fffffffu);   // a wait ran out: the outputs say so
         }
-        store_rows32<T>(p, z, staging, lane, row0, n0 + c);
+      } else if constexpr (sizeof(T) == 2) {
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t acc[32], z[16];
+          umma::tmem_load32(from + c, acc);
+          umma::tmem_load_wait();
+          if (c == 96) read_out();
+          if (col0 + c >= p.n) continue;
+#pragma unroll
+          for (int e = 0; e < 16; e++) z[e] = pack_pair<T>(value(acc[2 * e], c + 2 * e), value(acc[2 * e + 1], c + 2 * e + 1));
+          store_rows64(static_cast<T*>(p.c) + row0 * p.ldc + col0 + c, p.ldc, rows, p.n - col0 - c, p.vec, z, staging, lane);
+        }
       }
     }
     if (!ok) umma::drain_copies();
@@ -386,7 +423,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     int items = p.splits > 1 ? 1 : p.doubles / pairs;
     if (p.splits == 1 && p.singles > pair) items += (p.singles - pair + pairs - 1) / pairs;
     const int64_t total = int64_t(items) * steps;
-    RingAt<S::kBack ? S::kRaws : 1> rw;
+    RingOf rw{raws};
     RingAt<S::kStages> cv;
     float sc[2], next[2];
     auto factors = [&](int block, float (&f)[2]) {
@@ -403,7 +440,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       block = (block + kConvGroups) % p.blocks;
       factors(block, next);   // a turn ahead: the load's latency stays out of the wait
       if (!umma::bar_wait(raw_full(rw.slot), rw.parity)) { ok = false; break; }
-      const uint32_t in = base + S::kOffRaw + rw.slot * kRawBytes + (w * 16 + r8) * 128;
+      const uint32_t in = raw_tile(rw.slot) + (w * 16 + r8) * 128;
       uint32_t q[4][4];
 #pragma unroll
       for (int i = 0; i < 4; i++)   // rows + 8 (i / 2), 64 columns (i % 2)
