@@ -167,24 +167,30 @@ __device__ __forceinline__ void store_rows64(T* c, int64_t ld, int rows, int64_t
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(staging + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)),
                  "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3]) : "memory");
   __syncwarp();
-  const int j = lane & 3;
+  const int j = lane & 3, r0 = lane >> 2;   // rows r0, r0 + 8, ..: the same place in the swizzle
+  uint32_t v[4][4];
+#pragma unroll
+  for (int k = 0; k < 4; k++)
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[k][0]), "=r"(v[k][1]), "=r"(v[k][2]), "=r"(v[k][3])
+                 : "r"(staging + r0 * 64 + k * 512 + ((j ^ ((r0 >> 1) & 3)) << 4)));
+  T* to = c + r0 * ld + j * kPer;
+  if (vec && rows == 32 && cols >= 4 * kPer) {   // uniform
+#pragma unroll
+    for (int k = 0; k < 4; k++) *reinterpret_cast<uint4*>(to + k * 8 * ld) = make_uint4(v[k][0], v[k][1], v[k][2], v[k][3]);
+    return;
+  }
 #pragma unroll
   for (int k = 0; k < 4; k++) {
-    const int r = k * 8 + (lane >> 2);
-    uint32_t v[4];
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                 : "r"(staging + r * 64 + ((j ^ ((r >> 1) & 3)) << 4)));
-    if (r < rows) {
-      T* to = c + r * ld + j * kPer;
-      if (vec && (j + 1) * kPer <= cols) {
-        *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
-      } else {
-        T e[kPer];
-        __builtin_memcpy(e, v, 16);
+    if (r0 + 8 * k >= rows) break;
+    T* at = to + k * 8 * ld;
+    if (vec && (j + 1) * kPer <= cols) {
+      *reinterpret_cast<uint4*>(at) = make_uint4(v[k][0], v[k][1], v[k][2], v[k][3]);
+    } else {
+      T e[kPer];
+      __builtin_memcpy(e, v[k], 16);
 #pragma unroll
-        for (int i = 0; i < kPer; i++)
-          if (j * kPer + i < cols) to[i] = e[i];
-      }
+      for (int i = 0; i < kPer; i++)
+        if (j * kPer + i < cols) at[i] = e[i];
     }
   }
 }
