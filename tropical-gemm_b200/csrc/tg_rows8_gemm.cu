@@ -47,12 +47,18 @@ struct Operand8 {
       : q(q_), ld(ld_), rows(rows_), cols(cols_), pad(!tma_rows8(q_, ld_, rows_, cols_)) {}
   int64_t padded() const { return std::max<int64_t>(16, round_up(cols, 16)); }
   size_t scratch() const { return pad ? Scratch::size_of<int8_t>(size_t(rows) * size_t(padded())) : 0; }
-  // A padded copy where the rows are not aligned; cols stays the sum's own
-  // length (at least 1: a sum of nothing is a sum over one zero).
-  void make(Scratch& s, cudaStream_t st) {
+  // Takes the place of a padded copy where the rows are not aligned, to be
+  // filled by pad_operands; a sum of nothing becomes a sum over one zero.
+  void place(Scratch& s, tg8::PadArgs& p, int& count) {
     if (pad) {
       int8_t* out = s.take<int8_t>(size_t(rows) * size_t(padded()));
-      tg8::pad8_kernel<<<row_grid(1024, padded(), rows), 256, 0, st>>>(rows, cols, q, ld, out, padded());
+      p.q[count] = q;
+      p.out[count] = out;
+      p.rows[count] = rows;
+      p.cols[count] = cols;
+      p.ldq[count] = ld;
+      p.ldo[count] = padded();
+      count++;
       q = out;
       ld = padded();
       cols = std::max<int64_t>(cols, 1);
@@ -64,6 +70,12 @@ struct Operand8 {
     return encode_tma(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q, cols, rows, ld, 1, 0, box_cols, box_rows, m);
   }
 };
+
+void pad_operands(const tg8::PadArgs& p, int count, cudaStream_t st) {
+  int64_t most = 0;
+  for (int i = 0; i < count; i++) most = std::max(most, (p.rows[i] * (p.ldo[i] / 16) + 255) / 256);
+  if (most) tg8::pad8_kernel<<<dim3(unsigned(std::min<int64_t>(most, 8192)), 1, unsigned(count)), 256, 0, st>>>(p);
+}
 
 template <int MODE, typename T>
 tg_status launch_product(const CUtensorMap& a, const CUtensorMap& b, ProductArgs p, cudaStream_t st) {
@@ -166,8 +178,11 @@ tg_status tg_rows8_gemm(tg_dtype dtype, int64_t m, int64_t n, int64_t k, const i
     const cudaError_t e = scratch.reserve(need);
     if (e != cudaSuccess) return fail(TG_ERR_CUDA, "rows8 gemm scratch: %s", cudaGetErrorString(e));
   }
-  oa.make(scratch, st);
-  ob.make(scratch, st);
+  tg8::PadArgs pads{};
+  int padded = 0;
+  oa.place(scratch, pads, padded);
+  ob.place(scratch, pads, padded);
+  pad_operands(pads, padded, st);
   ProductArgs p{};
   p.m = m; p.n = n; p.ldc = ldc; p.c = c; p.row_scale = a_scale; p.col_scale = b_scale; p.bias = bias;
   p.sum = int(k);
@@ -223,7 +238,10 @@ tg_status tg_rows8_gemm_backward(tg_dtype grad_dtype, tg_dtype out_dtype, int tr
     const cudaError_t e = scratch.reserve(need);
     if (e != cudaSuccess) return fail(TG_ERR_CUDA, "rows8 gemm backward scratch: %s", cudaGetErrorString(e));
   }
-  oq.make(scratch, st);
+  tg8::PadArgs pads{};
+  int padded = 0;
+  oq.place(scratch, pads, padded);
+  pad_operands(pads, padded, st);
   if (!direct) {
     tg8::bf16* parts = scratch.take<tg8::bf16>(part_count);
     const tg_status s = with_type8(grad_dtype, [&](auto t) {

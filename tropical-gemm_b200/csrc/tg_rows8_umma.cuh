@@ -712,16 +712,36 @@ __global__ void __launch_bounds__(256) split_kernel(int64_t rows, int64_t cols, 
   }
 }
 
-// 8-bit rows copied to rows of ldo, a multiple of 16, zeros behind.
-__global__ void __launch_bounds__(256) pad8_kernel(int64_t rows, int64_t cols, const int8_t* q, int64_t ldq, int8_t* out, int64_t ldo) {
-  const int64_t c = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4;
-  if (c >= ldo) return;
-  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
-    uint32_t v = 0;
+// 8-bit rows copied to rows of ldo, a multiple of 16, zeros behind; up to two
+// matrices in one launch (blockIdx.z).  16 bytes per thread: five aligned
+// words, each with at least one byte of the row, shifted into place.
+struct PadArgs {
+  const int8_t* q[2];
+  int8_t* out[2];
+  int64_t rows[2], cols[2], ldq[2], ldo[2];
+};
+__global__ void __launch_bounds__(256) pad8_kernel(const PadArgs p) {
+  const int z = blockIdx.z;
+  const int64_t per = p.ldo[z] / 16, total = p.rows[z] * per;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+    const int64_t r = i / per, c = (i - r * per) * 16;
+    const int64_t left = p.cols[z] - c;   // bytes of the row from c on
+    uint32_t o[4] = {0, 0, 0, 0};
+    if (left > 0) {
+      const int8_t* from = p.q[z] + r * p.ldq[z] + c;
+      const uint32_t skew = uint32_t(reinterpret_cast<uintptr_t>(from) & 3);
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(from - skew);
+      uint32_t w[5];
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (c + e < cols) v |= uint32_t(uint8_t(q[r * ldq + c + e])) << (8 * e);
-    *reinterpret_cast<uint32_t*>(out + r * ldo + c) = v;
+      for (int k = 0; k < 5; k++) w[k] = 4 * k < left + skew ? words[k] : 0u;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        o[k] = __funnelshift_r(w[k], w[k + 1], skew * 8);
+        const int64_t valid = left - 4 * k;
+        if (valid < 4) o[k] = valid <= 0 ? 0u : o[k] & ((1u << (8 * valid)) - 1);
+      }
+    }
+    *reinterpret_cast<uint4*>(p.out[z] + r * p.ldo[z] + c) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
