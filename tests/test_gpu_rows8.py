@@ -501,3 +501,51 @@ def test_refusals(call):
     x = torch.ones(4, 8, device="cuda")
     with pytest.raises(ValueError):
         call(x, rows8.quantize(x))
+
+
+# ------------------------------------------------------------------- example
+def test_example_trains_and_serves():
+    """The example block learns, and serving gives the trained block's bits:
+    the integer sums are exact, whatever kernel a number of tokens takes."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "rows8_block.py")
+    spec = importlib.util.spec_from_file_location("rows8_block", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    got = example.main(steps=60, tokens=512, width=256)
+    assert got["last"] < 0.5 * got["first"]
+    assert got["served equals trained"] and got["one token at a time equals all"]
+
+
+@pytest.mark.parametrize("m", [1, 5, 16, 17, 40, 64, 100, 128, 200, 512, 513, 700])
+@pytest.mark.parametrize("n, k", [(16, 16), (130, 1000), (4096, 640), (300, 12000)])
+def test_matmul_bits_do_not_depend_on_the_number_of_tokens(m, n, k):
+    """Every kernel and split gives the same bits for a token: exact sums, one epilogue."""
+    g = gen(n + k)
+    a, b = rand8(g, 1024, k), rand8(g, n, k)
+    bias = randn(g, n, dtype=torch.bfloat16)
+    whole = rows8.matmul(a, b, bias=bias)
+    assert torch.equal(rows8.matmul(Rows8(a.q[:m], a.scale[:m]), b, bias=bias), whole[:m])
+
+
+def test_graph_capture():
+    """Norm and product capture into a CUDA graph and replay on new inputs."""
+    g = gen(77)
+    x, res, w = randn(g, 8, 512, dtype=torch.bfloat16), randn(g, 8, 512, dtype=torch.bfloat16), randn(g, 512, dtype=torch.bfloat16)
+    b = rand8(g, 256, 512)
+
+    def run():
+        n = rows8.rmsnorm(x, w, residual=res, checkpoint=True)
+        z = rows8.matmul(n.rows, b)
+        return z, rows8.matmul_backward(z, n.rows, b)[1]
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    x.copy_(randn(g, 8, 512, dtype=torch.bfloat16))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(out, run()))

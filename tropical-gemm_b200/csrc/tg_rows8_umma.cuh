@@ -179,18 +179,29 @@ __device__ __forceinline__ void store_rows64(T* c, int64_t ld, int rows, int64_t
     for (int k = 0; k < 4; k++) *reinterpret_cast<uint4*>(to + k * 8 * ld) = make_uint4(v[k][0], v[k][1], v[k][2], v[k][3]);
     return;
   }
+  if (vec && cols % kPer == 0) {   // whole chunks only
 #pragma unroll
-  for (int k = 0; k < 4; k++) {
-    if (r0 + 8 * k >= rows) break;
-    T* at = to + k * 8 * ld;
-    if (vec && (j + 1) * kPer <= cols) {
-      *reinterpret_cast<uint4*>(at) = make_uint4(v[k][0], v[k][1], v[k][2], v[k][3]);
-    } else {
-      T e[kPer];
-      __builtin_memcpy(e, v[k], 16);
-#pragma unroll
-      for (int i = 0; i < kPer; i++)
-        if (j * kPer + i < cols) at[i] = e[i];
+    for (int k = 0; k < 4; k++)
+      if (r0 + 8 * k < rows && (j + 1) * kPer <= cols) *reinterpret_cast<uint4*>(to + k * 8 * ld) = make_uint4(v[k][0], v[k][1], v[k][2], v[k][3]);
+    return;
+  }
+  // any alignment: lanes along the row, one element each
+  constexpr int kWide = 64 / int(sizeof(T));   // 16 or 32 elements: two rows or one at a time
+  const int e = lane % kWide;
+  if (e < cols) {
+    T* at = c + e;
+#pragma unroll 8
+    for (int r = lane / kWide; r < rows; r += 32 / kWide) {
+      const uint32_t from = staging + r * 64 + (((e / kPer) ^ ((r >> 1) & 3)) << 4) + (e % kPer) * int(sizeof(T));
+      if constexpr (sizeof(T) == 4) {
+        uint32_t x;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(from));
+        reinterpret_cast<uint32_t*>(at)[r * ld] = x;
+      } else {
+        uint16_t x;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(from));
+        reinterpret_cast<uint16_t*>(at)[r * ld] = x;
+      }
     }
   }
 }
