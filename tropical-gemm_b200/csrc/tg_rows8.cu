@@ -107,19 +107,23 @@ __global__ void __launch_bounds__(G == 1 ? 1024 : 512) rows_kernel(RowArgs p) {
   };
 
   RowStats s{0.f, 0u, 0u};
+  float top_h = 0.f, top_y = 0.f;
 #pragma unroll
   for (int g = 0; g < G; g++) {
     float w[8];
     if (NORM) weight_of(g, w);
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      s.top_h = max(s.top_h, mag_bits(v[g][e]));
+    for (int e = 0; e < 8; e += 2) {
+      top_h = mag_max(v[g][e], v[g][e + 1], top_h);
       if (NORM) {
         s.sum = fmaf(v[g][e], v[g][e], s.sum);
-        s.top_y = max(s.top_y, mag_bits(v[g][e] * w[e]));
+        s.sum = fmaf(v[g][e + 1], v[g][e + 1], s.sum);
+        top_y = mag_max(v[g][e] * w[e], v[g][e + 1] * w[e + 1], top_y);
       }
     }
   }
+  s.top_h = __float_as_uint(top_h);
+  s.top_y = __float_as_uint(top_y);
   s = row_reduce(s, p.tpr, warp_stats);
 
   float u = 1.f;
@@ -184,6 +188,129 @@ __global__ void __launch_bounds__(G == 1 ? 1024 : 512) rows_kernel(RowArgs p) {
           if (NORM && p.h) h[c] = from_f32<T>(v[g][e]);
         }
       }
+    }
+  }
+}
+
+// Sums and maxima over the tpr threads of a row: one named barrier per row, two
+// sets of partial results in turn.  The order is the same in every thread.
+struct RowJoin {
+  float4 (*stats)[16];   // [2][warps of the block]
+  int tpr, sub, turn;
+  __device__ __forceinline__ void barrier() const { asm volatile("bar.sync %0, %1;" ::"r"(sub + 1), "r"(tpr) : "memory"); }
+  __device__ __forceinline__ RowStats operator()(RowStats s) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) s.sum += __shfl_xor_sync(0xffffffffu, s.sum, d);
+    s.top_y = __reduce_max_sync(0xffffffffu, s.top_y);
+    s.top_h = __reduce_max_sync(0xffffffffu, s.top_h);
+    if (tpr > 32) {
+      const int lane = threadIdx.x & 31, warps = tpr >> 5, first = sub * warps;
+      if (lane == 0) stats[turn][threadIdx.x >> 5] = make_float4(s.sum, __uint_as_float(s.top_y), __uint_as_float(s.top_h), 0.f);
+      barrier();
+      const float4 o = stats[turn][first + (lane & (warps - 1))];
+      turn ^= 1;
+      s.sum = o.x;
+      for (int d = warps >> 1; d; d >>= 1) s.sum += __shfl_xor_sync(0xffffffffu, s.sum, d);
+      s.top_y = __reduce_max_sync(0xffffffffu, __float_as_uint(o.y));
+      s.top_h = __reduce_max_sync(0xffffffffu, __float_as_uint(o.z));
+    }
+    return s;
+  }
+};
+
+// The norm for many aligned rows: persistent, tpr threads per row with a fixed
+// set of columns each, so the weights stay in registers as f32, and the next
+// row is on its way while this one is worked on.  The kernel above is bound by
+// instructions (78 % of the issue slots for 4096 x 8192 bf16, weights unpacked
+// twice per row); this one needs about half of them.
+template <typename T, int G>
+__global__ void __launch_bounds__(512) norm_stream_kernel(RowArgs p) {
+  __shared__ float4 stats[2][16];
+  const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, per_block = blockDim.x / p.tpr;
+  const int cols = int(p.cols);
+  auto at = [&](int g) { return (g * p.tpr + t) * 8; };
+  RowJoin join{stats, p.tpr, sub, 0};
+  float w[G][8];
+  Vec8<T> nx[G], nr[G];
+  const T *x = static_cast<const T*>(p.x), *res = static_cast<const T*>(p.residual);
+#pragma unroll
+  for (int g = 0; g < G; g++) {
+    if (at(g) < cols) nx[g].load(static_cast<const T*>(p.weight) + at(g)); else nx[g].zero();
+    nx[g].get(w[g]);
+  }
+  auto load = [&](int64_t row) {
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      const bool in = at(g) < cols;
+      if (in) nx[g].load(x + row * p.ldx + at(g)); else nx[g].zero();
+      if (in && res) nr[g].load(res + row * p.ldr + at(g)); else nr[g].zero();
+    }
+  };
+  const int64_t stride = int64_t(gridDim.x) * per_block;
+  int64_t row = int64_t(blockIdx.x) * per_block + sub;
+  if (row < p.rows) load(row);
+  for (; row < p.rows; row += stride) {
+    float v[G][8];
+    RowStats s{0.f, 0u, 0u};
+    float top_h = 0.f, top_y = 0.f;
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      float r[8];
+      nx[g].get(v[g]);
+      if (res) {
+        nr[g].get(r);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[g][e] += r[e];
+      }
+    }
+    if (row + stride < p.rows) load(row + stride);
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        top_h = mag_max(v[g][e], v[g][e + 1], top_h);
+        s.sum = fmaf(v[g][e], v[g][e], s.sum);
+        s.sum = fmaf(v[g][e + 1], v[g][e + 1], s.sum);
+        top_y = mag_max(v[g][e] * w[g][e], v[g][e + 1] * w[g][e + 1], top_y);
+      }
+    s.top_h = __float_as_uint(top_h);
+    s.top_y = __float_as_uint(top_y);
+    s = join(s);
+    const float u = 1.f / sqrtf(s.sum / float(cols) + p.eps);
+    const Quant qh = quant_of(s.top_h);
+    // y = (h * weight) * u, so y / scale = (h * weight) * (127 / max|h * weight|),
+    // unless the product left f32's comfortable range
+    Quant qy;
+    const bool redo = !(__uint_as_float(s.top_y) > 1e-25f && __uint_as_float(s.top_y) < 1e25f);
+    if (redo) {   // uniform over the row's threads; zero rows, tiny or huge values
+      RowStats r{0.f, 0u, 0u};
+#pragma unroll
+      for (int g = 0; g < G; g++)
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (at(g) < cols) r.top_y = max(r.top_y, mag_bits(v[g][e] * u * w[g][e]));
+      qy = quant_of(join(r).top_y);
+    } else {
+      qy = quant_of(s.top_y);
+      qy.scale = quant_of(mag_bits(__uint_as_float(s.top_y) * u)).scale;
+    }
+    if (t == 0) {
+      p.scale[row] = qy.scale;
+      if (p.ckpt) {
+        p.ckpt_scale[row] = qh.scale;
+        p.rstd[row] = u;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      const int c = at(g);
+      if (c >= cols) continue;
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) y[e] = redo ? v[g][e] * u * w[g][e] : v[g][e] * w[g][e];
+      *reinterpret_cast<uint2*>(p.q + row * p.ldq + c) = quant_pack8(y, qy.inv);
+      if (p.ckpt) *reinterpret_cast<uint2*>(p.ckpt + row * p.ldk + c) = quant_pack8(v[g], qh.inv);
+      if (p.h) store8(static_cast<T*>(p.h) + row * p.ldh + c, v[g]);
     }
   }
 }
@@ -350,72 +477,67 @@ template <typename T, typename GT, int G> struct BackRow<T, GT, G, false> {
 // one's sum is joined, so a row is always on its way.
 template <typename T, typename GT, int G, bool VEC>
 __global__ void __launch_bounds__(512) norm_backward_kernel(BackArgs p) {
-  __shared__ float warp_sums[2][16];
+  __shared__ float4 stats[2][16];
   const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, per_block = blockDim.x / p.tpr;
   const int cols = int(p.cols);
   const T* wgt = static_cast<const T*>(p.weight);
   auto at = [&](int g, int e) { return VEC ? (g * p.tpr + t) * 8 + e : (g * 8 + e) * p.tpr + t; };
-  auto weight_of = [&](int g, float (&w)[8]) {
+  RowJoin join{stats, p.tpr, sub, 0};
+  // what fits the registers: the next row (up to 16 elements per thread, aligned), and
+  // the weights as f32 beside 16-bit rows; else the weights come from L1
+  constexpr bool kAhead = G <= 2 && VEC, kHold = G <= 2 && sizeof(T) == 2 && VEC;
+  float dw[G][8] = {}, held[kHold ? G : 1][8];
+  auto weight_of = [&](int i, float (&w)[8]) {
     if (VEC) {
       Vec8<T> a;
-      if (at(g, 0) < cols) a.load(wgt + at(g, 0)); else a.zero();
+      if (at(i, 0) < cols) a.load(wgt + at(i, 0)); else a.zero();
       a.get(w);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; e++) w[e] = at(g, e) < cols ? to_f32(wgt[at(g, e)]) : 0.f;
+      for (int e = 0; e < 8; e++) w[e] = at(i, e) < cols ? to_f32(wgt[at(i, e)]) : 0.f;
     }
   };
-  float dw[G][8] = {};
+  if constexpr (kHold) {
+#pragma unroll
+    for (int i = 0; i < G; i++) weight_of(i, held[i]);
+  }
   const float inv_cols = 1.f / float(cols);
-  const int64_t first = int64_t(blockIdx.x) * per_block;
+  const int64_t slot = int64_t(blockIdx.x) * per_block + sub;
   BackRow<T, GT, G, VEC> next;
-  if (first + sub < p.rows) next.load(p, first + sub, t);
-  int turn = 0;
-  // the same number of turns in every thread of the block: the sums synchronise
-  for (int64_t base = first; base < p.rows; base += p.slots, turn ^= 1) {
-    const int64_t row = base + sub;
-    const bool live = row < p.rows;
-    const BackRow<T, GT, G, VEC> cur = next;
-    if (row + p.slots < p.rows) next.load(p, row + p.slots, t);
+  int64_t row = slot;
+  if (kAhead && row < p.rows) next.load(p, row, t);
+  for (; row < p.rows; row += p.slots) {
+    if (!kAhead) next.load(p, row, t);
+    float gw[G][8], v[G][8];
+    const BackRow<T, GT, G, VEC> cur = next;   // of which grad_h is needed below
     const float u = cur.u, s = cur.s * u;
     float dot = 0.f;
-    if (live) {
 #pragma unroll
-      for (int i = 0; i < G; i++) {
-        float w[8], g[8], v[8];
-        weight_of(i, w);
-        cur.get(i, g, v);
+    for (int i = 0; i < G; i++) {
+      float g[8], w[8];
+      cur.get(i, g, v[i]);
+      if constexpr (!kHold) weight_of(i, w);
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          if (at(i, VEC ? 0 : e) < cols) {   // a NaN scale must not reach columns that are not there
-            v[e] *= s;
-            dw[i][e] = fmaf(g[e], v[e], dw[i][e]);
-            dot = fmaf(g[e] * w[e], v[e], dot);
-          }
+      for (int e = 0; e < 8; e++) {
+        gw[i][e] = 0.f;
+        if (at(i, VEC ? 0 : e) < cols) {   // a NaN scale must not reach columns that are not there
+          v[i][e] *= s;
+          dw[i][e] = fmaf(g[e], v[i][e], dw[i][e]);
+          gw[i][e] = g[e] * (kHold ? held[kHold ? i : 0][e] : w[e]);
+          dot = fmaf(gw[i][e], v[i][e], dot);
         }
       }
     }
+    if (kAhead && row + p.slots < p.rows) next.load(p, row + p.slots, t);
     if (!p.grad_x) continue;   // uniform over the grid
-#pragma unroll
-    for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-    if (p.tpr > 32) {   // two sets of sums in turn: one barrier per row
-      const int first_warp = sub * (p.tpr >> 5);
-      if ((threadIdx.x & 31) == 0) warp_sums[turn][threadIdx.x >> 5] = dot;
-      __syncthreads();
-      dot = warp_sums[turn][first_warp];
-      for (int w = 1; w < p.tpr >> 5; w++) dot += warp_sums[turn][first_warp + w];
-    }
-    const float mean = dot * inv_cols;
-    if (!live) continue;
+    const float mean = join(RowStats{dot, 0u, 0u}).sum * inv_cols;
     T* out = static_cast<T*>(p.grad_x) + row * p.ldx;
 #pragma unroll
     for (int i = 0; i < G; i++) {
-      float w[8], g[8], v[8], h[8], o[8];
-      weight_of(i, w);
-      cur.get(i, g, v);
+      float o[8], h[8];
       cur.get_h(i, h);
 #pragma unroll
-      for (int e = 0; e < 8; e++) o[e] = fmaf(u, g[e] * w[e] - v[e] * s * mean, h[e]);
+      for (int e = 0; e < 8; e++) o[e] = fmaf(u, fmaf(-mean, v[i][e], gw[i][e]), h[e]);
       if (VEC) {
         if (at(i, 0) < cols) store8(out + at(i, 0), o);
       } else {
@@ -425,7 +547,6 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(BackArgs p) {
       }
     }
   }
-  const int64_t slot = first + sub;
   if (p.partial && slot < p.slots) {
     float* o = p.partial + slot * p.cols;
 #pragma unroll
@@ -528,6 +649,23 @@ tg_status launch_rows(RowArgs p, bool vec, cudaStream_t st) {
     if (p.rows > kGridLimit) return fail(TG_ERR_UNSUPPORTED, "%lld rows", (long long)p.rows);
     tg8::rows_long_kernel<T, NORM><<<unsigned(p.rows), 1024, 0, st>>>(p);
     return check_launch("rows8");
+  }
+  if constexpr (NORM) {
+    // many aligned rows: persistent, 32 elements per thread (f32: 16, which
+    // holds 8192 columns).  8192 x 8192 bf16 with the checkpoint: 96 us, one
+    // row per block 124.  The plain quantisation has no weights to keep and
+    // gains nothing (46 us either way).
+    constexpr int kGroups = sizeof(T) == 4 ? 2 : 4;
+    if (vec && p.rows >= 4 * int64_t(sm_count()) && p.cols <= 512 * 8 * kGroups) {
+      const RowShape s = row_shape(p.rows, p.cols, kGroups, 512);
+      p.tpr = s.tpr;
+      const int per = s.block / s.tpr;
+      const int64_t blocks = std::min<int64_t>((p.rows + per - 1) / per, int64_t(sm_count()) * (512 / s.block));
+      if (s.groups == 1) tg8::norm_stream_kernel<T, 1><<<unsigned(blocks), s.block, 0, st>>>(p);
+      else if (s.groups == 2) tg8::norm_stream_kernel<T, 2><<<unsigned(blocks), s.block, 0, st>>>(p);
+      else if constexpr (kGroups == 4) tg8::norm_stream_kernel<T, 4><<<unsigned(blocks), s.block, 0, st>>>(p);
+      return check_launch("rows8");
+    }
   }
   const RowShape s = row_shape(p.rows, p.cols, 4, 1024);
   p.tpr = s.tpr;

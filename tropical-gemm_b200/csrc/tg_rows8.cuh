@@ -75,6 +75,13 @@ __device__ __forceinline__ void store8(f16* p, const float (&v)[8]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// max(|a|, |b|, m) that keeps a NaN.
+__device__ __forceinline__ float mag_max(float a, float b, float m) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(m));
+  return r;
+}
+
 // One row's quantisation from its largest magnitude, given as the maximum of
 // the values' bit patterns without the sign: unsigned order is magnitude
 // order, with infinities and NaN on top, so a maximum never loses a NaN.
