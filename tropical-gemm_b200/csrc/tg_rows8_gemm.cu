@@ -92,11 +92,15 @@ tg_status launch_product(const CUtensorMap& a, const CUtensorMap& b, ProductArgs
   const int most = std::max(1, sm_count() / 2), steps = p.blocks * p.planes;
   p.splits = 1;
   // Few tiles and a long sum: several pairs share a tile's sum and a second
-  // kernel joins the parts (~3 us).  4096 x 4096 weights, one token: 16.4 us
-  // whole, JOINED in four parts.
-  if (tm * tn * 2 <= most && steps >= 16) {
-    p.split_steps = std::max<int>(4, int((steps * tm * tn + most - 1) / most));
-    p.splits = (steps + p.split_steps - 1) / p.split_steps;
+  // kernel joins the parts.  A stage takes about 0.35 us (backward 0.5) when few
+  // pairs run; the parts cost their write and read and a launch.
+  if (tm * tn * 2 <= most) {
+    const int split_steps = std::max<int>(8, int((steps * tm * tn + most - 1) / most)), splits = (steps + split_steps - 1) / split_steps;
+    const double saved = (S::kBack ? 0.5 : 0.35) * (steps - split_steps), cost = 5.0 + 8e-6 * splits * double(p.m) * double(p.n) / 4.0;
+    if (splits > 1 && saved > cost) {
+      p.split_steps = split_steps;
+      p.splits = splits;
+    }
   }
   const int pairs = p.splits > 1 ? int(tm * tn) * p.splits : int(std::min<int64_t>(tm * tn, most));
   const int64_t couples = (tm / 2) * tn;
@@ -115,9 +119,13 @@ tg_status launch_product(const CUtensorMap& a, const CUtensorMap& b, ProductArgs
   return check_launch("rows8 product");
 }
 
-// Tokens per tile of the few-token kernel, or 0 for the paired one.
-int token_tile(int64_t m) {
-  return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 512 ? 128 : 0;
+// Tokens per tile of the few-token kernel, or 0 for the paired one.  Up to 64
+// tokens the weights' read decides (4096 x 4096, one token: 8.3 us, paired 18).
+// Above, the few-token kernel's split sum pays while the sum is long (256 tokens,
+// 4096 x 4096: 17.8 us, paired 28; 512 x 512: 12.3 against 8.2).
+int token_tile(int64_t m, int blocks) {
+  if (m > 64) return m <= 512 && blocks >= 24 ? 128 : 0;
+  return m <= 16 ? 16 : m <= 32 ? 32 : 64;
 }
 
 template <int NT, typename T>
@@ -189,7 +197,7 @@ tg_status tg_rows8_gemm(tg_dtype dtype, int64_t m, int64_t n, int64_t k, const i
   p.planes = 1;
   p.blocks = std::max(1, int((k + 127) / 128));
   CUtensorMap ma, mb;
-  const int nt = token_tile(m);
+  const int nt = token_tile(m, p.blocks);
   if (!oa.map(128, nt ? nt : 128, &ma) || !ob.map(128, 128, &mb)) return fail(TG_ERR_CUDA, "rows8 gemm: tensor map encoding failed");
   return with_type8(dtype, [&](auto t) {
     using T = decltype(t);
