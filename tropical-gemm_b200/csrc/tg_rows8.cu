@@ -55,6 +55,7 @@ __device__ __forceinline__ uint32_t mag_bits(float v) { return __float_as_uint(v
 template <typename T, int G, bool VEC, bool NORM>
 __global__ void __launch_bounds__(G == 1 ? 1024 : 512) rows_kernel(RowArgs p) {
   __shared__ RowStats warp_stats[32];
+  after_previous_kernel();
   const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, per_block = blockDim.x / p.tpr;
   const int64_t row = int64_t(blockIdx.x) * per_block + sub;
   const bool live = row < p.rows;
@@ -226,6 +227,7 @@ struct RowJoin {
 template <typename T, int G>
 __global__ void __launch_bounds__(512) norm_stream_kernel(RowArgs p) {
   __shared__ float4 stats[2][16];
+  after_previous_kernel();
   const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, per_block = blockDim.x / p.tpr;
   const int cols = int(p.cols);
   auto at = [&](int g) { return (g * p.tpr + t) * 8; };
@@ -320,6 +322,7 @@ __global__ void __launch_bounds__(512) norm_stream_kernel(RowArgs p) {
 template <typename T, bool NORM>
 __global__ void __launch_bounds__(1024) rows_long_kernel(RowArgs p) {
   __shared__ RowStats warp_stats[32];
+  after_previous_kernel();
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.ldr : nullptr;
@@ -361,6 +364,7 @@ __global__ void __launch_bounds__(1024) rows_long_kernel(RowArgs p) {
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dequantize_kernel(int64_t rows, int64_t cols, const int8_t* q, int64_t ldq,
                                                          const float* scale, T* y, int64_t ldy) {
+  after_previous_kernel();
   const int64_t per = VEC ? cols / 16 : cols, total = rows * per;
   const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (i >= total) return;
@@ -478,6 +482,7 @@ template <typename T, typename GT, int G> struct BackRow<T, GT, G, false> {
 template <typename T, typename GT, int G, bool VEC>
 __global__ void __launch_bounds__(512) norm_backward_kernel(BackArgs p) {
   __shared__ float4 stats[2][16];
+  after_previous_kernel();
   const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, per_block = blockDim.x / p.tpr;
   const int cols = int(p.cols);
   const T* wgt = static_cast<const T*>(p.weight);
@@ -566,6 +571,7 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(BackArgs p) {
 template <typename T, typename GT>
 __global__ void __launch_bounds__(1024) norm_backward_long_kernel(BackArgs p) {
   __shared__ float warp_sums[32];
+  after_previous_kernel();
   const int64_t row = blockIdx.x;
   const float u = p.rstd[row], s = p.ckpt_scale[row] * u;
   const GT* grad = static_cast<const GT*>(p.grad) + row * p.ldg;
@@ -587,6 +593,7 @@ template <typename GT>
 __global__ void __launch_bounds__(256) column_partial_kernel(int64_t rows, int64_t cols, const GT* x, int64_t ldx,
                                                              const int8_t* ckpt, int64_t ldk, const float* ckpt_scale,
                                                              const float* rstd, float* partial) {
+  after_previous_kernel();
   const int64_t c = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (c >= cols) return;
   float s = 0.f;
@@ -602,6 +609,7 @@ __global__ void __launch_bounds__(256) column_partial_kernel(int64_t rows, int64
 template <typename T>
 __global__ void __launch_bounds__(256) column_join_kernel(int64_t slots, int64_t cols, const float* partial, T* out) {
   __shared__ float part[8][33];
+  after_previous_kernel();
   const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int64_t c = int64_t(blockIdx.x) * 32 + lane;
   float s = 0.f;
@@ -647,7 +655,7 @@ template <typename T, bool NORM>
 tg_status launch_rows(RowArgs p, bool vec, cudaStream_t st) {
   if (p.cols > kRowLimit) {
     if (p.rows > kGridLimit) return fail(TG_ERR_UNSUPPORTED, "%lld rows", (long long)p.rows);
-    tg8::rows_long_kernel<T, NORM><<<unsigned(p.rows), 1024, 0, st>>>(p);
+    launch_kernel(tg8::rows_long_kernel<T, NORM>, unsigned(p.rows), 1024, 0, 0, st, p);
     return check_launch("rows8");
   }
   if constexpr (NORM) {
@@ -661,9 +669,9 @@ tg_status launch_rows(RowArgs p, bool vec, cudaStream_t st) {
       p.tpr = s.tpr;
       const int per = s.block / s.tpr;
       const int64_t blocks = std::min<int64_t>((p.rows + per - 1) / per, int64_t(sm_count()) * (512 / s.block));
-      if (s.groups == 1) tg8::norm_stream_kernel<T, 1><<<unsigned(blocks), s.block, 0, st>>>(p);
-      else if (s.groups == 2) tg8::norm_stream_kernel<T, 2><<<unsigned(blocks), s.block, 0, st>>>(p);
-      else if constexpr (kGroups == 4) tg8::norm_stream_kernel<T, 4><<<unsigned(blocks), s.block, 0, st>>>(p);
+      if (s.groups == 1) launch_kernel(tg8::norm_stream_kernel<T, 1>, unsigned(blocks), s.block, 0, 0, st, p);
+      else if (s.groups == 2) launch_kernel(tg8::norm_stream_kernel<T, 2>, unsigned(blocks), s.block, 0, 0, st, p);
+      else if constexpr (kGroups == 4) launch_kernel(tg8::norm_stream_kernel<T, 4>, unsigned(blocks), s.block, 0, 0, st, p);
       return check_launch("rows8");
     }
   }
@@ -674,9 +682,9 @@ tg_status launch_rows(RowArgs p, bool vec, cudaStream_t st) {
   if (grid > kGridLimit) return fail(TG_ERR_UNSUPPORTED, "%lld rows", (long long)p.rows);
   auto go = [&](auto vec_c) {
     constexpr bool V = decltype(vec_c)::value;
-    if (s.groups == 1) tg8::rows_kernel<T, 1, V, NORM><<<unsigned(grid), s.block, 0, st>>>(p);
-    else if (s.groups == 2) tg8::rows_kernel<T, 2, V, NORM><<<unsigned(grid), s.block, 0, st>>>(p);
-    else tg8::rows_kernel<T, 4, V, NORM><<<unsigned(grid), s.block, 0, st>>>(p);
+    if (s.groups == 1) launch_kernel(tg8::rows_kernel<T, 1, V, NORM>, unsigned(grid), s.block, 0, 0, st, p);
+    else if (s.groups == 2) launch_kernel(tg8::rows_kernel<T, 2, V, NORM>, unsigned(grid), s.block, 0, 0, st, p);
+    else launch_kernel(tg8::rows_kernel<T, 4, V, NORM>, unsigned(grid), s.block, 0, 0, st, p);
   };
   if (vec) go(std::true_type{}); else go(std::false_type{});
   return check_launch("rows8");
@@ -698,23 +706,22 @@ tg_status launch_norm_backward(BackArgs p, T* grad_w, bool vec, cudaStream_t st)
     p.partial = static_cast<float*>(scratch);
   }
   if (lng) {
-    if (p.grad_x && p.rows) tg8::norm_backward_long_kernel<T, GT><<<unsigned(p.rows), 1024, 0, st>>>(p);
+    if (p.grad_x && p.rows) launch_kernel(tg8::norm_backward_long_kernel<T, GT>, unsigned(p.rows), 1024, 0, 0, st, p);
     if (grad_w)
-      tg8::column_partial_kernel<GT><<<dim3(unsigned((p.cols + 255) / 256), unsigned(p.slots)), 256, 0, st>>>(
-          p.rows, p.cols, static_cast<const GT*>(p.grad), p.ldg, p.ckpt, p.ldk, p.ckpt_scale, p.rstd, p.partial);
+      launch_kernel(tg8::column_partial_kernel<GT>, dim3(unsigned((p.cols + 255) / 256), unsigned(p.slots)), 256, 0, 0, st, p.rows, p.cols, static_cast<const GT*>(p.grad), p.ldg, p.ckpt, p.ldk, p.ckpt_scale, p.rstd, p.partial);
   } else {
     auto go = [&](auto vec_c) {
       constexpr bool V = decltype(vec_c)::value;
-      if (s.groups == 1) tg8::norm_backward_kernel<T, GT, 1, V><<<unsigned(blocks), s.block, 0, st>>>(p);
-      else if (s.groups == 2) tg8::norm_backward_kernel<T, GT, 2, V><<<unsigned(blocks), s.block, 0, st>>>(p);
-      else tg8::norm_backward_kernel<T, GT, 4, V><<<unsigned(blocks), s.block, 0, st>>>(p);
+      if (s.groups == 1) launch_kernel(tg8::norm_backward_kernel<T, GT, 1, V>, unsigned(blocks), s.block, 0, 0, st, p);
+      else if (s.groups == 2) launch_kernel(tg8::norm_backward_kernel<T, GT, 2, V>, unsigned(blocks), s.block, 0, 0, st, p);
+      else launch_kernel(tg8::norm_backward_kernel<T, GT, 4, V>, unsigned(blocks), s.block, 0, 0, st, p);
     };
     if (vec) go(std::true_type{}); else go(std::false_type{});
   }
   tg_status r = check_launch("rows8 norm backward");
   if (grad_w) {
     if (r == TG_OK) {
-      tg8::column_join_kernel<T><<<unsigned((p.cols + 31) / 32), 256, 0, st>>>(p.slots, p.cols, p.partial, grad_w);
+      launch_kernel(tg8::column_join_kernel<T>, unsigned((p.cols + 31) / 32), 256, 0, 0, st, p.slots, p.cols, p.partial, grad_w);
       r = check_launch("rows8 norm backward");
     }
     scratch_free(scratch, st);
@@ -780,8 +787,8 @@ tg_status tg_rows8_dequantize(tg_dtype dtype, int64_t rows, int64_t cols, const 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return with_type8(dtype, [&](auto t) {
     using T = decltype(t);
-    if (vec) tg8::dequantize_kernel<T, true><<<grid, 256, 0, st>>>(rows, cols, q, ldq, scale, static_cast<T*>(y), ldy);
-    else tg8::dequantize_kernel<T, false><<<grid, 256, 0, st>>>(rows, cols, q, ldq, scale, static_cast<T*>(y), ldy);
+    if (vec) launch_kernel(tg8::dequantize_kernel<T, true>, grid, 256, 0, 0, st, rows, cols, q, ldq, scale, static_cast<T*>(y), ldy);
+    else launch_kernel(tg8::dequantize_kernel<T, false>, grid, 256, 0, 0, st, rows, cols, q, ldq, scale, static_cast<T*>(y), ldy);
     return check_launch("rows8 dequantize");
   });
 }
@@ -870,14 +877,13 @@ tg_status tg_rows8_column_sum(tg_dtype dtype, tg_dtype out_dtype, int64_t rows, 
   float* partial = static_cast<float*>(scratch);
   tg_status r = with_type8(dtype, [&](auto t) {
     using T = decltype(t);
-    tg8::column_partial_kernel<T><<<dim3(unsigned(strips), unsigned(slots)), 256, 0, st>>>(
-        rows, cols, static_cast<const T*>(x), ldx, nullptr, 0, nullptr, nullptr, partial);
+    launch_kernel(tg8::column_partial_kernel<T>, dim3(unsigned(strips), unsigned(slots)), 256, 0, 0, st, rows, cols, static_cast<const T*>(x), ldx, nullptr, 0, nullptr, nullptr, partial);
     return check_launch("rows8 column sum");
   });
   if (r == TG_OK)
     r = with_type8(out_dtype, [&](auto t) {
       using T = decltype(t);
-      tg8::column_join_kernel<T><<<unsigned((cols + 31) / 32), 256, 0, st>>>(slots, cols, partial, static_cast<T*>(out));
+      launch_kernel(tg8::column_join_kernel<T>, unsigned((cols + 31) / 32), 256, 0, 0, st, slots, cols, partial, static_cast<T*>(out));
       return check_launch("rows8 column sum");
     });
   scratch_free(scratch, st);

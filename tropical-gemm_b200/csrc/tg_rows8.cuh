@@ -126,9 +126,36 @@ __device__ __forceinline__ void bytes_f32(uint2 w, float (&v)[8]) {
   v[4] = byte_f32<0>(b); v[5] = byte_f32<1>(b); v[6] = byte_f32<2>(b); v[7] = byte_f32<3>(b);
 }
 
+// Kernels of these calls are launched with programmatic stream serialisation:
+// a kernel may be set up while the one before it ends, waits here before it
+// touches global memory until that one is complete, and lets the next one be
+// set up.  (norm, product: about 1 us less between two kernels.)
+__device__ __forceinline__ void after_previous_kernel() {
+  asm volatile("griddepcontrol.wait;\ngriddepcontrol.launch_dependents;" ::: "memory");
+}
+
 }  // namespace tg8
 
 namespace tgi {
+
+// A launch of one of these kernels; clusters of `cluster` blocks along x.
+// Errors are left to check_launch.
+template <typename... P, typename... A>
+void launch_kernel(void (*kern)(P...), dim3 grid, int block, size_t smem, int cluster, cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(block));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {unsigned(cluster), 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster ? 2 : 1;   // 0: the kernel's own cluster size, if any
+  (void)cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+}
 
 inline size_t elem8_size(tg_dtype t) { return t == TG_F32 ? 4 : (t == TG_BF16 || t == TG_F16) ? 2 : 0; }
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }

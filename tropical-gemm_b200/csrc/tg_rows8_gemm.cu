@@ -74,7 +74,7 @@ struct Operand8 {
 void pad_operands(const tg8::PadArgs& p, int count, cudaStream_t st) {
   int64_t most = 0;
   for (int i = 0; i < count; i++) most = std::max(most, (p.rows[i] * (p.ldo[i] / 16) + 255) / 256);
-  if (most) tg8::pad8_kernel<<<dim3(unsigned(std::min<int64_t>(most, 8192)), 1, unsigned(count)), 256, 0, st>>>(p);
+  if (most) launch_kernel(tg8::pad8_kernel, dim3(unsigned(std::min<int64_t>(most, 8192)), 1, unsigned(count)), 256, 0, 0, st, p);
 }
 
 template <int MODE, typename T>
@@ -114,8 +114,8 @@ tg_status launch_product(const CUtensorMap& a, const CUtensorMap& b, ProductArgs
     if (e != cudaSuccess) return fail(TG_ERR_CUDA, "rows8 product scratch: %s", cudaGetErrorString(e));
     p.part = scratch.take<uint32_t>(count);
   }
-  kern<<<2 * pairs, S::kThreads, S::kSmem, st>>>(a, b, p);
-  if (p.splits > 1) tg8::join_kernel<MODE == tg8::kForward, T><<<row_grid(1024, p.n, p.m), 256, 0, st>>>(p);
+  launch_kernel(kern, 2 * pairs, S::kThreads, S::kSmem, 0, st, a, b, p);
+  if (p.splits > 1) launch_kernel(tg8::join_kernel<MODE == tg8::kForward, T>, row_grid(1024, p.n, p.m), 256, 0, 0, st, p);
   return check_launch("rows8 product");
 }
 
@@ -143,22 +143,8 @@ tg_status launch_tokens(const CUtensorMap& tokens, const CUtensorMap& weights, P
   auto kern = tg8::tokens_kernel<NT, T>;
   const tg_status s = ensure_smem(reinterpret_cast<const void*>(kern), size_t(S::kMost) * S::kStage + S::kExchange + 1024);
   if (s != TG_OK) return s;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(tiles * split), unsigned(tt));
-  cfg.blockDim = dim3(128);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {unsigned(split), 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tokens, weights, p, split, stages);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return fail(TG_ERR_CUDA, "rows8 gemm: %s", cudaGetErrorString(e));
-  }
-  return TG_OK;
+  launch_kernel(kern, dim3(unsigned(tiles * split), unsigned(tt)), 128, smem, split, st, tokens, weights, p, split, stages);
+  return check_launch("rows8 gemm");
 }
 
 }  // namespace tgi
@@ -254,7 +240,7 @@ tg_status tg_rows8_gemm_backward(tg_dtype grad_dtype, tg_dtype out_dtype, int tr
     tg8::bf16* parts = scratch.take<tg8::bf16>(part_count);
     const tg_status s = with_type8(grad_dtype, [&](auto t) {
       using T = decltype(t);
-      tg8::split_kernel<T><<<row_grid(256, ldp, g_rows), 256, 0, st>>>(g_rows, g_cols, static_cast<const T*>(g), ldg,
+      launch_kernel(tg8::split_kernel<T>, row_grid(256, ldp, g_rows), 256, 0, 0, st, g_rows, g_cols, static_cast<const T*>(g), ldg,
                                                                         planes > 1 ? scale : nullptr, transposed != 0, parts, ldp, planes);
       return check_launch("rows8 gemm backward");
     });

@@ -263,6 +263,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     umma::bar_init_fence();
   }
   if (warp == 2) umma::tmem_alloc<2>(base + S::kOffSlot, 512);
+  after_previous_kernel();
   umma::fence_before();
   umma::cluster_sync();
   umma::fence_after();
@@ -552,6 +553,7 @@ __global__ void __launch_bounds__(128) tokens_kernel(const __grid_constant__ CUt
     umma::bar_init_fence();
   }
   if (warp == 2) umma::tmem_alloc<1>(umma::smem_u32(&slot), S::kColumns);
+  after_previous_kernel();
   umma::fence_before();
   __syncthreads();
   umma::fence_after();
@@ -669,6 +671,7 @@ __global__ void __launch_bounds__(128) tokens_kernel(const __grid_constant__ CUt
 // and bias, backward f32 sums.  Four columns per thread.
 template <bool FORWARD, typename T>
 __global__ void __launch_bounds__(256) join_kernel(const ProductArgs p) {
+  after_previous_kernel();
   const int64_t c0 = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4;
   if (c0 >= p.n) return;
   for (int64_t row = blockIdx.y; row < p.m; row += gridDim.y) {
@@ -705,6 +708,7 @@ __global__ void __launch_bounds__(256) join_kernel(const ProductArgs p) {
 template <typename GT>
 __global__ void __launch_bounds__(256) split_kernel(int64_t rows, int64_t cols, const GT* g, int64_t ldg, const float* scale,
                                                     int scale_rows, bf16* out, int64_t ldo, int planes) {
+  after_previous_kernel();
   const int64_t c = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (c >= ldo) return;
   for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
@@ -732,6 +736,7 @@ struct PadArgs {
   int64_t rows[2], cols[2], ldq[2], ldo[2];
 };
 __global__ void __launch_bounds__(256) pad8_kernel(const PadArgs p) {
+  after_previous_kernel();
   const int z = blockIdx.z;
   const int64_t per = p.ldo[z] / 16, total = p.rows[z] * per;
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
