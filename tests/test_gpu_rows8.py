@@ -451,6 +451,13 @@ def test_autograd_partial_needs_and_frozen_weight():
     assert torch.equal(z, z2) and not z2.requires_grad
 
 
+def test_autograd_refuses_a_second_derivative():
+    x = torch.randn(4, 32, device="cuda", requires_grad=True)
+    z, _ = tp.rmsnorm_linear_rows8(x, torch.ones(32, device="cuda"), torch.randn(8, 32, device="cuda"))
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(z.sum(), x, create_graph=True)
+
+
 def test_linear_gradient_against_differences():
     """z is bilinear in the held values: differences are exact up to rounding."""
     g = gen(8)

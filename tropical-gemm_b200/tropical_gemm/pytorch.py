@@ -177,59 +177,18 @@ def tropical_maxmul_matmul_batched(a: torch.Tensor, b: torch.Tensor) -> torch.Te
     return TropicalMaxMulMatmulBatched.apply(a, b)
 
 
-class RMSNormLinearRows8(torch.autograd.Function):
-    """norm of x + residual -> linear, both in 8-bit rows.  What is kept for
-    the backward is 8-bit: the normalised activations (the product's own
-    operand), h, and the weight's rows."""
-
-    @staticmethod
-    def forward(ctx, x, norm_weight, weight, weight_scale, residual, bias, eps):
-        kept = weight_scale is None   # a float weight: quantised here, and it has a gradient
-        train = any(ctx.needs_input_grad)
-        r = rows8.rmsnorm(x, norm_weight, residual, eps, checkpoint=train)
-        b = rows8.quantize(weight) if kept else rows8.Rows8(weight, weight_scale)
-        z = rows8.matmul(r.rows, b, bias, x.dtype)
-        if train:
-            ctx.save_for_backward(*r.rows, *r.checkpoint, r.rstd, *b, norm_weight)
-        ctx.set_materialize_grads(False)
-        if residual is None:
-            return z, x.view_as(x)   # an output must not be the input itself
-        return z, r.h
-
-    @staticmethod
-    def backward(ctx, grad_z, grad_h):
-        aq, a_scale, hq, h_scale, rstd, bq, b_scale, norm_weight = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        grad_x = grad_norm = grad_w = grad_bias = None
-        if grad_z is not None:
-            norm = need[0] or need[1] or need[4]
-            # the norm's incoming gradient stays float32: one rounding less, at its output
-            grad_y, grad_w = rows8.matmul_backward(
-                grad_z, rows8.Rows8(aq, a_scale) if need[2] else None, rows8.Rows8(bq, b_scale) if norm else None,
-                dtype_a=torch.float32)
-            if norm:
-                grad_x, grad_norm = rows8.rmsnorm_backward(grad_y, rows8.Rows8(hq, h_scale), rstd, norm_weight, grad_h)
-            if need[5]:
-                grad_bias = rows8.column_sum(grad_z)
-        elif grad_h is not None:
-            grad_x = grad_h
-        return (grad_x if need[0] else None, grad_norm if need[1] else None, grad_w, None, grad_x if need[4] else None,
-                grad_bias, None)
-
-
 def rmsnorm_linear_rows8(x: torch.Tensor, norm_weight: torch.Tensor, weight, residual=None, bias=None, eps: float = 1e-6):
     """(z, h): h = x + residual, z = rmsnorm(h) weight^T + bias, the norm's
     output and the weight in 8-bit rows, with autograd.
 
     `weight` is a (N, K) tensor of x's type, quantised at every call, or
-    `rows8.Rows8` (frozen: no gradient).  Gradients are those of the product
-    of the 8-bit values, passed straight through the rounding.  CUDA tensors
-    of float32, float16 or bfloat16."""
-    if isinstance(weight, rows8.Rows8):
-        return RMSNormLinearRows8.apply(x, norm_weight, weight.q, weight.scale, residual, bias, eps)
-    if weight.dtype != x.dtype or weight.dim() != 2:
-        raise ValueError(f"weight must be a two-dimensional {x.dtype} tensor or Rows8, got {weight.dtype} {tuple(weight.shape)}")
-    return RMSNormLinearRows8.apply(x, norm_weight, weight, None, residual, bias, eps)
+    `rows8.Rows8` (frozen: no gradient).  Between forward and backward only
+    8-bit rows are kept (the norm's output, h, the weight).  Gradients are those
+    of the product of the 8-bit values, passed straight through the rounding;
+    they cannot be differentiated again.  CUDA tensors of float32, float16 or
+    bfloat16."""
+    w, w_scale = weight if isinstance(weight, rows8.Rows8) else (weight, None)
+    return rows8._x().rmsnorm_linear(x, norm_weight, w, w_scale, residual, bias, eps)
 
 
 __all__ = [
@@ -239,6 +198,6 @@ __all__ = [
     "tropical_maxplus_matmul", "tropical_minplus_matmul", "tropical_maxmul_matmul",
     "tropical_maxplus_matmul_gpu", "tropical_minplus_matmul_gpu", "tropical_maxmul_matmul_gpu",
     "tropical_maxplus_matmul_batched", "tropical_minplus_matmul_batched", "tropical_maxmul_matmul_batched",
-    "RMSNormLinearRows8", "rmsnorm_linear_rows8",
+    "rmsnorm_linear_rows8",
     "GPU_AVAILABLE", "_DLPACK_AVAILABLE",
 ]
