@@ -369,6 +369,33 @@ def test_matmul_backward_strides_and_none(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_matmul_backward_of_nothing(dtype):
+    """Sums of no terms are zero, outputs of no rows or columns are empty."""
+    g = gen(1)
+    ga, gb = rows8.matmul_backward(randn(g, 5, 0, dtype=dtype), rand8(g, 5, 8), rand8(g, 0, 8))
+    assert ga.shape == (5, 8) and not ga.any() and gb.shape == (0, 8)
+    ga, gb = rows8.matmul_backward(randn(g, 0, 6, dtype=dtype), rand8(g, 0, 8), rand8(g, 6, 8))
+    assert ga.shape == (0, 8) and gb.shape == (6, 8) and not gb.any()
+    ga, gb = rows8.matmul_backward(randn(g, 5, 6, dtype=dtype), rand8(g, 5, 0), rand8(g, 6, 0))
+    assert ga.shape == (5, 0) and gb.shape == (6, 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_matmul_backward_of_a_long_sum(dtype):
+    """A sum over two million rows, few outputs and many."""
+    g = gen(6)
+    r = 2_000_003
+    a = Rows8(torch.randint(-127, 128, (r, 24), generator=g, device="cuda", dtype=torch.int8), torch.full((r,), 2.0 ** -9, device="cuda"))
+    grad = randn(g, r, 8, dtype=dtype)
+    _, gb = rows8.matmul_backward(grad, a, None, dtype_b=torch.float32)
+    v = values(a)
+    want, mag = grad.double().t() @ v, grad.double().abs().t() @ v.abs()
+    # power-of-two scales: the bf16 factors are exact.  Sums of 2e6 terms with a
+    # rounding or truncation each 16 terms
+    assert_near(gb, want, mag * (2.0 ** -22 + r / 16 * 2 * U))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_matmul_backward_non_finite(dtype):
     """A NaN gradient reaches what it is a factor of, and nothing else."""
     g = gen(2)

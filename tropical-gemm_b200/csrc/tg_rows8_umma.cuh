@@ -383,7 +383,11 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (row < p.m) rs = p.row_scale[row];
       }
-      if (ok && !umma::bar_wait(acc_full(buf), (n >> 1) & 1)) ok = false;
+      if (ok) {   // a whole tile's sum: the limit grows with its length
+        bool done = false;
+        for (int k = 0; k <= steps >> 10 && !done; k++) done = umma::bar_wait(acc_full(buf), (n >> 1) & 1);
+        ok = done;
+      }
       umma::fence_after();
       const uint32_t from = tmem + buf * kTile + half * 128 + (uint32_t(w * 32) << 16);
       const int64_t col0 = n0 + half * 128;
