@@ -128,6 +128,45 @@ def test_rmsnorm(dtype, rows, cols, with_residual):
     assert torch.equal(plain.rows.q, n.rows.q) and torch.equal(plain.rows.scale, n.rows.scale)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, cols, ld, first", [(700, 13, 13, 0), (900, 1001, 1001, 0), (650, 8185, 8185, 0), (600, 16380, 16380, 0),
+                                                   (800, 250, 264, 0), (800, 250, 264, 3), (800, 256, 264, 5), (20, 77, 81, 2), (5, 3, 9, 4)])
+def test_rows_that_start_anywhere(dtype, rows, cols, ld, first):
+    """Rows off the 16-byte boundaries, all operands alike or not, against the same rows packed."""
+    g = gen(rows + cols)
+
+    def view(t):   # the same values at an offset inside a wider matrix
+        wide = torch.full((rows, ld), float("nan"), device="cuda", dtype=torch.float32).to(t.dtype)
+        wide[:, first:first + cols] = t
+        return wide[:, first:first + cols]
+
+    x, res, gr, w = (randn(g, *s, dtype=dtype) for s in ((rows, cols), (rows, cols), (rows, cols), (cols,)))
+    x[::7] = 0
+    res[::7] = 0
+    n = rows8.rmsnorm(x, w, residual=res, checkpoint=True, eps=1e-5)
+    h = (x.float() + res.float()).double()
+    u = (h.square().mean(-1) + 1e-5).rsqrt()
+    check_rows(n.rows, h * u[:, None] * w.double(), (0.5 * 128 + 6) * U)
+    check_rows(n.checkpoint, h, 0.0)
+    assert torch.equal(n.h, (x.float() + res.float()).to(dtype))
+    m = rows8.rmsnorm(view(x), w, residual=view(res), checkpoint=True, eps=1e-5)
+    for a, b in ((n.rows, m.rows), (n.checkpoint, m.checkpoint)):
+        assert_near(values(a), values(b), 1.001 * a.scale.double()[:, None])   # a step at most: the sums' order may differ
+    check_rows(rows8.quantize(view(x)), x.double(), 0.0)
+    d = Rows8(n.rows.q, n.rows.scale)
+    assert torch.equal(rows8.dequantize(Rows8(view(d.q.float()).to(torch.int8), d.scale), dtype), rows8.dequantize(d, dtype))
+    dx, dw = rows8.rmsnorm_backward(gr, n.checkpoint, n.rstd, w, grad_h=res)
+    dx2, dw2 = rows8.rmsnorm_backward(view(gr), n.checkpoint, n.rstd, w, grad_h=view(res))
+    v, ud = values(n.checkpoint) * n.rstd.double()[:, None], n.rstd.double()[:, None]
+    G, W, H = gr.double(), w.double(), res.double()
+    want_x, want_w = norm_gradients(G, v, ud[:, 0], W, H)
+    c_abs = (G * W * v).abs().mean(-1, keepdim=True)
+    tol = 8 * U * (ud * (G * W).abs() + ud * v.abs() * c_abs + H.abs()) + ud * v.abs() * c_abs * 140 * U
+    for a, b in ((dx, dw), (dx2, dw2)):
+        assert_near(a, want_x, tol + want_x.abs() * OUT[dtype] + TINY[dtype])
+        assert_near(b, want_w, (G * v).abs().sum(0) * (rows + 12) * U + want_w.abs() * OUT[dtype] + TINY[dtype])
+
+
 def test_rmsnorm_of_zero_huge_and_non_finite_rows():
     x = torch.ones(6, 64, device="cuda")
     x[1] = 0

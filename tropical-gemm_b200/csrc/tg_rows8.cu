@@ -49,10 +49,9 @@ __device__ __forceinline__ RowStats row_reduce(RowStats s, int tpr, RowStats* wa
 __device__ __forceinline__ uint32_t mag_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // One row per tpr threads, G groups of 8 elements per thread held in f32
-// registers.  VEC: 16-byte accesses; otherwise element by element, any
-// alignment.  NORM: root-mean-square norm (and the checkpoint when asked
-// for); otherwise the plain quantisation.
-template <typename T, int G, bool VEC, bool NORM>
+// registers.  NORM: root-mean-square norm (and the checkpoint when asked for);
+// otherwise the plain quantisation.
+template <typename T, int G, int ACCESS, bool NORM>
 __global__ void __launch_bounds__(G == 1 ? 1024 : 512) rows_kernel(RowArgs p) {
   __shared__ RowStats warp_stats[32];
   after_previous_kernel();
@@ -62,17 +61,19 @@ __global__ void __launch_bounds__(G == 1 ? 1024 : 512) rows_kernel(RowArgs p) {
   const T* x = static_cast<const T*>(p.x) + (live ? row : 0) * p.ldx;
   const T* res = p.residual ? static_cast<const T*>(p.residual) + (live ? row : 0) * p.ldr : nullptr;
   const T* wgt = static_cast<const T*>(p.weight);
-  const int cols = int(p.cols);
-  auto at = [&](int g, int e) { return VEC ? (g * p.tpr + t) * 8 + e : (g * 8 + e) * p.tpr + t; };
+  const int cols = int(p.cols), shift = ACCESS == kShifted ? row_shift(x) : 0;
+  auto at = [&](int g, int e) { return ACCESS == kScalar ? (g * 8 + e) * p.tpr + t : (g * p.tpr + t) * 8 + e - shift; };
+  auto inside = [&](int g, int e) { return at(g, e) < cols && (ACCESS != kShifted || at(g, e) >= 0); };
 
   float v[G][8];
-  if (VEC) {
+  if constexpr (ACCESS != kScalar) {
     Vec8<T> a[G], b[G];
 #pragma unroll
     for (int g = 0; g < G; g++) {
-      const bool in = live && at(g, 0) < cols;
-      if (in) a[g].load(x + at(g, 0)); else a[g].zero();
-      if (NORM && res && in) b[g].load(res + at(g, 0)); else b[g].zero();
+      a[g].zero();
+      b[g].zero();
+      if (live) load_group<ACCESS>(a[g], x, at(g, 0), cols);
+      if (NORM && res && live) load_group<ACCESS>(b[g], res, at(g, 0), cols);
     }
 #pragma unroll
     for (int g = 0; g < G; g++) {
@@ -97,13 +98,13 @@ __global__ void __launch_bounds__(G == 1 ? 1024 : 512) rows_kernel(RowArgs p) {
   }
 
   auto weight_of = [&](int g, float (&w)[8]) {
-    if (VEC) {
+    if constexpr (ACCESS == kAligned) {
       Vec8<T> a;
-      if (at(g, 0) < cols) a.load(wgt + at(g, 0)); else a.zero();
+      load_group<ACCESS>(a, wgt, at(g, 0), cols);
       a.get(w);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; e++) w[e] = at(g, e) < cols ? to_f32(wgt[at(g, e)]) : 0.f;
+      for (int e = 0; e < 8; e++) w[e] = inside(g, e) ? to_f32(wgt[at(g, e)]) : 0.f;
     }
   };
 
@@ -142,8 +143,7 @@ __global__ void __launch_bounds__(G == 1 ? 1024 : 512) rows_kernel(RowArgs p) {
         weight_of(g, w);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          const int c = at(g, VEC ? 0 : e);
-          if (c < cols) r.top_y = max(r.top_y, mag_bits(v[g][e] * u * w[e]));
+          if (inside(g, e)) r.top_y = max(r.top_y, mag_bits(v[g][e] * u * w[e]));
         }
       }
       r = row_reduce(r, p.tpr, warp_stats);
@@ -172,13 +172,11 @@ __global__ void __launch_bounds__(G == 1 ? 1024 : 512) rows_kernel(RowArgs p) {
     if (NORM) weight_of(g, w);
 #pragma unroll
     for (int e = 0; e < 8; e++) y[e] = NORM ? v[g][e] * u * w[e] : v[g][e];
-    if (VEC) {
+    if constexpr (ACCESS != kScalar) {
       const int c = at(g, 0);
-      if (c < cols) {
-        *reinterpret_cast<uint2*>(q + c) = quant_pack8(y, qy.inv);
-        if (NORM && k) *reinterpret_cast<uint2*>(k + c) = quant_pack8(v[g], qh.inv);
-        if (NORM && p.h) store8(h + c, v[g]);
-      }
+      store_bytes<ACCESS>(q, c, cols, quant_pack8(y, qy.inv));
+      if (NORM && k) store_bytes<ACCESS>(k, c, cols, quant_pack8(v[g], qh.inv));
+      if (NORM && p.h) store_group<ACCESS>(h, c, cols, v[g]);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; e++) {
@@ -224,28 +222,36 @@ struct RowJoin {
 // row is on its way while this one is worked on.  The kernel above is bound by
 // instructions (78 % of the issue slots for 4096 x 8192 bf16, weights unpacked
 // twice per row); this one needs about half of them.
-template <typename T, int G>
+// Rows that start anywhere take their weights from shared memory instead.
+template <typename T, int G, int ACCESS>
 __global__ void __launch_bounds__(512) norm_stream_kernel(RowArgs p) {
+  extern __shared__ float shared_weight[];   // kShifted
   __shared__ float4 stats[2][16];
   after_previous_kernel();
   const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, per_block = blockDim.x / p.tpr;
   const int cols = int(p.cols);
-  auto at = [&](int g) { return (g * p.tpr + t) * 8; };
+  int shift = 0;   // of the row being loaded
+  auto at = [&](int g) { return (g * p.tpr + t) * 8 - shift; };
   RowJoin join{stats, p.tpr, sub, 0};
   float w[G][8];
   Vec8<T> nx[G], nr[G];
-  const T *x = static_cast<const T*>(p.x), *res = static_cast<const T*>(p.residual);
-#pragma unroll
-  for (int g = 0; g < G; g++) {
-    if (at(g) < cols) nx[g].load(static_cast<const T*>(p.weight) + at(g)); else nx[g].zero();
-    nx[g].get(w[g]);
-  }
-  auto load = [&](int64_t row) {
+  const T *x = static_cast<const T*>(p.x), *res = static_cast<const T*>(p.residual), *wgt = static_cast<const T*>(p.weight);
+  if constexpr (ACCESS == kShifted) {
+    for (int c = int(threadIdx.x) - 8; c < cols + 8; c += blockDim.x) shared_weight[padded_at(c)] = c >= 0 && c < cols ? to_f32(wgt[c]) : 0.f;
+    __syncthreads();
+  } else {
 #pragma unroll
     for (int g = 0; g < G; g++) {
-      const bool in = at(g) < cols;
-      if (in) nx[g].load(x + row * p.ldx + at(g)); else nx[g].zero();
-      if (in && res) nr[g].load(res + row * p.ldr + at(g)); else nr[g].zero();
+      load_group<ACCESS>(nx[g], wgt, at(g), cols);
+      nx[g].get(w[g]);
+    }
+  }
+  auto load = [&](int64_t row) {
+    if (ACCESS == kShifted) shift = row_shift(x + row * p.ldx);
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      load_group<ACCESS>(nx[g], x + row * p.ldx, at(g), cols);
+      if (res) load_group<ACCESS>(nr[g], res + row * p.ldr, at(g), cols);
     }
   };
   const int64_t stride = int64_t(gridDim.x) * per_block;
@@ -265,7 +271,17 @@ __global__ void __launch_bounds__(512) norm_stream_kernel(RowArgs p) {
         for (int e = 0; e < 8; e++) v[g][e] += r[e];
       }
     }
+    const int here = shift;   // of this row
     if (row + stride < p.rows) load(row + stride);
+    if constexpr (ACCESS == kShifted) {
+#pragma unroll
+      for (int g = 0; g < G; g++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int c = (g * p.tpr + t) * 8 - here + e;
+          w[g][e] = c < cols + 8 ? shared_weight[padded_at(c)] : 0.f;
+        }
+    }
 #pragma unroll
     for (int g = 0; g < G; g++)
 #pragma unroll
@@ -290,7 +306,7 @@ __global__ void __launch_bounds__(512) norm_stream_kernel(RowArgs p) {
       for (int g = 0; g < G; g++)
 #pragma unroll
         for (int e = 0; e < 8; e++)
-          if (at(g) < cols) r.top_y = max(r.top_y, mag_bits(v[g][e] * u * w[g][e]));
+          if (const int c = (g * p.tpr + t) * 8 - here + e; c >= 0 && c < cols) r.top_y = max(r.top_y, mag_bits(v[g][e] * u * w[g][e]));
       qy = quant_of(join(r).top_y);
     } else {
       qy = quant_of(s.top_y);
@@ -305,14 +321,14 @@ __global__ void __launch_bounds__(512) norm_stream_kernel(RowArgs p) {
     }
 #pragma unroll
     for (int g = 0; g < G; g++) {
-      const int c = at(g);
+      const int c = (g * p.tpr + t) * 8 - here;
       if (c >= cols) continue;
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; e++) y[e] = redo ? v[g][e] * u * w[g][e] : v[g][e] * w[g][e];
-      *reinterpret_cast<uint2*>(p.q + row * p.ldq + c) = quant_pack8(y, qy.inv);
-      if (p.ckpt) *reinterpret_cast<uint2*>(p.ckpt + row * p.ldk + c) = quant_pack8(v[g], qh.inv);
-      if (p.h) store8(static_cast<T*>(p.h) + row * p.ldh + c, v[g]);
+      store_bytes<ACCESS>(p.q + row * p.ldq, c, cols, quant_pack8(y, qy.inv));
+      if (p.ckpt) store_bytes<ACCESS>(p.ckpt + row * p.ldk, c, cols, quant_pack8(v[g], qh.inv));
+      if (p.h) store_group<ACCESS>(static_cast<T*>(p.h) + row * p.ldh, c, cols, v[g]);
     }
   }
 }
@@ -360,20 +376,20 @@ __global__ void __launch_bounds__(1024) rows_long_kernel(RowArgs p) {
   }
 }
 
-// y = q * scale: 16 elements per thread (VEC) or one.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) dequantize_kernel(int64_t rows, int64_t cols, const int8_t* q, int64_t ldq,
+// y = q * scale: 16 elements per thread, a shifted group of 8, or one.
+template <typename T, int ACCESS>
+__global__ void __launch_bounds__(256) dequantize_kernel(int64_t rows, int64_t cols, int64_t per, const int8_t* q, int64_t ldq,
                                                          const float* scale, T* y, int64_t ldy) {
   after_previous_kernel();
-  const int64_t per = VEC ? cols / 16 : cols, total = rows * per;
+  const int64_t total = rows * per;
   const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (i >= total) return;
   const int64_t row = total <= 0xffffffffll ? int64_t(uint32_t(i) / uint32_t(per)) : i / per;
   const int64_t c = i - row * per;
   const float s = scale[row];
-  if (VEC) {
+  float v[8];
+  if constexpr (ACCESS == kAligned) {
     const uint4 w = *reinterpret_cast<const uint4*>(q + row * ldq + c * 16);
-    float v[8];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       bytes_f32(h ? make_uint2(w.z, w.w) : make_uint2(w.x, w.y), v);
@@ -381,6 +397,12 @@ __global__ void __launch_bounds__(256) dequantize_kernel(int64_t rows, int64_t c
       for (int e = 0; e < 8; e++) v[e] *= s;
       store8(y + row * ldy + c * 16 + h * 8, v);
     }
+  } else if constexpr (ACCESS == kShifted) {
+    const int first = int(c * 8) - row_shift(y + row * ldy);
+    bytes_f32(load_bytes<ACCESS>(q + row * ldq, first, int(cols)), v);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] *= s;
+    store_group<ACCESS>(y + row * ldy, first, int(cols), v);
   } else {
     y[row * ldy + c] = from_f32<T>(float(q[row * ldq + c]) * s);
   }
@@ -413,31 +435,27 @@ __device__ __forceinline__ float row_sum(float s, int tpr, float* warp_sums) {
   return s;
 }
 
-// What one thread reads of a row, as loaded.
-template <typename T, typename GT, int G, bool VEC> struct BackRow;
-template <typename T, typename GT, int G> struct BackRow<T, GT, G, true> {
+// What one thread reads of a row, as loaded; the columns are at(group, element).
+template <typename T, typename GT, int G, int ACCESS> struct BackRow {
   Vec8<GT> grad[G];
   Vec8<T> gh[G];
   uint2 q[G];
   float u, s;
+  int shift;
   __device__ __forceinline__ void load(const BackArgs& p, int64_t row, int t) {
     u = p.rstd[row];
     s = p.ckpt_scale[row];
     const GT* g = static_cast<const GT*>(p.grad) + row * p.ldg;
     const T* h = p.grad_h ? static_cast<const T*>(p.grad_h) + row * p.ldgh : nullptr;
     const int8_t* k = p.ckpt + row * p.ldk;
+    const int cols = int(p.cols);
+    shift = ACCESS == kShifted ? row_shift(g) : 0;
 #pragma unroll
     for (int i = 0; i < G; i++) {
-      const int c = (i * p.tpr + t) * 8;
-      if (c < p.cols) {
-        grad[i].load(g + c);
-        q[i] = *reinterpret_cast<const uint2*>(k + c);
-        if (h) gh[i].load(h + c); else gh[i].zero();
-      } else {
-        grad[i].zero();
-        gh[i].zero();
-        q[i] = make_uint2(0, 0);
-      }
+      const int c = (i * p.tpr + t) * 8 - shift;
+      load_group<ACCESS>(grad[i], g, c, cols);
+      q[i] = load_bytes<ACCESS>(k, c, cols);
+      if (h) load_group<ACCESS>(gh[i], h, c, cols); else gh[i].zero();
     }
   }
   __device__ __forceinline__ void get(int i, float (&g)[8], float (&v)[8]) const {
@@ -446,11 +464,12 @@ template <typename T, typename GT, int G> struct BackRow<T, GT, G, true> {
   }
   __device__ __forceinline__ void get_h(int i, float (&h)[8]) const { gh[i].get(h); }
 };
-template <typename T, typename GT, int G> struct BackRow<T, GT, G, false> {
+template <typename T, typename GT, int G> struct BackRow<T, GT, G, kScalar> {
   GT grad[G][8];
   T gh[G][8];
   int8_t q[G][8];
   float u, s;
+  static constexpr int shift = 0;
   __device__ __forceinline__ void load(const BackArgs& p, int64_t row, int t) {
     u = p.rstd[row];
     s = p.ckpt_scale[row];
@@ -475,67 +494,85 @@ template <typename T, typename GT, int G> struct BackRow<T, GT, G, false> {
   }
 };
 
-// Each slot (tpr threads) walks its rows with a fixed set of columns per
-// thread, so the sums over rows stay in registers; they are joined by
-// column_join_kernel in a fixed order.  The next row is loaded before this
-// one's sum is joined, so a row is always on its way.
-template <typename T, typename GT, int G, bool VEC>
+// Each slot (tpr threads) walks its rows; the sums over its rows stay with it
+// and are joined by column_join_kernel in a fixed order.  A thread has a fixed
+// set of columns and keeps their sums in registers, except where rows start
+// anywhere: there sums and weights are in shared memory (a column has one
+// thread per row, and a barrier lies between rows).  The next row is loaded
+// before this one's sum is joined, so a row is always on its way.
+template <typename T, typename GT, int G, int ACCESS>
 __global__ void __launch_bounds__(512) norm_backward_kernel(BackArgs p) {
+  constexpr bool kShift = ACCESS == kShifted;
+  extern __shared__ float shared_cols[];   // kShifted: the weights, then a slot's sums each
   __shared__ float4 stats[2][16];
   after_previous_kernel();
   const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, per_block = blockDim.x / p.tpr;
   const int cols = int(p.cols);
   const T* wgt = static_cast<const T*>(p.weight);
-  auto at = [&](int g, int e) { return VEC ? (g * p.tpr + t) * 8 + e : (g * 8 + e) * p.tpr + t; };
+  auto at = [&](int g, int e, int shift) { return ACCESS == kScalar ? (g * 8 + e) * p.tpr + t : (g * p.tpr + t) * 8 + e - shift; };
   RowJoin join{stats, p.tpr, sub, 0};
-  // what fits the registers: the next row (up to 16 elements per thread, aligned), and
+  float* sums = shared_cols + (1 + sub) * (padded_bytes(cols) / 4);
+  if constexpr (kShift) {
+    for (int c = int(threadIdx.x) - 8; c < cols + 8; c += blockDim.x) shared_cols[padded_at(c)] = c >= 0 && c < cols ? to_f32(wgt[c]) : 0.f;
+    for (int c = t; c < cols; c += p.tpr) sums[padded_at(c)] = 0.f;
+    __syncthreads();
+  }
+  // what fits the registers: the next row (up to 16 elements per thread), and
   // the weights as f32 beside 16-bit rows; else the weights come from L1
-  constexpr bool kAhead = G <= 2 && VEC, kHold = G <= 2 && sizeof(T) == 2 && VEC;
-  float dw[G][8] = {}, held[kHold ? G : 1][8];
-  auto weight_of = [&](int i, float (&w)[8]) {
-    if (VEC) {
+  constexpr bool kAhead = G <= 2 && ACCESS != kScalar, kHold = G <= 2 && sizeof(T) == 2 && ACCESS == kAligned;
+  float dw[kShift ? 1 : G][8] = {}, held[kHold ? G : 1][8];
+  auto weight_of = [&](int i, int shift, float (&w)[8]) {
+    if constexpr (ACCESS == kAligned) {
       Vec8<T> a;
-      if (at(i, 0) < cols) a.load(wgt + at(i, 0)); else a.zero();
+      load_group<ACCESS>(a, wgt, at(i, 0, 0), cols);
       a.get(w);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; e++) w[e] = at(i, e) < cols ? to_f32(wgt[at(i, e)]) : 0.f;
+      for (int e = 0; e < 8; e++) {
+        const int c = at(i, e, shift);
+        if (kShift) w[e] = c < cols + 8 ? shared_cols[padded_at(c)] : 0.f;
+        else w[e] = c < cols ? to_f32(wgt[c]) : 0.f;
+      }
     }
   };
   if constexpr (kHold) {
 #pragma unroll
-    for (int i = 0; i < G; i++) weight_of(i, held[i]);
+    for (int i = 0; i < G; i++) weight_of(i, 0, held[i]);
   }
   const float inv_cols = 1.f / float(cols);
   const int64_t slot = int64_t(blockIdx.x) * per_block + sub;
-  BackRow<T, GT, G, VEC> next;
+  BackRow<T, GT, G, ACCESS> next;
   int64_t row = slot;
   if (kAhead && row < p.rows) next.load(p, row, t);
   for (; row < p.rows; row += p.slots) {
     if (!kAhead) next.load(p, row, t);
     float gw[G][8], v[G][8];
-    const BackRow<T, GT, G, VEC> cur = next;   // of which grad_h is needed below
+    const BackRow<T, GT, G, ACCESS> cur = next;   // of which grad_h is needed below
     const float u = cur.u, s = cur.s * u;
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < G; i++) {
       float g[8], w[8];
       cur.get(i, g, v[i]);
-      if constexpr (!kHold) weight_of(i, w);
+      if constexpr (!kHold) weight_of(i, cur.shift, w);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
+        const int c = at(i, ACCESS == kAligned ? 0 : e, cur.shift);
         gw[i][e] = 0.f;
-        if (at(i, VEC ? 0 : e) < cols) {   // a NaN scale must not reach columns that are not there
+        if (c < cols && (!kShift || c >= 0)) {   // a NaN scale must not reach columns that are not there
           v[i][e] *= s;
-          dw[i][e] = fmaf(g[e], v[i][e], dw[i][e]);
+          if (kShift) sums[padded_at(c)] += g[e] * v[i][e];
+          else dw[kShift ? 0 : i][e] = fmaf(g[e], v[i][e], dw[kShift ? 0 : i][e]);
           gw[i][e] = g[e] * (kHold ? held[kHold ? i : 0][e] : w[e]);
           dot = fmaf(gw[i][e], v[i][e], dot);
         }
       }
     }
     if (kAhead && row + p.slots < p.rows) next.load(p, row + p.slots, t);
-    if (!p.grad_x) continue;   // uniform over the grid
-    const float mean = join(RowStats{dot, 0u, 0u}).sum * inv_cols;
+    if (!p.grad_x && !kShift) continue;   // uniform over the grid
+    const float mean = join(RowStats{dot, 0u, 0u}).sum * inv_cols;   // kShifted: also the barrier between rows' sums
+    if (kShift) __syncwarp();
+    if (!p.grad_x) continue;
     T* out = static_cast<T*>(p.grad_x) + row * p.ldx;
 #pragma unroll
     for (int i = 0; i < G; i++) {
@@ -543,25 +580,31 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(BackArgs p) {
       cur.get_h(i, h);
 #pragma unroll
       for (int e = 0; e < 8; e++) o[e] = fmaf(u, fmaf(-mean, v[i][e], gw[i][e]), h[e]);
-      if (VEC) {
-        if (at(i, 0) < cols) store8(out + at(i, 0), o);
+      if constexpr (ACCESS != kScalar) {
+        store_group<ACCESS>(out, at(i, 0, cur.shift), cols, o);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; e++)
-          if (at(i, e) < cols) out[at(i, e)] = from_f32<T>(o[e]);
+          if (at(i, e, 0) < cols) out[at(i, e, 0)] = from_f32<T>(o[e]);
       }
     }
   }
   if (p.partial && slot < p.slots) {
     float* o = p.partial + slot * p.cols;
+    if constexpr (kShift) {
+      join(RowStats{0.f, 0u, 0u});   // the last row's sums are complete
+      __syncwarp();
+      for (int c = t; c < cols; c += p.tpr) o[c] = sums[padded_at(c)];
+    } else {
 #pragma unroll
-    for (int i = 0; i < G; i++) {
-      if (VEC) {
-        if (at(i, 0) < cols) store8(o + at(i, 0), dw[i]);
-      } else {
+      for (int i = 0; i < G; i++) {
+        if constexpr (ACCESS == kAligned) {
+          if (at(i, 0, 0) < cols) store8(o + at(i, 0, 0), dw[i]);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (at(i, e) < cols) o[at(i, e)] = dw[i][e];
+          for (int e = 0; e < 8; e++)
+            if (at(i, e, 0) < cols) o[at(i, e, 0)] = dw[i][e];
+        }
       }
     }
   }
@@ -651,8 +694,14 @@ RowShape row_shape(int64_t rows, int64_t cols, int max_groups, int max_threads) 
   return {tpr, g, std::max(tpr, 128)};
 }
 
+template <typename F> void with_access(int access, F&& f) {
+  if (access == tg8::kAligned) f(std::integral_constant<int, tg8::kAligned>{});
+  else if (access == tg8::kShifted) f(std::integral_constant<int, tg8::kShifted>{});
+  else f(std::integral_constant<int, tg8::kScalar>{});
+}
+
 template <typename T, bool NORM>
-tg_status launch_rows(RowArgs p, bool vec, cudaStream_t st) {
+tg_status launch_rows(RowArgs p, int access, cudaStream_t st) {
   if (p.cols > kRowLimit) {
     if (p.rows > kGridLimit) return fail(TG_ERR_UNSUPPORTED, "%lld rows", (long long)p.rows);
     launch_kernel(tg8::rows_long_kernel<T, NORM>, unsigned(p.rows), 1024, 0, 0, st, p);
@@ -664,36 +713,51 @@ tg_status launch_rows(RowArgs p, bool vec, cudaStream_t st) {
     // row per block 124.  The plain quantisation has no weights to keep and
     // gains nothing (46 us either way).
     constexpr int kGroups = sizeof(T) == 4 ? 2 : 4;
-    if (vec && p.rows >= 4 * int64_t(sm_count()) && p.cols <= 512 * 8 * kGroups) {
-      const RowShape s = row_shape(p.rows, p.cols, kGroups, 512);
+    const int64_t span = p.cols + (access == tg8::kShifted ? 7 : 0);   // a shifted row may need a group more
+    if (access != tg8::kScalar && p.rows >= 4 * int64_t(sm_count()) && span <= 512 * 8 * kGroups) {
+      const RowShape s = row_shape(p.rows, span, kGroups, 512);
       p.tpr = s.tpr;
       const int per = s.block / s.tpr;
       const int64_t blocks = std::min<int64_t>((p.rows + per - 1) / per, int64_t(sm_count()) * (512 / s.block));
-      if (s.groups == 1) launch_kernel(tg8::norm_stream_kernel<T, 1>, unsigned(blocks), s.block, 0, 0, st, p);
-      else if (s.groups == 2) launch_kernel(tg8::norm_stream_kernel<T, 2>, unsigned(blocks), s.block, 0, 0, st, p);
-      else if constexpr (kGroups == 4) launch_kernel(tg8::norm_stream_kernel<T, 4>, unsigned(blocks), s.block, 0, 0, st, p);
-      return check_launch("rows8");
+      auto go = [&](auto access_c) {
+        constexpr int A = decltype(access_c)::value;
+        const size_t smem = A == tg8::kShifted ? tg8::padded_bytes(p.cols) : 0;
+        auto run = [&](auto kern) {
+          if (smem) {
+            const tg_status r = ensure_smem(reinterpret_cast<const void*>(kern), tg8::padded_bytes(kRowLimit));
+            if (r != TG_OK) return r;
+          }
+          launch_kernel(kern, unsigned(blocks), s.block, smem, 0, st, p);
+          return check_launch("rows8");
+        };
+        if (s.groups == 1) return run(tg8::norm_stream_kernel<T, 1, A>);
+        if (s.groups == 2 || kGroups == 2) return run(tg8::norm_stream_kernel<T, 2, A>);
+        return run(tg8::norm_stream_kernel<T, kGroups, A>);
+      };
+      return access == tg8::kAligned ? go(std::integral_constant<int, tg8::kAligned>{}) : go(std::integral_constant<int, tg8::kShifted>{});
     }
   }
-  const RowShape s = row_shape(p.rows, p.cols, 4, 1024);
+  if (access == tg8::kShifted && p.cols + 7 > kRowLimit) access = tg8::kScalar;
+  const RowShape s = row_shape(p.rows, p.cols + (access == tg8::kShifted ? 7 : 0), 4, 1024);
   p.tpr = s.tpr;
   const int per = s.block / s.tpr;
   const int64_t grid = (p.rows + per - 1) / per;
   if (grid > kGridLimit) return fail(TG_ERR_UNSUPPORTED, "%lld rows", (long long)p.rows);
-  auto go = [&](auto vec_c) {
-    constexpr bool V = decltype(vec_c)::value;
+  auto go = [&](auto access_c) {
+    constexpr int V = decltype(access_c)::value;
     if (s.groups == 1) launch_kernel(tg8::rows_kernel<T, 1, V, NORM>, unsigned(grid), s.block, 0, 0, st, p);
     else if (s.groups == 2) launch_kernel(tg8::rows_kernel<T, 2, V, NORM>, unsigned(grid), s.block, 0, 0, st, p);
     else launch_kernel(tg8::rows_kernel<T, 4, V, NORM>, unsigned(grid), s.block, 0, 0, st, p);
   };
-  if (vec) go(std::true_type{}); else go(std::false_type{});
+  with_access(access, go);
   return check_launch("rows8");
 }
 
 template <typename T, typename GT>
-tg_status launch_norm_backward(BackArgs p, T* grad_w, bool vec, cudaStream_t st) {
+tg_status launch_norm_backward(BackArgs p, T* grad_w, int access, cudaStream_t st) {
   const bool lng = p.cols > kRowLimit;
-  RowShape s = lng ? RowShape{1024, 4, 1024} : row_shape(p.rows, p.cols, 2, 512);
+  if (access == tg8::kShifted && p.cols + 7 > kRowLimit) access = tg8::kScalar;
+  RowShape s = lng ? RowShape{1024, 4, 1024} : row_shape(p.rows, p.cols + (access == tg8::kShifted ? 7 : 0), 2, 512);
   const int per = s.block / s.tpr;
   p.tpr = s.tpr;
   const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((p.rows + per - 1) / per, sm_count() * int64_t(std::max(1, 1024 / s.block))));
@@ -710,13 +774,22 @@ tg_status launch_norm_backward(BackArgs p, T* grad_w, bool vec, cudaStream_t st)
     if (grad_w)
       launch_kernel(tg8::column_partial_kernel<GT>, dim3(unsigned((p.cols + 255) / 256), unsigned(p.slots)), 256, 0, 0, st, p.rows, p.cols, static_cast<const GT*>(p.grad), p.ldg, p.ckpt, p.ldk, p.ckpt_scale, p.rstd, p.partial);
   } else {
-    auto go = [&](auto vec_c) {
-      constexpr bool V = decltype(vec_c)::value;
-      if (s.groups == 1) launch_kernel(tg8::norm_backward_kernel<T, GT, 1, V>, unsigned(blocks), s.block, 0, 0, st, p);
-      else if (s.groups == 2) launch_kernel(tg8::norm_backward_kernel<T, GT, 2, V>, unsigned(blocks), s.block, 0, 0, st, p);
-      else launch_kernel(tg8::norm_backward_kernel<T, GT, 4, V>, unsigned(blocks), s.block, 0, 0, st, p);
-    };
-    if (vec) go(std::true_type{}); else go(std::false_type{});
+    tg_status sized = TG_OK;
+    with_access(access, [&](auto access_c) {
+      constexpr int A = decltype(access_c)::value;
+      const size_t smem = A == tg8::kShifted ? size_t(1 + per) * tg8::padded_bytes(p.cols) : 0;
+      auto run = [&](auto kern) {
+        if (smem) sized = ensure_smem(reinterpret_cast<const void*>(kern), 2 * tg8::padded_bytes(kRowLimit));
+        if (sized == TG_OK) launch_kernel(kern, unsigned(blocks), s.block, smem, 0, st, p);
+      };
+      if (s.groups == 1) run(tg8::norm_backward_kernel<T, GT, 1, A>);
+      else if (s.groups == 2) run(tg8::norm_backward_kernel<T, GT, 2, A>);
+      else run(tg8::norm_backward_kernel<T, GT, 4, A>);
+    });
+    if (sized != TG_OK) {
+      if (scratch) scratch_free(scratch, st);
+      return sized;
+    }
   }
   tg_status r = check_launch("rows8 norm backward");
   if (grad_w) {
@@ -766,9 +839,10 @@ tg_status tg_rows8_quantize(tg_dtype dtype, int64_t rows, int64_t cols, const vo
   TG8_CHECK(check_ld("ldq", ldq, cols));
   RowArgs p{};
   p.rows = rows; p.cols = cols; p.x = x; p.ldx = ldx; p.q = q; p.ldq = ldq; p.scale = scale;
-  const size_t e = elem8_size(dtype);
-  const bool vec = cols % 8 == 0 && rows_vec(x, ldx, e) && rows_vec(q, ldq, 1, 8);
-  return with_type8(dtype, [&](auto t) { return launch_rows<decltype(t), false>(p, vec, static_cast<cudaStream_t>(stream)); });
+  RowAccess access(cols);
+  access.add(x, ldx, elem8_size(dtype));
+  access.add(q, ldq, 1);
+  return with_type8(dtype, [&](auto t) { return launch_rows<decltype(t), false>(p, access.get(), static_cast<cudaStream_t>(stream)); });
 }
 
 tg_status tg_rows8_dequantize(tg_dtype dtype, int64_t rows, int64_t cols, const int8_t* q, int64_t ldq,
@@ -780,15 +854,20 @@ tg_status tg_rows8_dequantize(tg_dtype dtype, int64_t rows, int64_t cols, const 
   if (!q || !scale || !y) return fail(TG_ERR_INVALID_ARGUMENT, "null operand");
   TG8_CHECK(check_ld("ldq", ldq, cols));
   TG8_CHECK(check_ld("ldy", ldy, cols));
-  const bool vec = cols % 16 == 0 && rows_vec(y, ldy, elem8_size(dtype)) && rows_vec(q, ldq, 1);
-  const int64_t per = vec ? cols / 16 : cols;
+  RowAccess access(cols);
+  access.add(y, ldy, elem8_size(dtype));
+  access.add(q, ldq, 1);
+  int how = access.get();
+  if (how == tg8::kAligned && (cols % 16 || ldq % 16 || !aligned(q, 16))) how = tg8::kShifted;   // by 8 elements, without edges
+  const int64_t per = how == tg8::kAligned ? cols / 16 : how == tg8::kShifted ? (cols + 7 + 7) / 8 : cols;
   if (rows > (kGridLimit * 256) / per) return fail(TG_ERR_UNSUPPORTED, "%lld x %lld elements", (long long)rows, (long long)cols);
   const unsigned grid = unsigned((rows * per + 255) / 256);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return with_type8(dtype, [&](auto t) {
     using T = decltype(t);
-    if (vec) launch_kernel(tg8::dequantize_kernel<T, true>, grid, 256, 0, 0, st, rows, cols, q, ldq, scale, static_cast<T*>(y), ldy);
-    else launch_kernel(tg8::dequantize_kernel<T, false>, grid, 256, 0, 0, st, rows, cols, q, ldq, scale, static_cast<T*>(y), ldy);
+    with_access(how, [&](auto access_c) {
+      launch_kernel(tg8::dequantize_kernel<T, decltype(access_c)::value>, grid, 256, 0, 0, st, rows, cols, per, q, ldq, scale, static_cast<T*>(y), ldy);
+    });
     return check_launch("rows8 dequantize");
   });
 }
@@ -822,9 +901,14 @@ tg_status tg_rows8_rmsnorm(tg_dtype dtype, int64_t rows, int64_t cols, const voi
   p.eps = eps; p.h = h; p.ldh = ldh; p.q = q; p.ldq = ldq; p.scale = scale;
   p.ckpt = ckpt; p.ldk = ldk; p.ckpt_scale = ckpt_scale; p.rstd = rstd;
   const size_t e = elem8_size(dtype);
-  const bool vec = cols % 8 == 0 && rows_vec(x, ldx, e) && rows_vec(residual, ldr, e) && aligned(weight, 16) &&
-                   rows_vec(h, ldh, e) && rows_vec(q, ldq, 1, 8) && rows_vec(ckpt, ldk, 1, 8);
-  return with_type8(dtype, [&](auto t) { return launch_rows<decltype(t), true>(p, vec, static_cast<cudaStream_t>(stream)); });
+  RowAccess access(cols);
+  access.add(x, ldx, e);
+  access.add(residual, ldr, e);
+  access.add(h, ldh, e);
+  access.add(q, ldq, 1);
+  access.add(ckpt, ldk, 1);
+  const int how = access.get() == tg8::kAligned && !aligned(weight, 16) ? tg8::kScalar : access.get();
+  return with_type8(dtype, [&](auto t) { return launch_rows<decltype(t), true>(p, how, static_cast<cudaStream_t>(stream)); });
 }
 
 tg_status tg_rows8_rmsnorm_backward(tg_dtype dtype, tg_dtype grad_dtype, int64_t rows, int64_t cols, const void* grad,
@@ -848,13 +932,17 @@ tg_status tg_rows8_rmsnorm_backward(tg_dtype dtype, tg_dtype grad_dtype, int64_t
   p.ckpt = ckpt; p.ldk = ldk; p.ckpt_scale = ckpt_scale; p.rstd = rstd; p.grad_x = grad_x; p.ldx = ldx;
   if (rows == 0 && !grad_weight) return TG_OK;
   const size_t e = elem8_size(dtype);
-  const bool vec = cols % 8 == 0 && rows_vec(grad, ldg, elem8_size(grad_dtype)) && rows_vec(grad_h, ldgh, e) &&
-                   aligned(weight, 16) && rows_vec(ckpt, ldk, 1, 8) && rows_vec(grad_x, ldx, e);
+  RowAccess access(cols);
+  access.add(grad, ldg, elem8_size(grad_dtype));
+  access.add(grad_h, ldgh, e);
+  access.add(ckpt, ldk, 1);
+  access.add(grad_x, ldx, e);
+  const int how = access.get() == tg8::kAligned && !aligned(weight, 16) ? tg8::kScalar : access.get();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return with_type8(dtype, [&](auto t) {
     using T = decltype(t);
-    if (grad_dtype == dtype) return launch_norm_backward<T, T>(p, static_cast<T*>(grad_weight), vec, st);
-    return launch_norm_backward<T, float>(p, static_cast<T*>(grad_weight), vec, st);
+    if (grad_dtype == dtype) return launch_norm_backward<T, T>(p, static_cast<T*>(grad_weight), how, st);
+    return launch_norm_backward<T, float>(p, static_cast<T*>(grad_weight), how, st);
   });
 }
 

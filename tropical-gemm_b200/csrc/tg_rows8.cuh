@@ -75,6 +75,65 @@ __device__ __forceinline__ void store8(f16* p, const float (&v)[8]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// How a row kernel reaches its rows.
+//   kScalar  element by element, any alignment
+//   kAligned groups of 8 elements that start on 16-byte boundaries
+//   kShifted the same groups for rows that start anywhere: group k is elements
+//            8 k - s .. 8 k - s + 7 with s the row start's distance from a boundary
+//            of 8 elements, equal in all operands; the groups at both ends of the
+//            row go element by element
+enum Access { kScalar, kAligned, kShifted };
+
+template <typename T> __device__ __forceinline__ int row_shift(const T* row) { return int((reinterpret_cast<uintptr_t>(row) / sizeof(T)) & 7); }
+
+template <int ACCESS, typename T> __device__ __forceinline__ void load_group(Vec8<T>& v, const T* row, int c, int cols) {
+  if (ACCESS == kAligned ? c < cols : c >= 0 && c + 8 <= cols) {
+    v.load(row + c);
+  } else {
+    v.zero();
+    if (ACCESS == kShifted && c > -8 && c < cols) {
+      alignas(16) T e[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) e[i] = c + i >= 0 && c + i < cols ? row[c + i] : T(0.f);
+      __builtin_memcpy(&v, e, sizeof(v));
+    }
+  }
+}
+template <int ACCESS, typename T> __device__ __forceinline__ void store_group(T* row, int c, int cols, const float (&v)[8]) {
+  if (ACCESS == kAligned ? c < cols : c >= 0 && c + 8 <= cols) {
+    store8(row + c, v);
+  } else if (ACCESS == kShifted) {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (c + i >= 0 && c + i < cols) row[c + i] = from_f32<T>(v[i]);
+  }
+}
+template <int ACCESS> __device__ __forceinline__ uint2 load_bytes(const int8_t* row, int c, int cols) {
+  if (ACCESS == kAligned ? c < cols : c >= 0 && c + 8 <= cols) return *reinterpret_cast<const uint2*>(row + c);
+  uint2 w = make_uint2(0, 0);
+  if (ACCESS == kShifted) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const uint32_t b = c + i >= 0 && c + i < cols ? uint32_t(uint8_t(row[c + i])) << (8 * (i & 3)) : 0u;
+      if (i < 4) w.x |= b; else w.y |= b;
+    }
+  }
+  return w;
+}
+template <int ACCESS> __device__ __forceinline__ void store_bytes(int8_t* row, int c, int cols, uint2 w) {
+  if (ACCESS == kAligned ? c < cols : c >= 0 && c + 8 <= cols) {
+    *reinterpret_cast<uint2*>(row + c) = w;
+  } else if (ACCESS == kShifted) {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (c + i >= 0 && c + i < cols) row[c + i] = int8_t(((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 0xff);
+  }
+}
+// Place of column c in a row of f32 held in shared memory, c from -8: a word of
+// padding after every eight, so that lanes eight columns apart meet all banks.
+__device__ __forceinline__ int padded_at(int c) { return c + 8 + ((c + 8) >> 3); }
+__host__ __device__ __forceinline__ size_t padded_bytes(int64_t cols) { return size_t(cols + 16 + (cols + 16) / 8 + 1) * 4; }
+
 // max(|a|, |b|, m) that keeps a NaN.
 __device__ __forceinline__ float mag_max(float a, float b, float m) {
   float r;
@@ -159,10 +218,27 @@ void launch_kernel(void (*kern)(P...), dim3 grid, int block, size_t smem, int cl
 
 inline size_t elem8_size(tg_dtype t) { return t == TG_F32 ? 4 : (t == TG_BF16 || t == TG_F16) ? 2 : 0; }
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
-// p null, or 16-byte aligned rows of `elem`-byte elements
-inline bool rows_vec(const void* p, int64_t ld, size_t elem, size_t bytes = 16) {
-  return !p || (aligned(p, bytes) && (ld * int64_t(elem)) % int64_t(bytes) == 0);
-}
+
+// The access that a call's operands allow: kAligned when all rows start on a
+// boundary of 8 elements, kShifted when all are the same distance from one.
+class RowAccess {
+ public:
+  explicit RowAccess(int64_t cols) : cols_(cols) {}
+  void add(const void* p, int64_t ld, size_t elem) {
+    if (!p) return;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    const int phase = a % elem ? -1 : int(a / elem % 8), step = int(ld % 8);
+    if (!any_) { phase_ = phase; step_ = step; }
+    any_ = true;
+    same_ = same_ && phase >= 0 && phase == phase_ && step == step_;
+  }
+  int get() const { return !same_ ? tg8::kScalar : phase_ == 0 && step_ == 0 && cols_ % 8 == 0 ? tg8::kAligned : tg8::kShifted; }
+
+ private:
+  int64_t cols_;
+  int phase_ = 0, step_ = 0;
+  bool any_ = false, same_ = true;
+};
 
 // f(T{}) for the element type of a tg_rows8 call; the caller has checked dtype.
 template <typename F> tg_status with_type8(tg_dtype t, F&& f) {
