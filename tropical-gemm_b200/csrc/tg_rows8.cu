@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(G == 1 ? 1024 : 512) rows_kernel(RowArgs p) {
 #pragma unroll
         for (int e = 0; e < 8; e++) v[g][e] += r[e];
       }
+      mask_group<ACCESS>(v[g], at(g, 0), cols);
     }
   } else {
 #pragma unroll
@@ -222,36 +223,29 @@ struct RowJoin {
 // row is on its way while this one is worked on.  The kernel above is bound by
 // instructions (78 % of the issue slots for 4096 x 8192 bf16, weights unpacked
 // twice per row); this one needs about half of them.
-// Rows that start anywhere take their weights from shared memory instead.
-template <typename T, int G, int ACCESS>
+// Rows that start anywhere would take their weights from shared memory and are
+// slower so (16384 x 4001 bf16: 169 us, one row per block 137).
+template <typename T, int G>
 __global__ void __launch_bounds__(512) norm_stream_kernel(RowArgs p) {
-  extern __shared__ float shared_weight[];   // kShifted
   __shared__ float4 stats[2][16];
   after_previous_kernel();
   const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, per_block = blockDim.x / p.tpr;
   const int cols = int(p.cols);
-  int shift = 0;   // of the row being loaded
-  auto at = [&](int g) { return (g * p.tpr + t) * 8 - shift; };
+  auto at = [&](int g) { return (g * p.tpr + t) * 8; };
   RowJoin join{stats, p.tpr, sub, 0};
   float w[G][8];
   Vec8<T> nx[G], nr[G];
-  const T *x = static_cast<const T*>(p.x), *res = static_cast<const T*>(p.residual), *wgt = static_cast<const T*>(p.weight);
-  if constexpr (ACCESS == kShifted) {
-    for (int c = int(threadIdx.x) - 8; c < cols + 8; c += blockDim.x) shared_weight[padded_at(c)] = c >= 0 && c < cols ? to_f32(wgt[c]) : 0.f;
-    __syncthreads();
-  } else {
+  const T *x = static_cast<const T*>(p.x), *res = static_cast<const T*>(p.residual);
 #pragma unroll
-    for (int g = 0; g < G; g++) {
-      load_group<ACCESS>(nx[g], wgt, at(g), cols);
-      nx[g].get(w[g]);
-    }
+  for (int g = 0; g < G; g++) {
+    load_group<kAligned>(nx[g], static_cast<const T*>(p.weight), at(g), cols);
+    nx[g].get(w[g]);
   }
   auto load = [&](int64_t row) {
-    if (ACCESS == kShifted) shift = row_shift(x + row * p.ldx);
 #pragma unroll
     for (int g = 0; g < G; g++) {
-      load_group<ACCESS>(nx[g], x + row * p.ldx, at(g), cols);
-      if (res) load_group<ACCESS>(nr[g], res + row * p.ldr, at(g), cols);
+      load_group<kAligned>(nx[g], x + row * p.ldx, at(g), cols);
+      if (res) load_group<kAligned>(nr[g], res + row * p.ldr, at(g), cols);
     }
   };
   const int64_t stride = int64_t(gridDim.x) * per_block;
@@ -271,17 +265,7 @@ __global__ void __launch_bounds__(512) norm_stream_kernel(RowArgs p) {
         for (int e = 0; e < 8; e++) v[g][e] += r[e];
       }
     }
-    const int here = shift;   // of this row
     if (row + stride < p.rows) load(row + stride);
-    if constexpr (ACCESS == kShifted) {
-#pragma unroll
-      for (int g = 0; g < G; g++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const int c = (g * p.tpr + t) * 8 - here + e;
-          w[g][e] = c < cols + 8 ? shared_weight[padded_at(c)] : 0.f;
-        }
-    }
 #pragma unroll
     for (int g = 0; g < G; g++)
 #pragma unroll
@@ -306,7 +290,7 @@ __global__ void __launch_bounds__(512) norm_stream_kernel(RowArgs p) {
       for (int g = 0; g < G; g++)
 #pragma unroll
         for (int e = 0; e < 8; e++)
-          if (const int c = (g * p.tpr + t) * 8 - here + e; c >= 0 && c < cols) r.top_y = max(r.top_y, mag_bits(v[g][e] * u * w[g][e]));
+          if (at(g) < cols) r.top_y = max(r.top_y, mag_bits(v[g][e] * u * w[g][e]));
       qy = quant_of(join(r).top_y);
     } else {
       qy = quant_of(s.top_y);
@@ -321,14 +305,14 @@ __global__ void __launch_bounds__(512) norm_stream_kernel(RowArgs p) {
     }
 #pragma unroll
     for (int g = 0; g < G; g++) {
-      const int c = (g * p.tpr + t) * 8 - here;
+      const int c = at(g);
       if (c >= cols) continue;
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; e++) y[e] = redo ? v[g][e] * u * w[g][e] : v[g][e] * w[g][e];
-      store_bytes<ACCESS>(p.q + row * p.ldq, c, cols, quant_pack8(y, qy.inv));
-      if (p.ckpt) store_bytes<ACCESS>(p.ckpt + row * p.ldk, c, cols, quant_pack8(v[g], qh.inv));
-      if (p.h) store_group<ACCESS>(static_cast<T*>(p.h) + row * p.ldh, c, cols, v[g]);
+      store_bytes<kAligned>(p.q + row * p.ldq, c, cols, quant_pack8(y, qy.inv));
+      if (p.ckpt) store_bytes<kAligned>(p.ckpt + row * p.ldk, c, cols, quant_pack8(v[g], qh.inv));
+      if (p.h) store_group<kAligned>(static_cast<T*>(p.h) + row * p.ldh, c, cols, v[g]);
     }
   }
 }
@@ -399,7 +383,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(int64_t rows, int64_t c
     }
   } else if constexpr (ACCESS == kShifted) {
     const int first = int(c * 8) - row_shift(y + row * ldy);
-    bytes_f32(load_bytes<ACCESS>(q + row * ldq, first, int(cols)), v);
+    bytes_f32(load_bytes(q + row * ldq, first, int(cols)), v);
 #pragma unroll
     for (int e = 0; e < 8; e++) v[e] *= s;
     store_group<ACCESS>(y + row * ldy, first, int(cols), v);
@@ -454,7 +438,7 @@ template <typename T, typename GT, int G, int ACCESS> struct BackRow {
     for (int i = 0; i < G; i++) {
       const int c = (i * p.tpr + t) * 8 - shift;
       load_group<ACCESS>(grad[i], g, c, cols);
-      q[i] = load_bytes<ACCESS>(k, c, cols);
+      q[i] = load_bytes(k, c, cols);
       if (h) load_group<ACCESS>(gh[i], h, c, cols); else gh[i].zero();
     }
   }
@@ -526,13 +510,13 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(BackArgs p) {
       Vec8<T> a;
       load_group<ACCESS>(a, wgt, at(i, 0, 0), cols);
       a.get(w);
+    } else if constexpr (kShift) {
+      const float* from = shared_cols + padded_at(at(i, 0, shift));
+#pragma unroll
+      for (int e = 0; e < 8; e++) w[e] = at(i, 0, shift) < cols ? from[padded_offset(shift, e)] : 0.f;
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const int c = at(i, e, shift);
-        if (kShift) w[e] = c < cols + 8 ? shared_cols[padded_at(c)] : 0.f;
-        else w[e] = c < cols ? to_f32(wgt[c]) : 0.f;
-      }
+      for (int e = 0; e < 8; e++) w[e] = at(i, e, 0) < cols ? to_f32(wgt[at(i, e, 0)]) : 0.f;
     }
   };
   if constexpr (kHold) {
@@ -561,7 +545,7 @@ __global__ void __launch_bounds__(512) norm_backward_kernel(BackArgs p) {
         gw[i][e] = 0.f;
         if (c < cols && (!kShift || c >= 0)) {   // a NaN scale must not reach columns that are not there
           v[i][e] *= s;
-          if (kShift) sums[padded_at(c)] += g[e] * v[i][e];
+          if (kShift) sums[padded_at(at(i, 0, cur.shift)) + padded_offset(cur.shift, e)] += g[e] * v[i][e];
           else dw[kShift ? 0 : i][e] = fmaf(g[e], v[i][e], dw[kShift ? 0 : i][e]);
           gw[i][e] = g[e] * (kHold ? held[kHold ? i : 0][e] : w[e]);
           dot = fmaf(gw[i][e], v[i][e], dot);
@@ -680,18 +664,20 @@ constexpr int64_t kGridLimit = 0x7fffffff;
 // Threads per row and groups of 8 elements per thread (1, 2 or 4), for rows of
 // at most kRowLimit: as few threads as max_groups allows (more loads in
 // flight per thread, cheaper sums) when there are rows enough to fill the GPU;
-// one group per thread when there are not, and latency counts.
+// one group per thread when there are not, and latency counts.  Threads are a
+// power of two (RowJoin), or a multiple of `step`.
 struct RowShape {
   int tpr, groups, block;
 };
-RowShape row_shape(int64_t rows, int64_t cols, int max_groups, int max_threads) {
+RowShape row_shape(int64_t rows, int64_t cols, int max_groups, int max_threads, int step = 0) {
   const int64_t groups = (cols + 7) / 8;
   int g = rows >= 2 * sm_count() ? max_groups : 1;
   while (groups > int64_t(g) * (g == 1 ? max_threads : 512)) g *= 2;
   int tpr = 32;
   while (int64_t(tpr) * g < groups) tpr *= 2;
   while (g > 1 && int64_t(tpr) * (g / 2) >= groups) g /= 2;
-  return {tpr, g, std::max(tpr, 128)};
+  if (step) tpr = std::max(step, int(((groups + g - 1) / g + step - 1) / step * step));
+  return {tpr, g, tpr >= 128 ? tpr : 128 / tpr * tpr};
 }
 
 template <typename F> void with_access(int access, F&& f) {
@@ -713,32 +699,20 @@ tg_status launch_rows(RowArgs p, int access, cudaStream_t st) {
     // row per block 124.  The plain quantisation has no weights to keep and
     // gains nothing (46 us either way).
     constexpr int kGroups = sizeof(T) == 4 ? 2 : 4;
-    const int64_t span = p.cols + (access == tg8::kShifted ? 7 : 0);   // a shifted row may need a group more
-    if (access != tg8::kScalar && p.rows >= 4 * int64_t(sm_count()) && span <= 512 * 8 * kGroups) {
-      const RowShape s = row_shape(p.rows, span, kGroups, 512);
+    if (access == tg8::kAligned && p.rows >= 4 * int64_t(sm_count()) && p.cols <= 512 * 8 * kGroups) {
+      const RowShape s = row_shape(p.rows, p.cols, kGroups, 512);
       p.tpr = s.tpr;
       const int per = s.block / s.tpr;
       const int64_t blocks = std::min<int64_t>((p.rows + per - 1) / per, int64_t(sm_count()) * (512 / s.block));
-      auto go = [&](auto access_c) {
-        constexpr int A = decltype(access_c)::value;
-        const size_t smem = A == tg8::kShifted ? tg8::padded_bytes(p.cols) : 0;
-        auto run = [&](auto kern) {
-          if (smem) {
-            const tg_status r = ensure_smem(reinterpret_cast<const void*>(kern), tg8::padded_bytes(kRowLimit));
-            if (r != TG_OK) return r;
-          }
-          launch_kernel(kern, unsigned(blocks), s.block, smem, 0, st, p);
-          return check_launch("rows8");
-        };
-        if (s.groups == 1) return run(tg8::norm_stream_kernel<T, 1, A>);
-        if (s.groups == 2 || kGroups == 2) return run(tg8::norm_stream_kernel<T, 2, A>);
-        return run(tg8::norm_stream_kernel<T, kGroups, A>);
-      };
-      return access == tg8::kAligned ? go(std::integral_constant<int, tg8::kAligned>{}) : go(std::integral_constant<int, tg8::kShifted>{});
+      if (s.groups == 1) launch_kernel(tg8::norm_stream_kernel<T, 1>, unsigned(blocks), s.block, 0, 0, st, p);
+      else if (s.groups == 2) launch_kernel(tg8::norm_stream_kernel<T, 2>, unsigned(blocks), s.block, 0, 0, st, p);
+      else launch_kernel(tg8::norm_stream_kernel<T, kGroups>, unsigned(blocks), s.block, 0, 0, st, p);
+      return check_launch("rows8");
     }
   }
   if (access == tg8::kShifted && p.cols + 7 > kRowLimit) access = tg8::kScalar;
-  const RowShape s = row_shape(p.rows, p.cols + (access == tg8::kShifted ? 7 : 0), 4, 1024);
+  // a shifted row may need a group more
+  const RowShape s = row_shape(p.rows, p.cols + (access == tg8::kShifted ? 7 : 0), 4, 1024, 32);
   p.tpr = s.tpr;
   const int per = s.block / s.tpr;
   const int64_t grid = (p.rows + per - 1) / per;

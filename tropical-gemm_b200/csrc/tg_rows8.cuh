@@ -80,23 +80,33 @@ __device__ __forceinline__ void store8(f16* p, const float (&v)[8]) {
 //   kAligned groups of 8 elements that start on 16-byte boundaries
 //   kShifted the same groups for rows that start anywhere: group k is elements
 //            8 k - s .. 8 k - s + 7 with s the row start's distance from a boundary
-//            of 8 elements, equal in all operands; the groups at both ends of the
-//            row go element by element
+//            of 8 elements, equal in all operands.  A group at an end of the row is
+//            loaded whole where its 16 bytes hold an element of the row (they are
+//            mapped then) and masked; it is stored element by element
 enum Access { kScalar, kAligned, kShifted };
 
 template <typename T> __device__ __forceinline__ int row_shift(const T* row) { return int((reinterpret_cast<uintptr_t>(row) / sizeof(T)) & 7); }
 
+__device__ __forceinline__ void load_touching(Vec8<float>& v, const float* row, int c, int cols) {
+  if (c + 4 > 0) v.a = *reinterpret_cast<const float4*>(row + c);
+  if (c + 4 < cols) v.b = *reinterpret_cast<const float4*>(row + c + 4);
+}
+template <typename T> __device__ __forceinline__ void load_touching(Vec8<T>& v, const T* row, int c, int) { v.load(row + c); }
+
 template <int ACCESS, typename T> __device__ __forceinline__ void load_group(Vec8<T>& v, const T* row, int c, int cols) {
-  if (ACCESS == kAligned ? c < cols : c >= 0 && c + 8 <= cols) {
-    v.load(row + c);
+  if constexpr (ACCESS == kAligned) {
+    if (c < cols) v.load(row + c); else v.zero();
   } else {
     v.zero();
-    if (ACCESS == kShifted && c > -8 && c < cols) {
-      alignas(16) T e[8];
+    if (c < cols) load_touching(v, row, c, cols);   // c > -8
+  }
+}
+// Zeros for what a group at a row's end holds of its neighbours.
+template <int ACCESS> __device__ __forceinline__ void mask_group(float (&v)[8], int c, int cols) {
+  if (ACCESS == kShifted && (c < 0 || c + 8 > cols)) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) e[i] = c + i >= 0 && c + i < cols ? row[c + i] : T(0.f);
-      __builtin_memcpy(&v, e, sizeof(v));
-    }
+    for (int i = 0; i < 8; i++)
+      if (c + i < 0 || c + i >= cols) v[i] = 0.f;
   }
 }
 template <int ACCESS, typename T> __device__ __forceinline__ void store_group(T* row, int c, int cols, const float (&v)[8]) {
@@ -108,17 +118,8 @@ template <int ACCESS, typename T> __device__ __forceinline__ void store_group(T*
       if (c + i >= 0 && c + i < cols) row[c + i] = from_f32<T>(v[i]);
   }
 }
-template <int ACCESS> __device__ __forceinline__ uint2 load_bytes(const int8_t* row, int c, int cols) {
-  if (ACCESS == kAligned ? c < cols : c >= 0 && c + 8 <= cols) return *reinterpret_cast<const uint2*>(row + c);
-  uint2 w = make_uint2(0, 0);
-  if (ACCESS == kShifted) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const uint32_t b = c + i >= 0 && c + i < cols ? uint32_t(uint8_t(row[c + i])) << (8 * (i & 3)) : 0u;
-      if (i < 4) w.x |= b; else w.y |= b;
-    }
-  }
-  return w;
+__device__ __forceinline__ uint2 load_bytes(const int8_t* row, int c, int cols) {
+  return c < cols ? *reinterpret_cast<const uint2*>(row + c) : make_uint2(0, 0);
 }
 template <int ACCESS> __device__ __forceinline__ void store_bytes(int8_t* row, int c, int cols, uint2 w) {
   if (ACCESS == kAligned ? c < cols : c >= 0 && c + 8 <= cols) {
@@ -132,6 +133,9 @@ template <int ACCESS> __device__ __forceinline__ void store_bytes(int8_t* row, i
 // Place of column c in a row of f32 held in shared memory, c from -8: a word of
 // padding after every eight, so that lanes eight columns apart meet all banks.
 __device__ __forceinline__ int padded_at(int c) { return c + 8 + ((c + 8) >> 3); }
+// padded_at(c + e) = padded_at(c) + padded_offset(shift, e) for the group that
+// starts at c = 8 k - shift: an offset per element that a row's groups share.
+__device__ __forceinline__ int padded_offset(int shift, int e) { return e + ((((8 - shift) & 7) + e) >> 3); }
 __host__ __device__ __forceinline__ size_t padded_bytes(int64_t cols) { return size_t(cols + 16 + (cols + 16) / 8 + 1) * 4; }
 
 // max(|a|, |b|, m) that keeps a NaN.
