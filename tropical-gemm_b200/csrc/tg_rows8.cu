@@ -631,24 +631,27 @@ __global__ void __launch_bounds__(256) column_partial_kernel(int64_t rows, int64
   partial[int64_t(blockIdx.y) * cols + c] = s;
 }
 
-// out[c] = sum over slots of partial[slot, c]: 32 columns x 8 slot lanes per
+// out[c] = sum over slots of partial[slot, c]: 32 columns x 32 slot lanes per
 // block, joined in a fixed order.
 template <typename T>
-__global__ void __launch_bounds__(256) column_join_kernel(int64_t slots, int64_t cols, const float* partial, T* out) {
-  __shared__ float part[8][33];
+__global__ void __launch_bounds__(1024) column_join_kernel(int64_t slots, int64_t cols, const float* partial, T* out) {
+  __shared__ float part[32][33];
   after_previous_kernel();
   const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int64_t c = int64_t(blockIdx.x) * 32 + lane;
   float s = 0.f;
-  if (c < cols)
-    for (int64_t r = y; r < slots; r += 8) s += partial[r * cols + c];
+  if (c < cols) {
+#pragma unroll 8
+    for (int64_t r = y; r < slots; r += 32) s += partial[r * cols + c];
+  }
   part[y][lane] = s;
   __syncthreads();
-  if (y == 0 && c < cols) {
+  // warp y joins column y of the strip
+  s = part[lane][y];
 #pragma unroll
-    for (int i = 1; i < 8; i++) s += part[i][lane];
-    out[c] = from_f32<T>(s);
-  }
+  for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  const int64_t column = int64_t(blockIdx.x) * 32 + y;
+  if (lane == 0 && column < cols) out[column] = from_f32<T>(s);
 }
 
 }  // namespace tg8
@@ -734,7 +737,8 @@ tg_status launch_norm_backward(BackArgs p, T* grad_w, int access, cudaStream_t s
   RowShape s = lng ? RowShape{1024, 4, 1024} : row_shape(p.rows, p.cols + (access == tg8::kShifted ? 7 : 0), 2, 512);
   const int per = s.block / s.tpr;
   p.tpr = s.tpr;
-  const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((p.rows + per - 1) / per, sm_count() * int64_t(std::max(1, 1024 / s.block))));
+  // at most four slots per SM: each leaves a row of sums to be joined
+  const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((p.rows + per - 1) / per, sm_count() * int64_t(std::max(1, std::min(4 / per, 1024 / s.block)))));
   p.slots = lng ? std::max<int64_t>(1, std::min<int64_t>(p.rows, 64)) : blocks * per;
   if (lng && p.rows > kGridLimit) return fail(TG_ERR_UNSUPPORTED, "%lld rows", (long long)p.rows);
   void* scratch = nullptr;
@@ -768,7 +772,7 @@ tg_status launch_norm_backward(BackArgs p, T* grad_w, int access, cudaStream_t s
   tg_status r = check_launch("rows8 norm backward");
   if (grad_w) {
     if (r == TG_OK) {
-      launch_kernel(tg8::column_join_kernel<T>, unsigned((p.cols + 31) / 32), 256, 0, 0, st, p.slots, p.cols, p.partial, grad_w);
+      launch_kernel(tg8::column_join_kernel<T>, unsigned((p.cols + 31) / 32), 1024, 0, 0, st, p.slots, p.cols, p.partial, grad_w);
       r = check_launch("rows8 norm backward");
     }
     scratch_free(scratch, st);
@@ -945,7 +949,7 @@ tg_status tg_rows8_column_sum(tg_dtype dtype, tg_dtype out_dtype, int64_t rows, 
   if (r == TG_OK)
     r = with_type8(out_dtype, [&](auto t) {
       using T = decltype(t);
-      launch_kernel(tg8::column_join_kernel<T>, unsigned((cols + 31) / 32), 256, 0, 0, st, slots, cols, partial, static_cast<T*>(out));
+      launch_kernel(tg8::column_join_kernel<T>, unsigned((cols + 31) / 32), 1024, 0, 0, st, slots, cols, partial, static_cast<T*>(out));
       return check_launch("rows8 column sum");
     });
   scratch_free(scratch, st);
