@@ -79,7 +79,8 @@ void pad_operands(const tg8::PadArgs& p, int count, cudaStream_t st) {
 
 template <int MODE, typename T>
 tg_status launch_product(const CUtensorMap& a, const CUtensorMap& b, ProductArgs p, cudaStream_t st) {
-  const int64_t tm = (p.m + tg8::kTile - 1) / tg8::kTile, tn = (p.n + tg8::kTile - 1) / tg8::kTile;
+  p.half_n = p.n <= 128 ? 64 : 128;   // narrow outputs: half the products and expansions are not wasted
+  const int64_t tm = (p.m + tg8::kTile - 1) / tg8::kTile, tn = (p.n + 2 * p.half_n - 1) / (2 * p.half_n);
   if (tm * tn > 0x3fffffff || p.m > 0x7ffffc00 || p.n > 0x7ffffc00)
     return fail(TG_ERR_UNSUPPORTED, "%lld x %lld outputs", (long long)p.m, (long long)p.n);
   p.tiles_m = int(tm);
@@ -89,30 +90,35 @@ tg_status launch_product(const CUtensorMap& a, const CUtensorMap& b, ProductArgs
   using S = tg8::ProductShape<MODE>;
   const tg_status s = ensure_smem(reinterpret_cast<const void*>(kern), S::kSmem);
   if (s != TG_OK) return s;
-  const int most = std::max(1, sm_count() / 2), steps = p.blocks * p.planes;
+  const int most = std::max(1, sm_count() / 2);
   p.splits = 1;
   // Few tiles and a long sum: several pairs share a tile's sum and a second
   // kernel joins the parts.  A stage takes about 0.35 us (backward 0.5) when few
   // pairs run; the parts cost their write and read and a launch.
   if (tm * tn * 2 <= most) {
-    const int split_steps = std::max<int>(8, int((steps * tm * tn + most - 1) / most)), splits = (steps + split_steps - 1) / split_steps;
-    const double saved = (S::kBack ? 0.5 : 0.35) * (steps - split_steps), cost = 5.0 + 8e-6 * splits * double(p.m) * double(p.n) / 4.0;
+    const int split_blocks = std::max<int>((8 + p.planes - 1) / p.planes, int((p.blocks * tm * tn + most - 1) / most));
+    const int splits = (p.blocks + split_blocks - 1) / split_blocks;
+    const double saved = (S::kBack ? 0.5 : 0.35) * (p.blocks - split_blocks) * p.planes, cost = 5.0 + 8e-6 * splits * double(p.m) * double(p.n) / 4.0;
     if (splits > 1 && saved > cost) {
-      p.split_steps = split_steps;
+      p.split_blocks = split_blocks;
       p.splits = splits;
     }
   }
+  p.chunk = p.planes == 3 ? 32 : std::max(1, p.blocks);
+  const bool chunked = p.chunk < (p.splits > 1 ? p.split_blocks : p.blocks);
   const int pairs = p.splits > 1 ? int(tm * tn) * p.splits : int(std::min<int64_t>(tm * tn, most));
   const int64_t couples = (tm / 2) * tn;
   p.doubles = S::kHalves == 2 && p.splits == 1 ? int(couples / pairs * pairs) : 0;
   p.singles = int(tm * tn - 2 * int64_t(p.doubles));
   Scratch scratch(st);
-  if (p.splits > 1) {
-    p.ldp = round_up(p.n, 4);
-    const size_t count = size_t(p.splits) * size_t(p.m) * size_t(p.ldp);
-    const cudaError_t e = scratch.reserve(count * sizeof(uint32_t));
+  p.ldp = round_up(p.n, 4);
+  const size_t parts = p.splits > 1 ? size_t(p.splits) * size_t(p.m) * size_t(p.ldp) : 0;
+  const size_t sums = chunked ? size_t(pairs) * 4 * tg8::kEpiWarps * 1024 : 0;   // two tiles of a pair
+  if (parts || sums) {
+    const cudaError_t e = scratch.reserve(Scratch::size_of<uint32_t>(parts) + Scratch::size_of<float4>(sums));
     if (e != cudaSuccess) return fail(TG_ERR_CUDA, "rows8 product scratch: %s", cudaGetErrorString(e));
-    p.part = scratch.take<uint32_t>(count);
+    p.part = scratch.take<uint32_t>(parts);
+    p.work = scratch.take<float4>(sums);
   }
   launch_kernel(kern, 2 * pairs, S::kThreads, S::kSmem, 0, st, a, b, p);
   if (p.splits > 1) launch_kernel(tg8::join_kernel<MODE == tg8::kForward, T>, row_grid(1024, p.n, p.m), 256, 0, 0, st, p);
@@ -137,8 +143,8 @@ tg_status launch_tokens(const CUtensorMap& tokens, const CUtensorMap& weights, P
   // least two stages of the sum
   int split = 1;
   while (split < 8 && tiles * tt * split * 2 <= sm_count() && p.blocks >= 4 * split) split *= 2;
-  p.split_steps = (p.blocks + split - 1) / split;
-  const int stages = std::min(S::kMost, p.split_steps);
+  p.split_blocks = (p.blocks + split - 1) / split;
+  const int stages = std::min(S::kMost, p.split_blocks);
   const size_t smem = size_t(stages) * S::kStage + (split > 1 ? S::kExchange : 0) + 1024;
   auto kern = tg8::tokens_kernel<NT, T>;
   const tg_status s = ensure_smem(reinterpret_cast<const void*>(kern), size_t(S::kMost) * S::kStage + S::kExchange + 1024);

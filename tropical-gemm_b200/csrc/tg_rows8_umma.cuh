@@ -37,7 +37,10 @@ struct ProductArgs {
   int sum;                    // length of the sum (of one plane)
   int blocks, planes;         // stages per plane, planes of g
   int tiles_m, tiles_n;       // 256 x 256 tiles
-  int splits, split_steps;    // the sum in parts, one pair each (1: whole); stages per part
+  int half_n;                 // columns of a tile per CTA: 128, or 64 for outputs of at most 128 columns
+  int splits, split_blocks;   // the sum in parts, one pair each (1: whole); blocks per part
+  int chunk;                  // blocks after which the accumulator is added up in f32 (see Walk)
+  float4* work;               // those sums of the pairs' current tiles, or null
   uint32_t* part;             // raw sums of the parts, (splits x m x ldp), joined by join_kernel
   int64_t ldp;
   int doubles;                // two-tile items, taken first (a multiple of the pairs)
@@ -68,7 +71,7 @@ template <int MODE> struct ProductShape {
   static constexpr int kOwnRaws = kBack ? 2 : 0, kRaws = kBack ? 2 + 2 * kStages : 0;
   // a slot belongs to one conv group for good: a group that met a slot every
   // other turn could take the parity of a turn it did not see for its own
-  static_assert(kOwnRaws % kConvGroups == 0 && kRaws % kConvGroups == 0 && kStages % kConvGroups == 0, "rings and groups");
+  static_assert(kConvGroups == 2 && kOwnRaws % kConvGroups == 0 && kRaws % kConvGroups == 0 && kStages % kConvGroups == 0, "rings and groups");
   static constexpr int kThreads = 32 * (4 + kEpiWarps + (kBack ? kConvWarps * kConvGroups : 0));
   static constexpr int kOffRaw = kStages * kStage;
   static constexpr int kOffStaging = kOffRaw + kOwnRaws * kRawBytes;
@@ -114,18 +117,23 @@ struct RingOf {
 // below it.  Double items first, in whole rounds of all pairs; then the rest
 // one tile at a time, so the last round is as even as single tiles make it.
 // Doubles go in groups of 4 (8 panels of 256 rows), columns outside rows.
+// b0 .. b1: the item's blocks of the sum.
 struct Item {
   int64_t m0, n0;
-  int halves;
+  int halves, b0, b1;
 };
 __device__ __forceinline__ bool item_at(const ProductArgs& p, int pair, int pairs, int i, Item& it) {
   if (p.splits > 1) {   // one part of one tile per pair
-    const int tile = pair / p.splits;
+    const int tile = pair / p.splits, part = pair - tile * p.splits;
     it.m0 = int64_t(tile % p.tiles_m) * kTile;
-    it.n0 = int64_t(tile / p.tiles_m) * kTile;
+    it.n0 = int64_t(tile / p.tiles_m) * 2 * p.half_n;
     it.halves = 1;
+    it.b0 = part * p.split_blocks;
+    it.b1 = min(p.blocks, it.b0 + p.split_blocks);
     return i == 0;
   }
+  it.b0 = 0;
+  it.b1 = p.blocks;
   constexpr int kGroup = 4;
   const int panels = p.tiles_m >> 1;
   int d, half = 0;
@@ -140,16 +148,39 @@ __device__ __forceinline__ bool item_at(const ProductArgs& p, int pair, int pair
     half = int(s & 1);
     if (d >= panels * p.tiles_n) {   // the last panel, when their number is odd
       it.m0 = int64_t(p.tiles_m - 1) * kTile;
-      it.n0 = (s - 2 * int64_t(panels * p.tiles_n - p.doubles)) * kTile;
+      it.n0 = (s - 2 * int64_t(panels * p.tiles_n - p.doubles)) * 2 * p.half_n;
       return true;
     }
   }
   const int per = kGroup * p.tiles_n, g = d / per, first = g * kGroup, rows = min(kGroup, panels - first);
   const int in = d - g * per;
   it.m0 = int64_t(2 * (first + in % rows) + half) * kTile;
-  it.n0 = int64_t(in / rows) * kTile;
+  it.n0 = int64_t(in / rows) * 2 * p.half_n;
   return true;
 }
+
+// The order of an item's stages: chunks of blocks, in each the planes of g from
+// the smallest parts to the largest, in each the chunk's blocks.  With three
+// planes (f32) a chunk is 32 blocks: the tensor core's f32 sums lose about the
+// square root of the additions (a sum of 8014 terms was off by 2.2e-6, the
+// plain f32 product by 1.2e-6), so after a chunk the epilogue adds the
+// accumulator to a running f32 sum.  Otherwise one chunk is the whole sum.
+struct Walk {
+  int block, plane, c0, c1, chunk, b1, planes;
+  __device__ __forceinline__ Walk(const ProductArgs& p, const Item& it)
+      : block(it.b0), plane(0), c0(it.b0), c1(min(it.b0 + p.chunk, it.b1)), chunk(p.chunk), b1(it.b1), planes(p.planes) {}
+  __device__ __forceinline__ bool first() const { return block == c0 && plane == 0; }   // of a chunk
+  __device__ __forceinline__ bool last() const { return block + 1 == c1 && plane + 1 == planes; }
+  __device__ __forceinline__ bool more() const { return c0 < b1; }
+  __device__ __forceinline__ void next() {
+    if (++block < c1) return;
+    block = c0;
+    if (++plane < planes) return;
+    plane = 0;
+    block = c0 = c1;
+    c1 = min(c1 + chunk, b1);
+  }
+};
 
 // 64 bytes of each of 32 rows, one row per lane, to global memory through
 // shared memory, so that a warp's store covers 8 rows' 64 bytes (a store of 32
@@ -242,8 +273,6 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // warp: uniform
   const uint32_t rank = umma::cta_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int step0 = p.splits > 1 ? pair % p.splits * p.split_steps : 0;   // this pair's part of the sum
-  const int steps = min(p.blocks * p.planes - step0, p.splits > 1 ? p.split_steps : p.blocks * p.planes);
 
   if (warp == 0 && lane == 0) {
     umma::tma_prefetch(&map_a);
@@ -276,11 +305,11 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     RingAt<S::kStages> at;
     Item item;
     for (int i = 0; ok && item_at(p, pair, pairs, i, item); i++) {
-      const int row = int(item.m0) + int(rank) * kHalf, col = int(item.n0) + int(rank) * kHalf;
-      int plane = step0 / p.blocks, block = step0 - plane * p.blocks;
-      for (int step = 0; step < steps; step++, at.next()) {
+      const int row = int(item.m0) + int(rank) * kHalf, col = int(item.n0) + int(rank) * p.half_n;
+      for (Walk at_sum(p, item); at_sum.more(); at_sum.next(), at.next()) {
         if (!umma::bar_wait(empty(at.slot), at.parity ^ 1)) { ok = false; break; }
         const uint32_t b = base + at.slot * S::kStage, bar = umma::map_rank(full(at.slot), 0);
+        const int block = at_sum.block, plane = at_sum.plane;
         if (issue) {
           if (rank == 0) umma::bar_expect(full(at.slot), 2 * kOperand * (item.halves + (S::kBack ? 0 : 1)));
           if (MODE == kForward) umma::tma_load_3d_pair(b, &map_b, block * 128, col, 0, bar);
@@ -299,7 +328,6 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             }
           }
         }
-        if (++block == p.blocks) { block = 0; plane++; }
       }
     }
     if (!ok) umma::drain_copies();
@@ -309,22 +337,20 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     RingOf at{raws};
     Item item;
     for (int i = 0; ok && item_at(p, pair, pairs, i, item); i++) {
-      const int col = int(item.n0) + int(rank) * kHalf;
-      int block = step0 % p.blocks;
-      for (int step = 0; step < steps; step++, at.next()) {
+      const int col = int(item.n0) + int(rank) * p.half_n;
+      for (Walk at_sum(p, item); at_sum.more(); at_sum.next(), at.next()) {
         if (!umma::bar_wait(raw_empty(at.slot), at.parity ^ 1)) { ok = false; break; }
         if (issue) {
           umma::bar_expect(raw_full(at.slot), kRawBytes);
-          umma::tma_load_3d_pair(raw_tile(at.slot), &map_b, col, block * 64, 0, umma::map_rank(raw_full(at.slot), rank));
+          umma::tma_load_3d_pair(raw_tile(at.slot), &map_b, col, at_sum.block * 64, 0, umma::map_rank(raw_full(at.slot), rank));
         }
-        if (++block == p.blocks) block = 0;
       }
     }
     if (!ok) umma::drain_copies();
   } else if (warp == 1 && rank == 0) {
     // ---- products, issued by one thread of the leader for both SMs
-    constexpr uint32_t idesc = MODE == kForward ? umma::instr_desc(2, 1, false, false, kTile, kTile)
-                                                : umma::instr_desc(1, 1, MODE == kBackCols, true, kTile, kTile);
+    const uint32_t idesc = MODE == kForward ? umma::instr_desc(2, 1, false, false, kTile, 2 * p.half_n)
+                                            : umma::instr_desc(1, 1, MODE == kBackCols, true, kTile, 2 * p.half_n);
     // bytes from one instruction's slice of the sum to the next: 32 along a
     // 128-byte row, or 16 rows
     constexpr uint32_t step_a = MODE == kBackCols ? 2048 : 32, step_b = MODE == kForward ? 32 : 2048;
@@ -335,29 +361,33 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const bool issue = umma::elect_one();
     RingAt<S::kStages> at;
     Item item;
-    int n = 0;   // tiles so far: tile n sums into accumulator n % 2
-    for (int i = 0; ok && item_at(p, pair, pairs, i, item); n += item.halves, i++) {
-      for (int step = 0; step < steps; step++, at.next()) {
+    int n = 0;   // sums so far: sum n goes into accumulator n % 2
+    for (int i = 0; ok && item_at(p, pair, pairs, i, item); i++) {
+      for (Walk at_sum(p, item); at_sum.more(); at_sum.next(), at.next()) {
         if (!umma::bar_wait<S::kBack>(full(at.slot), at.parity)) { ok = false; break; }
         const uint32_t off = at.slot * (S::kStage >> 4);
+        const bool first = at_sum.first();
 #pragma unroll
         for (int h = 0; h < S::kHalves; h++) {
           if (h == item.halves) break;
           const int buf = (n + h) & 1;
-          if (step == 0 && !umma::bar_wait<true>(acc_empty(buf), (((n + h) >> 1) & 1) ^ 1)) { ok = false; break; }
+          if (first && !umma::bar_wait<true>(acc_empty(buf), (((n + h) >> 1) & 1) ^ 1)) { ok = false; break; }
           umma::fence_after();
           const uint32_t offa = off + h * (kOperand >> 4);
           if (issue) {
 #pragma unroll
             for (int j = 0; j < 4; j++)
-              umma::mma<2, MODE == kForward>(tmem + buf * kTile, da0 + (offa + (j * step_a >> 4)), db0 + (off + (j * step_b >> 4)), idesc, step | j);
+              umma::mma<2, MODE == kForward>(tmem + buf * kTile, da0 + (offa + (j * step_a >> 4)), db0 + (off + (j * step_b >> 4)), idesc, !first || j);
           }
         }
         if (!ok) break;
         if (issue) umma::mma_commit<2>(empty(at.slot));
+        if (at_sum.last()) {
+          if (issue)
+            for (int h = 0; h < item.halves; h++) umma::mma_commit<2>(acc_full((n + h) & 1));
+          n += item.halves;
+        }
       }
-      if (issue && ok)
-        for (int h = 0; h < item.halves; h++) umma::mma_commit<2>(acc_full((n + h) & 1));
       __syncwarp();
     }
     if (!ok) umma::drain_copies();
@@ -369,69 +399,99 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     float* cols = reinterpret_cast<float*>(smem + S::kOffCols);
     Item item;
     int n = 0;
-    for (int i = 0, h = 0; item_at(p, pair, pairs, i, item); n++) {   // h: the tile within the item
-      const int64_t n0 = item.n0, row0 = item.m0 + h * kTile + rank * kHalf + w * 32, row = row0 + lane;
-      const int rows = int(max(int64_t(0), min(int64_t(32), p.m - row0)));
-      const int buf = n & 1;
-      if (++h == item.halves) { h = 0; i++; }
-      float rs = 0.f;
-      if (MODE == kForward && p.splits == 1) {
-        asm volatile("bar.sync 1, 256;" ::: "memory");   // the last tile's columns are no longer read
-        const bool in = n0 + tid < p.n;
-        cols[tid] = in ? p.col_scale[n0 + tid] : 0.f;
-        cols[kTile + tid] = in && p.bias ? to_f32(static_cast<const T*>(p.bias)[n0 + tid]) : 0.f;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (row < p.m) rs = p.row_scale[row];
-      }
-      if (ok) {   // a whole tile's sum: the limit grows with its length
-        bool done = false;
-        for (int k = 0; k <= steps >> 10 && !done; k++) done = umma::bar_wait(acc_full(buf), (n >> 1) & 1);
-        ok = done;
-      }
-      umma::fence_after();
-      const uint32_t from = tmem + buf * kTile + half * 128 + (uint32_t(w * 32) << 16);
-      const int64_t col0 = n0 + half * 128;
-      auto read_out = [&] {   // the next tile's products may have the accumulator
-        umma::fence_before();
-        __syncwarp();
-        if (lane == 0) umma::bar_arrive_cluster(umma::map_rank(acc_empty(buf), 0));
-      };
-      auto value = [&](uint32_t acc, int c) {
-        float z = __uint_as_float(acc);
-        if (MODE == kForward) z = float(int(acc)) * rs * cols[half * 128 + c] + cols[kTile + half * 128 + c];
-        return ok ? z : __uint_as_float(0x7fffffffu);   // a wait ran out: the outputs say so
-      };
-      if (p.splits > 1 || sizeof(T) == 4) {
-#pragma unroll 1
-        for (int c = 0; c < 128; c += 16) {
-          uint32_t acc[16];
-          umma::tmem_load16(from + c, acc);
-          umma::tmem_load_wait();
-          if (c == 112) read_out();
-          if (col0 + c >= p.n) continue;
-          if (p.splits > 1) {
-            if (!ok) {   // NaN, or a value no integer sum takes
-#pragma unroll
-              for (int e = 0; e < 16; e++) acc[e] = MODE == kForward ? 0x80000000u : 0x7fffffffu;
-            }
-            store_rows64(p.part + (int64_t(pair % p.splits) * p.m + row0) * p.ldp + col0 + c, p.ldp, rows, p.ldp - col0 - c, true, acc, staging, lane);
-          } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int e = 0; e < 16; e++) acc[e] = __float_as_uint(value(acc[e], c + e));
-            store_rows64(static_cast<T*>(p.c) + row0 * p.ldc + col0 + c, p.ldc, rows, p.n - col0 - c, p.vec, acc, staging, lane);
-          }
+    for (int i = 0; item_at(p, pair, pairs, i, item); i++) {
+      const int chunks = (item.b1 - item.b0 + p.chunk - 1) / p.chunk;
+      for (int ch = 0, h = 0; ch < chunks; n++) {   // h: the tile within the item
+        const int tile = h, buf = n & 1;
+        const bool first = ch == 0, last = ch + 1 == chunks;
+        const int64_t n0 = item.n0, row0 = item.m0 + tile * kTile + rank * kHalf + w * 32, row = row0 + lane;
+        const int rows = int(max(int64_t(0), min(int64_t(32), p.m - row0)));
+        const int columns = min(128, 2 * p.half_n - half * 128);   // of this warp's half: none in narrow tiles' second
+        if (++h == item.halves) { h = 0; ch++; }
+        float rs = 0.f;
+        if (MODE == kForward && p.splits == 1) {
+          asm volatile("bar.sync 1, 256;" ::: "memory");   // the last tile's columns are no longer read
+          const bool in = n0 + tid < p.n;
+          cols[tid] = in ? p.col_scale[n0 + tid] : 0.f;
+          cols[kTile + tid] = in && p.bias ? to_f32(static_cast<const T*>(p.bias)[n0 + tid]) : 0.f;
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+          if (row < p.m) rs = p.row_scale[row];
         }
-      } else if constexpr (sizeof(T) == 2) {
-#pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
-          uint32_t acc[32], z[16];
-          umma::tmem_load32(from + c, acc);
-          umma::tmem_load_wait();
-          if (c == 96) read_out();
-          if (col0 + c >= p.n) continue;
+        if (ok) {   // a whole sum: the limit grows with its length
+          bool done = false;
+          for (int k = 0; k <= (item.b1 - item.b0) * p.planes >> 10 && !done; k++) done = umma::bar_wait(acc_full(buf), (n >> 1) & 1);
+          ok = done;
+        }
+        umma::fence_after();
+        const uint32_t from = tmem + buf * kTile + half * 128 + (uint32_t(w * 32) << 16);
+        const int64_t col0 = n0 + half * 128;
+        auto read_out = [&] {   // the next sum may have the accumulator
+          umma::fence_before();
+          __syncwarp();
+          if (lane == 0) umma::bar_arrive_cluster(umma::map_rank(acc_empty(buf), 0));
+        };
+        auto value = [&](uint32_t acc, int c) {
+          float z = __uint_as_float(acc);
+          if (MODE == kForward) z = float(int(acc)) * rs * cols[half * 128 + c] + cols[kTile + half * 128 + c];
+          return ok ? z : __uint_as_float(0x7fffffffu);   // a wait ran out: the outputs say so
+        };
+        // 16 columns' sums so far, kept where the same thread finds them again
+        auto add_up = [&](uint32_t* acc, int c) {
+          if (!S::kBack || (first && last)) return;
+          float4* kept = p.work + (((int64_t(pair) * 2 + rank) * 2 + tile) * kEpiWarps + (warp - 4)) * 1024 + c / 4 * 32 + lane;
 #pragma unroll
-          for (int e = 0; e < 16; e++) z[e] = pack_pair<T>(value(acc[2 * e], c + 2 * e), value(acc[2 * e + 1], c + 2 * e + 1));
-          store_rows64(static_cast<T*>(p.c) + row0 * p.ldc + col0 + c, p.ldc, rows, p.n - col0 - c, p.vec, z, staging, lane);
+          for (int j = 0; j < 4; j++) {
+            float4 o = first ? make_float4(0.f, 0.f, 0.f, 0.f) : kept[j * 32];
+            o.x += __uint_as_float(acc[4 * j]);
+            o.y += __uint_as_float(acc[4 * j + 1]);
+            o.z += __uint_as_float(acc[4 * j + 2]);
+            o.w += __uint_as_float(acc[4 * j + 3]);
+            if (!last) kept[j * 32] = o;
+            acc[4 * j] = __float_as_uint(o.x);
+            acc[4 * j + 1] = __float_as_uint(o.y);
+            acc[4 * j + 2] = __float_as_uint(o.z);
+            acc[4 * j + 3] = __float_as_uint(o.w);
+          }
+        };
+        if (columns <= 0) {
+          read_out();
+        } else if (p.splits > 1 || sizeof(T) == 4) {
+#pragma unroll 1
+          for (int c = 0; c < columns; c += 16) {
+            uint32_t acc[16];
+            umma::tmem_load16(from + c, acc);
+            umma::tmem_load_wait();
+            if (c + 16 == columns) read_out();
+            if (col0 + c >= p.n) continue;
+            add_up(acc, c);
+            if (!last) continue;
+            if (p.splits > 1) {
+              if (!ok) {   // NaN, or a value no integer sum takes
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[e] = MODE == kForward ? 0x80000000u : 0x7fffffffu;
+              }
+              store_rows64(p.part + (int64_t(pair % p.splits) * p.m + row0) * p.ldp + col0 + c, p.ldp, rows, p.ldp - col0 - c, true, acc, staging, lane);
+            } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+              for (int e = 0; e < 16; e++) acc[e] = __float_as_uint(value(acc[e], c + e));
+              store_rows64(static_cast<T*>(p.c) + row0 * p.ldc + col0 + c, p.ldc, rows, p.n - col0 - c, p.vec, acc, staging, lane);
+            }
+          }
+        } else if constexpr (sizeof(T) == 2) {
+#pragma unroll 1
+          for (int c = 0; c < columns; c += 32) {
+            uint32_t acc[32], z[16];
+            umma::tmem_load32(from + c, acc);
+            umma::tmem_load_wait();
+            if (c + 32 == columns) read_out();
+            if (col0 + c >= p.n) continue;
+            add_up(acc, c);
+            add_up(acc + 16, c + 16);
+            if (!last) continue;
+#pragma unroll
+            for (int e = 0; e < 16; e++) z[e] = pack_pair<T>(value(acc[2 * e], c + 2 * e), value(acc[2 * e + 1], c + 2 * e + 1));
+            store_rows64(static_cast<T*>(p.c) + row0 * p.ldc + col0 + c, p.ldc, rows, p.n - col0 - c, p.vec, z, staging, lane);
+          }
         }
       }
     }
@@ -442,9 +502,6 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     // swizzle spreads them over all banks on both sides.
     const int w = (warp - 4 - kEpiWarps) % kConvWarps, group = (warp - 4 - kEpiWarps) / kConvWarps;
     const int r8 = lane & 7, c4 = lane >> 3;
-    int items = p.splits > 1 ? 1 : p.doubles / pairs;
-    if (p.splits == 1 && p.singles > pair) items += (p.singles - pair + pairs - 1) / pairs;
-    const int64_t total = int64_t(items) * steps;
     RingOf rw{raws};
     RingAt<S::kStages> cv;
     float sc[2], next[2];
@@ -453,25 +510,36 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
       for (int i = 0; i < 2; i++) f[i] = p.sum_scale ? (r0 + 8 * i < p.sum ? p.sum_scale[r0 + 8 * i] : 0.f) : 1.f;
     };
-    int block = (step0 + group) % p.blocks;
-    factors(block, next);
     for (int i = 0; i < group; i++) { rw.next(); cv.next(); }
-    for (int64_t it = group; it < total; it += kConvGroups) {
+    Item item;
+    bool started = false;
+    int turn = 0;   // stages go to the groups in turn
+    for (int i = 0; ok && item_at(p, pair, pairs, i, item); i++)
+    for (Walk at_sum(p, item); at_sum.more(); at_sum.next(), turn ^= 1) {
+      if (turn != group) continue;
+      if (!started) factors(at_sum.block, next);
+      started = true;
       sc[0] = next[0];
       sc[1] = next[1];
-      block = (block + kConvGroups) % p.blocks;
-      factors(block, next);   // a turn ahead: the load's latency stays out of the wait
+      // a turn ahead, so that the load's latency stays out of the wait (factors
+      // are there only with one plane, whose walk is straight, and all items of a
+      // pair have the same blocks)
+      int ahead = at_sum.block + kConvGroups;
+      while (ahead >= item.b1) ahead -= item.b1 - item.b0;
+      factors(ahead, next);
       if (!umma::bar_wait(raw_full(rw.slot), rw.parity)) { ok = false; break; }
       const uint32_t in = raw_tile(rw.slot) + (w * 16 + r8) * 128;
+      const bool wide = p.half_n == 128;   // else the first 64 columns only
       uint32_t q[4][4];
 #pragma unroll
       for (int i = 0; i < 4; i++)   // rows + 8 (i / 2), 64 columns (i % 2)
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q[i][0]), "=r"(q[i][1]), "=r"(q[i][2]), "=r"(q[i][3])
+        if (wide || !(i & 1)) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q[i][0]), "=r"(q[i][1]), "=r"(q[i][2]), "=r"(q[i][3])
                      : "r"(in + (i >> 1) * 1024 + ((((i & 1) * 4 + c4) ^ r8) << 4)));
       if (!umma::bar_wait(empty(cv.slot), cv.parity ^ 1)) { ok = false; break; }
       const uint32_t out = base + cv.slot * S::kStage + (w * 16 + r8) * 128;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
+        if (!wide && (i & 1)) continue;
         uint32_t o[8];
         const float f = sc[i >> 1];
 #pragma unroll
@@ -544,7 +612,7 @@ __global__ void __launch_bounds__(128) tokens_kernel(const __grid_constant__ CUt
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = blockIdx.x % split;
   const int n0 = int(blockIdx.x / split) * 128, t0 = int(blockIdx.y) * NT, tokens = min(NT, int(p.m) - t0);
-  const int first = rank * p.split_steps, steps = max(0, min(p.split_steps, p.blocks - first));   // the last CTAs may have no share
+  const int first = rank * p.split_blocks, steps = max(0, min(p.split_blocks, p.blocks - first));   // the last CTAs may have no share
 
   if (warp == 0 && lane == 0) {
     umma::tma_prefetch(&map_weights);
