@@ -14,12 +14,13 @@
 // Persistent: a pair walks tiles in groups of row panels, so what it reads
 // stays in L2.
 //
-// What bounds it: shared memory.  Per 256 x 256 x (128 bytes) step an SM's
-// tensor core needs 512 cycles, and reads 32 KB (256 cycles at 128 bytes per
-// cycle); TMA writes 32 KB more (forward: 512 in all).  Backward, a step
-// writes 16 + 8 KB, and the expansion reads 8 and writes 16: 640 cycles, and
-// measured 860.  Two tiles that share the right operand need 896 (forward)
-// and 1024 (backward) cycles per 1024 of tensor work.
+// What bounds it: power for long sums (8192^3 forward: 0.33 ms, with zero operands
+// 0.25), and shared memory.  Per 256 x 256 x (128 bytes) step an SM's tensor core
+// needs 512 cycles and reads 32 KB (256 cycles at 128 bytes per cycle); TMA writes
+// 32 KB more (forward: 512 in all).  Backward a step writes 16 + 8 KB, and the
+// expansion reads 8 and writes 16: 640 cycles.  Two tiles that share the right
+// operand bring that to 1024 per 1024 of tensor work (8192 x 8192 x 4096: 0.44 ms
+// one tile at a time, 0.37 two); forward they gain nothing (0.176, 0.196 ms).
 #pragma once
 #include "tg_rows8.cuh"
 #include "tg_umma.cuh"
@@ -40,7 +41,7 @@ struct ProductArgs {
   int half_n;                 // columns of a tile per CTA: 128, or 64 for outputs of at most 128 columns
   int splits, split_blocks;   // the sum in parts, one pair each (1: whole); blocks per part
   int chunk;                  // blocks after which the accumulator is added up in f32 (see Walk)
-  float4* work;               // those sums of the pairs' current tiles, or null
+  float4* work;               // those sums of the pairs' current tiles, or null; L2 keeps them
   uint32_t* part;             // raw sums of the parts, (splits x m x ldp), joined by join_kernel
   int64_t ldp;
   int doubles;                // two-tile items, taken first (a multiple of the pairs)
@@ -161,10 +162,11 @@ __device__ __forceinline__ bool item_at(const ProductArgs& p, int pair, int pair
 
 // The order of an item's stages: chunks of blocks, in each the planes of g from
 // the smallest parts to the largest, in each the chunk's blocks.  With three
-// planes (f32) a chunk is 32 blocks: the tensor core's f32 sums lose about the
-// square root of the additions (a sum of 8014 terms was off by 2.2e-6, the
-// plain f32 product by 1.2e-6), so after a chunk the epilogue adds the
-// accumulator to a running f32 sum.  Otherwise one chunk is the whole sum.
+// planes (f32) a chunk is 16 blocks, 1024 terms: the tensor core's f32 sums
+// lose in proportion to the additions (relative error 1.3e-6 after 2048 terms,
+// 6.6e-7 after 1024, 3.1e-7 after 512; the plain f32 product of 8192 terms
+// 1.6e-6), so after a chunk the epilogue adds the accumulator to a running f32
+// sum.  Otherwise one chunk is the whole sum.
 struct Walk {
   int block, plane, c0, c1, chunk, b1, planes;
   __device__ __forceinline__ Walk(const ProductArgs& p, const Item& it)
@@ -777,24 +779,41 @@ __global__ void __launch_bounds__(256) join_kernel(const ProductArgs p) {
 // ldo: parts 0 .. planes - 1 from the smallest to the largest, so that the
 // sums take the small ones first.  The upper parts are truncations, which
 // leaves an exact rest: three parts hold all 24 bits, two hold 16 rounded.
+// Eight columns per thread; vec: g's rows are 16-byte aligned.
 template <typename GT>
 __global__ void __launch_bounds__(256) split_kernel(int64_t rows, int64_t cols, const GT* g, int64_t ldg, const float* scale,
-                                                    int scale_rows, bf16* out, int64_t ldo, int planes) {
+                                                    int scale_rows, bf16* out, int64_t ldo, int planes, int vec) {
   after_previous_kernel();
-  const int64_t c = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t c = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 8;
   if (c >= ldo) return;
+  float by_col[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) by_col[e] = scale && !scale_rows && c + e < cols ? scale[c + e] : 1.f;
   for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
-    float v = 0.f;
-    if (c < cols) {
-      v = to_f32(g[r * ldg + c]);
-      if (scale) v *= scale[scale_rows ? r : c];
+    float v[8];
+    if (vec && c + 8 <= cols) {
+      Vec8<GT> a;
+      a.load(g + r * ldg + c);
+      a.get(v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = c + e < cols ? to_f32(g[r * ldg + c + e]) : 0.f;
     }
-    const bool finite = fabsf(v) < __uint_as_float(0x7f800000u);
+    const float by_row = scale && scale_rows ? scale[r] : 1.f;
+    bool finite[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      v[e] *= scale_rows ? by_row : by_col[e];
+      finite[e] = fabsf(v[e]) < __uint_as_float(0x7f800000u);
+    }
     for (int i = planes - 1; i >= 0; i--) {
-      const uint32_t bits = __float_as_uint(v) & 0xffff0000u;
-      bf16 part = i && finite ? __ushort_as_bfloat16(uint16_t(bits >> 16)) : __float2bfloat16_rn(v);
-      out[(int64_t(i) * rows + r) * ldo + c] = part;
-      v = finite ? v - __bfloat162float(part) : 0.f;
+      float part[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        part[e] = i && finite[e] ? __uint_as_float(__float_as_uint(v[e]) & 0xffff0000u) : __bfloat162float(__float2bfloat16_rn(v[e]));
+        v[e] = finite[e] ? v[e] - part[e] : 0.f;
+      }
+      store8(out + (int64_t(i) * rows + r) * ldo + c, part);
     }
   }
 }
