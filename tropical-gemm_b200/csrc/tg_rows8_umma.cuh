@@ -819,31 +819,39 @@ __global__ void __launch_bounds__(256) split_kernel(int64_t rows, int64_t cols, 
 }
 
 // 8-bit rows copied to rows of ldo, a multiple of 16, zeros behind; up to two
-// matrices in one launch (blockIdx.z).  16 bytes per thread: five aligned
-// words, each with at least one byte of the row, shifted into place.
+// matrices in one launch (blockIdx.z).  16 bytes per thread: the one or two
+// aligned 16-byte words that hold them (each with at least one byte of the
+// row), shifted into place.
 struct PadArgs {
   const int8_t* q[2];
   int8_t* out[2];
   int64_t rows[2], cols[2], ldq[2], ldo[2];
 };
-__global__ void __launch_bounds__(256) pad8_kernel(const PadArgs p) {
+__global__ void __launch_bounds__(256) pad8_kernel(const __grid_constant__ PadArgs p) {   // indexed in place: a copy per thread took 17 of 31 us at 4096 x 4095
   after_previous_kernel();
   const int z = blockIdx.z;
   const int64_t per = p.ldo[z] / 16, total = p.rows[z] * per;
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
-    const int64_t r = i / per, c = (i - r * per) * 16;
+    const int64_t r = total <= 0xffffffffll ? int64_t(uint32_t(i) / uint32_t(per)) : i / per, c = (i - r * per) * 16;
     const int64_t left = p.cols[z] - c;   // bytes of the row from c on
     uint32_t o[4] = {0, 0, 0, 0};
     if (left > 0) {
       const int8_t* from = p.q[z] + r * p.ldq[z] + c;
-      const uint32_t skew = uint32_t(reinterpret_cast<uintptr_t>(from) & 3);
-      const uint32_t* words = reinterpret_cast<const uint32_t*>(from - skew);
-      uint32_t w[5];
+      const uint32_t skew = uint32_t(reinterpret_cast<uintptr_t>(from) & 15);
+      const uint4* words = reinterpret_cast<const uint4*>(from - skew);
+      const uint4 lo = words[0], hi = skew && 16 < left + skew ? words[1] : make_uint4(0, 0, 0, 0);
+      uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      if (skew & 8) {
 #pragma unroll
-      for (int k = 0; k < 5; k++) w[k] = 4 * k < left + skew ? words[k] : 0u;
+        for (int k = 0; k < 6; k++) w[k] = w[k + 2];
+      }
+      if (skew & 4) {
+#pragma unroll
+        for (int k = 0; k < 5; k++) w[k] = w[k + 1];
+      }
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        o[k] = __funnelshift_r(w[k], w[k + 1], skew * 8);
+        o[k] = __funnelshift_r(w[k], w[k + 1], (skew & 3) * 8);
         const int64_t valid = left - 4 * k;
         if (valid < 4) o[k] = valid <= 0 ? 0u : o[k] & ((1u << (8 * valid)) - 1);
       }
