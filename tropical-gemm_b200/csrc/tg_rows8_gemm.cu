@@ -86,10 +86,7 @@ tg_status launch_product(const CUtensorMap& a, const CUtensorMap& b, ProductArgs
   p.tiles_m = int(tm);
   p.tiles_n = int(tn);
   p.vec = aligned(p.c, 16) && (p.ldc * int64_t(sizeof(T))) % 16 == 0;
-  auto kern = tg8::product_kernel<MODE, T>;
   using S = tg8::ProductShape<MODE>;
-  const tg_status s = ensure_smem(reinterpret_cast<const void*>(kern), S::kSmem);
-  if (s != TG_OK) return s;
   const int most = std::max(1, sm_count() / 2);
   p.splits = 1;
   // Few tiles and a long sum: several pairs share a tile's sum and a second
@@ -122,7 +119,15 @@ tg_status launch_product(const CUtensorMap& a, const CUtensorMap& b, ProductArgs
     p.part = scratch.take<uint32_t>(parts);
     p.work = scratch.take<float4>(sums);
   }
-  launch_kernel(kern, 2 * pairs, S::kThreads, S::kSmem, 0, st, a, b, p);
+  auto run = [&](auto kern) {
+    const tg_status s = ensure_smem(reinterpret_cast<const void*>(kern), S::kSmem);
+    if (s == TG_OK) launch_kernel(kern, 2 * pairs, S::kThreads, S::kSmem, 0, st, a, b, p);
+    return s;
+  };
+  tg_status launched;
+  if constexpr (S::kBack) launched = chunked ? run(tg8::product_kernel<MODE, T, true>) : run(tg8::product_kernel<MODE, T, false>);
+  else launched = run(tg8::product_kernel<MODE, T, false>);
+  if (launched != TG_OK) return launched;
   if (p.splits > 1) launch_kernel(tg8::join_kernel<MODE == tg8::kForward, T>, row_grid(1024, p.n, p.m), 256, 0, 0, st, p);
   return check_launch("rows8 product");
 }

@@ -249,7 +249,9 @@ template <> __device__ __forceinline__ uint32_t pack_pair<f16>(float a, float b)
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-template <int MODE, typename T>
+// SUMS: the sum has several chunks (kept out of the other instances: a short
+// product is on the GPU for 5 us and pays for every instruction it fetches).
+template <int MODE, typename T, bool SUMS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ProductShape<MODE>::kThreads, 1)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs p) {
   using S = ProductShape<MODE>;
@@ -402,10 +404,10 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     Item item;
     int n = 0;
     for (int i = 0; item_at(p, pair, pairs, i, item); i++) {
-      const int chunks = (item.b1 - item.b0 + p.chunk - 1) / p.chunk;
+      const int chunks = SUMS ? (item.b1 - item.b0 + p.chunk - 1) / p.chunk : 1;
       for (int ch = 0, h = 0; ch < chunks; n++) {   // h: the tile within the item
         const int tile = h, buf = n & 1;
-        const bool first = ch == 0, last = ch + 1 == chunks;
+        const bool first = !SUMS || ch == 0, last = !SUMS || ch + 1 == chunks;
         const int64_t n0 = item.n0, row0 = item.m0 + tile * kTile + rank * kHalf + w * 32, row = row0 + lane;
         const int rows = int(max(int64_t(0), min(int64_t(32), p.m - row0)));
         const int columns = min(128, 2 * p.half_n - half * 128);   // of this warp's half: none in narrow tiles' second
@@ -439,7 +441,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         };
         // 16 columns' sums so far, kept where the same thread finds them again
         auto add_up = [&](uint32_t* acc, int c) {
-          if (!S::kBack || (first && last)) return;
+          if (!SUMS || (first && last)) return;
           float4* kept = p.work + (((int64_t(pair) * 2 + rank) * 2 + tile) * kEpiWarps + (warp - 4)) * 1024 + c / 4 * 32 + lane;
 #pragma unroll
           for (int j = 0; j < 4; j++) {
