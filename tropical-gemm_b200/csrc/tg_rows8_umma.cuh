@@ -37,7 +37,7 @@ struct ProductArgs {
   const float* sum_scale;     // backward: one factor per index of the sum, or null (taken into g)
   int sum;                    // length of the sum (of one plane)
   int blocks, planes;         // stages per plane, planes of g
-  int tiles_m, tiles_n;       // 256 x 256 tiles
+  int tiles_m, tiles_n;       // tiles of 256 x 2 half_n
   int half_n;                 // columns of a tile per CTA: 128, or 64 for outputs of at most 128 columns
   int splits, split_blocks;   // the sum in parts, one pair each (1: whole); blocks per part
   int chunk;                  // blocks after which the accumulator is added up in f32 (see Walk)
@@ -518,8 +518,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     Item item;
     bool started = false;
     int turn = 0;   // stages go to the groups in turn
-    for (int i = 0; ok && item_at(p, pair, pairs, i, item); i++)
-    for (Walk at_sum(p, item); at_sum.more(); at_sum.next(), turn ^= 1) {
+    for (int it = 0; ok && item_at(p, pair, pairs, it, item); it++)
+    for (Walk at_sum(p, item); at_sum.more(); at_sum.next(), turn ^= 1) {   // one nest: every stage of every item
       if (turn != group) continue;
       if (!started) factors(at_sum.block, next);
       started = true;
