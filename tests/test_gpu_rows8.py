@@ -622,3 +622,29 @@ def test_graph_capture():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(out, run()))
+
+
+def test_products_on_several_streams_at_once():
+    """Few-token and paired products, splits and joins, side by side: the same bits as alone."""
+    g = gen(31)
+    cases = []
+    for m, n, k in ((1, 4096, 4096), (40, 1000, 2048), (100, 700, 4096), (700, 1300, 512), (3, 515, 1111)):
+        a, b, grad = rand8(g, m, k), rand8(g, n, k), randn(g, m, n)
+        cases.append((a, b, grad, grad.bfloat16()))
+
+    def run(c):
+        a, b, grad, grad16 = c
+        return (rows8.matmul(a, b), *rows8.matmul_backward(grad, a, b), *rows8.matmul_backward(grad16, a, b))
+
+    want = [run(c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for turn in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                j = (turn + i) % len(cases)
+                got.append((j, run(cases[j])))
+    torch.cuda.synchronize()
+    for j, r in got:
+        assert all(torch.equal(x, y) for x, y in zip(r, want[j]))
