@@ -202,7 +202,9 @@ tg_status tg_gemm_i32_noalloc(tg_semiring semiring, tg_layout layout,
  * ------------------------------------------------------------------------ */
 
 /* q, scale = x in 8-bit rows: scale = max|x[r,:]| / 127, q = x / scale
- * rounded to nearest even, in [-127, 127].  A row whose largest magnitude is
+ * rounded to nearest even, in [-127, 127] (ties of x * 127 / max exactly; a
+ * quotient within 2^-15 of a tie that is none may take either neighbour, the
+ * division being f32).  A row whose largest magnitude is
  * below 2^-120 becomes zeros with scale 0; a row that holds a NaN or an
  * infinity gets scale NaN, so that everything made of it is NaN. */
 tg_status tg_rows8_quantize(tg_dtype dtype, int64_t rows, int64_t cols,

@@ -175,16 +175,16 @@ __global__ void __launch_bounds__(G == 1 ? 1024 : 512) rows_kernel(RowArgs p) {
     for (int e = 0; e < 8; e++) y[e] = NORM ? v[g][e] * u * w[e] : v[g][e];
     if constexpr (ACCESS != kScalar) {
       const int c = at(g, 0);
-      store_bytes<ACCESS>(q, c, cols, quant_pack8(y, qy.inv));
-      if (NORM && k) store_bytes<ACCESS>(k, c, cols, quant_pack8(v[g], qh.inv));
+      store_bytes<ACCESS>(q, c, cols, quant_pack8(y, qy));
+      if (NORM && k) store_bytes<ACCESS>(k, c, cols, quant_pack8(v[g], qh));
       if (NORM && p.h) store_group<ACCESS>(h, c, cols, v[g]);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const int c = at(g, e);
         if (c < cols) {
-          q[c] = int8_t(quant8(y[e], qy.inv));
-          if (NORM && k) k[c] = int8_t(quant8(v[g][e], qh.inv));
+          q[c] = int8_t(quant8(y[e], qy));
+          if (NORM && k) k[c] = int8_t(quant8(v[g][e], qh));
           if (NORM && p.h) h[c] = from_f32<T>(v[g][e]);
         }
       }
@@ -310,8 +310,8 @@ __global__ void __launch_bounds__(512) norm_stream_kernel(RowArgs p) {
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; e++) y[e] = redo ? v[g][e] * u * w[g][e] : v[g][e] * w[g][e];
-      store_bytes<kAligned>(p.q + row * p.ldq, c, cols, quant_pack8(y, qy.inv));
-      if (p.ckpt) store_bytes<kAligned>(p.ckpt + row * p.ldk, c, cols, quant_pack8(v[g], qh.inv));
+      store_bytes<kAligned>(p.q + row * p.ldq, c, cols, quant_pack8(y, qy));
+      if (p.ckpt) store_bytes<kAligned>(p.ckpt + row * p.ldk, c, cols, quant_pack8(v[g], qh));
       if (p.h) store_group<kAligned>(static_cast<T*>(p.h) + row * p.ldh, c, cols, v[g]);
     }
   }
@@ -354,8 +354,8 @@ __global__ void __launch_bounds__(1024) rows_long_kernel(RowArgs p) {
   }
   for (int64_t c = threadIdx.x; c < p.cols; c += blockDim.x) {
     const float v = value(c);
-    p.q[row * p.ldq + c] = int8_t(quant8(NORM ? v * u * to_f32(wgt[c]) : v, qy.inv));
-    if (NORM && p.ckpt) p.ckpt[row * p.ldk + c] = int8_t(quant8(v, qh.inv));
+    p.q[row * p.ldq + c] = int8_t(quant8(NORM ? v * u * to_f32(wgt[c]) : v, qy));
+    if (NORM && p.ckpt) p.ckpt[row * p.ldk + c] = int8_t(quant8(v, qh));
     if (NORM && p.h) static_cast<T*>(p.h)[row * p.ldh + c] = from_f32<T>(v);
   }
 }
@@ -698,7 +698,7 @@ tg_status launch_rows(RowArgs p, int access, cudaStream_t st) {
   }
   if constexpr (NORM) {
     // many aligned rows: persistent, 32 elements per thread (f32: 16, which
-    // holds 8192 columns).  8192 x 8192 bf16 with the checkpoint: 96 us, one
+    // holds 8192 columns).  8192 x 8192 bf16 with the checkpoint: 99 us, one
     // row per block 124.  The plain quantisation has no weights to keep and
     // gains nothing (46 us either way).
     constexpr int kGroups = sizeof(T) == 4 ? 2 : 4;

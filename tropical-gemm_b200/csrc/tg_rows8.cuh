@@ -148,12 +148,25 @@ __device__ __forceinline__ float mag_max(float a, float b, float m) {
 // One row's quantisation from its largest magnitude, given as the maximum of
 // the values' bit patterns without the sign: unsigned order is magnitude
 // order, with infinities and NaN on top, so a maximum never loses a NaN.
+//
+// A code is y * inv, rounded by adding `first` and then 1.5 * 2^23 - first, which
+// leaves the integer in the low mantissa bits.  inv is 127 / top rounded up, off by
+// less than 2^-23 of itself, and for most rows first = 1.5 * 2^23, one rounding:
+// a quotient within 127 * 2^-23 of a tie may go to either side.  Ties themselves,
+// 2 * 127 |y| = (2n + 1) top, go to the even code.  127 is a prime, so either
+// 2n + 1 = 127 (y is half the largest value, 16-bit inputs hit it often): 63.5,
+// made no less by inv, goes to 64.  Or 127 divides top's significand (by chance
+// one row in 127): top / 127 is exact then, and first = 384.  384 + y * inv has
+// units of 2^-15, so inv's error, below 126.5 * 2^-23 < 2^-16, is rounded away
+// and the tie is met exactly by the second rounding.
 struct Quant {
-  float scale, inv;
+  float scale, inv, first;
 };
+constexpr float kWhole = 12582912.f;   // 1.5 * 2^23
 __device__ __forceinline__ Quant quant_of(uint32_t top_bits) {
   Quant s;
   const float top = __uint_as_float(top_bits);
+  s.first = kWhole;
   if (top_bits >= 0x7f800000u) {   // an infinity or a NaN: the row reads as NaN
     s.scale = __uint_as_float(0x7fffffffu);
     s.inv = 0.f;
@@ -161,23 +174,27 @@ __device__ __forceinline__ Quant quant_of(uint32_t top_bits) {
     s.scale = s.inv = 0.f;
   } else {
     s.scale = top / 127.f;
-    // rounded up: a value of exactly half the largest one is a tie at 63.5,
-    // which goes to the even 64, and 16-bit inputs hit it often
     s.inv = __fdiv_ru(127.f, top);
+    if (fmaf(s.scale, 127.f, -top) == 0.f) s.first = 384.f;
   }
   return s;
 }
-// y * inv rounded to nearest even, as the low byte of the result: adding
-// 1.5 * 2^23 leaves the integer in the low mantissa bits (|y * inv| < 128).
-__device__ __forceinline__ uint32_t quant8(float y, float inv) {
-  return __float_as_uint(fmaf(y, inv, 12582912.f));
+// The code as the low byte of the result (|y * inv| < 128).
+__device__ __forceinline__ uint32_t quant8(float y, const Quant& s) {
+  return __float_as_uint(fmaf(y, s.inv, s.first) + (kWhole - s.first));
 }
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
-__device__ __forceinline__ uint2 quant_pack8(const float (&v)[8], float inv) {
-  return make_uint2(pack4(quant8(v[0], inv), quant8(v[1], inv), quant8(v[2], inv), quant8(v[3], inv)),
-                    pack4(quant8(v[4], inv), quant8(v[5], inv), quant8(v[6], inv), quant8(v[7], inv)));
+__device__ __forceinline__ uint2 quant_pack8(const float (&v)[8], const Quant& s) {
+  uint32_t q[8];
+#pragma unroll
+  for (int e = 0; e < 8; e += 2)   // two at a time
+    asm("{\n.reg .b64 y, i, f, r;\nmov.b64 y, {%2, %3};\nmov.b64 i, {%4, %4};\nmov.b64 f, {%5, %5};\nmov.b64 r, {%6, %6};\n"
+        "fma.rn.f32x2 y, y, i, f;\nadd.rn.f32x2 y, y, r;\nmov.b64 {%0, %1}, y;\n}\n"
+        : "=r"(q[e]), "=r"(q[e + 1])
+        : "f"(v[e]), "f"(v[e + 1]), "f"(s.inv), "f"(s.first), "f"(kWhole - s.first));
+  return make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
 }
 // Byte i of w as a signed integer in f32, by way of 2^23 + (byte + 128).
 template <int I> __device__ __forceinline__ float byte_f32(uint32_t w_biased) {
