@@ -748,7 +748,7 @@ tg_status launch_norm_backward(BackArgs p, T* grad_w, int access, cudaStream_t s
     p.partial = static_cast<float*>(scratch);
   }
   if (lng) {
-    if (p.grad_x && p.rows) launch_kernel(tg8::norm_backward_long_kernel<T, GT>, unsigned(p.rows), 1024, 0, 0, st, p);
+    if (p.grad_x) launch_kernel(tg8::norm_backward_long_kernel<T, GT>, unsigned(p.rows), 1024, 0, 0, st, p);
     if (grad_w)
       launch_kernel(tg8::column_partial_kernel<GT>, dim3(unsigned((p.cols + 255) / 256), unsigned(p.slots)), 256, 0, 0, st, p.rows, p.cols, static_cast<const GT*>(p.grad), p.ldg, p.ckpt, p.ldk, p.ckpt_scale, p.rstd, p.partial);
   } else {
@@ -898,17 +898,19 @@ tg_status tg_rows8_rmsnorm_backward(tg_dtype dtype, tg_dtype grad_dtype, int64_t
   if (grad_dtype != dtype && grad_dtype != TG_F32) return fail(TG_ERR_INVALID_ARGUMENT, "grad is of type dtype or f32, got dtype %d", int(grad_dtype));
   TG8_CHECK(check_rows(rows, cols));
   if (cols == 0 || (!grad_x && !grad_weight)) return TG_OK;
-  if (rows && (!grad || !weight || !ckpt || !ckpt_scale || !rstd)) return fail(TG_ERR_INVALID_ARGUMENT, "null operand");
-  if (rows) {
-    TG8_CHECK(check_ld("ldg", ldg, cols));
-    if (grad_h) TG8_CHECK(check_ld("ldgh", ldgh, cols));
-    TG8_CHECK(check_ld("ldk", ldk, cols));
-    if (grad_x) TG8_CHECK(check_ld("ldx", ldx, cols));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {   // a sum of nothing; the operands, the weight among them, may be null
+    const cudaError_t e = grad_weight ? cudaMemsetAsync(grad_weight, 0, size_t(cols) * elem8_size(dtype), st) : cudaSuccess;
+    return e == cudaSuccess ? TG_OK : fail(TG_ERR_CUDA, "memset: %s", cudaGetErrorString(e));
   }
+  if (!grad || !weight || !ckpt || !ckpt_scale || !rstd) return fail(TG_ERR_INVALID_ARGUMENT, "null operand");
+  TG8_CHECK(check_ld("ldg", ldg, cols));
+  if (grad_h) TG8_CHECK(check_ld("ldgh", ldgh, cols));
+  TG8_CHECK(check_ld("ldk", ldk, cols));
+  if (grad_x) TG8_CHECK(check_ld("ldx", ldx, cols));
   BackArgs p{};
   p.rows = rows; p.cols = cols; p.grad = grad; p.ldg = ldg; p.grad_h = grad_h; p.ldgh = ldgh; p.weight = weight;
   p.ckpt = ckpt; p.ldk = ldk; p.ckpt_scale = ckpt_scale; p.rstd = rstd; p.grad_x = grad_x; p.ldx = ldx;
-  if (rows == 0 && !grad_weight) return TG_OK;
   const size_t e = elem8_size(dtype);
   RowAccess access(cols);
   access.add(grad, ldg, elem8_size(grad_dtype));
@@ -916,7 +918,6 @@ tg_status tg_rows8_rmsnorm_backward(tg_dtype dtype, tg_dtype grad_dtype, int64_t
   access.add(ckpt, ldk, 1);
   access.add(grad_x, ldx, e);
   const int how = access.get() == tg8::kAligned && !aligned(weight, 16) ? tg8::kScalar : access.get();
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   return with_type8(dtype, [&](auto t) {
     using T = decltype(t);
     if (grad_dtype == dtype) return launch_norm_backward<T, T>(p, static_cast<T*>(grad_weight), how, st);
