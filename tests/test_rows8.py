@@ -87,3 +87,12 @@ def test_tropical_calls_refuse_the_16_bit_types():
     for t in (BF16, F16):
         assert L.tg_gemm(0, t, 0, 4, 4, 4, P, 4, P, 4, P, 4, None, None) == N.TG_ERR_INVALID_ARGUMENT
         assert L.tg_backward_a(0, t, 0, 1, 4, 4, 4, P, 4, 16, P, None, 4, 16, P, 4, 16, 0, None) == N.TG_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("m, n", [(1, 0x7ffffc01), (64, 1 << 31), (40, 1 << 34), (0x7ffffc01, 16), (1 << 33, 16)])
+@pytest.mark.parametrize("ld", [16, 24])
+def test_products_of_too_many_rows_or_columns_are_refused(m, n, ld):
+    """Whatever kernel the number of tokens would take, and before any scratch or launch."""
+    L = N.lib()
+    assert L.tg_rows8_gemm(BF16, m, n, 16, P, ld, P, P, ld, P, None, P, n, None) == N.TG_ERR_UNSUPPORTED
+    assert b"outputs" in L.tg_last_error()

@@ -30,6 +30,10 @@ class Scratch {
   cudaStream_t st_;
 };
 
+// Rows and columns of C: the kernels count them, and the edges of the last tiles,
+// in 32 bits (TMA's coordinates are 32-bit too).
+constexpr int64_t kMostOutputs = 0x7ffffc00;
+
 int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 dim3 row_grid(int64_t cols_per_block, int64_t cols, int64_t rows) {
   return dim3(unsigned((cols + cols_per_block - 1) / cols_per_block), unsigned(std::min<int64_t>(rows, 16384)));
@@ -81,7 +85,7 @@ template <int MODE, typename T>
 tg_status launch_product(const CUtensorMap& a, const CUtensorMap& b, ProductArgs p, cudaStream_t st) {
   p.half_n = p.n <= 128 ? 64 : 128;   // narrow outputs: half the products and expansions are not wasted
   const int64_t tm = (p.m + tg8::kTile - 1) / tg8::kTile, tn = (p.n + 2 * p.half_n - 1) / (2 * p.half_n);
-  if (tm * tn > 0x3fffffff || p.m > 0x7ffffc00 || p.n > 0x7ffffc00)
+  if (tm * tn > 0x3fffffff)
     return fail(TG_ERR_UNSUPPORTED, "%lld x %lld outputs", (long long)p.m, (long long)p.n);
   p.tiles_m = int(tm);
   p.tiles_n = int(tn);
@@ -145,7 +149,6 @@ template <int NT, typename T>
 tg_status launch_tokens(const CUtensorMap& tokens, const CUtensorMap& weights, ProductArgs p, cudaStream_t st) {
   using S = tg8::TokensShape<NT>;
   const int64_t tiles = (p.n + 127) / 128, tt = (p.m + NT - 1) / NT;
-  if (tiles > 0x0fffffff) return fail(TG_ERR_UNSUPPORTED, "n=%lld", (long long)p.n);
   // as many CTAs of a cluster per tile as give every SM one, each with at
   // least two stages of the sum
   int split = 1;
@@ -173,6 +176,7 @@ tg_status tg_rows8_gemm(tg_dtype dtype, int64_t m, int64_t n, int64_t k, const i
   if (!elem8_size(dtype)) return fail(TG_ERR_INVALID_ARGUMENT, "8-bit rows need f32, f16 or bf16, got dtype %d", int(dtype));
   if (m < 0 || n < 0 || k < 0) return fail(TG_ERR_INVALID_ARGUMENT, "negative size (m=%lld n=%lld k=%lld)", (long long)m, (long long)n, (long long)k);
   if (m == 0 || n == 0) return TG_OK;
+  if (m > kMostOutputs || n > kMostOutputs) return fail(TG_ERR_UNSUPPORTED, "%lld x %lld outputs", (long long)m, (long long)n);
   if (k >= (int64_t(1) << 17)) return fail(TG_ERR_UNSUPPORTED, "k=%lld: 32-bit sums of 8-bit products are exact below 131072", (long long)k);
   if (!c || !a_scale || !b_scale || (k && (!a || !b))) return fail(TG_ERR_INVALID_ARGUMENT, "null operand");
   if (lda < k) return fail(TG_ERR_DIMENSION_MISMATCH, "lda=%lld < %lld", (long long)lda, (long long)k);
@@ -223,7 +227,7 @@ tg_status tg_rows8_gemm_backward(tg_dtype grad_dtype, tg_dtype out_dtype, int tr
   if (r && ldg < need) return fail(TG_ERR_DIMENSION_MISMATCH, "ldg=%lld < %lld", (long long)ldg, (long long)need);
   if (r && ldq < cols) return fail(TG_ERR_DIMENSION_MISMATCH, "ldq=%lld < %lld", (long long)ldq, (long long)cols);
   if (ldo < cols) return fail(TG_ERR_DIMENSION_MISMATCH, "ldo=%lld < %lld", (long long)ldo, (long long)cols);
-  if (p > 0x7ffffc00 || cols > 0x7ffffc00 || r > 0x3ffffc00)
+  if (p > kMostOutputs || cols > kMostOutputs || r > 0x3ffffc00)
     return fail(TG_ERR_UNSUPPORTED, "p=%lld cols=%lld r=%lld", (long long)p, (long long)cols, (long long)r);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (r == 0) {   // a sum of nothing
