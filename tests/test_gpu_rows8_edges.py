@@ -21,3 +21,18 @@ def test_norm_backward_of_no_rows_needs_no_operands(dtype, f32_grad, cols):
     N.check(N.lib().tg_rows8_rmsnorm_backward(code, 0 if f32_grad else code, 0, cols, None, cols, None, cols, None, None, cols,
                                               None, None, None, cols, out.data_ptr(), stream))
     assert not out[:cols].any() and (out[cols:] == 3).all()
+
+
+@pytest.mark.parametrize("cols", [2 ** 31 - 1, 2 ** 31 - 8, 2 ** 31 - 24, 2 ** 31 - 33, 2 ** 31 - 40])
+def test_dequantize_the_longest_rows(cols):
+    """A row of as many columns as are accepted, of 8-element groups whose ends lie past 2^31 - 1."""
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB")
+    q = torch.empty(1, cols, device="cuda", dtype=torch.int8)
+    ramp = torch.arange(1 << 20, device="cuda").remainder(251).sub(125).to(torch.int8)
+    for at in range(0, cols, 1 << 20):
+        q[0, at:at + (1 << 20)] = ramp[:min(1 << 20, cols - at)]
+    y = rows8.dequantize(Rows8(q, torch.full((1,), 0.5, device="cuda")), torch.float16)
+    for at in range(0, cols, 1 << 28):   # exact: codes of 8 bits, halved
+        part = slice(at, min(at + (1 << 28), cols))
+        assert torch.equal(y[:, part], q[:, part].half() * 0.5)

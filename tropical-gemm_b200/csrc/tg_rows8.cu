@@ -837,6 +837,7 @@ tg_status tg_rows8_dequantize(tg_dtype dtype, int64_t rows, int64_t cols, const 
   access.add(q, ldq, 1);
   int how = access.get();
   if (how == tg8::kAligned && (cols % 16 || ldq % 16 || !aligned(q, 16))) how = tg8::kShifted;   // by 8 elements, without edges
+  if (how == tg8::kShifted && cols > kGridLimit - 32) how = tg8::kScalar;   // a shifted group counts its columns in 32 bits, to 22 past the row
   const int64_t per = how == tg8::kAligned ? cols / 16 : how == tg8::kShifted ? (cols + 7 + 7) / 8 : cols;
   if (rows > (kGridLimit * 256) / per) return fail(TG_ERR_UNSUPPORTED, "%lld x %lld elements", (long long)rows, (long long)cols);
   const unsigned grid = unsigned((rows * per + 255) / 256);
