@@ -260,7 +260,9 @@ tg_status tg_rows8_gemm(tg_dtype dtype, int64_t m, int64_t n, int64_t k,
  *   out[p, c] = sum_i g(p, i) * scale[i] * q[i, c]
  * transposed == 0: g is (p x r), g(p, i) = g[p*ldg + i]  (grad_A = grad B)
  * transposed != 0: g is (r x p), g(p, i) = g[i*ldg + p]  (grad_B = grad^T A)
- * g is of type grad_dtype, out (p x cols) of type out_dtype.  Sums are f32.
+ * g is of type grad_dtype, out (p x cols) of type out_dtype.  Sums are f32, the
+ * tensor core's for some thousand terms and then added up, so that their error
+ * does not grow with r.
  * Rounding of the factors: a TG_BF16 gradient meets the 8-bit operand's
  * values rounded once to bf16; TG_F16 and TG_F32 gradients are carried with
  * 16 and 24 significant bits. */

@@ -105,7 +105,8 @@ tg_status launch_product(const CUtensorMap& a, const CUtensorMap& b, ProductArgs
       p.splits = splits;
     }
   }
-  p.chunk = p.planes == 3 ? 16 : std::max(1, p.blocks);
+  // stages whose sum the tensor core may keep (see Walk); integer sums are exact
+  p.chunk = p.planes == 3 ? 16 : S::kBack ? 256 / p.planes : std::max(1, p.blocks);
   const bool chunked = p.chunk < (p.splits > 1 ? p.split_blocks : p.blocks);
   const int pairs = p.splits > 1 ? int(tm * tn) * p.splits : int(std::min<int64_t>(tm * tn, most));
   const int64_t couples = (tm / 2) * tn;
