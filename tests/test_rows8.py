@@ -1,4 +1,7 @@
 """8-bit rows without a GPU: refusals of the Python surface and of the C ABI."""
+import os
+import subprocess
+
 import pytest
 import torch
 
@@ -96,3 +99,13 @@ def test_products_of_too_many_rows_or_columns_are_refused(m, n, ld):
     L = N.lib()
     assert L.tg_rows8_gemm(BF16, m, n, 16, P, ld, P, P, ld, P, None, P, n, None) == N.TG_ERR_UNSUPPORTED
     assert b"outputs" in L.tg_last_error()
+
+
+def test_the_library_builds_without_torch():
+    """The C library and its probe need nvcc alone; the torch binding is a target of its own."""
+    def commands(*target):
+        pkg = os.path.dirname(os.path.dirname(os.path.abspath(N.__file__)))
+        return subprocess.run(["make", "-n", "-B", "-C", pkg, "PYTHON=no-such-python", *target], check=True, capture_output=True, text=True).stdout
+
+    assert "libtropical_gemm_b200.so" in commands() and "rows8_torch" not in commands() and "no-such-python" not in commands()
+    assert "rows8_torch" in commands("torch") and "libtropical_gemm_b200.so" in commands("torch")

@@ -35,7 +35,7 @@ def _x():
         path = os.path.join(os.path.dirname(N.LIB_PATH), "_rows8_torch.so")
         if not os.path.exists(path):
             raise ImportError(f"{path} not found: build it with `python __graft_entry__.py build` "
-                              "(or `make -C tropical-gemm_b200`)")
+                              "(or `make -C tropical-gemm_b200 torch`)")
         from . import _rows8_torch
         _ext = _rows8_torch
     return _ext
