@@ -49,3 +49,47 @@ def test_sums_of_16_bit_gradients_keep_16_bits_at_any_length(dtype, p, c, r, row
     ga, gb = rows8.matmul_backward(grad, None if rows else b, b if rows else None, dtype_a=torch.float32, dtype_b=torch.float32)
     want = (grad.double() if rows else grad.double().t()) @ values(b)
     assert error(ga if rows else gb, want) < 2.0 ** -15
+
+
+# outputs p x c of sums of r terms, f32: one tile and few blocks; sums in parts with chunks in each; several tiles per
+# pair with chunks, whole and ragged edges; narrow outputs
+F32 = [(512, 256, 512), (300, 200, 5000), (24, 8, 200_000), (2100, 4100, 4100), (2048, 4096, 1024), (3000, 100, 8191), (513, 1025, 1087)]
+
+
+@pytest.mark.parametrize("p, c, r", F32)
+@pytest.mark.parametrize("rows", [True, False])
+def test_f32_gradients_are_f32(p, c, r, rows):
+    """A product of f32 operands in f32 would lose 4e-7 to 2.5e-6 here.  This one carries all 24 bits of g and lets the tensor
+    core add 1024 terms at most, which loses 6.6e-7.  Without the chunks 4100 terms lose 2.9e-6, without the third
+    part of g every sum 4.9e-6."""
+    g = gen(p + c)
+    b, grad = rand8(g, r, c, torch.float32), randn(g, *((p, r) if rows else (r, p)))
+    ga, gb = rows8.matmul_backward(grad, None if rows else b, b if rows else None)
+    want = (grad.double() if rows else grad.double().t()) @ values(b)
+    assert error(ga if rows else gb, want) < 1e-6
+
+
+# p x c outputs of r terms where pairs take two tiles at a time (more than 74 couples of 256-row tiles): an even and an odd
+# number of row tiles, single tiles after the doubles, ragged edges, rings that wrap (11 blocks and more) and a short sum
+DOUBLE = [(4700, 4300, 700), (5000, 4097, 64), (4864, 4096, 1000), (7200, 2600, 1337), (40000, 200, 390)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("p, c, r", DOUBLE)
+@pytest.mark.parametrize("rows", [True, False])
+def test_gradients_two_tiles_at_a_time(dtype, p, c, r, rows):
+    """Errors as above: factors of 16 bits (f16: 4.9e-6 at random) or exact (bf16 with scales of powers of two), and sums
+    that lose 1e-9 per term, 2e-6 at most here; a tile that is wrong, missing or in another's place shows at once.  Each tile is
+    held to the bound too, its own error over its own size."""
+    g = gen(p + c + r)
+    b, grad = rand8(g, r, c, dtype), randn(g, *((p, r) if rows else (r, p)), dtype=dtype)
+    ga, gb = rows8.matmul_backward(grad, None if rows else b, b if rows else None, dtype_a=torch.float32, dtype_b=torch.float32)
+    got = (ga if rows else gb).double()
+    want = (grad.double() if rows else grad.double().t()) @ values(b)
+    bound = 2.0 ** -16
+    assert error(got, want) < bound
+    pad = (0, -c % 256, 0, -p % 256)
+    tiles = [torch.nn.functional.pad(v, pad).square().unflatten(0, (-1, 256)).unflatten(2, (-1, 256)).sum((1, 3)) for v in (got - want, want)]
+    assert (tiles[0] <= bound ** 2 * tiles[1]).all()
+    ga, gb = rows8.matmul_backward(grad, None if rows else b, b if rows else None)   # and in its own type
+    assert torch.equal(ga if rows else gb, got.to(dtype))
