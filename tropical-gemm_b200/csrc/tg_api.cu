@@ -62,6 +62,7 @@ bool fast_f32_ok(const Problem& P) {
 std::mutex g_cfg_mu;
 std::set<std::pair<int, const void*>> g_cfg_done;
 int g_sm_count[64] = {0};
+int g_clusters[64][4] = {};
 
 tg_status ensure_smem(const void* kern, size_t smem) {
   int dev = 0;
@@ -128,6 +129,34 @@ int sm_count() {
     g_sm_count[dev] = n;
   }
   return g_sm_count[dev];
+}
+
+int clusters_at_once(const void* kern, int size) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int log = size >= 8 ? 3 : size >= 4 ? 2 : size >= 2 ? 1 : 0, sms = sm_count();
+  if (dev < 0 || dev >= 64 || log == 0) return sms >> log;
+  std::lock_guard<std::mutex> lock(g_cfg_mu);
+  if (!g_clusters[dev][log]) {
+    int n = 0, smem = 0;
+    cudaFuncAttributes fa;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {1u << log, 1, 1};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(sms >> log << log));
+    cfg.blockDim = dim3(128);
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaFuncGetAttributes(&fa, kern) == cudaSuccess) smem = fa.maxDynamicSharedSizeBytes;   // as opted in: an SM's worth
+    cfg.dynamicSmemBytes = size_t(smem);
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      return sms >> log;
+    }
+    g_clusters[dev][log] = n;
+  }
+  return g_clusters[dev][log];
 }
 
 // Stream-ordered scratch comes from a memory pool the library creates on

@@ -26,6 +26,10 @@ tg_status check_launch(const char* what);
 tg_status ensure_smem(const void* kern, size_t smem);
 // SM count of the current device (cached).
 int sm_count();
+// How many clusters of `size` CTAs (1, 2, 4 or 8) run on the current device at
+// once when each CTA of `kern` takes an SM (cached): a cluster stays within a
+// group of SMs, so fewer than sm_count() / size.
+int clusters_at_once(const void* kern, int size);
 // Stream-ordered scratch from the library's own memory pool on the current
 // device (the i32 / i64 conversion copies).
 cudaError_t scratch_alloc(void** p, size_t bytes, cudaStream_t st);

@@ -139,10 +139,17 @@ tg_status launch_product(const CUtensorMap& a, const CUtensorMap& b, ProductArgs
 
 // Tokens per tile of the few-token kernel, or 0 for the paired one.  Up to 64
 // tokens the weights' read decides (4096 x 4096, one token: 8.3 us, paired 18).
-// Above, the few-token kernel's split sum pays while the sum is long (256 tokens,
-// 4096 x 4096: 17.8 us, paired 28; 512 x 512: 12.3 against 8.2).
-int token_tile(int64_t m, int blocks) {
-  if (m > 64) return m <= 512 && blocks >= 24 ? 128 : 0;
+// Above, what the few-token kernel has to offer is its split sum: it is taken for
+// long sums of so few tiles that two CTAs or more share one.  us, few-token /
+// paired, tokens x channels:
+//   sums of 8192    128 x 2048 14.0 / 16.4, 128 x 4096 15.6 / 25.9, 256 x 4096 19.8 / 26.9,
+//                   512 x 2048 19.0 / 26.0, 128 x 8192 22.8 / 31.0
+//   of 4096         128 x 2048 10.4 / 12.4, 128 x 4096 12.1 / 14.7, 256 x 4096 15.3 / 14.8,
+//                   512 x 2048 14.2 / 14.7, 128 x 8192 16.7 / 15.2
+//   of 2048         128 x 2048 9.6 / 9.7, 128 x 4096 10.0 / 9.9, 256 x 4096 12.0 / 9.9
+//   without a split (8192)   512 x 4096 25.8 / 24.1, 256 x 8192 28.6 / 24.4, 512 x 8192 54 / 27, 512 x 16384 125 / 51
+int token_tile(int64_t m, int64_t n, int blocks) {
+  if (m > 64) return m <= 512 && blocks >= 24 && (n + 127) / 128 * ((m + 127) / 128) * 2 <= sm_count() ? 128 : 0;
   return m <= 16 ? 16 : m <= 32 ? 32 : 64;
 }
 
@@ -150,16 +157,19 @@ template <int NT, typename T>
 tg_status launch_tokens(const CUtensorMap& tokens, const CUtensorMap& weights, ProductArgs p, cudaStream_t st) {
   using S = tg8::TokensShape<NT>;
   const int64_t tiles = (p.n + 127) / 128, tt = (p.m + NT - 1) / NT;
-  // as many CTAs of a cluster per tile as give every SM one, each with at
-  // least two stages of the sum
-  int split = 1;
-  while (split < 8 && tiles * tt * split * 2 <= sm_count() && p.blocks >= 4 * split) split *= 2;
-  p.split_blocks = (p.blocks + split - 1) / split;
-  const int stages = std::min(S::kMost, p.split_blocks);
-  const size_t smem = size_t(stages) * S::kStage + (split > 1 ? S::kExchange : 0) + 1024;
   auto kern = tg8::tokens_kernel<NT, T>;
   const tg_status s = ensure_smem(reinterpret_cast<const void*>(kern), size_t(S::kMost) * S::kStage + S::kExchange + 1024);
   if (s != TG_OK) return s;
+  // as many CTAs of a cluster per tile as run at once, each with at least two
+  // stages of the sum.  15 clusters of 8 and 33 of 4 do: one more is a second
+  // round (us, split in 8 / 4 / 2, sums of 8192: 1 x 1920 6.2 / 6.9 / 9.0,
+  // 1 x 2048 10.4 / 7.0 / 9.1, 128 x 2048 22.5 / 14.0 / 18.7; in 4 / 2: 1 x 4096
+  // 9.4 / 9.8, 1 x 4352 13.9 / 9.9, 128 x 4608 28.2 / 19.9).
+  int split = 1;
+  while (split < 8 && tiles * tt <= clusters_at_once(reinterpret_cast<const void*>(kern), 2 * split) && p.blocks >= 4 * split) split *= 2;
+  p.split_blocks = (p.blocks + split - 1) / split;
+  const int stages = std::min(S::kMost, p.split_blocks);
+  const size_t smem = size_t(stages) * S::kStage + (split > 1 ? S::kExchange : 0) + 1024;
   launch_kernel(kern, dim3(unsigned(tiles * split), unsigned(tt)), 128, smem, split, st, tokens, weights, p, split, stages);
   return check_launch("rows8 gemm");
 }
@@ -201,7 +211,7 @@ tg_status tg_rows8_gemm(tg_dtype dtype, int64_t m, int64_t n, int64_t k, const i
   p.planes = 1;
   p.blocks = std::max(1, int((k + 127) / 128));
   CUtensorMap ma, mb;
-  const int nt = token_tile(m, p.blocks);
+  const int nt = token_tile(m, n, p.blocks);
   if (!oa.map(128, nt ? nt : 128, &ma) || !ob.map(128, 128, &mb)) return fail(TG_ERR_CUDA, "rows8 gemm: tensor map encoding failed");
   return with_type8(dtype, [&](auto t) {
     using T = decltype(t);
