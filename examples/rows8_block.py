@@ -6,7 +6,10 @@
 
 Trains the block on a synthetic target (activations kept in 8 bits between
 forward and backward), then serves it with frozen 8-bit weights, all tokens at
-once and one at a time.
+once and one at a time.  Serving as many tokens as were trained on gives the
+trained block's bits.  One token at a time gives them too at the sizes below;
+wider norms of many tokens take their sums in another order than those of a
+few, and a code next to a tie may come out as its neighbour.
 
     python examples/rows8_block.py [--steps 60] [--tokens 512] [--width 256]
 """

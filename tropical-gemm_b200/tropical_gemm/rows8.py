@@ -74,7 +74,8 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tens
     """Root-mean-square norm of h = x + residual over the last dimension,
     times `weight`, in 8-bit rows.  `checkpoint` also keeps h in 8-bit rows
     and the row's factor, which is what `rmsnorm_backward` reads.  Without a
-    residual h is x itself."""
+    residual h is x itself.  The order of a row's sum of squares may depend on
+    the number of rows; h and the checkpoint do not."""
     q, scale, h, ck, ck_scale, rstd = _x().rmsnorm(x, weight, residual, eps, checkpoint)
     return NormRows8(Rows8(q, scale), h, None if ck is None else Rows8(ck, ck_scale), rstd)
 
