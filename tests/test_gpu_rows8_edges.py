@@ -36,3 +36,15 @@ def test_dequantize_the_longest_rows(cols):
     for at in range(0, cols, 1 << 28):   # exact: codes of 8 bits, halved
         part = slice(at, min(at + (1 << 28), cols))
         assert torch.equal(y[:, part], q[:, part].half() * 0.5)
+
+
+def test_calls_record_no_graph():
+    """Only the autograd layer is differentiable; the calls below it return plain results for any arguments."""
+    x, res, w, weight, bias = (torch.randn(*s, device="cuda").requires_grad_(True) for s in ((6, 32), (6, 32), (32,), (5, 32), (5,)))
+    n = rows8.rmsnorm(x, w, residual=res, checkpoint=True)
+    b = rows8.quantize(weight)
+    z = rows8.matmul(n.rows, b, bias=bias, dtype=torch.float32)
+    grads = rows8.matmul_backward(z, n.rows, b) + rows8.rmsnorm_backward(x, n.checkpoint, n.rstd, w, grad_h=res)
+    for t in (n.h, n.rows.scale, n.checkpoint.scale, n.rstd, b.scale, z, rows8.column_sum(x), rows8.dequantize(b), *grads):
+        assert not t.requires_grad and t.grad_fn is None
+    assert rows8.rmsnorm(x, w).h is x or rows8.rmsnorm(x, w).h.data_ptr() == x.data_ptr()

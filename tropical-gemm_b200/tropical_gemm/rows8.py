@@ -10,6 +10,10 @@ element of x between its forward and its backward (the norm's output and h).
     z = rows8.matmul(r.rows, rows8.quantize(weight))          # tokens x output channels
 
 `tropical_gemm.pytorch.rmsnorm_linear_rows8` is the same chain with autograd.
+The calls of this module record no graph: what they return requires no
+gradient, whatever their arguments do, and `rmsnorm_backward`, `matmul_backward`
+and `column_sum` are how gradients are taken.  (Without a residual `rmsnorm`
+hands x through as h, as it came.)
 
 Tensors are CUDA tensors of float32, float16 or bfloat16 with any leading
 dimensions; rows may be strided, their elements are contiguous (other layouts
