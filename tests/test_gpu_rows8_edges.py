@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import tropical_gemm.pytorch as tp
 from tropical_gemm import _native as N
 from tropical_gemm import rows8
 from tropical_gemm.rows8 import Rows8
@@ -48,3 +49,16 @@ def test_calls_record_no_graph():
     for t in (n.h, n.rows.scale, n.checkpoint.scale, n.rstd, b.scale, z, rows8.column_sum(x), rows8.dequantize(b), *grads):
         assert not t.requires_grad and t.grad_fn is None
     assert rows8.rmsnorm(x, w).h is x or rows8.rmsnorm(x, w).h.data_ptr() == x.data_ptr()
+
+
+@pytest.mark.parametrize("needed", [False, True])
+def test_frozen_scales_take_no_gradient(needed):
+    """A frozen weight is a constant, whatever its scale says."""
+    x, w = torch.randn(4, 32, device="cuda", requires_grad=needed), rows8.quantize(torch.randn(8, 32, device="cuda"))
+    scale = w.scale.clone().requires_grad_(True)
+    norm = torch.ones(32, device="cuda")
+    z, _ = tp.rmsnorm_linear_rows8(x, norm, Rows8(w.q, scale))
+    assert torch.equal(z, tp.rmsnorm_linear_rows8(x, norm, w)[0]) and z.requires_grad == needed
+    if needed:
+        z.sum().backward()
+        assert x.grad is not None and scale.grad is None

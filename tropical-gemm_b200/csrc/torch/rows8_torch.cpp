@@ -320,7 +320,10 @@ std::tuple<Tensor, Tensor> rmsnorm_linear(const Tensor& x, const Tensor& norm_we
   const bool train = at::GradMode::is_enabled() &&
                      (x.requires_grad() || norm_weight.requires_grad() || (!weight_scale && weight.requires_grad()) ||
                       (residual && residual->requires_grad()) || (bias && bias->requires_grad()));
-  auto out = NormLinear::apply(x, norm_weight, weight, weight_scale, residual, bias, eps, train);
+  // frozen rows are constants, their scales included: else a scale that requires a
+  // gradient would make a node of a call that kept nothing for its backward
+  const OptTensor frozen = weight_scale && weight_scale->requires_grad() ? OptTensor(weight_scale->detach()) : weight_scale;
+  auto out = NormLinear::apply(x, norm_weight, weight, frozen, residual, bias, eps, train);
   return {out[0], out[1]};
 }
 
