@@ -211,7 +211,7 @@ tg_status tg_rows8_quantize(tg_dtype dtype, int64_t rows, int64_t cols,
                             const void* x, int64_t ldx,
                             int8_t* q, int64_t ldq, float* scale, void* stream);
 
-/* y = q * scale, rounded once to dtype. */
+/* y = q * scale, the f32 product rounded to dtype. */
 tg_status tg_rows8_dequantize(tg_dtype dtype, int64_t rows, int64_t cols,
                               const int8_t* q, int64_t ldq, const float* scale,
                               void* y, int64_t ldy, void* stream);
@@ -221,6 +221,8 @@ tg_status tg_rows8_dequantize(tg_dtype dtype, int64_t rows, int64_t cols,
  * q, scale = y in 8-bit rows (as tg_rows8_quantize).  All arithmetic and
  * the statistics are f32 on the unrounded sum; x, residual, weight and h are
  * of type dtype.  residual and h may be null (no addition; h not written).
+ * Finite rows whose sum of squares passes f32's range (|h| from about 1e19 on)
+ * have u = 0 and read as zeros.
  * For training, ckpt (ldk) and ckpt_scale receive h in 8-bit rows and rstd
  * receives u: what tg_rows8_rmsnorm_backward reads.  The three may be null. */
 tg_status tg_rows8_rmsnorm(tg_dtype dtype, int64_t rows, int64_t cols,

@@ -1,8 +1,11 @@
 // Row kernels of the 8-bit row operators: quantisation, the root-mean-square
 // norm with the residual's addition, its backward, and column sums.
 //
-// All are bound by memory: each reads its inputs once, keeps the row in
-// registers between the statistics and the output, and writes once.
+// All are bound by memory.  A row of up to 16384 columns is read once, kept in
+// registers between the statistics and the output, and written once; the norm
+// reads its weights again for the output, from L1 (norm_stream_kernel keeps them).
+// Longer rows are read two or three times, the later ones mostly from L2
+// (2048 x 53248 bf16: quantise 186 us, 1.8 TB/s; norm with checkpoint 540).
 #include <algorithm>
 #include "tg_rows8.cuh"
 

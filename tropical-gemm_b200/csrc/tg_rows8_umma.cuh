@@ -14,13 +14,13 @@
 // Persistent: a pair walks tiles in groups of row panels, so what it reads
 // stays in L2.
 //
-// What bounds it: power for long sums (8192^3 forward: 0.33 ms, with zero operands
-// 0.25), and shared memory.  Per 256 x 256 x (128 bytes) step an SM's tensor core
+// What bounds it: power for long sums (8192^3 forward: one call 0.33 ms, called on
+// end 0.38, with zero operands 0.25), and shared memory.  Per 256 x 256 x (128 bytes) step an SM's tensor core
 // needs 512 cycles and reads 32 KB (256 cycles at 128 bytes per cycle); TMA writes
 // 32 KB more (forward: 512 in all).  Backward a step writes 16 + 8 KB, and the
 // expansion reads 8 and writes 16: 640 cycles.  Two tiles that share the right
 // operand bring that to 1024 per 1024 of tensor work (8192 x 8192 x 4096: 0.44 ms
-// one tile at a time, 0.37 two); forward they gain nothing (0.176, 0.196 ms).
+// one tile at a time, 0.36 two, called on end 0.43); forward they gain nothing (0.176, 0.196 ms).
 #pragma once
 #include "tg_rows8.cuh"
 #include "tg_umma.cuh"

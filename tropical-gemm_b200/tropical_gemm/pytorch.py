@@ -184,8 +184,9 @@ def rmsnorm_linear_rows8(x: torch.Tensor, norm_weight: torch.Tensor, weight, res
     `weight` is a (N, K) tensor of x's type, quantised at every call, or
     `rows8.Rows8` (frozen: no gradient).  Between forward and backward only
     8-bit rows are kept (the norm's output, h, the weight).  Gradients are those
-    of the product of the 8-bit values, passed straight through the rounding;
-    they cannot be differentiated again.  CUDA tensors of float32, float16 or
+    of the product of the 8-bit values, passed straight through the rounding
+    (float32 and float16 gradients meet them with 24 and 16 bits, bfloat16 ones
+    rounded once to bfloat16); they cannot be differentiated again.  CUDA tensors of float32, float16 or
     bfloat16."""
     w, w_scale = weight if isinstance(weight, rows8.Rows8) else (weight, None)
     return rows8._x().rmsnorm_linear(x, norm_weight, w, w_scale, residual, bias, eps)

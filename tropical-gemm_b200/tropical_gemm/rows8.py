@@ -68,7 +68,7 @@ def quantize(x: torch.Tensor) -> Rows8:
 
 
 def dequantize(r: Rows8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values that 8-bit rows stand for, rounded once to `dtype`."""
+    """The values that 8-bit rows stand for: q * scale in float32, rounded to `dtype`."""
     q, scale = r
     return _x().dequantize(q, scale, dtype)
 
