@@ -279,6 +279,126 @@ tg_status tg_rows8_gemm_backward(tg_dtype grad_dtype, tg_dtype out_dtype, int tr
 tg_status tg_rows8_column_sum(tg_dtype dtype, tg_dtype out_dtype, int64_t rows, int64_t cols,
                               const void* x, int64_t ldx, void* out, void* stream);
 
+/* --------------------------------------------------------------------------
+ * Layer norm.  Row-major; dtype is TG_F32, TG_F16 or TG_BF16; conventions as
+ * for the 8-bit rows above (device pointers, stream order, status codes, sizes
+ * of 0 rows accepted, scratch from the library's own pool).  No reference
+ * counterpart.
+ * ------------------------------------------------------------------------ */
+
+/* h = x + residual;  u = (h - mean) * rstd;  y = u * weight + bias
+ * with a row's mean and rstd = 1 / sqrt(variance + eps), the variance being the
+ * mean square of h - mean.  All arithmetic is f32 on the unrounded sum; x,
+ * residual, weight, bias, h and y are of type dtype.  residual, weight (ones),
+ * bias (zeros), h, mean and rstd may be null, mean and rstd together.  Equal
+ * rows of one call give equal bits. */
+tg_status tg_layernorm(tg_dtype dtype, int64_t rows, int64_t cols,
+                       const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                       const void* weight, const void* bias, float eps,
+                       void* h, int64_t ldh, void* y, int64_t ldy,
+                       float* mean, float* rstd, void* stream);
+
+/* Backward of the norm.  With u = (h - mean) * rstd and a = grad * weight:
+ *   grad_x = rstd * (a - mean(a) - u * mean(a * u)) + grad_h
+ *   grad_weight = sum over rows of grad * u;  grad_bias = sum over rows of grad
+ * All of type dtype except mean and rstd (f32).  grad_h and weight may be
+ * null, and each of the three results.  The sums over rows have a fixed order:
+ * equal inputs give equal bits. */
+tg_status tg_layernorm_backward(tg_dtype dtype, int64_t rows, int64_t cols,
+                                const void* grad, int64_t ldg, const void* grad_h, int64_t ldgh,
+                                const void* weight, const void* h, int64_t ldh,
+                                const float* mean, const float* rstd,
+                                void* grad_x, int64_t ldx, void* grad_weight, void* grad_bias, void* stream);
+
+/* --------------------------------------------------------------------------
+ * Matrices held in 8-bit floating point (e4m3, as bytes) with a scale for each
+ * block of 128: element (r, c) stands for q[r*ldq + c] times the scale of
+ *   its row's block of 128 columns   (tall == 1)
+ *   its tile of 128 rows x columns   (tall == 128)
+ * which is scale[(r / tall) * scale_row + (c / 128) * scale_block], f32.
+ * A block at the matrix's edge is shorter.  Conventions as above; dtype is
+ * TG_F32, TG_F16 or TG_BF16.
+ *
+ * The quantising calls take the least power of two, from 2^-126 on, that
+ * brings a block's largest magnitude to 448 (the largest e4m3 value) or below,
+ * and round to nearest even: a float code's precision does not depend on its
+ * scale's mantissa, and with a power of two the rounding to 8 bits is the only
+ * one.  A block that holds a NaN or an infinity gets scale NaN, so that
+ * everything made of it is NaN.  The products take any f32 scales; the product
+ * of two scales that meet is taken in f32.
+ * ------------------------------------------------------------------------ */
+
+/* q, scale = x with a scale per row and block of 128 columns.  qt (cols x
+ * rows, or null): x transposed, with blocks of 128 along ITS rows; its element
+ * (c, r) has the scale scale_t[c * scale_t_row + (r / 128) * scale_t_block].
+ * q may be null when qt is not. */
+tg_status tg_blocks8_quantize(tg_dtype dtype, int64_t rows, int64_t cols, const void* x, int64_t ldx,
+                              void* q, int64_t ldq, float* scale, int64_t scale_row, int64_t scale_block,
+                              void* qt, int64_t ldqt, float* scale_t, int64_t scale_t_row, int64_t scale_t_block,
+                              void* stream);
+
+/* q, scale = x with a scale per tile of 128 x 128.  qt (cols x rows, or null)
+ * gets the same codes transposed, whose scales are scale transposed. */
+tg_status tg_blocks8_quantize_tiles(tg_dtype dtype, int64_t rows, int64_t cols, const void* x, int64_t ldx,
+                                    void* q, int64_t ldq, float* scale, int64_t scale_row, int64_t scale_block,
+                                    void* qt, int64_t ldqt, void* stream);
+
+/* Codes transposed: qt (cols x rows) = q (rows x cols).  A matrix in tiles of
+ * 128 x 128 transposed has its scales transposed too. */
+tg_status tg_blocks8_transpose(int64_t rows, int64_t cols, const void* q, int64_t ldq, void* qt, int64_t ldqt, void* stream);
+
+/* y = q * scale, the f32 product rounded to dtype; tall is 1 or 128. */
+tg_status tg_blocks8_dequantize(tg_dtype dtype, int64_t rows, int64_t cols, int tall,
+                                const void* q, int64_t ldq, const float* scale, int64_t scale_row, int64_t scale_block,
+                                void* y, int64_t ldy, void* stream);
+
+/* tg_layernorm with its output in 8-bit blocks (tall == 1), quantised from the
+ * unrounded f32 values. */
+tg_status tg_blocks8_layernorm(tg_dtype dtype, int64_t rows, int64_t cols,
+                               const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                               const void* weight, const void* bias, float eps, void* h, int64_t ldh,
+                               void* q, int64_t ldq, float* scale, int64_t scale_row, int64_t scale_block,
+                               float* mean, float* rstd, void* stream);
+
+/* C[i,j] = sum over blocks b of a_scale(i, b) * b_scale(j, b) * sum over k in b
+ * of A[i,k] * B[j,k], + bias[j]: A (m x k) with tall == 1, B (n x k) with
+ * b_tall 1 or 128, C (m x n) and bias (n, or null) of type dtype.  Sums are
+ * f32: the tensor core's within a block of 128, then added up in order. */
+tg_status tg_blocks8_gemm(tg_dtype dtype, int64_t m, int64_t n, int64_t k,
+                          const void* a, int64_t lda, const float* a_scale, int64_t a_scale_row, int64_t a_scale_block,
+                          const void* b, int64_t ldb, int b_tall, const float* b_scale, int64_t b_scale_row, int64_t b_scale_block,
+                          const void* bias, void* c, int64_t ldc, void* stream);
+
+/* --------------------------------------------------------------------------
+ * What a model answers with: log probabilities of tokens.  logits (rows x
+ * vocab) of type dtype; conventions as above.
+ *   p = softmax(row);  logprob = log p[token];  entropy = -sum p log p
+ * Logits of -infinity have no part in it.  A row of nothing else has logprob
+ * and alternatives -infinity, entropy 0 and no gradient; a row that holds a
+ * NaN or +infinity gives NaN.  token == ignore_index gives logprob 0 and has
+ * no part in the gradient; any other token outside 0 .. vocab - 1 gives NaN.
+ * ------------------------------------------------------------------------ */
+
+/* tokens and logprob may be null together; entropy and stats may be null.
+ * stats (2 per row): the row's largest logit m, and log sum exp(logit - m).
+ * top (0 .. 32, at most vocab): that many most likely tokens per row, and
+ * their log probabilities, from the most likely on; of equal logits the lower
+ * token comes first. */
+tg_status tg_token_logprobs(tg_dtype dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld,
+                            const int64_t* tokens, int64_t ignore_index, float* logprob, float* entropy, float* stats,
+                            int top, float* top_logprobs, int64_t* top_tokens, void* stream);
+
+/* grad_logits[r, v] = grad_logprob[r] * ([v == token] - p_v)
+ *                   - grad_entropy[r] * p_v * (log p_v + entropy[r])
+ * from stats and entropy as tg_token_logprobs gave them.  grad_logprob or
+ * grad_entropy may be null (zeros); tokens may be null with grad_logprob,
+ * entropy with grad_entropy.  grad_logits, of type dtype, may be the logits
+ * themselves (same address and ld). */
+tg_status tg_token_logprobs_backward(tg_dtype dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld,
+                                     const int64_t* tokens, int64_t ignore_index, const float* stats, const float* entropy,
+                                     const float* grad_logprob, const float* grad_entropy,
+                                     void* grad_logits, int64_t ldg, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

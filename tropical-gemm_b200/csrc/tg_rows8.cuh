@@ -214,6 +214,29 @@ __device__ __forceinline__ void after_previous_kernel() {
   asm volatile("griddepcontrol.wait;\ngriddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// out[c] = sum over slots of partial[slot, c]: 32 columns x 32 slot lanes per
+// block, joined in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(1024) column_join_kernel(int64_t slots, int64_t cols, const float* partial, T* out) {
+  __shared__ float part[32][33];
+  after_previous_kernel();
+  const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t c = int64_t(blockIdx.x) * 32 + lane;
+  float s = 0.f;
+  if (c < cols) {
+#pragma unroll 8
+    for (int64_t r = y; r < slots; r += 32) s += partial[r * cols + c];
+  }
+  part[y][lane] = s;
+  __syncthreads();
+  // warp y joins column y of the strip
+  s = part[lane][y];
+#pragma unroll
+  for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  const int64_t column = int64_t(blockIdx.x) * 32 + y;
+  if (lane == 0 && column < cols) out[column] = from_f32<T>(s);
+}
+
 }  // namespace tg8
 
 namespace tgi {

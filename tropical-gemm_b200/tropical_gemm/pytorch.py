@@ -19,7 +19,7 @@ import torch
 
 import tropical_gemm
 from . import _native as N
-from . import rows8
+from . import _layers, blocks8, rows8
 
 GPU_AVAILABLE = tropical_gemm.cuda_available()
 _DLPACK_AVAILABLE = GPU_AVAILABLE
@@ -192,6 +192,38 @@ def rmsnorm_linear_rows8(x: torch.Tensor, norm_weight: torch.Tensor, weight, res
     return rows8._x().rmsnorm_linear(x, norm_weight, w, w_scale, residual, bias, eps)
 
 
+def layernorm(x: torch.Tensor, weight=None, bias=None, residual=None, eps: float = 1e-5):
+    """(y, h): h = x + residual, y = (h - mean) / sqrt(variance + eps) * weight + bias
+    over the last dimension, with autograd (`norms.layernorm`).  Kept for the
+    backward: h and two float32 values per row.  Gradients cannot be
+    differentiated again."""
+    return _layers.ext().layernorm_grad(x, weight, bias, residual, eps)
+
+
+def linear_blocks8(x: torch.Tensor, weight, bias=None) -> torch.Tensor:
+    """x weight^T + bias in 8-bit floating point with a scale for each block of
+    128, with autograd: x in blocks along its rows, the weight in tiles.
+
+    `weight` is a (N, K) tensor of x's type, quantised at every call, or
+    `blocks8.Blocks8` (frozen: no gradient; in tiles, if x takes one).  The
+    gradients are products in 8-bit blocks too, of z's gradient in blocks along
+    each sum: grad W for x, grad^T x for the weight, with x in blocks along the
+    tokens.  They pass straight through the rounding; the bias's gradient is a
+    float32 sum of the unrounded gradient.  Between forward and backward x and
+    the weight are kept in 8 bits.  Gradients cannot be differentiated again.
+    CUDA tensors of float32, float16 or bfloat16."""
+    w, w_scale = weight if isinstance(weight, blocks8.Blocks8) else (weight, None)
+    return _layers.ext().linear(x, w, w_scale, bias)
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, ignore_index: int = -100):
+    """(logprob, entropy) of each row of logits (.., vocabulary), float32, with
+    autograd (`logprobs.token_logprobs`): log p[token] and -sum p log p with
+    p = softmax(row).  Kept for the backward: the logits and three float32
+    values per row.  Gradients cannot be differentiated again."""
+    return _layers.ext().token_logprobs_grad(logits, tokens, ignore_index)
+
+
 __all__ = [
     "TropicalMaxPlusMatmul", "TropicalMinPlusMatmul", "TropicalMaxMulMatmul",
     "TropicalMaxPlusMatmulGPU", "TropicalMinPlusMatmulGPU", "TropicalMaxMulMatmulGPU",
@@ -199,6 +231,6 @@ __all__ = [
     "tropical_maxplus_matmul", "tropical_minplus_matmul", "tropical_maxmul_matmul",
     "tropical_maxplus_matmul_gpu", "tropical_minplus_matmul_gpu", "tropical_maxmul_matmul_gpu",
     "tropical_maxplus_matmul_batched", "tropical_minplus_matmul_batched", "tropical_maxmul_matmul_batched",
-    "rmsnorm_linear_rows8",
+    "rmsnorm_linear_rows8", "layernorm", "linear_blocks8", "token_logprobs",
     "GPU_AVAILABLE", "_DLPACK_AVAILABLE",
 ]
