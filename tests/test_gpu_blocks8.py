@@ -202,7 +202,7 @@ def test_linear_gradient_against_the_formula():
         a, b = p.abs(), q.abs()
         limit = ((a * (1 + 2.0 ** -4) + floor) @ (b * (1 + 2.0 ** -4) + floor)) - a @ b
         assert ((got.detach().double() - p @ q).abs() <= limit).all()
-            assert float((got.detach().double() - p @ q).norm() / (p @ q).norm()) < 2 * 2.0 ** -4
+        assert float((got.detach().double() - p @ q).norm() / (p @ q).norm()) < 2 * 2.0 ** -4
 
 
 def test_linear_frozen_and_needs():
