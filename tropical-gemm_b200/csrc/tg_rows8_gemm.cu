@@ -2,83 +2,15 @@
 // integers and the products of its backward.
 #include <algorithm>
 #include "tg_rows8.cuh"
+#include "tg_operand8.cuh"
 #include "tg_rows8_umma.cuh"
 
 namespace tgi {
 
 using tg8::ProductArgs;
 
-// Scratch of one call, freed in stream order when the call returns.
-class Scratch {
- public:
-  explicit Scratch(cudaStream_t st) : st_(st) {}
-  Scratch(const Scratch&) = delete;
-  ~Scratch() {
-    if (p_) scratch_free(p_, st_);
-  }
-  cudaError_t reserve(size_t bytes) { return scratch_alloc(&p_, bytes, st_); }
-  template <typename T> T* take(size_t count) {
-    T* r = reinterpret_cast<T*>(static_cast<char*>(p_) + used_);
-    used_ += size_of<T>(count);
-    return r;
-  }
-  template <typename T> static size_t size_of(size_t count) { return (count * sizeof(T) + 255) & ~size_t(255); }
-
- private:
-  void* p_ = nullptr;
-  size_t used_ = 0;
-  cudaStream_t st_;
-};
-
-// Rows and columns of C: the kernels count them, and the edges of the last tiles,
-// in 32 bits (TMA's coordinates are 32-bit too).
-constexpr int64_t kMostOutputs = 0x7ffffc00;
-
-int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 dim3 row_grid(int64_t cols_per_block, int64_t cols, int64_t rows) {
   return dim3(unsigned((cols + cols_per_block - 1) / cols_per_block), unsigned(std::min<int64_t>(rows, 16384)));
-}
-
-// 8-bit rows a TMA load can take: 16-byte aligned rows of at least one byte.
-bool tma_rows8(const int8_t* q, int64_t ld, int64_t rows, int64_t cols) {
-  return cols > 0 && aligned(q, 16) && (ld % 16 == 0 || rows == 1);
-}
-struct Operand8 {
-  const int8_t* q;
-  int64_t ld, rows, cols;
-  bool pad;
-  Operand8(const int8_t* q_, int64_t ld_, int64_t rows_, int64_t cols_)
-      : q(q_), ld(ld_), rows(rows_), cols(cols_), pad(!tma_rows8(q_, ld_, rows_, cols_)) {}
-  int64_t padded() const { return std::max<int64_t>(16, round_up(cols, 16)); }
-  size_t scratch() const { return pad ? Scratch::size_of<int8_t>(size_t(rows) * size_t(padded())) : 0; }
-  // Takes the place of a padded copy where the rows are not aligned, to be
-  // filled by pad_operands; a sum of nothing becomes a sum over one zero.
-  void place(Scratch& s, tg8::PadArgs& p, int& count) {
-    if (pad) {
-      int8_t* out = s.take<int8_t>(size_t(rows) * size_t(padded()));
-      p.q[count] = q;
-      p.out[count] = out;
-      p.rows[count] = rows;
-      p.cols[count] = cols;
-      p.ldq[count] = ld;
-      p.ldo[count] = padded();
-      count++;
-      q = out;
-      ld = padded();
-      cols = std::max<int64_t>(cols, 1);
-    } else if (rows == 1) {
-      ld = padded();
-    }
-  }
-  bool map(uint32_t box_cols, uint32_t box_rows, CUtensorMap* m) const {
-    return encode_tma(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q, cols, rows, ld, 1, 0, box_cols, box_rows, m);
-  }
-};
-
-void pad_operands(const tg8::PadArgs& p, int count, cudaStream_t st) {
-  int64_t most = 0;
-  for (int i = 0; i < count; i++) most = std::max(most, (p.rows[i] * (p.ldo[i] / 16) + 255) / 256);
-  if (most) launch_kernel(tg8::pad8_kernel, dim3(unsigned(std::min<int64_t>(most, 8192)), 1, unsigned(count)), 256, 0, 0, st, p);
 }
 
 template <int MODE, typename T>

@@ -1,4 +1,4 @@
-// sm_100a building blocks of the 8-bit row products: mbarriers, TMA loads,
+// sm_100a building blocks of the 8-bit products: mbarriers, TMA loads,
 // tensor-core products with their accumulators in tensor memory.
 //
 // Waits are bounded: after kWaitPolls polls a wait reports failure and the
@@ -174,6 +174,20 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
   }
 #undef TG_MMA
 }
+// The same for 8-bit floating point, 32 of the sum per product.  Its instruction
+// descriptor: accumulator type f32 (1), operand type e4m3 (0).
+template <int CTAS> __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  const uint32_t acc = accumulate;
+  if constexpr (CTAS == 2)
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+  else
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+// Registers per thread of a warpgroup, all of whose threads come here.
+template <int N> __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 // The barrier at this offset, in this CTA (1) or in both of the pair (2),
 // gets one arrival when all products issued so far are done.
 template <int CTAS> __device__ __forceinline__ void mma_commit(uint32_t bar) {
