@@ -12,6 +12,7 @@ namespace {
 template <typename T, bool ROWS>
 tg_status launch_pairs(const CUtensorMap& a, const CUtensorMap& b, ProductArgs8 p, cudaStream_t st) {
   using S = tgb::PairShape;
+  using X = tgb::ScaledShape;
   p.half_n = p.n <= 128 ? 64 : 128;   // narrow outputs: half the products are not wasted
   const int64_t tm = (p.m + 255) / 256, tn = (p.n + 2 * p.half_n - 1) / (2 * p.half_n);
   if (tm * tn > 0x3fffffff) return fail(TG_ERR_UNSUPPORTED, "%lld x %lld outputs", (long long)p.m, (long long)p.n);
@@ -22,7 +23,7 @@ tg_status launch_pairs(const CUtensorMap& a, const CUtensorMap& b, ProductArgs8 
   p.splits = 1;
   // few tiles and a long sum: several pairs share a tile's sum and a second kernel joins the parts
   if (tm * tn * 2 <= most) {
-    const int split_blocks = std::max<int>(8, int((p.blocks * tm * tn + most - 1) / most));
+    const int split_blocks = std::max<int>(8, int((p.blocks * tm * tn + most - 1) / most + 3) / 4 * 4);
     const int splits = (p.blocks + split_blocks - 1) / split_blocks;
     const double saved = 0.35 * (p.blocks - split_blocks), cost = 5.0 + 8e-6 * splits * double(p.m) * double(p.n) / 4.0;   // us
     if (splits > 1 && saved > cost) {
@@ -31,21 +32,35 @@ tg_status launch_pairs(const CUtensorMap& a, const CUtensorMap& b, ProductArgs8 
     }
   }
   const int pairs = p.splits > 1 ? int(tm * tn) * p.splits : int(std::min<int64_t>(tm * tn, most));
+  p.chunk = sizeof(T) == 4 ? 8 : 64;
   Scratch scratch(st);
-  if (p.splits > 1) {
-    p.ldp = round_up(p.n, 4);
-    const size_t count = size_t(p.splits) * size_t(p.m) * size_t(p.ldp);
-    const cudaError_t e = scratch.reserve(Scratch::size_of<float>(count));
-    if (e != cudaSuccess) return fail(TG_ERR_CUDA, "blocks8 product scratch: %s", cudaGetErrorString(e));
-    p.part = scratch.take<float>(count);
-  }
-  auto kern = tgb::blocks_pair_kernel<T, ROWS>;
-  const void* entry = reinterpret_cast<const void*>(kern);
+  const size_t parts = p.splits > 1 ? size_t(p.splits) * size_t(p.m) * size_t(round_up(p.n, 4)) : 0;
+  const size_t groups = size_t(p.blocks + 3) / 4;
+  p.pitch_a = tm * 256;
+  p.pitch_b = tn * 2 * p.half_n;
+  const size_t words_a = groups * size_t(p.pitch_a), words_b = groups * size_t(p.pitch_b);
+  const cudaError_t e = scratch.reserve(Scratch::size_of<float>(parts) + Scratch::size_of<uint32_t>(words_a) + Scratch::size_of<uint32_t>(words_b) +
+                                        Scratch::size_of<int>(tgb::kPackBlocks));
+  if (e != cudaSuccess) return fail(TG_ERR_CUDA, "blocks8 product scratch: %s", cudaGetErrorString(e));
+  p.ldp = round_up(p.n, 4);
+  p.part = scratch.take<float>(parts);
+  p.words_a = scratch.take<uint32_t>(words_a);
+  p.words_b = scratch.take<uint32_t>(words_b);
+  p.other = scratch.take<int>(tgb::kPackBlocks);
+  auto scaled = tgb::blocks_scaled_kernel<T>;
+  auto any = tgb::blocks_pair_kernel<T, ROWS>;
+  const void *scaled_entry = reinterpret_cast<const void*>(scaled), *any_entry = reinterpret_cast<const void*>(any);
   // the epilogue's registers come from what the block was launched with
-  if (kernel_regs(entry) * S::kThreads < 128 * S::kLow + (S::kThreads - 128) * S::kHigh) return fail(TG_ERR_UNSUPPORTED, "blocks8 product: built with too few registers");
-  const tg_status s = ensure_smem(entry, S::kSmem);
+  if (kernel_regs(any_entry) * S::kThreads < 128 * S::kLow + (S::kThreads - 128) * S::kHigh ||
+      kernel_regs(scaled_entry) * X::kThreads < 256 * X::kLow + (X::kThreads - 256) * X::kHigh)
+    return fail(TG_ERR_UNSUPPORTED, "blocks8 product: built with too few registers");
+  tg_status s = ensure_smem(scaled_entry, X::kSmem);
+  if (s == TG_OK) s = ensure_smem(any_entry, S::kSmem);
   if (s != TG_OK) return s;
-  launch_kernel(kern, 2 * pairs, S::kThreads, S::kSmem, 0, st, a, b, p);
+  // The scales decide on the device which of the two kernels does the product; the other one returns at once.
+  launch_kernel(tgb::pack_scales_kernel, tgb::kPackBlocks, 256, 0, 0, st, p, ROWS ? 1 : 128);
+  launch_kernel(scaled, 2 * pairs, X::kThreads, X::kSmem, 0, st, a, b, p);
+  launch_kernel(any, 2 * pairs, S::kThreads, S::kSmem, 0, st, a, b, p);
   if (p.splits > 1)
     launch_kernel(tgb::blocks_join_kernel<T>, dim3(unsigned((p.n + 1023) / 1024), unsigned(std::min<int64_t>(p.m, 16384))), 256, 0, 0, st, p);
   return check_launch("blocks8 product");

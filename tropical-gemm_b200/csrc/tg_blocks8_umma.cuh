@@ -27,6 +27,11 @@ struct ProductArgs8 {
   float* part;                // sums of the parts, (splits x m x ldp)
   int64_t ldp;
   int vec;                    // 16-byte stores of C's rows
+  // scales that are powers of two, packed for the tensor core (pack_scales_kernel)
+  uint32_t *words_a, *words_b;   // (groups of 4 blocks) x (rows of A, of B, to whole tiles)
+  int64_t pitch_a, pitch_b;
+  int* other;                 // kPackBlocks flags: some scale is not a power of two
+  int chunk;                  // blocks that the tensor core may sum (scaled kernel)
 };
 
 // Two f32 values side by side.
@@ -51,6 +56,39 @@ __device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
 __device__ __forceinline__ void load_pairs(uint32_t from, uint64_t& a, uint64_t& b) {
   asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(from));
 }
+
+// ------------------------------------------------------------------------------- scales that are powers of two
+// Exponents of four blocks' scales per word, and whether all scales are powers of
+// two (from 2^-126 on) or NaN.  Rows past the last get zeros.
+constexpr int kPackBlocks = 256;
+static __global__ void __launch_bounds__(256) pack_scales_kernel(const ProductArgs8 p, int b_tall) {
+  after_previous_kernel();
+  const int64_t groups = (p.blocks + 3) / 4, total_a = groups * p.pitch_a, total = total_a + groups * p.pitch_b;
+  bool bad = false;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+    const bool is_a = i < total_a;
+    const int64_t at = is_a ? i : i - total_a, pitch = is_a ? p.pitch_a : p.pitch_b, g = at / pitch, r = at - g * pitch;
+    uint32_t w = 0;
+    if (r < (is_a ? p.m : p.n)) {
+      const float* s = is_a ? p.a_scale + r * p.a_row : p.b_scale + r / b_tall * p.b_row;
+      const int64_t step = is_a ? p.a_block : p.b_block;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (g * 4 + j >= p.blocks) break;
+        const uint32_t bits = __float_as_uint(s[(g * 4 + j) * step]);
+        uint32_t e = bits >> 23;   // 255: NaN
+        if ((bits & 0x7fffffffu) > 0x7f800000u) e = 255;
+        else if (bits & 0x007fffffu || e == 0 || e >= 255) bad = true;
+        w |= (e & 255) << (8 * j);
+      }
+    }
+    (is_a ? p.words_a : p.words_b)[at] = w;
+  }
+  bad = __syncthreads_or(bad);
+  if (threadIdx.x == 0) p.other[blockIdx.x] = bad;
+}
+// Whether some scale is not a power of two: the same in all threads.
+__device__ __forceinline__ bool other_scales(const int* other) { return __syncthreads_or(threadIdx.x < kPackBlocks && other[threadIdx.x]); }
 
 // ------------------------------------------------------------------------------- pairs of CTAs, tiles of 256 x 256
 // Persistent; CTA r of a pair holds rows 128 r .. of A's tile and half of B's, and
@@ -105,6 +143,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape::kThreads,
 blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs8 p) {
   using S = PairShape;
   using tg8::kOperand;
+  after_previous_kernel();
+  if (!other_scales(p.other)) return;   // blocks_scaled_kernel has done it
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (umma::smem_u32(smem_raw) + 1023) & ~1023u;
   uint8_t* smem = smem_raw + (base - umma::smem_u32(smem_raw));
@@ -132,7 +172,6 @@ blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     umma::bar_init_fence();
   }
   if (warp == 2) umma::tmem_alloc<2>(base + S::kOffSlot, 512);
-  after_previous_kernel();
   umma::fence_before();
   umma::cluster_sync();
   umma::fence_after();
@@ -292,6 +331,235 @@ blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             v.y += bias[half * 128 + c + 2 * e + 1];
             if (!ok) v.x = v.y = __uint_as_float(0x7fffffffu);
             z[e] = tg8::pack_pair<T>(v.x, v.y);
+          }
+          tg8::store_rows64(static_cast<T*>(p.c) + row0 * p.ldc + col0 + c, p.ldc, rows, p.n - col0 - c, p.vec, z, staging, lane);
+        }
+      }
+    }
+    if (!ok) umma::drain_copies();
+  }
+
+  __syncwarp();
+  umma::fence_before();
+  umma::cluster_sync();
+  if (warp == 2) {
+    umma::fence_after();
+    umma::tmem_free<2>(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------- the same for scales that are powers of two
+// The tensor core applies them itself, from tensor memory, so that a sum stays
+// there: blocks_pair_kernel's epilogue, per block a hand-over of 800 cycles and
+// 500 of reads and arithmetic with two accumulators, keeps the tensor core at 40 %
+// (8192^3 bf16: 0.70 ms; this kernel 0.38).
+//
+// Warps 4-7 bring the scales: four blocks' exponents are one word per row, of
+// which a CTA takes its 128 rows of A and all 256 of B to each quarter of the
+// lanes of its own tensor memory, in four slots in turn.  One accumulator of 256
+// columns fits beside them: a tile's sum is taken to registers before the next
+// one begins (about 1000 cycles; a tile of 8192 takes 33000).
+//
+// The tensor core's f32 sums lose in proportion to their length, so they are
+// taken out and added up in f32 every `chunk` blocks.
+struct ScaledShape {
+  static constexpr int kStages = 6, kStage = 2 * tg8::kOperand, kEpi = 8, kSlots = 4, kThreads = 512;
+  static constexpr int kLow = 48, kHigh = 208;   // registers per thread of the first two warpgroups, and of the epilogue's two
+  static constexpr int kOffStaging = kStages * kStage;
+  static constexpr int kOffBias = kOffStaging + kEpi * tg8::kStagingBytes;
+  static constexpr int kOffBars = kOffBias + 256 * 4;
+  static constexpr int kBars = 2 * (kStages + kSlots + 1);
+  static constexpr int kOffSlot = kOffBars + kBars * 8;
+  static constexpr int kSmem = kOffSlot + 16 + 1024;
+};
+static_assert(ScaledShape::kSmem <= 227 * 1024, "shared memory");
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ScaledShape::kThreads, 1)
+blocks_scaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs8 p) {
+  using S = ScaledShape;
+  using tg8::kOperand;
+  after_previous_kernel();
+  if (other_scales(p.other)) return;   // blocks_pair_kernel takes it
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (umma::smem_u32(smem_raw) + 1023) & ~1023u;
+  uint8_t* smem = smem_raw + (base - umma::smem_u32(smem_raw));
+  const uint32_t bars = base + S::kOffBars;
+  auto full = [&](int s) { return bars + 8 * s; };                              // operands in place in both CTAs (leader)
+  auto empty = [&](int s) { return bars + 8 * (S::kStages + s); };              // products that read them are done (each CTA)
+  auto scales_full = [&](int s) { return bars + 8 * (2 * S::kStages + s); };    // scales in both CTAs' tensor memory (leader)
+  auto scales_empty = [&](int s) { return bars + 8 * (2 * S::kStages + S::kSlots + s); };   // and used (each CTA)
+  const uint32_t acc_full = bars + 8 * (2 * S::kStages + 2 * S::kSlots), acc_empty = acc_full + 8;   // sum done (each CTA); taken out in both (leader)
+  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + S::kOffSlot);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t rank = umma::cta_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (warp == 0 && lane == 0) {
+    umma::tma_prefetch(&map_a);
+    umma::tma_prefetch(&map_b);
+    for (int s = 0; s < S::kStages; s++) {
+      umma::bar_init(full(s), 1);
+      umma::bar_init(empty(s), 1);
+    }
+    for (int s = 0; s < S::kSlots; s++) {
+      umma::bar_init(scales_full(s), 8);
+      umma::bar_init(scales_empty(s), 1);
+    }
+    umma::bar_init(acc_full, 1);
+    umma::bar_init(acc_empty, 2 * S::kEpi);
+    umma::bar_init_fence();
+  }
+  if (warp == 2) umma::tmem_alloc<2>(base + S::kOffSlot, 512);
+  umma::fence_before();
+  umma::cluster_sync();
+  umma::fence_after();
+  const uint32_t tmem = *slot, scales = tmem + 256;   // slot s: A's 4 columns at scales + 16 s, B's 8 behind them
+  bool ok = true;   // false once a wait of this role ran out
+
+  if (warp < 4) {
+    umma::registers_down<S::kLow>();
+    const bool issue = umma::elect_one();
+    tg8::RingAt<S::kStages> at;
+    PairItem item;
+    if (warp == 0) {
+      // ---- producer: this CTA's half of each operand
+      for (int i = 0; ok && pair_item(p, pair, pairs, i, item); i++) {
+        const int row = int(item.m0) + int(rank) * 128, col = int(item.n0) + int(rank) * p.half_n;
+        for (int b = item.b0; b < item.b1; b++, at.next()) {
+          if (!umma::bar_wait(empty(at.slot), at.parity ^ 1)) { ok = false; break; }
+          const uint32_t to = base + at.slot * S::kStage, bar = umma::map_rank(full(at.slot), 0);
+          if (issue) {
+            if (rank == 0) umma::bar_expect(full(at.slot), 4 * kOperand);
+            umma::tma_load_3d_pair(to, &map_b, b * 128, col, 0, bar);
+            umma::tma_load_3d_pair(to + kOperand, &map_a, b * 128, row, 0, bar);
+          }
+        }
+      }
+      if (!ok) umma::drain_copies();
+    } else if (warp == 1 && rank == 0) {
+      // ---- products, issued by one thread of the leader for both SMs
+      const uint32_t idesc = umma::instr_desc_scaled(256, 2 * p.half_n);
+      const uint64_t db0 = umma::smem_desc(base, 16, 1024), da0 = umma::smem_desc(base + kOperand, 16, 1024);
+      tg8::RingAt<S::kSlots> sc;
+      uint32_t n = 0;   // sums so far
+      for (int i = 0; ok && pair_item(p, pair, pairs, i, item); i++) {
+        for (int b = item.b0; b < item.b1; b++, at.next()) {
+          const int in = b - item.b0;
+          const bool first = in % p.chunk == 0, last = b + 1 == item.b1 || (in + 1) % p.chunk == 0;
+          if ((in & 3) == 0 && !umma::bar_wait<true>(scales_full(sc.slot), sc.parity)) { ok = false; break; }
+          if (first && !umma::bar_wait<true>(acc_empty, (n & 1) ^ 1)) { ok = false; break; }
+          if (!umma::bar_wait(full(at.slot), at.parity)) { ok = false; break; }
+          umma::fence_after();
+          const uint32_t off = at.slot * (S::kStage >> 4), sa = scales + 16 * sc.slot, id = idesc | umma::scale_byte(in & 3);
+          const bool group_done = (in & 3) == 3 || b + 1 == item.b1;
+          if (issue) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) umma::mma_f8_scaled<2>(tmem, da0 + (off + j * 2), db0 + (off + j * 2), id, sa, sa + 4, !first || j);
+            umma::mma_commit<2>(empty(at.slot));
+            if (group_done) umma::mma_commit<2>(scales_empty(sc.slot));
+            if (last) umma::mma_commit<2>(acc_full);
+          }
+          if (group_done) sc.next();
+          if (last) n++;
+        }
+        __syncwarp();
+      }
+      if (!ok) umma::drain_copies();
+    }
+  } else if (warp < 8) {
+    umma::registers_down<S::kLow>();
+    // ---- scales: each warp writes all of this CTA's to its quarter of the lanes
+    const uint32_t quarter = scales + (uint32_t((warp & 3) * 32) << 16);
+    tg8::RingAt<S::kSlots> sc;
+    PairItem item;
+    for (int i = 0; ok && pair_item(p, pair, pairs, i, item); i++) {
+      const int g1 = (item.b1 - 1) / 4;   // item.b0 is a multiple of 4
+      const uint32_t *wa = p.words_a + item.m0 + rank * 128 + lane, *wb = p.words_b + item.n0 + lane;
+      uint32_t a[4], b[8];
+      auto load = [&](int64_t g) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) a[j] = wa[g * p.pitch_a + 32 * j];
+#pragma unroll
+        for (int j = 0; j < 8; j++) b[j] = j < 4 || p.half_n == 128 ? wb[g * p.pitch_b + 32 * j] : 0u;
+      };
+      load(item.b0 / 4);
+      for (int g = item.b0 / 4; g <= g1; g++, sc.next()) {
+        if (!umma::bar_wait(scales_empty(sc.slot), sc.parity ^ 1)) { ok = false; break; }
+        umma::fence_after();
+        umma::tmem_store4(quarter + 16 * sc.slot, a);
+        umma::tmem_store8(quarter + 16 * sc.slot + 4, b);
+        if (g < g1) load(g + 1);
+        umma::tmem_store_wait();
+        umma::fence_before();
+        __syncwarp();
+        if (lane == 0) umma::bar_arrive_cluster(umma::map_rank(scales_full(sc.slot), 0));
+      }
+    }
+    if (!ok) umma::drain_copies();
+  } else {
+    umma::registers_up<S::kHigh>();
+    // ---- epilogue: warp w has lanes 32 (w % 4) .. of tensor memory and one half of the columns
+    const int w = warp & 3, half = (warp - 8) >> 2, tid = threadIdx.x - 256;
+    const uint32_t staging = base + S::kOffStaging + (warp - 8) * tg8::kStagingBytes;
+    float* bias = reinterpret_cast<float*>(smem + S::kOffBias);
+    const int columns = min(128, 2 * p.half_n - half * 128);   // of this warp's half: none in narrow tiles' second
+    const uint32_t from = tmem + half * 128 + (uint32_t(w * 32) << 16);
+    PairItem item;
+    uint32_t n = 0;
+    for (int i = 0; pair_item(p, pair, pairs, i, item); i++) {
+      const int64_t row0 = item.m0 + rank * 128 + w * 32, col0 = item.n0 + half * 128;
+      const bool parts = p.splits > 1;
+      if (!parts) {
+        asm volatile("bar.sync 1, 256;" ::: "memory");   // the last tile's bias is no longer read
+        bias[tid] = p.bias && item.n0 + tid < p.n ? to_f32(static_cast<const T*>(p.bias)[item.n0 + tid]) : 0.f;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+      float acc[128];
+      for (int b = item.b0; b < item.b1; b += p.chunk, n++) {
+        for (int k = 0; ok; k++) {   // a whole sum: the limit grows with its length
+          if (umma::bar_wait(acc_full, n & 1)) break;
+          if (k >= min(p.chunk, item.b1 - b) >> 10) ok = false;
+        }
+        umma::fence_after();
+        if (columns > 0) {
+          if (b == item.b0) {
+#pragma unroll
+            for (int c = 0; c < 128; c += 32) umma::tmem_load32(from + c, reinterpret_cast<uint32_t(&)[32]>(acc[c]));
+            umma::tmem_load_wait();
+          } else {
+#pragma unroll
+            for (int c = 0; c < 128; c += 16) {
+              uint32_t t[16];
+              umma::tmem_load16(from + c, t);
+              umma::tmem_load_wait();
+#pragma unroll
+              for (int e = 0; e < 16; e++) acc[c + e] += __uint_as_float(t[e]);
+            }
+          }
+        }
+        umma::fence_before();
+        __syncwarp();
+        if (lane == 0) umma::bar_arrive_cluster(umma::map_rank(acc_empty, 0));
+      }
+      if (columns <= 0) continue;
+      const int rows = int(max(int64_t(0), min(int64_t(32), p.m - row0)));
+#pragma unroll
+      for (int c = 0; c < 128; c += 16) {
+        if (c >= columns || col0 + c >= p.n) break;
+        uint32_t z[16];
+        if (parts || sizeof(T) == 4) {   // 16 columns
+#pragma unroll
+          for (int e = 0; e < 16; e++) z[e] = ok ? __float_as_uint(parts ? acc[c + e] : acc[c + e] + bias[half * 128 + c + e]) : 0x7fffffffu;   // a wait ran out: the outputs say so
+          if (parts) tg8::store_rows64(p.part + (int64_t(pair % p.splits) * p.m + row0) * p.ldp + col0 + c, p.ldp, rows, p.ldp - col0 - c, true, z, staging, lane);
+          else if constexpr (sizeof(T) == 4) tg8::store_rows64(static_cast<T*>(p.c) + row0 * p.ldc + col0 + c, p.ldc, rows, p.n - col0 - c, p.vec, z, staging, lane);
+        } else if constexpr (sizeof(T) == 2) {   // 32 columns
+          if (c % 32) continue;
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            float x = acc[c + 2 * e] + bias[half * 128 + c + 2 * e], y = acc[c + 2 * e + 1] + bias[half * 128 + c + 2 * e + 1];
+            if (!ok) x = y = __uint_as_float(0x7fffffffu);
+            z[e] = tg8::pack_pair<T>(x, y);
           }
           tg8::store_rows64(static_cast<T*>(p.c) + row0 * p.ldc + col0 + c, p.ldc, rows, p.n - col0 - c, p.vec, z, staging, lane);
         }

@@ -185,6 +185,31 @@ template <int CTAS> __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t 
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
+// e4m3 operands with scales, powers of two (e8m0) in tensor memory: one per row
+// of A and of B for the 32 of the sum.  Row r's scales of four products are the
+// bytes of the word at lane r % 32, column r / 32 of `sa` (of every quarter of
+// the lanes); the instruction descriptor chooses the byte.
+__host__ __device__ constexpr uint32_t instr_desc_scaled(uint32_t m, uint32_t n) { return (n >> 3) << 17 | 1u << 23 | (m >> 7) << 27; }
+__host__ __device__ constexpr uint32_t scale_byte(uint32_t byte) { return byte << 4 | byte << 29; }
+template <int CTAS>
+__device__ __forceinline__ void mma_f8_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, bool accumulate) {
+  const uint32_t acc = accumulate;
+  if constexpr (CTAS == 2)
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n}\n"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(sa), "r"(sb) : "memory");
+  else
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n}\n"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(sa), "r"(sb) : "memory");
+}
+// Columns of this warp's 32 lanes from registers.
+__device__ __forceinline__ void tmem_store4(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // Registers per thread of a warpgroup, all of whose threads come here.
 template <int N> __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
