@@ -91,21 +91,31 @@ static __global__ void __launch_bounds__(256) pack_scales_kernel(const ProductAr
 __device__ __forceinline__ bool other_scales(const int* other) { return __syncthreads_or(threadIdx.x < kPackBlocks && other[threadIdx.x]); }
 
 // ------------------------------------------------------------------------------- pairs of CTAs, tiles of 256 x 256
-// Persistent; CTA r of a pair holds rows 128 r .. of A's tile and half of B's, and
-// sums 128 x 256 outputs in the registers of 8 epilogue warps (128 each per
-// thread, for which the other warps give theirs up).
+// Persistent; CTA r of a pair holds rows 128 r .. of A's tile and half of B's.
 //
-// What bounds it: per block an SM's tensor core takes 512 cycles, the epilogue's
-// reads of tensor memory 256 (128 x 256 f32 at 512 bytes a cycle) and its f32
-// arithmetic 256 with a scale per tile of B, 512 with one per row and column.
+// Scales that are powers of two the tensor core applies itself, from tensor
+// memory, and the sum stays there.  Warps 4-7 bring them: four blocks' exponents
+// are one word per row, of which a CTA takes its 128 rows of A and all 256 of B
+// to each quarter of the lanes of its own tensor memory, in four slots in turn.
+// One accumulator of 256 columns fits beside them: a tile's sum is taken to
+// registers before the next one begins (about 1000 cycles; a tile of 8192 takes
+// 33000).  The tensor core's f32 sums lose in proportion to their length, so they
+// are taken out and added up in f32 every `chunk` blocks.
+//
+// With other scales each block goes into an accumulator of its own, of two in
+// turn, which the epilogue scales and adds up: a hand-over of 800 cycles and 500
+// of reads and arithmetic per block of 512, so this is 1.8 times slower
+// (8192^3 bf16: 0.39 and 0.70 ms).
+//
+// What bounds it: power (8192^3 2.8 PFLOP/s; 4096^3 57 us in four rounds of tiles).
 struct PairShape {
-  static constexpr int kStages = 6, kStage = 2 * tg8::kOperand, kEpi = 8, kThreads = 32 * (4 + kEpi);
-  static constexpr int kLow = 40, kHigh = 232;   // registers per thread of the first warpgroup, and of the other two
+  static constexpr int kStages = 6, kStage = 2 * tg8::kOperand, kEpi = 8, kSlots = 4, kThreads = 512;
+  static constexpr int kLow = 48, kHigh = 208;   // registers per thread of the first two warpgroups, and of the epilogue's two
   static constexpr int kOffStaging = kStages * kStage;
   static constexpr int kOffBias = kOffStaging + kEpi * tg8::kStagingBytes;
-  static constexpr int kOffScales = kOffBias + 256 * 4;      // ROWS: per warp two sets of 128 column scales
-  static constexpr int kOffBars = kOffScales + kEpi * 2 * 512;
-  static constexpr int kBars = 2 * (kStages + 2);
+  static constexpr int kOffScales = kOffBias + 256 * 4;      // other scales, ROWS: per epilogue warp 128 column scales
+  static constexpr int kOffBars = kOffScales + kEpi * 512;
+  static constexpr int kBars = 2 * (kStages + kSlots + 2);
   static constexpr int kOffSlot = kOffBars + kBars * 8;
   static constexpr int kSmem = kOffSlot + 16 + 1024;
 };
@@ -144,243 +154,7 @@ blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   using S = PairShape;
   using tg8::kOperand;
   after_previous_kernel();
-  if (!other_scales(p.other)) return;   // blocks_scaled_kernel has done it
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t base = (umma::smem_u32(smem_raw) + 1023) & ~1023u;
-  uint8_t* smem = smem_raw + (base - umma::smem_u32(smem_raw));
-  const uint32_t bars = base + S::kOffBars;
-  auto full = [&](int s) { return bars + 8 * s; };                        // operands in place in both CTAs (leader)
-  auto empty = [&](int s) { return bars + 8 * (S::kStages + s); };        // products that read them are done (each CTA)
-  auto acc_full = [&](int b) { return bars + 8 * (2 * S::kStages + b); };      // block summed (each CTA)
-  auto acc_empty = [&](int b) { return bars + 8 * (2 * S::kStages + 2 + b); };  // and taken out in both CTAs (leader)
-  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + S::kOffSlot);
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t rank = umma::cta_rank();
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-
-  if (warp == 0 && lane == 0) {
-    umma::tma_prefetch(&map_a);
-    umma::tma_prefetch(&map_b);
-    for (int s = 0; s < S::kStages; s++) {
-      umma::bar_init(full(s), 1);
-      umma::bar_init(empty(s), 1);
-    }
-    for (int b = 0; b < 2; b++) {
-      umma::bar_init(acc_full(b), 1);
-      umma::bar_init(acc_empty(b), 2 * S::kEpi);
-    }
-    umma::bar_init_fence();
-  }
-  if (warp == 2) umma::tmem_alloc<2>(base + S::kOffSlot, 512);
-  umma::fence_before();
-  umma::cluster_sync();
-  umma::fence_after();
-  const uint32_t tmem = *slot;
-  bool ok = true;   // false once a wait of this role ran out
-
-  if (warp < 4) {
-    umma::registers_down<S::kLow>();
-    const bool issue = umma::elect_one();
-    tg8::RingAt<S::kStages> at;
-    PairItem item;
-    if (warp == 0) {
-      // ---- producer: this CTA's half of each operand
-      for (int i = 0; ok && pair_item(p, pair, pairs, i, item); i++) {
-        const int row = int(item.m0) + int(rank) * 128, col = int(item.n0) + int(rank) * p.half_n;
-        for (int b = item.b0; b < item.b1; b++, at.next()) {
-          if (!umma::bar_wait(empty(at.slot), at.parity ^ 1)) { ok = false; break; }
-          const uint32_t to = base + at.slot * S::kStage, bar = umma::map_rank(full(at.slot), 0);
-          if (issue) {
-            if (rank == 0) umma::bar_expect(full(at.slot), 4 * kOperand);
-            umma::tma_load_3d_pair(to, &map_b, b * 128, col, 0, bar);
-            umma::tma_load_3d_pair(to + kOperand, &map_a, b * 128, row, 0, bar);
-          }
-        }
-      }
-      if (!ok) umma::drain_copies();
-    } else if (warp == 1 && rank == 0) {
-      // ---- products, issued by one thread of the leader for both SMs
-      const uint32_t idesc = umma::instr_desc(1, 0, false, false, 256, 2 * p.half_n);
-      const uint64_t db0 = umma::smem_desc(base, 16, 1024), da0 = umma::smem_desc(base + kOperand, 16, 1024);
-      uint32_t n = 0;   // blocks so far: block n goes into accumulator n % 2
-      for (int i = 0; ok && pair_item(p, pair, pairs, i, item); i++) {
-        for (int b = item.b0; b < item.b1; b++, at.next(), n++) {
-          const uint32_t buf = n & 1;
-          if (!umma::bar_wait(full(at.slot), at.parity) || !umma::bar_wait<true>(acc_empty(buf), ((n >> 1) & 1) ^ 1)) { ok = false; break; }
-          umma::fence_after();
-          const uint32_t off = at.slot * (S::kStage >> 4);
-          if (issue) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) umma::mma_f8<2>(tmem + buf * 256, da0 + (off + j * 2), db0 + (off + j * 2), idesc, j > 0);
-            umma::mma_commit<2>(empty(at.slot));
-            umma::mma_commit<2>(acc_full(buf));
-          }
-        }
-        __syncwarp();
-      }
-      if (!ok) umma::drain_copies();
-    }
-  } else {
-    umma::registers_up<S::kHigh>();
-    // ---- epilogue: warp w has lanes 32 (w % 4) .. of tensor memory and one half of the columns
-    const int w = (warp - 4) & 3, half = (warp - 4) >> 2, tid = threadIdx.x - 128;
-    const uint32_t staging = base + S::kOffStaging + (warp - 4) * tg8::kStagingBytes;
-    const uint32_t scales = base + S::kOffScales + (warp - 4) * 1024;
-    float* bias = reinterpret_cast<float*>(smem + S::kOffBias);
-    const int columns = min(128, 2 * p.half_n - half * 128);   // of this warp's half: none in narrow tiles' second
-    PairItem item;
-    uint32_t n = 0;
-    for (int i = 0; pair_item(p, pair, pairs, i, item); i++) {
-      const int64_t row0 = item.m0 + rank * 128 + w * 32, row = row0 + lane, col0 = item.n0 + half * 128;
-      const bool live = row < p.m && columns > 0;
-      if (p.splits == 1) {
-        asm volatile("bar.sync 1, 256;" ::: "memory");   // the last tile's bias is no longer read
-        bias[tid] = p.bias && item.n0 + tid < p.n ? to_f32(static_cast<const T*>(p.bias)[item.n0 + tid]) : 0.f;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-      }
-      // scales two blocks ahead: their way from memory stays out of the waits
-      const float* sa = p.a_scale + (live ? row : 0) * p.a_row;
-      const float* sb = p.b_scale + (col0 < p.n ? (ROWS ? col0 : col0 / kBlock) : 0) * p.b_row;
-      auto row_scale = [&](int b) { return live && b < item.b1 ? sa[b * p.a_block] : 0.f; };
-      auto tile_scale = [&](int b) { return !ROWS && b < item.b1 ? sb[b * p.b_block] : 0.f; };
-      float ra[2] = {row_scale(item.b0), row_scale(item.b0 + 1)}, rb[2] = {tile_scale(item.b0), tile_scale(item.b0 + 1)};
-      float rc[4];   // ROWS: columns lane, lane + 32, .. of the next block
-      auto column_scales = [&](int b) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int64_t col = lane + 32 * j;
-          rc[j] = b < item.b1 && col < columns && col0 + col < p.n ? sb[col * p.b_row + b * p.b_block] : 0.f;
-        }
-      };
-      if (ROWS) column_scales(item.b0);
-      uint64_t acc[64];
-#pragma unroll
-      for (int j = 0; j < 64; j++) acc[j] = 0;
-      const uint32_t quarter = tmem + half * 128 + (uint32_t(w * 32) << 16);
-#pragma unroll 1
-      for (int b = item.b0; b < item.b1; b++, n++) {
-        const uint32_t buf = n & 1;
-        const float s = ROWS ? ra[0] : ra[0] * rb[0];
-        ra[0] = ra[1]; rb[0] = rb[1];
-        ra[1] = row_scale(b + 2); rb[1] = tile_scale(b + 2);
-        const uint32_t mine = scales + (b & 1) * 512;
-        if (ROWS) {
-#pragma unroll
-          for (int j = 0; j < 4; j++) asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + (lane + 32 * j) * 4), "f"(rc[j]) : "memory");
-          __syncwarp();
-          column_scales(b + 1);
-        }
-        if (ok) ok = umma::bar_wait(acc_full(buf), (n >> 1) & 1);
-        umma::fence_after();
-        const uint64_t s2 = pair_of(s, s);
-        auto taken = [&] {   // the next block but one may have the accumulator
-          umma::fence_before();
-          __syncwarp();
-          if (lane == 0) umma::bar_arrive_cluster(umma::map_rank(acc_empty(buf), 0));
-        };
-        if (columns <= 0) {
-          taken();
-          continue;
-        }
-        uint32_t t[2][32];
-        umma::tmem_load32(quarter + buf * 256, t[0]);
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          umma::tmem_load_wait();
-          if (c < 3) umma::tmem_load32(quarter + buf * 256 + (c + 1) * 32, t[(c + 1) & 1]);
-          else taken();
-#pragma unroll
-          for (int j = 0; j < 8; j++) {
-            const uint64_t lo = pair_of(t[c & 1][4 * j], t[c & 1][4 * j + 1]), hi = pair_of(t[c & 1][4 * j + 2], t[c & 1][4 * j + 3]);
-            if constexpr (ROWS) {
-              uint64_t c0, c1;
-              load_pairs(mine + c * 128 + j * 16, c0, c1);
-              fma_pair(acc[c * 16 + 2 * j], mul_pair(lo, s2), c0);
-              fma_pair(acc[c * 16 + 2 * j + 1], mul_pair(hi, s2), c1);
-            } else {
-              fma_pair(acc[c * 16 + 2 * j], lo, s2);
-              fma_pair(acc[c * 16 + 2 * j + 1], hi, s2);
-            }
-          }
-        }
-      }
-      if (columns <= 0) continue;
-      const int rows = int(max(int64_t(0), min(int64_t(32), p.m - row0)));
-      const bool parts = p.splits > 1;
-#pragma unroll
-      for (int c = 0; c < 128; c += 16) {   // 16 columns; two bytes per output: 32
-        if (c >= columns || col0 + c >= p.n) break;
-        if (parts || sizeof(T) == 4) {
-          uint32_t z[16];
-#pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            float2 v = values_of(acc[(c + e) / 2]);
-            if (!parts) { v.x += bias[half * 128 + c + e]; v.y += bias[half * 128 + c + e + 1]; }
-            z[e] = ok ? __float_as_uint(v.x) : 0x7fffffffu;   // a wait ran out: the outputs say so
-            z[e + 1] = ok ? __float_as_uint(v.y) : 0x7fffffffu;
-          }
-          if (parts) tg8::store_rows64(p.part + (int64_t(pair % p.splits) * p.m + row0) * p.ldp + col0 + c, p.ldp, rows, p.ldp - col0 - c, true, z, staging, lane);
-          else if constexpr (sizeof(T) == 4) tg8::store_rows64(static_cast<T*>(p.c) + row0 * p.ldc + col0 + c, p.ldc, rows, p.n - col0 - c, p.vec, z, staging, lane);
-        } else if constexpr (sizeof(T) == 2) {
-          if (c % 32) continue;
-          uint32_t z[16];
-#pragma unroll
-          for (int e = 0; e < 16; e++) {
-            float2 v = values_of(acc[c / 2 + e]);
-            v.x += bias[half * 128 + c + 2 * e];
-            v.y += bias[half * 128 + c + 2 * e + 1];
-            if (!ok) v.x = v.y = __uint_as_float(0x7fffffffu);
-            z[e] = tg8::pack_pair<T>(v.x, v.y);
-          }
-          tg8::store_rows64(static_cast<T*>(p.c) + row0 * p.ldc + col0 + c, p.ldc, rows, p.n - col0 - c, p.vec, z, staging, lane);
-        }
-      }
-    }
-    if (!ok) umma::drain_copies();
-  }
-
-  __syncwarp();
-  umma::fence_before();
-  umma::cluster_sync();
-  if (warp == 2) {
-    umma::fence_after();
-    umma::tmem_free<2>(tmem, 512);
-  }
-}
-
-// ------------------------------------------------------------------------------- the same for scales that are powers of two
-// The tensor core applies them itself, from tensor memory, so that a sum stays
-// there: blocks_pair_kernel's epilogue, per block a hand-over of 800 cycles and
-// 500 of reads and arithmetic with two accumulators, keeps the tensor core at 40 %
-// (8192^3 bf16: 0.70 ms; this kernel 0.38).
-//
-// Warps 4-7 bring the scales: four blocks' exponents are one word per row, of
-// which a CTA takes its 128 rows of A and all 256 of B to each quarter of the
-// lanes of its own tensor memory, in four slots in turn.  One accumulator of 256
-// columns fits beside them: a tile's sum is taken to registers before the next
-// one begins (about 1000 cycles; a tile of 8192 takes 33000).
-//
-// The tensor core's f32 sums lose in proportion to their length, so they are
-// taken out and added up in f32 every `chunk` blocks.
-struct ScaledShape {
-  static constexpr int kStages = 6, kStage = 2 * tg8::kOperand, kEpi = 8, kSlots = 4, kThreads = 512;
-  static constexpr int kLow = 48, kHigh = 208;   // registers per thread of the first two warpgroups, and of the epilogue's two
-  static constexpr int kOffStaging = kStages * kStage;
-  static constexpr int kOffBias = kOffStaging + kEpi * tg8::kStagingBytes;
-  static constexpr int kOffBars = kOffBias + 256 * 4;
-  static constexpr int kBars = 2 * (kStages + kSlots + 1);
-  static constexpr int kOffSlot = kOffBars + kBars * 8;
-  static constexpr int kSmem = kOffSlot + 16 + 1024;
-};
-static_assert(ScaledShape::kSmem <= 227 * 1024, "shared memory");
-
-template <typename T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ScaledShape::kThreads, 1)
-blocks_scaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const ProductArgs8 p) {
-  using S = ScaledShape;
-  using tg8::kOperand;
-  after_previous_kernel();
-  if (other_scales(p.other)) return;   // blocks_pair_kernel takes it
+  const bool other = other_scales(p.other);
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (umma::smem_u32(smem_raw) + 1023) & ~1023u;
   uint8_t* smem = smem_raw + (base - umma::smem_u32(smem_raw));
@@ -389,7 +163,8 @@ blocks_scaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
   auto empty = [&](int s) { return bars + 8 * (S::kStages + s); };              // products that read them are done (each CTA)
   auto scales_full = [&](int s) { return bars + 8 * (2 * S::kStages + s); };    // scales in both CTAs' tensor memory (leader)
   auto scales_empty = [&](int s) { return bars + 8 * (2 * S::kStages + S::kSlots + s); };   // and used (each CTA)
-  const uint32_t acc_full = bars + 8 * (2 * S::kStages + 2 * S::kSlots), acc_empty = acc_full + 8;   // sum done (each CTA); taken out in both (leader)
+  auto acc_full = [&](int b) { return bars + 8 * (2 * S::kStages + 2 * S::kSlots + b); };       // sum done (each CTA)
+  auto acc_empty = [&](int b) { return bars + 8 * (2 * S::kStages + 2 * S::kSlots + 2 + b); };   // and taken out in both CTAs (leader)
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + S::kOffSlot);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = umma::cta_rank();
@@ -406,8 +181,10 @@ blocks_scaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
       umma::bar_init(scales_full(s), 8);
       umma::bar_init(scales_empty(s), 1);
     }
-    umma::bar_init(acc_full, 1);
-    umma::bar_init(acc_empty, 2 * S::kEpi);
+    for (int b = 0; b < 2; b++) {
+      umma::bar_init(acc_full(b), 1);
+      umma::bar_init(acc_empty(b), 2 * S::kEpi);
+    }
     umma::bar_init_fence();
   }
   if (warp == 2) umma::tmem_alloc<2>(base + S::kOffSlot, 512);
@@ -439,31 +216,50 @@ blocks_scaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
       if (!ok) umma::drain_copies();
     } else if (warp == 1 && rank == 0) {
       // ---- products, issued by one thread of the leader for both SMs
-      const uint32_t idesc = umma::instr_desc_scaled(256, 2 * p.half_n);
       const uint64_t db0 = umma::smem_desc(base, 16, 1024), da0 = umma::smem_desc(base + kOperand, 16, 1024);
-      tg8::RingAt<S::kSlots> sc;
       uint32_t n = 0;   // sums so far
-      for (int i = 0; ok && pair_item(p, pair, pairs, i, item); i++) {
-        for (int b = item.b0; b < item.b1; b++, at.next()) {
-          const int in = b - item.b0;
-          const bool first = in % p.chunk == 0, last = b + 1 == item.b1 || (in + 1) % p.chunk == 0;
-          if ((in & 3) == 0 && !umma::bar_wait<true>(scales_full(sc.slot), sc.parity)) { ok = false; break; }
-          if (first && !umma::bar_wait<true>(acc_empty, (n & 1) ^ 1)) { ok = false; break; }
-          if (!umma::bar_wait(full(at.slot), at.parity)) { ok = false; break; }
-          umma::fence_after();
-          const uint32_t off = at.slot * (S::kStage >> 4), sa = scales + 16 * sc.slot, id = idesc | umma::scale_byte(in & 3);
-          const bool group_done = (in & 3) == 3 || b + 1 == item.b1;
-          if (issue) {
+      if (other) {      // sum n, one block, goes into accumulator n % 2
+        const uint32_t idesc = umma::instr_desc(1, 0, false, false, 256, 2 * p.half_n);
+        for (int i = 0; ok && pair_item(p, pair, pairs, i, item); i++) {
+          for (int b = item.b0; b < item.b1; b++, at.next(), n++) {
+            const uint32_t buf = n & 1;
+            if (!umma::bar_wait(full(at.slot), at.parity) || !umma::bar_wait<true>(acc_empty(buf), ((n >> 1) & 1) ^ 1)) { ok = false; break; }
+            umma::fence_after();
+            const uint32_t off = at.slot * (S::kStage >> 4);
+            if (issue) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) umma::mma_f8_scaled<2>(tmem, da0 + (off + j * 2), db0 + (off + j * 2), id, sa, sa + 4, !first || j);
-            umma::mma_commit<2>(empty(at.slot));
-            if (group_done) umma::mma_commit<2>(scales_empty(sc.slot));
-            if (last) umma::mma_commit<2>(acc_full);
+              for (int j = 0; j < 4; j++) umma::mma_f8<2>(tmem + buf * 256, da0 + (off + j * 2), db0 + (off + j * 2), idesc, j > 0);
+              umma::mma_commit<2>(empty(at.slot));
+              umma::mma_commit<2>(acc_full(buf));
+            }
           }
-          if (group_done) sc.next();
-          if (last) n++;
+          __syncwarp();
         }
-        __syncwarp();
+      } else {
+        const uint32_t idesc = umma::instr_desc_scaled(256, 2 * p.half_n);
+        tg8::RingAt<S::kSlots> sc;
+        for (int i = 0; ok && pair_item(p, pair, pairs, i, item); i++) {
+          for (int b = item.b0; b < item.b1; b++, at.next()) {
+            const int in = b - item.b0;
+            const bool first = in % p.chunk == 0, last = b + 1 == item.b1 || (in + 1) % p.chunk == 0;
+            if ((in & 3) == 0 && !umma::bar_wait<true>(scales_full(sc.slot), sc.parity)) { ok = false; break; }
+            if (first && !umma::bar_wait<true>(acc_empty(0), (n & 1) ^ 1)) { ok = false; break; }
+            if (!umma::bar_wait(full(at.slot), at.parity)) { ok = false; break; }
+            umma::fence_after();
+            const uint32_t off = at.slot * (S::kStage >> 4), sa = scales + 16 * sc.slot, id = idesc | umma::scale_byte(in & 3);
+            const bool group_done = (in & 3) == 3 || b + 1 == item.b1;
+            if (issue) {
+#pragma unroll
+              for (int j = 0; j < 4; j++) umma::mma_f8_scaled<2>(tmem, da0 + (off + j * 2), db0 + (off + j * 2), id, sa, sa + 4, !first || j);
+              umma::mma_commit<2>(empty(at.slot));
+              if (group_done) umma::mma_commit<2>(scales_empty(sc.slot));
+              if (last) umma::mma_commit<2>(acc_full(0));
+            }
+            if (group_done) sc.next();
+            if (last) n++;
+          }
+          __syncwarp();
+        }
       }
       if (!ok) umma::drain_copies();
     }
@@ -473,7 +269,7 @@ blocks_scaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     const uint32_t quarter = scales + (uint32_t((warp & 3) * 32) << 16);
     tg8::RingAt<S::kSlots> sc;
     PairItem item;
-    for (int i = 0; ok && pair_item(p, pair, pairs, i, item); i++) {
+    for (int i = 0; ok && !other && pair_item(p, pair, pairs, i, item); i++) {
       const int g1 = (item.b1 - 1) / 4;   // item.b0 is a multiple of 4
       const uint32_t *wa = p.words_a + item.m0 + rank * 128 + lane, *wb = p.words_b + item.n0 + lane;
       uint32_t a[4], b[8];
@@ -516,18 +312,23 @@ blocks_scaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         asm volatile("bar.sync 1, 256;" ::: "memory");
       }
       float acc[128];
-      for (int b = item.b0; b < item.b1; b += p.chunk, n++) {
-        for (int k = 0; ok; k++) {   // a whole sum: the limit grows with its length
-          if (umma::bar_wait(acc_full, n & 1)) break;
-          if (k >= min(p.chunk, item.b1 - b) >> 10) ok = false;
-        }
-        umma::fence_after();
-        if (columns > 0) {
-          if (b == item.b0) {
+      auto taken = [&](int buf) {   // the next sum may have the accumulator
+        umma::fence_before();
+        __syncwarp();
+        if (lane == 0) umma::bar_arrive_cluster(umma::map_rank(acc_empty(buf), 0));
+      };
+      if (!other) {
+        for (int b = item.b0; b < item.b1; b += p.chunk, n++) {
+          for (int k = 0; ok; k++) {   // a whole sum: the limit grows with its length
+            if (umma::bar_wait(acc_full(0), n & 1)) break;
+            if (k >= min(p.chunk, item.b1 - b) >> 10) ok = false;
+          }
+          umma::fence_after();
+          if (columns > 0 && b == item.b0) {
 #pragma unroll
             for (int c = 0; c < 128; c += 32) umma::tmem_load32(from + c, reinterpret_cast<uint32_t(&)[32]>(acc[c]));
             umma::tmem_load_wait();
-          } else {
+          } else if (columns > 0) {
 #pragma unroll
             for (int c = 0; c < 128; c += 16) {
               uint32_t t[16];
@@ -537,10 +338,51 @@ blocks_scaled_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
               for (int e = 0; e < 16; e++) acc[c + e] += __uint_as_float(t[e]);
             }
           }
+          taken(0);
         }
-        umma::fence_before();
-        __syncwarp();
-        if (lane == 0) umma::bar_arrive_cluster(umma::map_rank(acc_empty, 0));
+      } else {
+        const int64_t row = row0 + lane;
+        const bool live = row < p.m && col0 < p.n && columns > 0;
+        const float* sa = p.a_scale + (live ? row : 0) * p.a_row;
+        const float* sb = p.b_scale + (col0 < p.n ? (ROWS ? col0 : col0 / kBlock) : 0) * p.b_row;
+        const uint32_t mine = base + S::kOffScales + (warp - 8) * 512;
+#pragma unroll
+        for (int c = 0; c < 128; c++) acc[c] = 0.f;
+#pragma unroll 1
+        for (int b = item.b0; b < item.b1; b++, n++) {
+          const uint32_t buf = n & 1;
+          float s = live ? sa[b * p.a_block] : 0.f;
+          if (ROWS) {
+            __syncwarp();   // the last block's are read
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const int64_t col = lane + 32 * j;
+              const float v = col < columns && col0 + col < p.n ? sb[col * p.b_row + b * p.b_block] : 0.f;
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + uint32_t(col) * 4), "f"(v) : "memory");
+            }
+            __syncwarp();
+          } else if (live) {
+            s *= sb[b * p.b_block];
+          }
+          if (ok) ok = umma::bar_wait(acc_full(buf), (n >> 1) & 1);
+          umma::fence_after();
+          if (columns > 0) {
+#pragma unroll
+            for (int c = 0; c < 128; c += 16) {
+              uint32_t t[16];
+              umma::tmem_load16(from + buf * 256 + c, t);
+              umma::tmem_load_wait();
+#pragma unroll
+              for (int e = 0; e < 16; e += 4) {
+                float k[4] = {1.f, 1.f, 1.f, 1.f};
+                if (ROWS) asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(k[0]), "=f"(k[1]), "=f"(k[2]), "=f"(k[3]) : "r"(mine + (c + e) * 4));
+#pragma unroll
+                for (int q = 0; q < 4; q++) acc[c + e + q] = ROWS ? fmaf(__uint_as_float(t[e + q]) * s, k[q], acc[c + e + q]) : fmaf(__uint_as_float(t[e + q]), s, acc[c + e + q]);
+              }
+            }
+          }
+          taken(buf);
+        }
       }
       if (columns <= 0) continue;
       const int rows = int(max(int64_t(0), min(int64_t(32), p.m - row0)));
