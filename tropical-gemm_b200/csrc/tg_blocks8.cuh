@@ -64,6 +64,55 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int64_t c, int64_t col
   }
 }
 
+// Two f32 values side by side.
+__device__ __forceinline__ uint64_t pair_of(uint32_t a, uint32_t b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair_of(float a, float b) { return pair_of(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ float2 values_of(uint64_t v) {
+  uint32_t a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+  return make_float2(__uint_as_float(a), __uint_as_float(b));
+}
+__device__ __forceinline__ uint64_t pair_of(float a) { return pair_of(a, a); }
+__device__ __forceinline__ void fma_pair(uint64_t& acc, uint64_t a, uint64_t b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b)); }
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_pair_of(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float sum_of(uint64_t v) {
+  const float2 f = values_of(v);
+  return f.x + f.y;
+}
+// Eight elements as four pairs: two f32 operations per instruction.
+template <typename T> __device__ __forceinline__ void get_pairs(const Vec8<T>& a, uint64_t (&v)[4]) {
+  float f[8];
+  a.get(f);
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] = pair_of(f[2 * i], f[2 * i + 1]);
+}
+__device__ __forceinline__ void from_pairs(const uint64_t (&v)[4], float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float2 x = values_of(v[i]);
+    f[2 * i] = x.x;
+    f[2 * i + 1] = x.y;
+  }
+}
+
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // A block's scale and its inverse, from the bit pattern of its largest

@@ -34,24 +34,6 @@ struct ProductArgs8 {
   int chunk;                  // blocks that the tensor core may sum (scaled kernel)
 };
 
-// Two f32 values side by side.
-__device__ __forceinline__ uint64_t pair_of(uint32_t a, uint32_t b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t pair_of(float a, float b) { return pair_of(__float_as_uint(a), __float_as_uint(b)); }
-__device__ __forceinline__ float2 values_of(uint64_t v) {
-  uint32_t a, b;
-  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
-  return make_float2(__uint_as_float(a), __uint_as_float(b));
-}
-__device__ __forceinline__ void fma_pair(uint64_t& acc, uint64_t a, uint64_t b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b)); }
-__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // Two pairs from shared memory.
 __device__ __forceinline__ void load_pairs(uint32_t from, uint64_t& a, uint64_t& b) {
   asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(from));

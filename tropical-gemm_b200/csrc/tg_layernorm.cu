@@ -5,9 +5,12 @@
 //   grad_x = rstd (a - mean(a) - u mean(a u)) + grad_h,  a = grad weight
 //
 // All are bound by memory: a row is read once, kept in registers between its
-// sums and its output, and written once.
+// sums and its output, and written once.  Many rows come by bulk copies into a
+// ring in shared memory, which keeps more of them on the way than registers
+// could; few rows are loaded directly.
 #include <algorithm>
 #include "tg_blocks8.cuh"
+#include "tg_umma.cuh"
 
 namespace tgb {
 
@@ -22,8 +25,9 @@ struct NormArgs {
   int tpr;                    // threads per row: 32 .. 512, a power of two
 };
 
-// Two sums over the tpr threads of a row: one named barrier per row, two sets
-// of partial results in turn.  The order is the same in every thread.
+// Two sums over the tpr threads of a row (a multiple of 32): one named barrier
+// per row, two sets of partial results in turn.  The order is the same in every
+// thread.
 struct PairJoin {
   float2 (*sums)[16];   // [2][warps of the block]
   int tpr, sub, turn;
@@ -37,12 +41,15 @@ struct PairJoin {
       const int lane = threadIdx.x & 31, warps = tpr >> 5, first = sub * warps;
       if (lane == 0) sums[turn][threadIdx.x >> 5] = s;
       asm volatile("bar.sync %0, %1;" ::"r"(sub + 1), "r"(tpr) : "memory");
-      s = sums[turn][first + (lane & (warps - 1))];
+      s = lane < warps ? sums[turn][first + lane] : make_float2(0.f, 0.f);
       turn ^= 1;
-      for (int d = warps >> 1; d; d >>= 1) {
+#pragma unroll
+      for (int d = 8; d; d >>= 1) {   // at most 16 warps
         s.x += __shfl_xor_sync(0xffffffffu, s.x, d);
         s.y += __shfl_xor_sync(0xffffffffu, s.y, d);
       }
+      s.x = __shfl_sync(0xffffffffu, s.x, 0);
+      s.y = __shfl_sync(0xffffffffu, s.y, 0);
     }
     return s;
   }
@@ -60,6 +67,15 @@ template <int ACCESS> __device__ __forceinline__ void mask_at(float (&v)[8], int
 #pragma unroll
   for (int e = 0; e < 8; e++)
     if (ACCESS != kAligned && !inside<ACCESS>(c, e, cols)) v[e] = 0.f;
+}
+template <int ACCESS> __device__ __forceinline__ void mask_pairs(uint64_t (&v)[4], int c, int cols) {
+  if (ACCESS != kAligned && (c < 0 || c + 8 > cols)) {   // a row's ends
+    float f[8];
+    from_pairs(v, f);
+    mask_at<ACCESS>(f, c, cols);
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = pair_of(f[2 * i], f[2 * i + 1]);
+  }
 }
 template <int ACCESS, typename T> __device__ __forceinline__ void store_at(T* row, int c, int cols, const float (&v)[8]) {
   if constexpr (ACCESS == kScalar) store_any(row, c, cols, v);
@@ -99,6 +115,75 @@ __device__ __forceinline__ void store_block(const NormArgs& p, int64_t row, int6
   if ((c & (kBlock - 1)) == 0) p.scale[row * p.scale_row + c / kBlock * p.scale_block] = s.scale;
 }
 
+// The two passes over a row that its threads hold: its statistics, and its
+// outputs.  Groups past the row take no part.
+template <int G, int ACCESS>
+__device__ __forceinline__ float2 row_stats(const uint64_t (&v)[G][4], int tpr, int t, int shift, int cols, float eps, PairJoin& join) {
+  auto at = [&](int g) { return (g * tpr + t) * 8 - shift; };
+  uint64_t sum = 0;
+#pragma unroll
+  for (int g = 0; g < G; g++) {
+    if (at(g) >= cols) continue;
+#pragma unroll
+    for (int i = 0; i < 4; i++) sum = add_pair(sum, v[g][i]);
+  }
+  const float n = float(cols), rough = join(make_float2(sum_of(sum), 0.f)).x / n;
+  const uint64_t minus = pair_of(-rough);
+  uint64_t off = 0, square = 0;
+#pragma unroll
+  for (int g = 0; g < G; g++) {
+    if (at(g) >= cols) continue;
+    uint64_t d[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) d[i] = add_pair(v[g][i], minus);
+    mask_pairs<ACCESS>(d, at(g), cols);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      off = add_pair(off, d[i]);
+      fma_pair(square, d[i], d[i]);
+    }
+  }
+  return finish_stats(rough, join(make_float2(sum_of(off), sum_of(square))), n, eps);
+}
+template <typename T, int G, int ACCESS, bool BLOCKS>
+__device__ __forceinline__ void finish_row(const NormArgs& p, int64_t row, int t, int shift, const uint64_t (&v)[G][4], const Vec8<T> (&w)[G],
+                                           const Vec8<T> (&b)[G], float2 st) {
+  if (t == 0 && p.mean) {
+    p.mean[row] = st.x;
+    p.rstd[row] = st.y;
+  }
+  const int cols = int(p.cols);
+  const uint64_t minus = pair_of(-st.x), scale = pair_of(st.y);
+  T* h = static_cast<T*>(p.h) + row * p.ldh;
+  T* out = static_cast<T*>(p.y) + row * p.ldy;
+#pragma unroll
+  for (int g = 0; g < G; g++) {
+    const int c = (g * p.tpr + t) * 8 - shift;
+    if (!BLOCKS && c >= cols) continue;
+    uint64_t y[4], k[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) y[i] = mul_pair(add_pair(v[g][i], minus), scale);
+    if (p.weight) {
+      get_pairs(w[g], k);
+#pragma unroll
+      for (int i = 0; i < 4; i++) y[i] = mul_pair(y[i], k[i]);
+    }
+    if (p.bias) {
+      get_pairs(b[g], k);
+#pragma unroll
+      for (int i = 0; i < 4; i++) y[i] = add_pair(y[i], k[i]);
+    }
+    float f[8];
+    if (p.h) {
+      from_pairs(v[g], f);
+      store_at<ACCESS>(h, c, cols, f);
+    }
+    from_pairs(y, f);
+    if constexpr (BLOCKS) store_block(p, row, c, f);
+    else store_at<ACCESS>(out, c, cols, f);
+  }
+}
+
 // tpr threads per row, G groups of 8 elements per thread.  A slot (tpr threads)
 // walks rows slot, slot + slots, ..; its threads have fixed columns, so weight
 // and bias stay in registers (rows that start anywhere: slots is a multiple of
@@ -130,61 +215,173 @@ __global__ void __launch_bounds__(512) layernorm_kernel(const NormArgs p) {
     if (p.weight) load_columns<ACCESS>(w[g], static_cast<const T*>(p.weight), at(g), cols);
     if (p.bias) load_columns<ACCESS>(b[g], static_cast<const T*>(p.bias), at(g), cols);
   }
-  const float n = float(cols);
   for (; row < p.rows; row += p.slots) {
-    float v[G][8], sum = 0.f;
+    uint64_t v[G][4];
 #pragma unroll
     for (int g = 0; g < G; g++) {
-      nx[g].get(v[g]);
+      get_pairs(nx[g], v[g]);
       if (res) {
-        float r[8];
-        nr[g].get(r);
+        uint64_t r[4];
+        get_pairs(nr[g], r);
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[g][e] += r[e];
+        for (int i = 0; i < 4; i++) v[g][i] = add_pair(v[g][i], r[i]);
       }
-      mask_at<ACCESS>(v[g], at(g), cols);
+      mask_pairs<ACCESS>(v[g], at(g), cols);
     }
     if (row + p.slots < p.rows) load(row + p.slots);
-#pragma unroll
-    for (int g = 0; g < G; g++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) sum += v[g][e];
-    const float rough = join(make_float2(sum, 0.f)).x / n;
-    float2 off = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int g = 0; g < G; g++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float d = inside<ACCESS>(at(g), e, cols) ? v[g][e] - rough : 0.f;
-        off.x += d;
-        off.y = fmaf(d, d, off.y);
-      }
-    const float2 st = finish_stats(rough, join(off), n, p.eps);
-    if (t == 0 && p.mean) {
-      p.mean[row] = st.x;
-      p.rstd[row] = st.y;
-    }
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-      const int c = at(g);
-      float y[8], k[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) y[e] = (v[g][e] - st.x) * st.y;
-      if (p.weight) {
-        w[g].get(k);
-#pragma unroll
-        for (int e = 0; e < 8; e++) y[e] *= k[e];
-      }
-      if (p.bias) {
-        b[g].get(k);
-#pragma unroll
-        for (int e = 0; e < 8; e++) y[e] += k[e];
-      }
-      if (p.h) store_at<ACCESS>(static_cast<T*>(p.h) + row * p.ldh, c, cols, v[g]);
-      if constexpr (BLOCKS) store_block(p, row, c, y);
-      else store_at<ACCESS>(static_cast<T*>(p.y) + row * p.ldy, c, cols, y);
-    }
+    const float2 st = row_stats<G, ACCESS>(v, p.tpr, t, shift, cols, p.eps, join);
+    finish_row<T, G, ACCESS, BLOCKS>(p, row, t, shift, v, w, b, st);
   }
+}
+
+// ------------------------------------------------------------------------------- rows by bulk copies
+// A stage holds one row of each of up to three operands for each of the `per`
+// rows that a block works on at once; a row is copied from the 16-byte boundary
+// before its first element, 16 bytes into its place.
+constexpr int kMostStages = 8;
+struct RowRing {
+  uint32_t base, full, empty;   // shared memory; barriers
+  int stages, per, ops, pitch;
+  __device__ __forceinline__ uint32_t at(int stage, int op, int sub) const { return base + uint32_t(((stage * ops + op) * per + sub) * pitch); }
+};
+// One warp starts the copies of a batch's rows into a stage.
+template <typename T>
+__device__ __forceinline__ void bring_rows(const RowRing& r, int64_t rows, int64_t cols, const void* const (&x)[3], const int64_t (&ld)[3], int64_t batch, int stage) {
+  const int lane = threadIdx.x & 31, here = int(min(int64_t(r.per), rows - batch * r.per));
+  uint32_t total = 0;
+  auto each = [&](auto&& f) {
+#pragma unroll
+    for (int op = 0; op < 3; op++)
+      if (op < r.ops)
+        for (int sub = lane; sub < here; sub += 32) {
+          const uintptr_t from = reinterpret_cast<uintptr_t>(static_cast<const T*>(x[op]) + (batch * r.per + sub) * ld[op]);
+          const uintptr_t a = from & ~uintptr_t(15), b = (from + cols * sizeof(T) + 15) & ~uintptr_t(15);
+          f(op, sub, a, uint32_t(b - a));
+        }
+  };
+  each([&](int, int, uintptr_t, uint32_t bytes) { total += bytes; });
+  total = __reduce_add_sync(0xffffffffu, total);
+  if (lane == 0) umma::bar_expect(r.full + 8 * stage, total);
+  __syncwarp();
+  each([&](int op, int sub, uintptr_t a, uint32_t bytes) {
+    umma::bulk_load(r.at(stage, op, sub) + 16, reinterpret_cast<const void*>(a), bytes, r.full + 8 * stage);
+  });
+}
+__device__ __forceinline__ uint4 load_shared16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+// Eight elements from shared memory; kScalar: from any element on.
+template <int ACCESS, typename T> __device__ __forceinline__ void take8(Vec8<T>& v, uint32_t at) {
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (ACCESS != kScalar) {
+      const uint4 a = load_shared16(at), b = load_shared16(at + 16);
+      v.a = make_float4(__uint_as_float(a.x), __uint_as_float(a.y), __uint_as_float(a.z), __uint_as_float(a.w));
+      v.b = make_float4(__uint_as_float(b.x), __uint_as_float(b.y), __uint_as_float(b.z), __uint_as_float(b.w));
+    } else {
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f[e]) : "r"(at + 4 * e));
+      v.a = make_float4(f[0], f[1], f[2], f[3]);
+      v.b = make_float4(f[4], f[5], f[6], f[7]);
+    }
+  } else if constexpr (ACCESS != kScalar) {
+    v.a = load_shared16(at);
+  } else {
+    const uint32_t skew = at & 15;
+    const uint4 lo = load_shared16(at - skew), hi = load_shared16(at - skew + 16);
+    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    if (skew & 8) {
+#pragma unroll
+      for (int k = 0; k < 6; k++) w[k] = w[k + 2];
+    }
+    if (skew & 4) {
+#pragma unroll
+      for (int k = 0; k < 5; k++) w[k] = w[k + 1];
+    }
+    const uint32_t bits = (skew & 2) * 8;
+    v.a = make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                     __funnelshift_r(w[3], w[4], bits));
+  }
+}
+template <typename T> __device__ __forceinline__ uint32_t skew_of(const T* row) { return uint32_t(reinterpret_cast<uintptr_t>(row) & 15); }
+
+// Many rows: as layernorm_kernel, `per` rows at once.  The first warp starts the
+// copies into a stage when all warps have read it.
+template <typename T, int G, int ACCESS, bool BLOCKS>
+__global__ void __launch_bounds__(512) layernorm_ring_kernel(const NormArgs p, int per, int stages, int pitch) {
+  extern __shared__ __align__(16) uint8_t ring_store[];
+  __shared__ __align__(8) uint64_t bars[2 * kMostStages];
+  __shared__ float2 sums[2][16];
+  const int workers = per * p.tpr, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  RowRing ring{umma::smem_u32(ring_store), umma::smem_u32(bars), umma::smem_u32(bars + kMostStages), stages, per, p.residual ? 2 : 1, pitch};
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; s++) {
+      umma::bar_init(ring.full + 8 * s, 1);
+      umma::bar_init(ring.empty + 8 * s, workers >> 5);
+    }
+    umma::bar_init_fence();
+  }
+  after_previous_kernel();
+  __syncthreads();
+  auto bring = [&](int64_t batch, int stage) { bring_rows<T>(ring, p.rows, p.cols, {p.x, p.residual, nullptr}, {p.ldx, p.ldr, 0}, batch, stage); };
+  if (warp == 0)
+    for (int s = 0; s < stages && (blockIdx.x + int64_t(s) * gridDim.x) * per < p.rows; s++) bring(blockIdx.x + int64_t(s) * gridDim.x, s);
+  const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, cols = int(p.cols);
+  const T *x = static_cast<const T*>(p.x), *res = static_cast<const T*>(p.residual);
+  // rows of a thread all start at the same distance from a boundary: gridDim.x * per is a multiple of 8, or each has one
+  const int shift = ACCESS == kShifted ? row_shift(x + (int64_t(blockIdx.x) * per + sub) * p.ldx) : 0;
+  auto at = [&](int g) { return (g * p.tpr + t) * 8 - shift; };
+  PairJoin join{sums, p.tpr, sub, 0};
+  Vec8<T> w[G], b[G];
+#pragma unroll
+  for (int g = 0; g < G; g++) {
+    if (p.weight) load_columns<ACCESS>(w[g], static_cast<const T*>(p.weight), at(g), cols);
+    if (p.bias) load_columns<ACCESS>(b[g], static_cast<const T*>(p.bias), at(g), cols);
+  }
+  int stage = 0;
+  uint32_t parity = 0;
+  bool ok = true;
+  for (int64_t batch = blockIdx.x; batch * per < p.rows; batch += gridDim.x) {
+    const int64_t row = batch * per + sub;
+    if (ok) ok = umma::bar_wait(ring.full + 8 * stage, parity);
+    uint64_t v[G][4];
+    if (row < p.rows) {
+      const uint32_t from = ring.at(stage, 0, sub) + 16 + (ACCESS == kAligned ? 0 : skew_of(x + row * p.ldx));
+      const uint32_t more = res ? ring.at(stage, 1, sub) + 16 + (ACCESS == kAligned ? 0 : skew_of(res + row * p.ldr)) : 0;
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        const int c = at(g);
+        if (c >= cols) continue;
+        Vec8<T> a;
+        take8<ACCESS>(a, from + c * int(sizeof(T)));
+        get_pairs(a, v[g]);
+        if (res) {
+          uint64_t r[4];
+          take8<ACCESS>(a, more + c * int(sizeof(T)));
+          get_pairs(a, r);
+#pragma unroll
+          for (int i = 0; i < 4; i++) v[g][i] = add_pair(v[g][i], r[i]);
+        }
+        mask_pairs<ACCESS>(v[g], c, cols);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) umma::bar_arrive(ring.empty + 8 * stage);
+    if (row < p.rows) {   // the same in all threads of a row
+      float2 st = row_stats<G, ACCESS>(v, p.tpr, t, shift, cols, p.eps, join);
+      if (!ok) st = make_float2(__uint_as_float(0x7fffffffu), __uint_as_float(0x7fffffffu));   // a wait ran out: the outputs say so
+      const int64_t ahead = batch + int64_t(stages) * gridDim.x;
+      if (warp == 0 && ahead * per < p.rows) {
+        if (ok) ok = umma::bar_wait(ring.empty + 8 * stage, parity);
+        if (ok) bring(ahead, stage);
+      }
+      finish_row<T, G, ACCESS, BLOCKS>(p, row, t, shift, v, w, b, st);
+    }
+    if (++stage == stages) { stage = 0; parity ^= 1; }
+  }
+  if (!ok) umma::drain_copies();
 }
 
 // Rows too long for registers: one block per row, which reads it three times
@@ -265,6 +462,43 @@ struct NormBackArgs {
   int tpr;
 };
 
+// The backward's two passes over a group: a = grad * weight and u, and their part
+// in the sums; then grad_x from the row's means.
+template <int ACCESS, typename T>
+__device__ __forceinline__ void back_group(const Vec8<T>& grad, const Vec8<T>& h, const Vec8<T>& w, bool weighted, int c, int cols, uint64_t minus,
+                                           uint64_t rstd, uint64_t (&a)[4], uint64_t (&u)[4], uint64_t (&dw)[4], uint64_t (&db)[4], uint64_t& s,
+                                           uint64_t& su) {
+  uint64_t k[4];
+  get_pairs(grad, a);
+  get_pairs(h, u);
+#pragma unroll
+  for (int i = 0; i < 4; i++) u[i] = mul_pair(add_pair(u[i], minus), rstd);
+  mask_pairs<ACCESS>(a, c, cols);
+  mask_pairs<ACCESS>(u, c, cols);
+  if (weighted) get_pairs(w, k);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    fma_pair(dw[i], a[i], u[i]);
+    db[i] = add_pair(db[i], a[i]);
+    if (weighted) a[i] = mul_pair(a[i], k[i]);
+    s = add_pair(s, a[i]);
+    fma_pair(su, a[i], u[i]);
+  }
+}
+// rstd * (a - mean - u * mean_u) + more
+template <bool MORE, typename T>
+__device__ __forceinline__ void back_out(const uint64_t (&a)[4], const uint64_t (&u)[4], uint64_t minus_mean, uint64_t minus_mean_u, uint64_t rstd,
+                                         const Vec8<T>& more, float (&o)[8]) {
+  uint64_t r[4], k[4];
+  if (MORE) get_pairs(more, k);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    r[i] = add_pair(fma_pair_of(u[i], minus_mean_u, a[i]), minus_mean);
+    r[i] = MORE ? fma_pair_of(r[i], rstd, k[i]) : mul_pair(r[i], rstd);
+  }
+  from_pairs(r, o);
+}
+
 // As layernorm_kernel; a thread also keeps its columns' sums of grad * u and of
 // grad over the slot's rows, joined by column_join_kernel in a fixed order.
 template <typename T, int G, int ACCESS>
@@ -282,7 +516,7 @@ __global__ void __launch_bounds__(512) layernorm_backward_kernel(const NormBackA
   constexpr bool kAhead = G * sizeof(T) <= 4;   // the next row fits the registers
   Vec8<T> ng[G], nh[G], w[G];
   float2 ns;
-  float dw[G][8] = {}, db[G][8] = {};
+  uint64_t dw[G][4] = {}, db[G][4] = {};
   auto load = [&](int64_t r) {
     ns = make_float2(p.mean[r], p.rstd[r]);
 #pragma unroll
@@ -304,58 +538,150 @@ __global__ void __launch_bounds__(512) layernorm_backward_kernel(const NormBackA
 #pragma unroll
       for (int g = 0; g < G; g++) load_at<ACCESS>(ch[g], gh + row * p.ldgh, at(g), cols);
     }
-    float a[G][8], u[G][8];
-    const float2 st = ns;
-    float2 s = make_float2(0.f, 0.f);
+    uint64_t a[G][4], u[G][4], s = 0, su = 0;
+    const uint64_t rstd = pair_of(ns.y), minus = pair_of(-ns.x);
 #pragma unroll
-    for (int g = 0; g < G; g++) {
-      ng[g].get(a[g]);
-      nh[g].get(u[g]);
-      float k[8];
-      if (p.weight) w[g].get(k);
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const bool in = inside<ACCESS>(at(g), e, cols);
-        u[g][e] = in ? (u[g][e] - st.x) * st.y : 0.f;
-        a[g][e] = in ? a[g][e] : 0.f;
-        dw[g][e] = fmaf(a[g][e], u[g][e], dw[g][e]);
-        db[g][e] += a[g][e];
-        if (p.weight) a[g][e] *= k[e];
-        if (ACCESS != kAligned && !in) a[g][e] = 0.f;
-        s.x += a[g][e];
-        s.y = fmaf(a[g][e], u[g][e], s.y);
-      }
-    }
+    for (int g = 0; g < G; g++)
+      if (at(g) < cols) back_group<ACCESS>(ng[g], nh[g], w[g], p.weight != nullptr, at(g), cols, minus, rstd, a[g], u[g], dw[g], db[g], s, su);
     if (kAhead && row + p.slots < p.rows) load(row + p.slots);
     if (!p.grad_x) continue;
-    s = join(s);
-    s.x /= n;
-    s.y /= n;
+    const float2 sums2 = join(make_float2(sum_of(s), sum_of(su)));
+    const uint64_t mean = pair_of(-sums2.x / n), mean_u = pair_of(-sums2.y / n);
     T* out = static_cast<T*>(p.grad_x) + row * p.ldx;
 #pragma unroll
     for (int g = 0; g < G; g++) {
+      if (at(g) >= cols) continue;
       float o[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) o[e] = st.y * (a[g][e] - s.x - u[g][e] * s.y);
-      if (gh) {
-        float k[8];
-        ch[g].get(k);
-#pragma unroll
-        for (int e = 0; e < 8; e++) o[e] += k[e];
-      }
+      if (gh) back_out<true>(a[g], u[g], mean, mean_u, rstd, ch[g], o);
+      else back_out<false>(a[g], u[g], mean, mean_u, rstd, ch[g], o);
       store_at<ACCESS>(out, at(g), cols, o);
     }
   }
 #pragma unroll
   for (int g = 0; g < G; g++) {
     const int c = at(g);
+    float fw[8], fb[8];
+    from_pairs(dw[g], fw);
+    from_pairs(db[g], fb);
 #pragma unroll
     for (int e = 0; e < 8; e++) {
       if (c + e < 0 || c + e >= cols) continue;
-      if (p.partial_w) p.partial_w[slot * p.cols + c + e] = dw[g][e];
-      if (p.partial_b) p.partial_b[slot * p.cols + c + e] = db[g][e];
+      if (p.partial_w) p.partial_w[slot * p.cols + c + e] = fw[e];
+      if (p.partial_b) p.partial_b[slot * p.cols + c + e] = fb[e];
     }
   }
+}
+
+// Many rows: as layernorm_backward_kernel, rows by bulk copies.  The block's
+// sums over its rows are joined across its `per` threads of a column at the end.
+template <typename T, int G, int ACCESS>
+__global__ void __launch_bounds__(512) layernorm_backward_ring_kernel(const NormBackArgs p, int per, int stages, int pitch) {
+  extern __shared__ __align__(16) uint8_t ring_store[];
+  __shared__ __align__(8) uint64_t bars[2 * kMostStages];
+  __shared__ float2 sums[2][16];
+  const int workers = per * p.tpr, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const T *grad = static_cast<const T*>(p.grad), *h = static_cast<const T*>(p.h), *gh = p.grad_x ? static_cast<const T*>(p.grad_h) : nullptr;
+  RowRing ring{umma::smem_u32(ring_store), umma::smem_u32(bars), umma::smem_u32(bars + kMostStages), stages, per, gh ? 3 : 2, pitch};
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; s++) {
+      umma::bar_init(ring.full + 8 * s, 1);
+      umma::bar_init(ring.empty + 8 * s, workers >> 5);
+    }
+    umma::bar_init_fence();
+  }
+  after_previous_kernel();
+  __syncthreads();
+  auto bring = [&](int64_t batch, int stage) { bring_rows<T>(ring, p.rows, p.cols, {grad, h, gh}, {p.ldg, p.ldh, p.ldgh}, batch, stage); };
+  if (warp == 0)
+    for (int s = 0; s < stages && (blockIdx.x + int64_t(s) * gridDim.x) * per < p.rows; s++) bring(blockIdx.x + int64_t(s) * gridDim.x, s);
+  const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, cols = int(p.cols);
+  const int shift = ACCESS == kShifted ? row_shift(grad + (int64_t(blockIdx.x) * per + sub) * p.ldg) : 0;
+  auto at = [&](int g) { return (g * p.tpr + t) * 8 - shift; };
+  PairJoin join{sums, p.tpr, sub, 0};
+  Vec8<T> w[G];
+#pragma unroll
+  for (int g = 0; g < G; g++)
+    if (p.weight) load_columns<ACCESS>(w[g], static_cast<const T*>(p.weight), at(g), cols);
+  uint64_t dw[G][4] = {}, db[G][4] = {};
+  const float n = float(cols);
+  int stage = 0;
+  uint32_t parity = 0;
+  bool ok = true;
+  float2 next = make_float2(0.f, 0.f);
+  if (int64_t(blockIdx.x) * per + sub < p.rows) next = make_float2(p.mean[int64_t(blockIdx.x) * per + sub], p.rstd[int64_t(blockIdx.x) * per + sub]);
+  for (int64_t batch = blockIdx.x; batch * per < p.rows; batch += gridDim.x) {
+    const int64_t row = batch * per + sub, after = row + int64_t(gridDim.x) * per;
+    const uint64_t rstd = pair_of(next.y), minus = pair_of(-next.x);
+    if (after < p.rows) next = make_float2(p.mean[after], p.rstd[after]);
+    if (ok) ok = umma::bar_wait(ring.full + 8 * stage, parity);
+    if (row < p.rows) {   // the same in all threads of a row
+      uint64_t a[G][4], u[G][4], s = 0, su = 0;
+      const uint32_t from = ring.at(stage, 0, sub) + 16 + (ACCESS == kAligned ? 0 : skew_of(grad + row * p.ldg));
+      const uint32_t from_h = ring.at(stage, 1, sub) + 16 + (ACCESS == kAligned ? 0 : skew_of(h + row * p.ldh));
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        const int c = at(g);
+        if (c >= cols) continue;
+        Vec8<T> vg, vh;
+        take8<ACCESS>(vg, from + c * int(sizeof(T)));
+        take8<ACCESS>(vh, from_h + c * int(sizeof(T)));
+        back_group<ACCESS>(vg, vh, w[g], p.weight != nullptr, c, cols, minus, rstd, a[g], u[g], dw[g], db[g], s, su);
+      }
+      if (p.grad_x) {
+        float2 sums2 = join(make_float2(sum_of(s), sum_of(su)));
+        if (!ok) sums2.x = __uint_as_float(0x7fffffffu);   // a wait ran out: the outputs say so
+        const uint64_t mean = pair_of(-sums2.x / n), mean_u = pair_of(-sums2.y / n);
+        const uint32_t more = gh ? ring.at(stage, 2, sub) + 16 + (ACCESS == kAligned ? 0 : skew_of(gh + row * p.ldgh)) : 0;
+        T* out = static_cast<T*>(p.grad_x) + row * p.ldx;
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          const int c = at(g);
+          if (c >= cols) continue;
+          float o[8];
+          Vec8<T> vh;
+          if (gh) {
+            take8<ACCESS>(vh, more + c * int(sizeof(T)));
+            back_out<true>(a[g], u[g], mean, mean_u, rstd, vh, o);
+          } else {
+            back_out<false>(a[g], u[g], mean, mean_u, rstd, vh, o);
+          }
+          store_at<ACCESS>(out, c, cols, o);
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) umma::bar_arrive(ring.empty + 8 * stage);
+    const int64_t ahead = batch + int64_t(stages) * gridDim.x;
+    if (warp == 0 && ahead * per < p.rows) {
+      if (ok) ok = umma::bar_wait(ring.empty + 8 * stage, parity);
+      if (ok) bring(ahead, stage);
+    }
+    if (++stage == stages) { stage = 0; parity ^= 1; }
+  }
+  if (!ok) umma::drain_copies();
+  // all rows have been used: the ring holds the sums of the block's threads of a column
+  float* store = reinterpret_cast<float*>(ring_store);
+  auto join_columns = [&](const uint64_t (&d)[G][4], float* partial) {
+    if (!partial) return;
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      float f[8];
+      from_pairs(d[g], f);
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (inside<kShifted>(at(g), e, cols)) store[sub * cols + at(g) + e] = ok ? f[e] : __uint_as_float(0x7fffffffu);
+    }
+    asm volatile("bar.sync 15, %0;" ::"r"(workers) : "memory");
+    for (int c = threadIdx.x; c < cols; c += workers) {
+      float sum = 0.f;
+      for (int i = 0; i < per; i++) sum += store[i * cols + c];
+      partial[int64_t(blockIdx.x) * p.cols + c] = sum;
+    }
+    asm volatile("bar.sync 15, %0;" ::"r"(workers) : "memory");
+  };
+  if (p.partial_w || p.partial_b) asm volatile("bar.sync 15, %0;" ::"r"(workers) : "memory");
+  join_columns(dw, p.partial_w);
+  join_columns(db, p.partial_b);
 }
 
 // Rows too long for registers, grad_x: one block per row, read twice.
@@ -443,6 +769,30 @@ __global__ void __launch_bounds__(128) layernorm_columns_kernel(const NormBackAr
   }
 }
 
+// out[c] = sum over slots of partial[slot, c], for the weight (blockIdx.y 0) and
+// the bias: 32 columns x 32 slot lanes per block, joined in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(1024) layernorm_join_kernel(int64_t slots, int64_t cols, const float* partial_w, const float* partial_b, T* grad_w, T* grad_b) {
+  __shared__ float part[32][33];
+  after_previous_kernel();
+  const float* partial = blockIdx.y || !grad_w ? partial_b : partial_w;
+  T* out = blockIdx.y || !grad_w ? grad_b : grad_w;
+  const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t c = int64_t(blockIdx.x) * 32 + lane;
+  float s = 0.f;
+  if (c < cols) {
+#pragma unroll 8
+    for (int64_t r = y; r < slots; r += 32) s += partial[r * cols + c];
+  }
+  part[y][lane] = s;
+  __syncthreads();
+  s = part[lane][y];   // warp y joins column y of the strip
+#pragma unroll
+  for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  const int64_t column = int64_t(blockIdx.x) * 32 + y;
+  if (lane == 0 && column < cols) out[column] = from_f32<T>(s);
+}
+
 }  // namespace tgb
 
 namespace tgi {
@@ -454,28 +804,63 @@ namespace {
 
 constexpr int64_t kColumnLimit = 0x7fffff00;
 
-// Threads per row (a power of two) and groups of 8 per thread, at most
-// `most`; `extra` elements may lie before a row's first group.
+// Groups of 8 elements of a row; one more where it may start behind a boundary.
+int64_t groups_of(int64_t cols, int access) { return (cols + (access == tg8::kShifted ? 7 : 0) + 7) / 8; }
+bool in_registers(int64_t cols, int access, int most) { return groups_of(cols, access) <= int64_t(most) * 512; }
+int64_t round32(int64_t v) { return (v + 31) / 32 * 32; }
+
+// Threads per row (a multiple of 32) and groups of 8 elements per thread, for
+// rows loaded directly: one group, for the latency, where 512 threads hold the row.
 struct RowPlan {
   int tpr, groups, block;
   int64_t blocks, slots;
 };
-RowPlan row_plan(int64_t rows, int64_t cols, int access, int most, int per_sm) {
-  const int64_t groups = (cols + (access == tg8::kShifted ? 7 : 0) + 7) / 8;
+RowPlan row_plan(int64_t rows, int64_t cols, int access) {
+  const int64_t groups = groups_of(cols, access);
   RowPlan r;
-  r.groups = rows >= 2 * int64_t(sm_count()) ? most : 1;
+  r.groups = 1;
   while (groups > int64_t(r.groups) * 512) r.groups *= 2;
-  r.tpr = 32;
-  while (int64_t(r.tpr) * r.groups < groups) r.tpr *= 2;
-  while (r.groups > 1 && int64_t(r.tpr) * (r.groups / 2) >= groups) r.groups /= 2;
-  r.block = std::max(r.tpr, 128);
-  const int per = r.block / r.tpr;
-  r.blocks = std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, int64_t(sm_count()) * per_sm * std::max(1, 512 / r.block)));
+  r.tpr = int(round32((groups + r.groups - 1) / r.groups));
+  const int per = std::max(1, 128 / r.tpr);
+  r.block = per * r.tpr;
+  r.blocks = std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, int64_t(sm_count()) * std::max(1, 512 / r.block)));
   r.slots = r.blocks * per;
   if (access == tg8::kShifted && r.slots < rows) {   // a slot's rows start alike
     r.slots = std::max<int64_t>(8, r.slots / 8 * 8);
     r.blocks = (r.slots + per - 1) / per;
   }
+  return r;
+}
+
+// The same for rows by bulk copies: up to `most` groups per thread, `workers`
+// threads per block that work, as many stages as its share of shared memory holds.
+struct RingPlan {
+  int tpr, groups, per, block, stages, pitch;
+  size_t smem;
+  int64_t blocks;
+  bool fits;
+};
+RingPlan ring_plan(int64_t rows, int64_t cols, size_t elem, int ops, int access, int most, int workers, int blocks_per_sm) {
+  RingPlan r{};
+  const int64_t groups = groups_of(cols, access);
+  if (groups > int64_t(most) * 512) return r;
+  r.groups = 1;
+  while (r.groups < most && groups > int64_t(r.groups) * 128) r.groups *= 2;   // up to 128 threads with one group each
+  r.tpr = int(round32((groups + r.groups - 1) / r.groups));
+  if (r.tpr > workers) blocks_per_sm = 1;
+  r.per = std::max(1, workers / r.tpr);
+  r.block = r.per * r.tpr;
+  r.pitch = int((cols * int64_t(elem) + 15) / 16 * 16 + 64);
+  const size_t stage = size_t(ops) * r.per * r.pitch, share = size_t(216 * 1024) / blocks_per_sm;
+  r.stages = int(std::min<size_t>(tgb::kMostStages, share / stage));
+  if (r.stages < 2) return r;
+  r.smem = r.stages * stage;
+  r.blocks = std::min<int64_t>((rows + r.per - 1) / r.per, int64_t(sm_count()) * blocks_per_sm);
+  if (access == tg8::kShifted && r.blocks * r.per < rows) {   // a thread's rows start alike
+    const int64_t unit = 8 / (r.per % 8 == 0 ? 8 : r.per % 4 == 0 ? 4 : r.per % 2 == 0 ? 2 : 1);
+    r.blocks = std::max(unit, r.blocks / unit * unit);
+  }
+  r.fits = true;
   return r;
 }
 template <typename F> void with_groups(int groups, F&& f) {
@@ -491,11 +876,33 @@ template <typename F> void with_mode(int access, F&& f) {
 
 template <typename T, bool BLOCKS> tg_status launch_norm(NormArgs p, int access, cudaStream_t st) {
   constexpr int kMost = sizeof(T) == 4 ? 2 : 4;
-  if (p.cols + 7 > 512 * 8 * kMost) {
+  if (access == tg8::kShifted && !in_registers(p.cols, access, kMost)) access = tg8::kScalar;
+  if (!in_registers(p.cols, access, kMost)) {
     launch_kernel(tgb::layernorm_long_kernel<T, BLOCKS>, unsigned(std::min<int64_t>(p.rows, 0x7fffffff)), 512, 0, 0, st, p);
     return check_launch("layernorm");
   }
-  const RowPlan r = row_plan(p.rows, p.cols, access, kMost, 1);
+  if (p.rows >= 2 * int64_t(sm_count())) {
+    const RingPlan r = ring_plan(p.rows, p.cols, sizeof(T), p.residual ? 2 : 1, access, kMost, 256, 2);
+    if (r.fits) {
+      p.tpr = r.tpr;
+      tg_status sized = TG_OK;
+      with_mode(access, [&](auto mode) {
+        constexpr int A = decltype(mode)::value;
+        if constexpr (!(BLOCKS && A == tg8::kShifted)) {
+          with_groups(r.groups, [&](auto g) {
+            constexpr int G = decltype(g)::value;
+            if constexpr (G <= kMost) {
+              auto kern = tgb::layernorm_ring_kernel<T, G, A, BLOCKS>;
+              sized = ensure_smem(reinterpret_cast<const void*>(kern), 216 * 1024);
+              if (sized == TG_OK) launch_kernel(kern, unsigned(r.blocks), r.block, r.smem, 0, st, p, r.per, r.stages, r.pitch);
+            }
+          });
+        }
+      });
+      return sized == TG_OK ? check_launch("layernorm") : sized;
+    }
+  }
+  const RowPlan r = row_plan(p.rows, p.cols, access);
   p.tpr = r.tpr;
   p.slots = r.slots;
   with_mode(access, [&](auto mode) {
@@ -558,11 +965,14 @@ tg_status norm_forward(tg_dtype dtype, NormArgs p, cudaStream_t st) {
 
 template <typename T> tg_status launch_backward(NormBackArgs p, T* grad_w, T* grad_b, int access, cudaStream_t st) {
   constexpr int kMost = 2;
-  const bool lng = p.cols + 7 > 512 * 8 * kMost;
-  RowPlan r = row_plan(p.rows, std::min<int64_t>(p.cols, 512 * 8), access, kMost, 1);
-  if (!lng) r = row_plan(p.rows, p.cols, access, kMost, 1);
-  p.tpr = r.tpr;
-  p.slots = lng ? std::max<int64_t>(1, std::min<int64_t>(p.rows, 64)) : r.slots;
+  if (access == tg8::kShifted && !in_registers(p.cols, access, kMost)) access = tg8::kScalar;
+  const bool lng = !in_registers(p.cols, access, kMost);
+  RingPlan ring{};
+  if (p.rows >= 2 * int64_t(sm_count())) ring = ring_plan(p.rows, p.cols, sizeof(T), p.grad_h && p.grad_x ? 3 : 2, access, kMost, 512, 1);
+  RowPlan r{};
+  if (lng) p.slots = std::max<int64_t>(1, std::min<int64_t>(p.rows, 64));
+  else if (ring.fits) { p.slots = ring.blocks; p.tpr = ring.tpr; }
+  else { r = row_plan(p.rows, p.cols, access); p.slots = r.slots; p.tpr = r.tpr; }
   void* scratch = nullptr;
   const size_t part = size_t(p.slots) * size_t(p.cols);
   if (grad_w || grad_b) {
@@ -572,20 +982,28 @@ template <typename T> tg_status launch_backward(NormBackArgs p, T* grad_w, T* gr
     if (grad_w) { p.partial_w = at; at += part; }
     if (grad_b) p.partial_b = at;
   }
+  tg_status s = TG_OK;
   if (lng) {
     if (p.grad_x) launch_kernel(tgb::layernorm_backward_long_kernel<T>, unsigned(std::min<int64_t>(p.rows, 0x7fffffff)), 512, 0, 0, st, p);
     if (scratch) launch_kernel(tgb::layernorm_columns_kernel<T>, dim3(unsigned((p.cols + 1023) / 1024), unsigned(p.slots)), 128, 0, 0, st, p);
   } else {
     with_mode(access, [&](auto mode) {
       constexpr int A = decltype(mode)::value;
-      if (r.groups == 1) launch_kernel(tgb::layernorm_backward_kernel<T, 1, A>, unsigned(r.blocks), r.block, 0, 0, st, p);
-      else launch_kernel(tgb::layernorm_backward_kernel<T, 2, A>, unsigned(r.blocks), r.block, 0, 0, st, p);
+      auto go = [&](auto direct, auto by_copies) {
+        if (!ring.fits) {
+          launch_kernel(direct, unsigned(r.blocks), r.block, 0, 0, st, p);
+        } else {
+          s = ensure_smem(reinterpret_cast<const void*>(by_copies), 216 * 1024);
+          if (s == TG_OK) launch_kernel(by_copies, unsigned(ring.blocks), ring.block, ring.smem, 0, st, p, ring.per, ring.stages, ring.pitch);
+        }
+      };
+      if ((ring.fits ? ring.groups : r.groups) == 1) go(tgb::layernorm_backward_kernel<T, 1, A>, tgb::layernorm_backward_ring_kernel<T, 1, A>);
+      else go(tgb::layernorm_backward_kernel<T, 2, A>, tgb::layernorm_backward_ring_kernel<T, 2, A>);
     });
   }
-  const unsigned strips = unsigned((p.cols + 31) / 32);
-  if (grad_w) launch_kernel(tg8::column_join_kernel<T>, strips, 1024, 0, 0, st, p.slots, p.cols, p.partial_w, grad_w);
-  if (grad_b) launch_kernel(tg8::column_join_kernel<T>, strips, 1024, 0, 0, st, p.slots, p.cols, p.partial_b, grad_b);
-  const tg_status s = check_launch("layernorm backward");
+  if (scratch && s == TG_OK)
+    launch_kernel(tgb::layernorm_join_kernel<T>, dim3(unsigned((p.cols + 31) / 32), grad_w && grad_b ? 2 : 1), 1024, 0, 0, st, p.slots, p.cols, p.partial_w, p.partial_b, grad_w, grad_b);
+  if (s == TG_OK) s = check_launch("layernorm backward");
   if (scratch) scratch_free(scratch, st);
   return s;
 }
