@@ -25,33 +25,43 @@ struct NormArgs {
   int tpr;                    // threads per row: 32 .. 512, a power of two
 };
 
-// Two sums over the tpr threads of a row (a multiple of 32): one named barrier
-// per row, two sets of partial results in turn.  The order is the same in every
-// thread.
-struct PairJoin {
+// Sums over the tpr threads of a row (a multiple of 32), one or two at a time:
+// one named barrier per row, two sets of partial results in turn.  The order is
+// the same in every thread.
+struct RowSums {
   float2 (*sums)[16];   // [2][warps of the block]
   int tpr, sub, turn;
-  __device__ __forceinline__ float2 operator()(float2 s) {
+  __device__ __forceinline__ float2 across(float2 s) {
+    if (tpr > 32) {
+      const int warps = tpr >> 5, first = sub * warps;
+      if ((threadIdx.x & 31) == 0) sums[turn][threadIdx.x >> 5] = s;
+      asm volatile("bar.sync %0, %1;" ::"r"(sub + 1), "r"(tpr) : "memory");
+      const float2* from = &sums[turn][first];
+      turn ^= 1;
+      uint64_t all = pair_of(from[0].x, from[0].y);
+      if (warps == 16) {
+#pragma unroll
+        for (int w = 1; w < 16; w++) all = add_pair(all, pair_of(from[w].x, from[w].y));
+      } else {
+#pragma unroll 4
+        for (int w = 1; w < warps; w++) all = add_pair(all, pair_of(from[w].x, from[w].y));
+      }
+      s = values_of(all);
+    }
+    return s;
+  }
+  __device__ __forceinline__ float one(float s) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    return across(make_float2(s, 0.f)).x;
+  }
+  __device__ __forceinline__ float2 two(float2 s) {
 #pragma unroll
     for (int d = 16; d; d >>= 1) {
       s.x += __shfl_xor_sync(0xffffffffu, s.x, d);
       s.y += __shfl_xor_sync(0xffffffffu, s.y, d);
     }
-    if (tpr > 32) {
-      const int lane = threadIdx.x & 31, warps = tpr >> 5, first = sub * warps;
-      if (lane == 0) sums[turn][threadIdx.x >> 5] = s;
-      asm volatile("bar.sync %0, %1;" ::"r"(sub + 1), "r"(tpr) : "memory");
-      s = lane < warps ? sums[turn][first + lane] : make_float2(0.f, 0.f);
-      turn ^= 1;
-#pragma unroll
-      for (int d = 8; d; d >>= 1) {   // at most 16 warps
-        s.x += __shfl_xor_sync(0xffffffffu, s.x, d);
-        s.y += __shfl_xor_sync(0xffffffffu, s.y, d);
-      }
-      s.x = __shfl_sync(0xffffffffu, s.x, 0);
-      s.y = __shfl_sync(0xffffffffu, s.y, 0);
-    }
-    return s;
+    return across(s);
   }
 };
 
@@ -81,25 +91,27 @@ template <int ACCESS, typename T> __device__ __forceinline__ void store_at(T* ro
   if constexpr (ACCESS == kScalar) store_any(row, c, cols, v);
   else store_group<ACCESS>(row, c, cols, v);
 }
-// A group of a vector over the columns (weight, bias), as it lies in memory.
-template <int ACCESS, typename T> __device__ __forceinline__ void load_columns(Vec8<T>& v, const T* from, int c, int cols) {
-  if constexpr (ACCESS == kAligned) {
+// A group of a vector over the columns (weight, bias), as it lies in memory;
+// `otherwise` in all places where there is none.
+template <int ACCESS, typename T> __device__ __forceinline__ void load_columns(Vec8<T>& v, const void* columns, float otherwise, int c, int cols) {
+  const T* from = static_cast<const T*>(columns);
+  if (ACCESS == kAligned && from) {
     load_group<kAligned>(v, from, c, cols);
   } else {
     union { Vec8<T> v; T e[8]; } u;
 #pragma unroll
-    for (int e = 0; e < 8; e++) u.e[e] = inside<ACCESS>(c, e, cols) ? from[c + e] : from_f32<T>(0.f);
+    for (int e = 0; e < 8; e++) u.e[e] = from && inside<ACCESS>(c, e, cols) ? from[c + e] : from_f32<T>(otherwise);
     v = u.v;
   }
 }
 
 // Mean and rstd from the row's mean (the sum's, rounded), the sum of h - mean and
 // of its square: what the rounding of the first mean left is taken out again.
-__device__ __forceinline__ float2 finish_stats(float mean, float2 off, float cols, float eps) {
-  const float d = off.x / cols;
-  float var = off.y / cols - d * d;
+__device__ __forceinline__ float2 finish_stats(float mean, float2 off, float inv_cols, float eps) {
+  const float d = off.x * inv_cols;
+  float var = fmaf(off.y, inv_cols, -d * d);
   if (var < 0.f) var = 0.f;   // a NaN stays
-  return make_float2(mean + d, 1.f / sqrtf(var + eps));
+  return make_float2(mean + d, rsqrtf(var + eps));   // within two units of the last place
 }
 
 // Codes and scale of eight outputs per lane, 16 lanes per block; c < 0 or past
@@ -118,7 +130,7 @@ __device__ __forceinline__ void store_block(const NormArgs& p, int64_t row, int6
 // The two passes over a row that its threads hold: its statistics, and its
 // outputs.  Groups past the row take no part.
 template <int G, int ACCESS>
-__device__ __forceinline__ float2 row_stats(const uint64_t (&v)[G][4], int tpr, int t, int shift, int cols, float eps, PairJoin& join) {
+__device__ __forceinline__ float2 row_stats(const uint64_t (&v)[G][4], int tpr, int t, int shift, int cols, float inv_cols, float eps, RowSums& join) {
   auto at = [&](int g) { return (g * tpr + t) * 8 - shift; };
   uint64_t sum = 0;
 #pragma unroll
@@ -127,7 +139,7 @@ __device__ __forceinline__ float2 row_stats(const uint64_t (&v)[G][4], int tpr, 
 #pragma unroll
     for (int i = 0; i < 4; i++) sum = add_pair(sum, v[g][i]);
   }
-  const float n = float(cols), rough = join(make_float2(sum_of(sum), 0.f)).x / n;
+  const float rough = join.one(sum_of(sum)) * inv_cols;
   const uint64_t minus = pair_of(-rough);
   uint64_t off = 0, square = 0;
 #pragma unroll
@@ -143,7 +155,7 @@ __device__ __forceinline__ float2 row_stats(const uint64_t (&v)[G][4], int tpr, 
       fma_pair(square, d[i], d[i]);
     }
   }
-  return finish_stats(rough, join(make_float2(sum_of(off), sum_of(square))), n, eps);
+  return finish_stats(rough, join.two(make_float2(sum_of(off), sum_of(square))), inv_cols, eps);
 }
 template <typename T, int G, int ACCESS, bool BLOCKS>
 __device__ __forceinline__ void finish_row(const NormArgs& p, int64_t row, int t, int shift, const uint64_t (&v)[G][4], const Vec8<T> (&w)[G],
@@ -156,28 +168,25 @@ __device__ __forceinline__ void finish_row(const NormArgs& p, int64_t row, int t
   const uint64_t minus = pair_of(-st.x), scale = pair_of(st.y);
   T* h = static_cast<T*>(p.h) + row * p.ldh;
   T* out = static_cast<T*>(p.y) + row * p.ldy;
+  if (p.h) {
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      const int c = (g * p.tpr + t) * 8 - shift;
+      float f[8];
+      from_pairs(v[g], f);
+      store_at<ACCESS>(h, c, cols, f);
+    }
+  }
 #pragma unroll
   for (int g = 0; g < G; g++) {
     const int c = (g * p.tpr + t) * 8 - shift;
     if (!BLOCKS && c >= cols) continue;
-    uint64_t y[4], k[4];
+    uint64_t y[4], kw[4], kb[4];
+    get_pairs(w[g], kw);
+    get_pairs(b[g], kb);
 #pragma unroll
-    for (int i = 0; i < 4; i++) y[i] = mul_pair(add_pair(v[g][i], minus), scale);
-    if (p.weight) {
-      get_pairs(w[g], k);
-#pragma unroll
-      for (int i = 0; i < 4; i++) y[i] = mul_pair(y[i], k[i]);
-    }
-    if (p.bias) {
-      get_pairs(b[g], k);
-#pragma unroll
-      for (int i = 0; i < 4; i++) y[i] = add_pair(y[i], k[i]);
-    }
+    for (int i = 0; i < 4; i++) y[i] = fma_pair_of(mul_pair(add_pair(v[g][i], minus), scale), kw[i], kb[i]);
     float f[8];
-    if (p.h) {
-      from_pairs(v[g], f);
-      store_at<ACCESS>(h, c, cols, f);
-    }
     from_pairs(y, f);
     if constexpr (BLOCKS) store_block(p, row, c, f);
     else store_at<ACCESS>(out, c, cols, f);
@@ -200,7 +209,7 @@ __global__ void __launch_bounds__(512) layernorm_kernel(const NormArgs p) {
   const T *x = static_cast<const T*>(p.x), *res = static_cast<const T*>(p.residual);
   const int shift = ACCESS == kShifted ? row_shift(x + row * p.ldx) : 0;
   auto at = [&](int g) { return (g * p.tpr + t) * 8 - shift; };
-  PairJoin join{sums, p.tpr, sub, 0};
+  RowSums join{sums, p.tpr, sub, 0};
   Vec8<T> nx[G], nr[G], w[G], b[G];
   auto load = [&](int64_t r) {
 #pragma unroll
@@ -212,9 +221,10 @@ __global__ void __launch_bounds__(512) layernorm_kernel(const NormArgs p) {
   load(row);
 #pragma unroll
   for (int g = 0; g < G; g++) {
-    if (p.weight) load_columns<ACCESS>(w[g], static_cast<const T*>(p.weight), at(g), cols);
-    if (p.bias) load_columns<ACCESS>(b[g], static_cast<const T*>(p.bias), at(g), cols);
+    load_columns<ACCESS>(w[g], p.weight, 1.f, at(g), cols);
+    load_columns<ACCESS>(b[g], p.bias, 0.f, at(g), cols);
   }
+  const float inv_cols = 1.f / float(cols);
   for (; row < p.rows; row += p.slots) {
     uint64_t v[G][4];
 #pragma unroll
@@ -229,7 +239,7 @@ __global__ void __launch_bounds__(512) layernorm_kernel(const NormArgs p) {
       mask_pairs<ACCESS>(v[g], at(g), cols);
     }
     if (row + p.slots < p.rows) load(row + p.slots);
-    const float2 st = row_stats<G, ACCESS>(v, p.tpr, t, shift, cols, p.eps, join);
+    const float2 st = row_stats<G, ACCESS>(v, p.tpr, t, shift, cols, inv_cols, p.eps, join);
     finish_row<T, G, ACCESS, BLOCKS>(p, row, t, shift, v, w, b, st);
   }
 }
@@ -244,29 +254,36 @@ struct RowRing {
   int stages, per, ops, pitch;
   __device__ __forceinline__ uint32_t at(int stage, int op, int sub) const { return base + uint32_t(((stage * ops + op) * per + sub) * pitch); }
 };
-// One warp starts the copies of a batch's rows into a stage.
-template <typename T>
-__device__ __forceinline__ void bring_rows(const RowRing& r, int64_t rows, int64_t cols, const void* const (&x)[3], const int64_t (&ld)[3], int64_t batch, int stage) {
-  const int lane = threadIdx.x & 31, here = int(min(int64_t(r.per), rows - batch * r.per));
-  uint32_t total = 0;
-  auto each = [&](auto&& f) {
-#pragma unroll
-    for (int op = 0; op < 3; op++)
-      if (op < r.ops)
-        for (int sub = lane; sub < here; sub += 32) {
-          const uintptr_t from = reinterpret_cast<uintptr_t>(static_cast<const T*>(x[op]) + (batch * r.per + sub) * ld[op]);
-          const uintptr_t a = from & ~uintptr_t(15), b = (from + cols * sizeof(T) + 15) & ~uintptr_t(15);
-          f(op, sub, a, uint32_t(b - a));
-        }
-  };
-  each([&](int, int, uintptr_t, uint32_t bytes) { total += bytes; });
-  total = __reduce_add_sync(0xffffffffu, total);
-  if (lane == 0) umma::bar_expect(r.full + 8 * stage, total);
-  __syncwarp();
-  each([&](int op, int sub, uintptr_t a, uint32_t bytes) {
-    umma::bulk_load(r.at(stage, op, sub) + 16, reinterpret_cast<const void*>(a), bytes, r.full + 8 * stage);
-  });
-}
+// One warp starts the copies of a batch's rows into a stage: a lane has one row
+// of one operand (ops * per is at most 32).
+template <int ACCESS, typename T> struct RowCopies {
+  const char* x;   // this lane's operand at row `sub` of batch 0
+  int64_t step;    // bytes from one batch to the next
+  int sub;
+  uint32_t to, bytes;
+  __device__ __forceinline__ RowCopies(const RowRing& r, int64_t cols, const void* const (&rows)[3], const int64_t (&ld)[3]) {
+    const int lane = threadIdx.x & 31, op = lane / r.per;
+    sub = lane - op * r.per;
+    if (op >= r.ops) sub = 1 << 30;
+    const void* from = op == 0 ? rows[0] : op == 1 ? rows[1] : rows[2];
+    const int64_t pitch = (op == 0 ? ld[0] : op == 1 ? ld[1] : ld[2]) * int64_t(sizeof(T));
+    x = static_cast<const char*>(from) + (op < r.ops ? sub * pitch : 0);
+    step = pitch * r.per;
+    bytes = uint32_t(cols * sizeof(T));
+    to = r.at(0, op < r.ops ? op : 0, op < r.ops ? sub : 0) + 16;
+  }
+  __device__ __forceinline__ void operator()(const RowRing& r, int64_t rows, int64_t batch, int stage) const {
+    const int here = int(min(int64_t(r.per), rows - batch * r.per));
+    const uintptr_t from = reinterpret_cast<uintptr_t>(x) + uintptr_t(batch * step), a = from & ~uintptr_t(15);
+    const uint32_t size = ACCESS == kAligned ? bytes : uint32_t(((from + bytes + 15) & ~uintptr_t(15)) - a);
+    const bool mine = sub < here;
+    uint32_t total = uint32_t(r.ops * here) * bytes;
+    if (ACCESS != kAligned) total = __reduce_add_sync(0xffffffffu, mine ? size : 0u);
+    if ((threadIdx.x & 31) == 0) umma::bar_expect(r.full + 8 * stage, total);
+    __syncwarp();
+    if (mine) umma::bulk_load(to + uint32_t(stage * r.ops * r.per * r.pitch), reinterpret_cast<const void*>(a), size, r.full + 8 * stage);
+  }
+};
 __device__ __forceinline__ uint4 load_shared16(uint32_t at) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
@@ -325,7 +342,8 @@ __global__ void __launch_bounds__(512) layernorm_ring_kernel(const NormArgs p, i
   }
   after_previous_kernel();
   __syncthreads();
-  auto bring = [&](int64_t batch, int stage) { bring_rows<T>(ring, p.rows, p.cols, {p.x, p.residual, nullptr}, {p.ldx, p.ldr, 0}, batch, stage); };
+  const RowCopies<ACCESS, T> copies(ring, p.cols, {p.x, p.residual, nullptr}, {p.ldx, p.ldr, 0});
+  auto bring = [&](int64_t batch, int stage) { copies(ring, p.rows, batch, stage); };
   if (warp == 0)
     for (int s = 0; s < stages && (blockIdx.x + int64_t(s) * gridDim.x) * per < p.rows; s++) bring(blockIdx.x + int64_t(s) * gridDim.x, s);
   const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, cols = int(p.cols);
@@ -333,13 +351,14 @@ __global__ void __launch_bounds__(512) layernorm_ring_kernel(const NormArgs p, i
   // rows of a thread all start at the same distance from a boundary: gridDim.x * per is a multiple of 8, or each has one
   const int shift = ACCESS == kShifted ? row_shift(x + (int64_t(blockIdx.x) * per + sub) * p.ldx) : 0;
   auto at = [&](int g) { return (g * p.tpr + t) * 8 - shift; };
-  PairJoin join{sums, p.tpr, sub, 0};
+  RowSums join{sums, p.tpr, sub, 0};
   Vec8<T> w[G], b[G];
 #pragma unroll
   for (int g = 0; g < G; g++) {
-    if (p.weight) load_columns<ACCESS>(w[g], static_cast<const T*>(p.weight), at(g), cols);
-    if (p.bias) load_columns<ACCESS>(b[g], static_cast<const T*>(p.bias), at(g), cols);
+    load_columns<ACCESS>(w[g], p.weight, 1.f, at(g), cols);
+    load_columns<ACCESS>(b[g], p.bias, 0.f, at(g), cols);
   }
+  const float inv_cols = 1.f / float(cols);
   int stage = 0;
   uint32_t parity = 0;
   bool ok = true;
@@ -370,7 +389,7 @@ __global__ void __launch_bounds__(512) layernorm_ring_kernel(const NormArgs p, i
     __syncwarp();
     if (lane == 0) umma::bar_arrive(ring.empty + 8 * stage);
     if (row < p.rows) {   // the same in all threads of a row
-      float2 st = row_stats<G, ACCESS>(v, p.tpr, t, shift, cols, p.eps, join);
+      float2 st = row_stats<G, ACCESS>(v, p.tpr, t, shift, cols, inv_cols, p.eps, join);
       if (!ok) st = make_float2(__uint_as_float(0x7fffffffu), __uint_as_float(0x7fffffffu));   // a wait ran out: the outputs say so
       const int64_t ahead = batch + int64_t(stages) * gridDim.x;
       if (warp == 0 && ahead * per < p.rows) {
@@ -390,8 +409,8 @@ template <typename T, bool BLOCKS>
 __global__ void __launch_bounds__(512) layernorm_long_kernel(const NormArgs p) {
   __shared__ float2 sums[2][16];
   after_previous_kernel();
-  PairJoin join{sums, 512, 0, 0};
-  const float n = float(p.cols);
+  RowSums join{sums, 512, 0, 0};
+  const float inv_cols = 1.f / float(p.cols);
   const int64_t last = (p.cols + 511 * 8 + 7) / (512 * 8);   // turns of the block
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
@@ -416,7 +435,7 @@ __global__ void __launch_bounds__(512) layernorm_long_kernel(const NormArgs p) {
 #pragma unroll
       for (int e = 0; e < 8; e++) sum += c + e < p.cols ? v[e] : 0.f;
     }
-    const float rough = join(make_float2(sum, 0.f)).x / n;
+    const float rough = join.one(sum) * inv_cols;
     float2 off = make_float2(0.f, 0.f);
     for (int64_t i = 0; i < last; i++) {
       const int64_t c = (i * 512 + threadIdx.x) * 8;
@@ -429,7 +448,7 @@ __global__ void __launch_bounds__(512) layernorm_long_kernel(const NormArgs p) {
         off.y = fmaf(d, d, off.y);
       }
     }
-    const float2 st = finish_stats(rough, join(off), n, p.eps);
+    const float2 st = finish_stats(rough, join.two(off), inv_cols, p.eps);
     if (threadIdx.x == 0 && p.mean) {
       p.mean[row] = st.x;
       p.rstd[row] = st.y;
@@ -465,7 +484,7 @@ struct NormBackArgs {
 // The backward's two passes over a group: a = grad * weight and u, and their part
 // in the sums; then grad_x from the row's means.
 template <int ACCESS, typename T>
-__device__ __forceinline__ void back_group(const Vec8<T>& grad, const Vec8<T>& h, const Vec8<T>& w, bool weighted, int c, int cols, uint64_t minus,
+__device__ __forceinline__ void back_group(const Vec8<T>& grad, const Vec8<T>& h, const Vec8<T>& w, int c, int cols, uint64_t minus,
                                            uint64_t rstd, uint64_t (&a)[4], uint64_t (&u)[4], uint64_t (&dw)[4], uint64_t (&db)[4], uint64_t& s,
                                            uint64_t& su) {
   uint64_t k[4];
@@ -475,12 +494,12 @@ __device__ __forceinline__ void back_group(const Vec8<T>& grad, const Vec8<T>& h
   for (int i = 0; i < 4; i++) u[i] = mul_pair(add_pair(u[i], minus), rstd);
   mask_pairs<ACCESS>(a, c, cols);
   mask_pairs<ACCESS>(u, c, cols);
-  if (weighted) get_pairs(w, k);
+  get_pairs(w, k);
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     fma_pair(dw[i], a[i], u[i]);
     db[i] = add_pair(db[i], a[i]);
-    if (weighted) a[i] = mul_pair(a[i], k[i]);
+    a[i] = mul_pair(a[i], k[i]);
     s = add_pair(s, a[i]);
     fma_pair(su, a[i], u[i]);
   }
@@ -512,7 +531,7 @@ __global__ void __launch_bounds__(512) layernorm_backward_kernel(const NormBackA
   const T *grad = static_cast<const T*>(p.grad), *h = static_cast<const T*>(p.h), *gh = static_cast<const T*>(p.grad_h);
   const int shift = ACCESS == kShifted ? row_shift(grad + slot * p.ldg) : 0;
   auto at = [&](int g) { return (g * p.tpr + t) * 8 - shift; };
-  PairJoin join{sums, p.tpr, sub, 0};
+  RowSums join{sums, p.tpr, sub, 0};
   constexpr bool kAhead = G * sizeof(T) <= 4;   // the next row fits the registers
   Vec8<T> ng[G], nh[G], w[G];
   float2 ns;
@@ -529,8 +548,8 @@ __global__ void __launch_bounds__(512) layernorm_backward_kernel(const NormBackA
   if (kAhead && row < p.rows) load(row);
 #pragma unroll
   for (int g = 0; g < G; g++)
-    if (p.weight) load_columns<ACCESS>(w[g], static_cast<const T*>(p.weight), at(g), cols);
-  const float n = float(cols);
+    load_columns<ACCESS>(w[g], p.weight, 1.f, at(g), cols);
+  const float inv_cols = 1.f / float(cols);
   for (; row < p.rows; row += p.slots) {
     if (!kAhead) load(row);
     Vec8<T> ch[G];
@@ -542,11 +561,11 @@ __global__ void __launch_bounds__(512) layernorm_backward_kernel(const NormBackA
     const uint64_t rstd = pair_of(ns.y), minus = pair_of(-ns.x);
 #pragma unroll
     for (int g = 0; g < G; g++)
-      if (at(g) < cols) back_group<ACCESS>(ng[g], nh[g], w[g], p.weight != nullptr, at(g), cols, minus, rstd, a[g], u[g], dw[g], db[g], s, su);
+      if (at(g) < cols) back_group<ACCESS>(ng[g], nh[g], w[g], at(g), cols, minus, rstd, a[g], u[g], dw[g], db[g], s, su);
     if (kAhead && row + p.slots < p.rows) load(row + p.slots);
     if (!p.grad_x) continue;
-    const float2 sums2 = join(make_float2(sum_of(s), sum_of(su)));
-    const uint64_t mean = pair_of(-sums2.x / n), mean_u = pair_of(-sums2.y / n);
+    const float2 sums2 = join.two(make_float2(sum_of(s), sum_of(su)));
+    const uint64_t mean = pair_of(-sums2.x * inv_cols), mean_u = pair_of(-sums2.y * inv_cols);
     T* out = static_cast<T*>(p.grad_x) + row * p.ldx;
 #pragma unroll
     for (int g = 0; g < G; g++) {
@@ -591,19 +610,20 @@ __global__ void __launch_bounds__(512) layernorm_backward_ring_kernel(const Norm
   }
   after_previous_kernel();
   __syncthreads();
-  auto bring = [&](int64_t batch, int stage) { bring_rows<T>(ring, p.rows, p.cols, {grad, h, gh}, {p.ldg, p.ldh, p.ldgh}, batch, stage); };
+  const RowCopies<ACCESS, T> copies(ring, p.cols, {grad, h, gh}, {p.ldg, p.ldh, p.ldgh});
+  auto bring = [&](int64_t batch, int stage) { copies(ring, p.rows, batch, stage); };
   if (warp == 0)
     for (int s = 0; s < stages && (blockIdx.x + int64_t(s) * gridDim.x) * per < p.rows; s++) bring(blockIdx.x + int64_t(s) * gridDim.x, s);
   const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, cols = int(p.cols);
   const int shift = ACCESS == kShifted ? row_shift(grad + (int64_t(blockIdx.x) * per + sub) * p.ldg) : 0;
   auto at = [&](int g) { return (g * p.tpr + t) * 8 - shift; };
-  PairJoin join{sums, p.tpr, sub, 0};
+  RowSums join{sums, p.tpr, sub, 0};
   Vec8<T> w[G];
 #pragma unroll
   for (int g = 0; g < G; g++)
-    if (p.weight) load_columns<ACCESS>(w[g], static_cast<const T*>(p.weight), at(g), cols);
+    load_columns<ACCESS>(w[g], p.weight, 1.f, at(g), cols);
   uint64_t dw[G][4] = {}, db[G][4] = {};
-  const float n = float(cols);
+  const float inv_cols = 1.f / float(cols);
   int stage = 0;
   uint32_t parity = 0;
   bool ok = true;
@@ -625,12 +645,12 @@ __global__ void __launch_bounds__(512) layernorm_backward_ring_kernel(const Norm
         Vec8<T> vg, vh;
         take8<ACCESS>(vg, from + c * int(sizeof(T)));
         take8<ACCESS>(vh, from_h + c * int(sizeof(T)));
-        back_group<ACCESS>(vg, vh, w[g], p.weight != nullptr, c, cols, minus, rstd, a[g], u[g], dw[g], db[g], s, su);
+        back_group<ACCESS>(vg, vh, w[g], c, cols, minus, rstd, a[g], u[g], dw[g], db[g], s, su);
       }
       if (p.grad_x) {
-        float2 sums2 = join(make_float2(sum_of(s), sum_of(su)));
+        float2 sums2 = join.two(make_float2(sum_of(s), sum_of(su)));
         if (!ok) sums2.x = __uint_as_float(0x7fffffffu);   // a wait ran out: the outputs say so
-        const uint64_t mean = pair_of(-sums2.x / n), mean_u = pair_of(-sums2.y / n);
+        const uint64_t mean = pair_of(-sums2.x * inv_cols), mean_u = pair_of(-sums2.y * inv_cols);
         const uint32_t more = gh ? ring.at(stage, 2, sub) + 16 + (ACCESS == kAligned ? 0 : skew_of(gh + row * p.ldgh)) : 0;
         T* out = static_cast<T*>(p.grad_x) + row * p.ldx;
 #pragma unroll
@@ -689,8 +709,8 @@ template <typename T>
 __global__ void __launch_bounds__(512) layernorm_backward_long_kernel(const NormBackArgs p) {
   __shared__ float2 sums[2][16];
   after_previous_kernel();
-  PairJoin join{sums, 512, 0, 0};
-  const float n = float(p.cols);
+  RowSums join{sums, 512, 0, 0};
+  const float inv_cols = 1.f / float(p.cols);
   const T* wgt = static_cast<const T*>(p.weight);
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const float mean = p.mean[row], rstd = p.rstd[row];
@@ -719,9 +739,9 @@ __global__ void __launch_bounds__(512) layernorm_backward_long_kernel(const Norm
         s.y = fmaf(a[e], u[e], s.y);
       }
     }
-    s = join(s);
-    s.x /= n;
-    s.y /= n;
+    s = join.two(s);
+    s.x *= inv_cols;
+    s.y *= inv_cols;
     for (int64_t c = threadIdx.x * 8; c < p.cols; c += 512 * 8) {
       float a[8], u[8];
       load(c, a, u);
@@ -848,7 +868,7 @@ RingPlan ring_plan(int64_t rows, int64_t cols, size_t elem, int ops, int access,
   while (r.groups < most && groups > int64_t(r.groups) * 128) r.groups *= 2;   // up to 128 threads with one group each
   r.tpr = int(round32((groups + r.groups - 1) / r.groups));
   if (r.tpr > workers) blocks_per_sm = 1;
-  r.per = std::max(1, workers / r.tpr);
+  r.per = std::min(std::max(1, workers / r.tpr), 32 / ops);   // a lane of the copying warp for each row
   r.block = r.per * r.tpr;
   r.pitch = int((cols * int64_t(elem) + 15) / 16 * 16 + 64);
   const size_t stage = size_t(ops) * r.per * r.pitch, share = size_t(216 * 1024) / blocks_per_sm;
