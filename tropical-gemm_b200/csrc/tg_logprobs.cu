@@ -5,46 +5,53 @@
 //   logprob = (x_token - m) - log S,  entropy = log S - E / S
 //   grad_v = g_lp ([v == token] - p_v) - g_H p_v (log p_v + entropy)
 //
-// One pass: each thread keeps m, S and E of what it has seen and rescales them
-// when a larger logit comes; each warp keeps its most likely tokens sorted
-// across its lanes.  Bound by memory, one exponential per logit beside it.
+// One pass, in powers of two: with t = (x - m) log2 e, S = sum 2^t, E = sum 2^t t:
+//   logprob = (x_token - m) - log S,  entropy = (log2 S - E / S) log 2
+// Each thread keeps m, S and E of what it has seen and rescales them when a
+// larger logit comes; each warp keeps its most likely tokens sorted across its
+// lanes.
+//
+// Bound by memory: beside a 16-bit logit's two bytes are one exponential (60 us
+// for 4096 x 65536 at 16 per clock and SM, the read 82) and six instructions.
 #include <algorithm>
 #include "tg_blocks8.cuh"
 #include "tg_umma.cuh"
 
 namespace tgb {
 
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kMostTop = 32;   // alternatives: one per lane
 constexpr int kWarps = 16;
+constexpr int kGroups = 4;     // of 8 logits per thread on their way at once
 
-__device__ __forceinline__ float exp2_fast(float x) {
+__device__ __forceinline__ float neg_inf() { return __int_as_float(int(0xff800000)); }
+__device__ __forceinline__ float exp2_fast(float x) {   // within 2^-22 of itself; 0 below 2^-126
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// x - m for the sums: below -1000 the exponential is zero either way, and a
-// product with it must not be 0 * infinity.  Keeps a NaN.
-__device__ __forceinline__ float below(float x, float m) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x - m), "f"(-1000.f));
-  return r;
-}
+// Where 2^t is zero its product with t is too (t may be -infinity).
+__device__ __forceinline__ float least_power(float t) { return fmaxf(t, -200.f); }
 
 struct Sums {
-  float m, s, e;   // largest logit, sum of exp(x - m), sum of exp(x - m) (x - m)
+  float m, s, e;   // largest logit, S, E
 };
-// What a thread with nothing but -infinity so far measures from: any finite value does.
-__device__ __forceinline__ float base_of(float m) { return m == -__int_as_float(0x7f800000) ? 0.f : m; }
+__device__ __forceinline__ Sums nothing() { return {neg_inf(), 0.f, 0.f}; }
+// What is measured from while there is nothing but -infinity: any finite value does.
+__device__ __forceinline__ float base_of(float m) { return m == neg_inf() ? 0.f : m; }
+// The same sums from m on, which is at least a.m.
 __device__ __forceinline__ Sums rebase(const Sums& a, float m) {
   if (a.m == m || a.s == 0.f) return {m, a.s, a.e};
-  const float d = below(a.m, m), f = exp2_fast(d * kLog2e);
-  return {m, a.s * f, (a.e + a.s * d) * f};
+  const float d = (base_of(a.m) - m) * kLog2e, f = exp2_fast(d);
+  return {m, a.s * f, fmaf(a.s, least_power(d), a.e) * f};
 }
 __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
   const float m = fmaxf(a.m, b.m);
   const Sums x = rebase(a, m), y = rebase(b, m);
   return {m, x.s + y.s, x.e + y.e};
+}
+__device__ __forceinline__ Sums from_lane(const Sums& a, int lane) {
+  return {__shfl_xor_sync(0xffffffffu, a.m, lane), __shfl_xor_sync(0xffffffffu, a.s, lane), __shfl_xor_sync(0xffffffffu, a.e, lane)};
 }
 
 // Order of the alternatives as one whole number: larger logits first (one zero,
@@ -84,6 +91,28 @@ struct Best {
   }
 };
 
+// A value's place in the order alone: larger for larger values, one zero, NaN on top.
+__device__ __forceinline__ uint32_t rank_of(float x) { return uint32_t(key_of(x, 0) >> 32); }
+__device__ __forceinline__ float value_of_rank(uint32_t r) { return __uint_as_float(r >> 31 ? r ^ 0x80000000u : ~r); }
+// The largest, or a NaN.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Descending over the lanes.
+__device__ __forceinline__ uint32_t sort_lanes(uint32_t v, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int d = size / 2; d; d >>= 1) {
+      const uint32_t o = __shfl_xor_sync(0xffffffffu, v, d);
+      const bool descending = (lane & size) == 0 || size == 32, low = (lane & d) == 0;
+      v = descending == low ? max(v, o) : min(v, o);
+    }
+  return v;
+}
+
 struct TokenArgs {
   int64_t rows, vocab, ld;
   const void* logits;
@@ -96,72 +125,156 @@ struct TokenArgs {
   int64_t share;    // groups of 8 logits of each
 };
 
+// The lists of `count` warps (or CTAs) to one: four warps take a quarter each, then warp 0 theirs.
+__device__ __forceinline__ void merge_lists(uint64_t (*lists)[kMostTop], int count, Best& best, int warp, int lane) {
+  if (count > 4) {
+    if (warp < 4) {
+      best.key = warp < count ? lists[warp][lane] : 0;
+      for (int i = warp + 4; i < count; i += 4) best.merge(lists[i][lane], lane);
+      lists[warp][lane] = best.key;   // only this warp reads or writes it
+    }
+    __syncthreads();
+  }
+  if (warp == 0) {
+    best.key = lists[0][lane];
+    for (int i = 1; i < min(count, 4); i++) best.merge(lists[i][lane], lane);
+  }
+}
+
 // One row per cluster of `split` CTAs, rows in turn.
+//
+// The alternatives: elements below a bound that k others are known to reach are
+// passed over.  After the first kGroups groups every warp sorts its lanes'
+// largest logits; with W warps the least of their ceil(k / W)-th ones is such a
+// bound (about six of 1024 normal logits reach it for k = 20 and 8 warps), and
+// later the warp's own k-th best.
 template <typename T, int ACCESS, bool TOP>
 __global__ void __launch_bounds__(512) token_logprobs_kernel(const TokenArgs p) {
   __shared__ Sums warp_sums[kWarps];
-  __shared__ Sums cta_sums[8];
+  __shared__ __align__(16) float4 cta_sums[8];   // m, S, E
   __shared__ uint64_t lists[kWarps][kMostTop];
   __shared__ uint64_t cta_lists[8][kMostTop];
+  __shared__ uint32_t bounds[kWarps];
   after_previous_kernel();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int rank = p.split > 1 ? int(umma::cta_rank()) : 0;
   const int64_t clusters = gridDim.x / p.split;
   if (p.split > 1) umma::cluster_arrive();   // all of the cluster has started: waited for before the first store to another CTA
   bool started = false;
+  const uint64_t log2e = pair_of(kLog2e);
   for (int64_t row = blockIdx.x / p.split; row < p.rows; row += clusters) {
     const T* x = static_cast<const T*>(p.logits) + row * p.ld;
     const int shift = ACCESS == kShifted ? row_shift(x) : 0;
-    const int64_t end = min((p.vocab + shift + 7) / 8, (rank + 1) * p.share);
-    Sums own{-__int_as_float(0x7f800000), 0.f, 0.f};
+    const int vocab = int(p.vocab), begin = int(rank * p.share), end = min((vocab - 1 + shift) / 8 + 1, begin + int(p.share));
+    Sums own = nothing();
+    uint64_t s = 0, e2 = 0, minus = 0;   // own.s, own.e and -own.m for pairs
     Best best{0};
-    uint64_t least = 0;   // the top-th best key so far
-    // whole warps go round together
-    for (int64_t g0 = rank * p.share + warp * 32; g0 < end; g0 += warps * 32) {
-      const int64_t g = g0 + lane, c = g * 8 - shift;
-      float v[8];
-      Vec8<T> a;
-      if (g < end) {
-        if constexpr (ACCESS == kScalar) load_any(a, x, c, p.vocab);
-        else load_group<ACCESS>(a, x, int(c), int(p.vocab));
-      } else {
-        a.zero();
-      }
+    uint64_t least = 0;          // the top-th best key so far
+    float bound = neg_inf();     // what is less is passed over
+    bool first = true;
+    auto logits_of = [&](const Vec8<T>& a, int g, float (&v)[8]) {
       a.get(v);
-      float top = -__int_as_float(0x7f800000);
+      if (ACCESS != kAligned) {
+        const int c = g * 8 - shift;
+        if (c < 0 || c > vocab - 8) {   // a row's ends
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        if (g >= end || c + e < 0 || c + e >= p.vocab) v[e] = -__int_as_float(0x7f800000);
-        top = fmaxf(top, v[e]);
-      }
-      if (top > own.m) own = rebase(own, top);
-      const float base = base_of(own.m);
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float d = below(v[e], base), f = exp2_fast(d * kLog2e);
-        own.s += f;
-        own.e = fmaf(f, d, own.e);
-      }
-      if constexpr (TOP) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const bool in = g < end && c + e >= 0 && c + e < p.vocab;
-          const uint64_t k = in ? key_of(v[e], uint32_t(c + e)) : 0;
-          uint32_t more = __ballot_sync(0xffffffffu, k > least);
-          while (more) {
-            const uint64_t next = __shfl_sync(0xffffffffu, k, __ffs(more) - 1);
-            more &= more - 1;
-            if (next <= least) continue;
-            best.insert(next, lane);
-            least = __shfl_sync(0xffffffffu, best.key, p.top - 1);
-          }
+          for (int e = 0; e < 8; e++)
+            if (c + e < 0 || c + e >= vocab) v[e] = neg_inf();
         }
       }
+    };
+    auto take = [&](const Vec8<T>& a, int g) {   // a group's alternatives; whole warps
+      const int c = g * 8 - shift;
+      float v[8];
+      uint32_t mine = 0;   // of this lane's eight
+      if (g < end) {
+        logits_of(a, g, v);
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (!(v[e] < bound) && (ACCESS == kAligned || (c + e >= 0 && c + e < vocab))) mine |= 1u << e;
+      }
+      while (const uint32_t lanes = __ballot_sync(0xffffffffu, mine != 0)) {
+        const int e = __ffs(mine) - 1;
+        float x1 = v[0];
+#pragma unroll
+        for (int i = 1; i < 8; i++)
+          if (e == i) x1 = v[i];
+        const int from = __ffs(lanes) - 1;
+        const uint64_t next = __shfl_sync(0xffffffffu, key_of(x1, uint32_t(c + e)), from);
+        if (lane == from) mine &= mine - 1;
+        if (next <= least) continue;
+        best.insert(next, lane);
+        least = __shfl_sync(0xffffffffu, best.key, p.top - 1);
+        if (least) bound = fmaxf(bound, value_of_rank(uint32_t(least >> 32)));   // a NaN is passed over by its key
+      }
+    };
+    // whole warps (TOP: the block) go round together
+    for (int g0 = begin; g0 < end || (TOP && first); g0 += int(blockDim.x) * kGroups) {
+      Vec8<T> a[kGroups];
+#pragma unroll
+      for (int u = 0; u < kGroups; u++) {
+        const int g = g0 + u * int(blockDim.x) + int(threadIdx.x), c = g * 8 - shift;
+        if (g < end) {
+          if constexpr (ACCESS == kScalar) load_any(a[u], x, c, vocab);
+          else load_group<ACCESS>(a[u], x, c, vocab);
+        }
+      }
+      float tops[kGroups];
+#pragma unroll
+      for (int u = 0; u < kGroups; u++) {
+        const int g = g0 + u * int(blockDim.x) + int(threadIdx.x);
+        tops[u] = neg_inf();
+        if (g >= end) continue;
+        float v[8];
+        logits_of(a[u], g, v);
+        // NaN stays out of m: it is in the sums
+        const float top = TOP ? max_nan(max_nan(v[0], v[1], v[2]), max_nan(v[3], v[4], v[5]), max_nan(v[6], v[7], v[7]))
+                              : fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+        tops[u] = top;
+        if (top > own.m) {
+          own.s = sum_of(s);
+          own.e = sum_of(e2);
+          own = rebase(own, top);
+          s = pair_of(own.s, 0.f);
+          e2 = pair_of(own.e, 0.f);
+          minus = pair_of(-own.m);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float2 t = values_of(mul_pair(add_pair(pair_of(v[2 * i], v[2 * i + 1]), minus), log2e));
+          const uint64_t f = pair_of(exp2_fast(t.x), exp2_fast(t.y));
+          s = add_pair(s, f);
+          fma_pair(e2, f, pair_of(least_power(t.x), least_power(t.y)));
+        }
+      }
+      if constexpr (TOP) {
+        if (first) {
+          // warps that have a logit come before those that have none; a lane that holds a NaN counts for nothing
+          const int working = min(warps, max(0, end - begin + 31) / 32), nth = working > 0 ? (p.top + working - 1) / working : kMostTop + 1;
+          float lane_top = neg_inf();
+#pragma unroll
+          for (int u = 0; u < kGroups; u++) lane_top = fmaxf(lane_top, tops[u]);
+          const uint32_t sorted = sort_lanes(rank_of(lane_top), lane);
+          const uint32_t nth_best = __shfl_sync(0xffffffffu, sorted, min(nth, 32) - 1);
+          if (lane == 0) bounds[warp] = nth_best;
+          __syncthreads();
+          uint32_t b = 0xffffffffu;
+          for (int w = 0; w < working; w++) b = min(b, bounds[w]);
+          if (nth <= 32) bound = value_of_rank(b);
+          first = false;
+        }
+#pragma unroll
+        for (int u = 0; u < kGroups; u++)
+          if (__any_sync(0xffffffffu, g0 + u * int(blockDim.x) + int(threadIdx.x) < end && !(tops[u] < bound)))
+            take(a[u], g0 + u * int(blockDim.x) + int(threadIdx.x));
+      }
     }
+    own.s = sum_of(s);
+    own.e = sum_of(e2);
     // the CTA's sums and list
 #pragma unroll
     for (int d = 16; d; d >>= 1) {
-      const Sums o{__shfl_xor_sync(0xffffffffu, own.m, d), __shfl_xor_sync(0xffffffffu, own.s, d), __shfl_xor_sync(0xffffffffu, own.e, d)};
+      const Sums o = from_lane(own, d);
       own = lane & d ? join(o, own) : join(own, o);
     }
     if (lane == 0) warp_sums[warp] = own;
@@ -169,48 +282,52 @@ __global__ void __launch_bounds__(512) token_logprobs_kernel(const TokenArgs p) 
     __syncthreads();
     if (p.split > 1 && !started) umma::cluster_wait();
     started = true;
+    if (TOP) merge_lists(lists, warps, best, warp, lane);
     if (warp == 0) {
-      own = warp_sums[0];
-      for (int w = 1; w < warps; w++) own = join(own, warp_sums[w]);
-      if (TOP)
-        for (int w = 1; w < warps; w++) best.merge(lists[w][lane], lane);
+      own = lane < warps ? warp_sums[lane] : nothing();
+#pragma unroll
+      for (int d = 8; d; d >>= 1) {
+        const Sums o = from_lane(own, d);
+        own = lane & d ? join(o, own) : join(own, o);
+      }
       if (p.split > 1) {
         const uint32_t to = umma::map_rank(umma::smem_u32(&cta_sums[rank]), 0);
-        if (lane == 0) {
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(own.m) : "memory");
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(own.s) : "memory");
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(own.e) : "memory");
-        }
+        if (lane == 0) umma::store_cluster(to, __float_as_uint(own.m), __float_as_uint(own.s), __float_as_uint(own.e), 0u);
         if (TOP)
           asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(umma::map_rank(umma::smem_u32(&cta_lists[rank][lane]), 0)), "l"(best.key) : "memory");
       }
     }
     if (p.split > 1) umma::cluster_sync();
+    if (p.split > 1 && rank == 0 && TOP) merge_lists(cta_lists, p.split, best, warp, lane);
     if (warp == 0 && rank == 0) {
       if (p.split > 1) {
-        own = cta_sums[0];
-        for (int r = 1; r < p.split; r++) own = join(own, cta_sums[r]);
-        if (TOP)
-          for (int r = 1; r < p.split; r++) best.merge(cta_lists[r][lane], lane);
+        own = lane < p.split ? Sums{cta_sums[lane].x, cta_sums[lane].y, cta_sums[lane].z} : nothing();
+#pragma unroll
+        for (int d = 4; d; d >>= 1) {
+          const Sums o = from_lane(own, d);
+          own = lane & d ? join(o, own) : join(own, o);
+        }
       }
-      const bool empty = own.m == -__int_as_float(0x7f800000) && own.s == 0.f;
+      own = {__shfl_sync(0xffffffffu, own.m, 0), __shfl_sync(0xffffffffu, own.s, 0), __shfl_sync(0xffffffffu, own.e, 0)};
+      const bool empty = own.m == neg_inf() && own.s == 0.f;
       const float logs = logf(own.s);
+      auto logp = [&](float v) { return empty ? neg_inf() : (v - own.m) - logs; };
       if (lane == 0) {
         if (p.logprob) {
           const int64_t token = p.tokens[row];
           float lp = __int_as_float(0x7fffffff);
           if (token == p.ignore) lp = 0.f;
-          else if (token >= 0 && token < p.vocab) lp = empty ? -__int_as_float(0x7f800000) : (to_f32(x[token]) - own.m) - logs;
+          else if (token >= 0 && token < p.vocab) lp = logp(to_f32(x[token]));
           p.logprob[row] = lp;
         }
-        if (p.entropy) p.entropy[row] = empty ? 0.f : logs - own.e / own.s;
+        if (p.entropy) p.entropy[row] = empty ? 0.f : logs - own.e / own.s * kLn2;
         if (p.stats) {
           p.stats[2 * row] = own.m;
-          p.stats[2 * row + 1] = logs;
+          p.stats[2 * row + 1] = logs;   // -infinity of an empty row
         }
       }
       if (TOP && lane < p.top) {
-        p.top_logprobs[row * p.top + lane] = empty ? -__int_as_float(0x7f800000) : (logit_of(best.key) - own.m) - logs;
+        p.top_logprobs[row * p.top + lane] = logp(logit_of(best.key));
         p.top_tokens[row * p.top + lane] = token_of(best.key);
       }
     }
@@ -228,36 +345,61 @@ struct TokenBackArgs {
   void* grad;
 };
 
+// Parts of kPart groups of a row, kGroups of 8 logits per thread at a time.
+constexpr int64_t kPart = 256 * kGroups * 2;
 template <typename T, int ACCESS>
-__global__ void __launch_bounds__(256) token_logprobs_backward_kernel(const TokenBackArgs p) {
+__global__ void __launch_bounds__(256) token_logprobs_backward_kernel(const TokenBackArgs p, int64_t parts) {
   after_previous_kernel();
-  for (int64_t row = blockIdx.y; row < p.rows; row += gridDim.y) {
+  const uint64_t log2e = pair_of(kLog2e);
+  for (int64_t item = blockIdx.x; item < p.rows * parts; item += gridDim.x) {
+    const int64_t row = item / parts, from = (item - row * parts) * kPart;
     const T* x = static_cast<const T*>(p.logits) + row * p.ld;
     T* out = static_cast<T*>(p.grad) + row * p.ldg;
     const int shift = ACCESS == kShifted ? row_shift(x) : 0;
+    const int64_t end = min((p.vocab + shift + 7) / 8, from + kPart);
     const float m = p.stats[2 * row], logs = p.stats[2 * row + 1];
-    const bool empty = m == -__int_as_float(0x7f800000) && logs == m;
+    const bool empty = m == neg_inf() && logs == m;
     const int64_t token = p.grad_logprob ? p.tokens[row] : p.ignore;
     float g = token != p.ignore ? p.grad_logprob[row] : 0.f;
     if (token != p.ignore && (token < 0 || token >= p.vocab)) g = __int_as_float(0x7fffffff);
     const float gh = p.grad_entropy ? p.grad_entropy[row] : 0.f, h = p.grad_entropy ? p.entropy[row] : 0.f;
-    const int64_t groups = (p.vocab + shift + 7) / 8;
-    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < groups; i += int64_t(gridDim.x) * 256) {
-      const int64_t c = i * 8 - shift;
-      Vec8<T> a;
-      float v[8];
-      if constexpr (ACCESS == kScalar) load_any(a, x, c, p.vocab);
-      else load_group<ACCESS>(a, x, int(c), int(p.vocab));
-      a.get(v);
+    const uint64_t minus_m = pair_of(-m), minus_s = pair_of(-logs);
+    const uint64_t slope = pair_of(-gh * kLn2), offset = pair_of(-fmaf(gh, h, g));
+    for (int64_t i = from + threadIdx.x; i < end; i += 256 * kGroups) {
+      Vec8<T> a[kGroups];
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float logp = below(v[e], m) - logs, prob = exp2_fast(logp * kLog2e);
-        float d = -prob * fmaf(gh, logp + h, g);
-        if (c + e == token) d += g;
-        v[e] = empty ? 0.f : d;
+      for (int u = 0; u < kGroups; u++) {
+        const int64_t c = (i + u * 256) * 8 - shift;
+        if (i + u * 256 < end) {
+          if constexpr (ACCESS == kScalar) load_any(a[u], x, c, p.vocab);
+          else load_group<ACCESS>(a[u], x, int(c), int(p.vocab));
+        }
       }
-      if constexpr (ACCESS == kScalar) store_any(out, c, p.vocab, v);
-      else store_group<ACCESS>(out, int(c), int(p.vocab), v);
+#pragma unroll
+      for (int u = 0; u < kGroups; u++) {
+        const int64_t c = (i + u * 256) * 8 - shift;
+        if (i + u * 256 >= end) continue;
+        uint64_t v[4];
+        float o[8];
+        get_pairs(a[u], v);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float2 t = values_of(mul_pair(add_pair(add_pair(v[j], minus_m), minus_s), log2e));   // log2 p
+          v[j] = mul_pair(pair_of(exp2_fast(t.x), exp2_fast(t.y)), fma_pair_of(pair_of(least_power(t.x), least_power(t.y)), slope, offset));
+        }
+        from_pairs(v, o);
+        if (token >= c && token < c + 8) {
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+            if (c + e == token) o[e] += g;
+        }
+        if (empty) {
+#pragma unroll
+          for (int e = 0; e < 8; e++) o[e] = 0.f;
+        }
+        if constexpr (ACCESS == kScalar) store_any(out, c, p.vocab, o);
+        else store_group<ACCESS>(out, int(c), int(p.vocab), o);
+      }
     }
   }
 }
@@ -266,6 +408,7 @@ __global__ void __launch_bounds__(256) token_logprobs_backward_kernel(const Toke
 
 namespace tgi {
 
+using tgb::kGroups;
 using tgb::TokenArgs;
 using tgb::TokenBackArgs;
 
@@ -315,11 +458,15 @@ tg_status tg_token_logprobs(tg_dtype dtype, int64_t rows, int64_t vocab, const v
   RowAccess access(vocab);
   access.add(logits, ld, elem8_size(dtype));
   const int64_t groups = (vocab + 7 + 7) / 8;
+  // Few rows: several CTAs share one, each with at least one round of its threads.
   p.split = 1;
-  while (p.split < 8 && rows * p.split * 2 <= 2 * int64_t(sm_count()) && groups >= 512 * 2 * p.split) p.split *= 2;
+  while (p.split < 8 && rows * p.split * 2 <= sm_count() && groups >= 512 * kGroups * p.split) p.split *= 2;
   p.share = (groups + p.split - 1) / p.split;
-  const int64_t clusters = std::min<int64_t>(rows, std::max<int64_t>(1, 4 * int64_t(sm_count()) / p.split));
-  const int threads = int(std::max<int64_t>(32, std::min<int64_t>(512, (p.share + 31) / 32 * 32)));
+  // Threads for one round of kGroups groups each.  Many rows: at most 256, so that fewer warps have a list and more rows
+  // are on an SM at once.
+  const int64_t most = rows * p.split >= 2 * int64_t(sm_count()) ? 256 : 512;
+  const int threads = int(std::max<int64_t>(32, std::min<int64_t>(most, (p.share + 32 * kGroups - 1) / (32 * kGroups) * 32)));
+  const int64_t clusters = std::min<int64_t>(rows, std::max<int64_t>(1, int64_t(sm_count()) * std::min(8, 2048 / threads) / p.split));
   return with_type8(dtype, [&](auto t) {
     using T = decltype(t);
     with_mode(access.get(), [&](auto mode) {
@@ -349,12 +496,12 @@ tg_status tg_token_logprobs_backward(tg_dtype dtype, int64_t rows, int64_t vocab
   RowAccess access(vocab);
   access.add(logits, ld, e);
   access.add(grad_logits, ldg, e);
-  const unsigned across = unsigned(std::min<int64_t>((vocab + 7 + 2047) / 2048, 64));
+  const int64_t parts = (vocab + 7 + 7) / 8 / tgb::kPart + 1;
+  const unsigned grid = unsigned(std::min<int64_t>(rows * parts, int64_t(sm_count()) * 8));
   return with_type8(dtype, [&](auto t) {
     using T = decltype(t);
     with_mode(access.get(), [&](auto mode) {
-      launch_kernel(tgb::token_logprobs_backward_kernel<T, decltype(mode)::value>, dim3(across, unsigned(std::min<int64_t>(rows, 65535))), 256, 0, 0,
-                    static_cast<cudaStream_t>(stream), p);
+      launch_kernel(tgb::token_logprobs_backward_kernel<T, decltype(mode)::value>, grid, 256, 0, 0, static_cast<cudaStream_t>(stream), p, parts);
     });
     return check_launch("token logprobs backward");
   });
