@@ -331,11 +331,12 @@ tg_status tg_layernorm_backward(tg_dtype dtype, int64_t rows, int64_t cols,
 /* q, scale = x with a scale per row and block of 128 columns.  qt (cols x
  * rows, or null): x transposed, with blocks of 128 along ITS rows; its element
  * (c, r) has the scale scale_t[c * scale_t_row + (r / 128) * scale_t_block].
- * q may be null when qt is not. */
+ * column_sum (cols, or null): the sums of x's columns, f32 sums in a fixed
+ * order, of type dtype.  One of q, qt and column_sum is there, all from one read. */
 tg_status tg_blocks8_quantize(tg_dtype dtype, int64_t rows, int64_t cols, const void* x, int64_t ldx,
                               void* q, int64_t ldq, float* scale, int64_t scale_row, int64_t scale_block,
                               void* qt, int64_t ldqt, float* scale_t, int64_t scale_t_row, int64_t scale_t_block,
-                              void* stream);
+                              void* column_sum, void* stream);
 
 /* q, scale = x with a scale per tile of 128 x 128.  qt (cols x rows, or null)
  * gets the same codes transposed, whose scales are scale transposed. */

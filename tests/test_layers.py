@@ -49,7 +49,7 @@ def test_wrong_types_and_shapes_are_value_errors(call):
 
 NORM = (BF16, 2, 8, P, 8, None, 0, P, P, 1e-5, None, 8, P, 8, None, None, None)
 NORM_BACK = (F16, 2, 8, P, 8, None, 0, P, P, 8, P, P, P, 8, P, P, None)
-QUANT = (F32, 2, 8, P, 8, P, 8, P, 1, 2, None, 0, None, 0, 0, None)
+QUANT = (F32, 2, 8, P, 8, P, 8, P, 1, 2, None, 0, None, 0, 0, None, None)
 TILES = (F32, 2, 8, P, 8, P, 8, P, 1, 1, None, 0, None)
 VALUES = (F32, 2, 8, 1, P, 8, P, 1, 1, P, 8, None)
 NORM8 = (BF16, 2, 8, P, 8, None, 0, P, P, 1e-5, None, 8, P, 8, P, 1, 2, None, None, None)

@@ -21,7 +21,7 @@ namespace tgb {
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kMostTop = 32;   // alternatives: one per lane
-constexpr int kWarps = 16;
+constexpr int kManyRows = 128, kFewRows = 512;   // threads per row and CTA
 constexpr int kGroups = 4;     // of 8 logits per thread on their way at once
 
 __device__ __forceinline__ float neg_inf() { return __int_as_float(int(0xff800000)); }
@@ -143,18 +143,24 @@ __device__ __forceinline__ void merge_lists(uint64_t (*lists)[kMostTop], int cou
 
 // One row per cluster of `split` CTAs, rows in turn.
 //
-// The alternatives: elements below a bound that k others are known to reach are
-// passed over.  After the first kGroups groups every warp sorts its lanes'
-// largest logits; with W warps the least of their ceil(k / W)-th ones is such a
-// bound (about six of 1024 normal logits reach it for k = 20 and 8 warps), and
-// later the warp's own k-th best.
-template <typename T, int ACCESS, bool TOP>
-__global__ void __launch_bounds__(512) token_logprobs_kernel(const TokenArgs p) {
+// The alternatives: logits below a bound that k of them are known to reach are
+// passed over.  It comes from the largest logits of the first batch's lanes, and
+// from the lists after one, two, four .. batches (of 8 warps' 1024 normal logits
+// each about three reach it in the second batch, for k = 20), and from the
+// warp's own k-th best.
+//
+// Many rows take 128 threads each (4096 x 65536 bf16, us without / with 20
+// alternatives: 512 threads 179 / 446, 256 144 / 266, 128 131 / 235, 64 125 / 236): fewer
+// lists to fill, more rows on an SM.  Few rows take 512, and several CTAs each (one
+// of 131072, 20 alternatives: 512 threads 11.5, 128 17.5).
+template <typename T, int ACCESS, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS, (TOP ? 768 : 1024) / THREADS) token_logprobs_kernel(const TokenArgs p) {
+  constexpr int kWarps = THREADS / 32;
   __shared__ Sums warp_sums[kWarps];
   __shared__ __align__(16) float4 cta_sums[8];   // m, S, E
   __shared__ uint64_t lists[kWarps][kMostTop];
   __shared__ uint64_t cta_lists[8][kMostTop];
-  __shared__ uint32_t bounds[kWarps];
+  __shared__ uint32_t bounds[2][32];
   after_previous_kernel();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int rank = p.split > 1 ? int(umma::cta_rank()) : 0;
@@ -171,7 +177,6 @@ __global__ void __launch_bounds__(512) token_logprobs_kernel(const TokenArgs p) 
     Best best{0};
     uint64_t least = 0;          // the top-th best key so far
     float bound = neg_inf();     // what is less is passed over
-    bool first = true;
     auto logits_of = [&](const Vec8<T>& a, int g, float (&v)[8]) {
       a.get(v);
       if (ACCESS != kAligned) {
@@ -208,8 +213,21 @@ __global__ void __launch_bounds__(512) token_logprobs_kernel(const TokenArgs p) 
         if (least) bound = fmaxf(bound, value_of_rank(uint32_t(least >> 32)));   // a NaN is passed over by its key
       }
     };
+    // A bound from what the block has seen: each warp gives its 32 / W best, `mine`
+    // being ranks in descending order over the lanes; k of them reach the k-th.
+    int bounded = 0;
+    auto tighten = [&](uint32_t mine) {
+      const int per = 32 / warps, set = bounded & 1;
+      if (lane < per) bounds[set][warp * per + lane] = mine;
+      __syncthreads();
+      const uint32_t sorted = sort_lanes(lane < per * warps ? bounds[set][lane] : 0u, lane);
+      const uint32_t kth = __shfl_sync(0xffffffffu, sorted, p.top - 1);
+      if (kth) bound = fmaxf(bound, value_of_rank(kth));
+      bounded++;
+    };
+    int batch = 0;
     // whole warps (TOP: the block) go round together
-    for (int g0 = begin; g0 < end || (TOP && first); g0 += int(blockDim.x) * kGroups) {
+    for (int g0 = begin; g0 < end || (TOP && batch == 0); g0 += int(blockDim.x) * kGroups, batch++) {
       Vec8<T> a[kGroups];
 #pragma unroll
       for (int u = 0; u < kGroups; u++) {
@@ -248,20 +266,13 @@ __global__ void __launch_bounds__(512) token_logprobs_kernel(const TokenArgs p) 
         }
       }
       if constexpr (TOP) {
-        if (first) {
-          // warps that have a logit come before those that have none; a lane that holds a NaN counts for nothing
-          const int working = min(warps, max(0, end - begin + 31) / 32), nth = working > 0 ? (p.top + working - 1) / working : kMostTop + 1;
+        if (batch == 0) {   // no lists yet: the lanes' largest logits; a lane that holds a NaN counts for nothing
           float lane_top = neg_inf();
 #pragma unroll
           for (int u = 0; u < kGroups; u++) lane_top = fmaxf(lane_top, tops[u]);
-          const uint32_t sorted = sort_lanes(rank_of(lane_top), lane);
-          const uint32_t nth_best = __shfl_sync(0xffffffffu, sorted, min(nth, 32) - 1);
-          if (lane == 0) bounds[warp] = nth_best;
-          __syncthreads();
-          uint32_t b = 0xffffffffu;
-          for (int w = 0; w < working; w++) b = min(b, bounds[w]);
-          if (nth <= 32) bound = value_of_rank(b);
-          first = false;
+          tighten(sort_lanes(lane_top == neg_inf() ? 0u : rank_of(lane_top), lane));
+        } else if ((batch & (batch - 1)) == 0) {
+          tighten(uint32_t(best.key >> 32));
         }
 #pragma unroll
         for (int u = 0; u < kGroups; u++)
@@ -409,6 +420,8 @@ __global__ void __launch_bounds__(256) token_logprobs_backward_kernel(const Toke
 namespace tgi {
 
 using tgb::kGroups;
+using tgb::kFewRows;
+using tgb::kManyRows;
 using tgb::TokenArgs;
 using tgb::TokenBackArgs;
 
@@ -460,21 +473,23 @@ tg_status tg_token_logprobs(tg_dtype dtype, int64_t rows, int64_t vocab, const v
   const int64_t groups = (vocab + 7 + 7) / 8;
   // Few rows: several CTAs share one, each with at least one round of its threads.
   p.split = 1;
-  while (p.split < 8 && rows * p.split * 2 <= sm_count() && groups >= 512 * kGroups * p.split) p.split *= 2;
+  while (p.split < 8 && rows * p.split * 2 <= sm_count() && groups >= kFewRows * kGroups * p.split) p.split *= 2;
   p.share = (groups + p.split - 1) / p.split;
-  // Threads for one round of kGroups groups each.  Many rows: at most 256, so that fewer warps have a list and more rows
-  // are on an SM at once.
-  const int64_t most = rows * p.split >= 2 * int64_t(sm_count()) ? 256 : 512;
-  const int threads = int(std::max<int64_t>(32, std::min<int64_t>(most, (p.share + 32 * kGroups - 1) / (32 * kGroups) * 32)));
-  const int64_t clusters = std::min<int64_t>(rows, std::max<int64_t>(1, int64_t(sm_count()) * std::min(8, 2048 / threads) / p.split));
+  const bool many = rows * p.split >= 3 * int64_t(sm_count());
+  // threads for one round of kGroups groups each
+  const int threads = int(std::max<int64_t>(32, std::min<int64_t>(many ? kManyRows : kFewRows, (p.share + 32 * kGroups - 1) / (32 * kGroups) * 32)));
+  const int64_t clusters = std::min<int64_t>(rows, int64_t(1) << 16);   // rows beyond that in turn
   return with_type8(dtype, [&](auto t) {
     using T = decltype(t);
     with_mode(access.get(), [&](auto mode) {
       constexpr int A = decltype(mode)::value;
       const dim3 grid(unsigned(clusters * p.split));
       const int cluster = p.split > 1 ? p.split : 0;
-      if (top) launch_kernel(tgb::token_logprobs_kernel<T, A, true>, grid, threads, 0, cluster, static_cast<cudaStream_t>(stream), p);
-      else launch_kernel(tgb::token_logprobs_kernel<T, A, false>, grid, threads, 0, cluster, static_cast<cudaStream_t>(stream), p);
+      auto go = [&](auto kern) { launch_kernel(kern, grid, threads, 0, cluster, static_cast<cudaStream_t>(stream), p); };
+      if (many && top) go(tgb::token_logprobs_kernel<T, A, true, kManyRows>);
+      else if (many) go(tgb::token_logprobs_kernel<T, A, false, kManyRows>);
+      else if (top) go(tgb::token_logprobs_kernel<T, A, true, kFewRows>);
+      else go(tgb::token_logprobs_kernel<T, A, false, kFewRows>);
     });
     return check_launch("token logprobs");
   });

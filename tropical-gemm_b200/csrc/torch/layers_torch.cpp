@@ -70,8 +70,8 @@ int check_blocks8(const Tensor& q, const Tensor& s, const char* what) {
   refuse(what, " needs one scale per row and block of 128 columns, or (two-dimensional) per tile of 128 x 128: q is ", shape(q.sizes()), ", scale is ", shape(s.sizes()));
 }
 
-// x along its rows, and with `turned` along its columns too (as rows of x^T; leading dimensions make one).
-void quantize_into(const Tensor& x, Blocks* rows, Blocks* turned) {
+// x along its rows, with `turned` along its columns (as rows of x^T; leading dimensions make one), and its columns' sums.
+void quantize_into(const Tensor& x, Blocks* rows, Blocks* turned, Tensor* sum = nullptr) {
   const tg_dtype code = type(x.scalar_type(), "x");
   on(x.device());
   if (x.dim() == 0) refuse("expected a tensor with at least one dimension");
@@ -91,7 +91,8 @@ void quantize_into(const Tensor& x, Blocks* rows, Blocks* turned) {
     turned->scale = make_scales({k, m}, x);
     qt = ptr(turned->q); st = f32(turned->scale); ldqt = pitch(turned->q);
   }
-  check(tg_blocks8_quantize(code, m, k, f.ptr(), f.ld, q, ldq, s, 1, m, qt, ldqt, st, 1, k, stream(x.device())));
+  if (sum) *sum = make({k}, x, x.scalar_type());
+  check(tg_blocks8_quantize(code, m, k, f.ptr(), f.ld, q, ldq, s, 1, m, qt, ldqt, st, 1, k, sum ? ptr(*sum) : nullptr, stream(x.device())));
 }
 
 std::tuple<Tensor, Tensor> quantize(const Tensor& x) {
@@ -167,14 +168,6 @@ Tensor matmul(const Tensor& aq, const Tensor& a_scale, const Tensor& bq, const T
   check(tg_blocks8_gemm(type(t, "dtype"), rows_of(aq), n, k, a.ptr(), a.ld, as.ptr(), as.row(), as.block(), b.ptr(), b.ld, tall,
                         bs.ptr(), bs.row(), bs.block(), ptr(bi), ptr(c), n, stream(dev)));
   return c;
-}
-
-Tensor column_sum(const Tensor& x, at::ScalarType t) {
-  const Flat f(x);
-  Tensor out = make({x.size(-1)}, x, t);
-  c10::cuda::CUDAGuard guard(x.device());
-  check(tg_rows8_column_sum(type(x.scalar_type(), "x"), type(t, "dtype"), rows_of(x), x.size(-1), f.ptr(), f.ld, ptr(out), stream(x.device())));
-  return out;
 }
 
 // ------------------------------------------------------------------------------------------------ layer norm
@@ -322,10 +315,9 @@ struct Linear : torch::autograd::Function<Linear> {
     Tensor grad_x, grad_w, grad_b;
     if (g.defined()) {
       Blocks rows, turned;
-      if (needs[0] || needs[1]) quantize_into(g, needs[0] ? &rows : nullptr, needs[1] ? &turned : nullptr);
+      quantize_into(g, needs[0] ? &rows : nullptr, needs[1] ? &turned : nullptr, needs[2] ? &grad_b : nullptr);
       if (needs[0]) grad_x = matmul(rows.q, rows.scale, saved[2], saved[3].t(), std::nullopt, g.scalar_type());
       if (needs[1]) grad_w = matmul(turned.q, turned.scale, saved[0], saved[1], std::nullopt, g.scalar_type());
-      if (needs[2]) grad_b = column_sum(g, g.scalar_type());
     }
     const Tensor none;
     return {grad_x, grad_w, none, grad_b, none};
