@@ -3,6 +3,8 @@
 // torch's current stream, autograd.  The work is the C ABI's
 // (include/tropical_gemm_b200.h).
 #include "binding.h"
+#include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <torch/csrc/autograd/variable.h>
 
 namespace {
 
@@ -252,6 +254,22 @@ bool any_wants(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 
+// A backward that is captured into a graph adds to its leaves on the stream of
+// the autograd graph that met them first.  Where an eager one is still alive
+// that is a stream outside of the capture, which breaks it off: said here,
+// while the forward is captured and nothing has gone wrong yet.
+void check_capture(std::initializer_list<const Tensor*> inputs) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  for (const Tensor* t : inputs) {
+    if (!wants(*t) || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (!node || !node->stream()) continue;
+    if (*node->stream() != at::cuda::getCurrentCUDAStream(t->device().index()).unwrap())
+      throw std::runtime_error("a leaf of this captured call belongs to an autograd graph that is alive on another stream: "
+                               "release what holds that graph (losses, outputs) before the capture");
+  }
+}
+
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias,
                                                 const OptTensor& residual, double eps, bool train) {
@@ -279,6 +297,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 };
 std::tuple<Tensor, Tensor> layernorm_grad(const Tensor& x, const OptTensor& weight, const OptTensor& bias, const OptTensor& residual, double eps) {
   const bool train = any_wants({&x, &or_none(weight), &or_none(bias), &or_none(residual)});
+  if (train) check_capture({&x, &or_none(weight), &or_none(bias), &or_none(residual)});
   auto out = LayerNorm::apply(x, weight, bias, residual, eps, train);
   return {out[0], out[1]};
 }
@@ -333,6 +352,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& weight_sca
   if (weight_scale && check_blocks8(weight, *weight_scale, "weight") != 128 && train && wants(x) && weight.size(0) > 1)
     refuse("a weight whose scales are per row has no gradient for x in 8-bit blocks: use tiles of 128 x 128");
   on(x.device(), {&weight, &or_none(weight_scale), &or_none(bias)});
+  if (train) check_capture({&x, &weight, &or_none(bias)});
   // frozen blocks are constants, their scales included
   const OptTensor frozen = weight_scale && weight_scale->requires_grad() ? OptTensor(weight_scale->detach()) : weight_scale;
   return Linear::apply(x, weight, frozen, bias, train)[0];
@@ -420,7 +440,9 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   }
 };
 std::tuple<Tensor, Tensor> token_logprobs_grad(const Tensor& logits, const Tensor& tokens, int64_t ignore) {
-  auto out = TokenLogprobs::apply(logits, tokens, ignore, any_wants({&logits}));
+  const bool train = any_wants({&logits});
+  if (train) check_capture({&logits});
+  auto out = TokenLogprobs::apply(logits, tokens, ignore, train);
   return {out[0], out[1]};
 }
 

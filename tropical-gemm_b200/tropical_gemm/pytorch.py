@@ -196,7 +196,9 @@ def layernorm(x: torch.Tensor, weight=None, bias=None, residual=None, eps: float
     """(y, h): h = x + residual, y = (h - mean) / sqrt(variance + eps) * weight + bias
     over the last dimension, with autograd (`norms.layernorm`).  Kept for the
     backward: h and two float32 values per row.  Gradients cannot be
-    differentiated again."""
+    differentiated again.  (A call that is captured into a CUDA graph refuses
+    leaves whose autograd graph of another stream is still alive; so do the two
+    below.)"""
     return _layers.ext().layernorm_grad(x, weight, bias, residual, eps)
 
 
