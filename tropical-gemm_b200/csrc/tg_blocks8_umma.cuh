@@ -221,24 +221,34 @@ blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         const uint32_t idesc = umma::instr_desc_scaled(256, 2 * p.half_n);
         tg8::RingAt<S::kSlots> sc;
         for (int i = 0; ok && pair_item(p, pair, pairs, i, item); i++) {
-          for (int b = item.b0; b < item.b1; b++, at.next()) {
-            const int in = b - item.b0;
-            const bool first = in % p.chunk == 0, last = b + 1 == item.b1 || (in + 1) % p.chunk == 0;
-            if ((in & 3) == 0 && !umma::bar_wait<true>(scales_full(sc.slot), sc.parity)) { ok = false; break; }
-            if (first && !umma::bar_wait<true>(acc_empty(0), (n & 1) ^ 1)) { ok = false; break; }
-            if (!umma::bar_wait(full(at.slot), at.parity)) { ok = false; break; }
-            umma::fence_after();
-            const uint32_t off = at.slot * (S::kStage >> 4), sa = scales + 16 * sc.slot, id = idesc | umma::scale_byte(in & 3);
-            const bool group_done = (in & 3) == 3 || b + 1 == item.b1;
-            if (issue) {
+          int left = 0;   // of the chunk
+          for (int b = item.b0; ok && b < item.b1; b += 4) {   // four blocks with one slot of scales
+            if (!umma::bar_wait<true>(scales_full(sc.slot), sc.parity)) { ok = false; break; }
+            const uint32_t sa = scales + 16 * sc.slot;
+            const int blocks = min(4, item.b1 - b);
 #pragma unroll
-              for (int j = 0; j < 4; j++) umma::mma_f8_scaled<2>(tmem, da0 + (off + j * 2), db0 + (off + j * 2), id, sa, sa + 4, !first || j);
-              umma::mma_commit<2>(empty(at.slot));
-              if (group_done) umma::mma_commit<2>(scales_empty(sc.slot));
-              if (last) umma::mma_commit<2>(acc_full(0));
+            for (int j = 0; j < 4; j++) {
+              if (j >= blocks) break;
+              const bool first = left == 0;
+              if (first) {
+                left = min(p.chunk, item.b1 - (b + j));
+                if (!umma::bar_wait<true>(acc_empty(0), (n & 1) ^ 1)) { ok = false; break; }
+              }
+              if (!umma::bar_wait(full(at.slot), at.parity)) { ok = false; break; }
+              umma::fence_after();
+              left--;
+              const uint32_t off = at.slot * (S::kStage >> 4), id = idesc | umma::scale_byte(j);
+              if (issue) {
+#pragma unroll
+                for (int q = 0; q < 4; q++) umma::mma_f8_scaled<2>(tmem, da0 + (off + q * 2), db0 + (off + q * 2), id, sa, sa + 4, !first || q);
+                umma::mma_commit<2>(empty(at.slot));
+                if (j + 1 == blocks) umma::mma_commit<2>(scales_empty(sc.slot));
+                if (left == 0) umma::mma_commit<2>(acc_full(0));
+              }
+              if (left == 0) n++;
+              at.next();
             }
-            if (group_done) sc.next();
-            if (last) n++;
+            sc.next();
           }
           __syncwarp();
         }
