@@ -5,9 +5,10 @@
 //   grad_x = rstd (a - mean(a) - u mean(a u)) + grad_h,  a = grad weight
 //
 // All are bound by memory: a row is read once, kept in registers between its
-// sums and its output, and written once.  Many rows come by bulk copies into a
-// ring in shared memory, which keeps more of them on the way than registers
-// could; few rows are loaded directly.
+// sums and its output, and written once.  The backward's rows, of three operands
+// beside the columns' sums, come by bulk copies into a ring in shared memory where
+// there are many, which keeps more of them on the way than registers could
+// (8192 x 8192 bf16 104 us, loaded directly 389 with f32 arithmetic one by one).
 #include <algorithm>
 #include "tg_blocks8.cuh"
 #include "tg_umma.cuh"
@@ -97,6 +98,8 @@ template <int ACCESS, typename T> __device__ __forceinline__ void load_columns(V
   const T* from = static_cast<const T*>(columns);
   if (ACCESS == kAligned && from) {
     load_group<kAligned>(v, from, c, cols);
+  } else if (from && c >= 0 && c + 8 <= cols) {
+    load_any(v, from, c, cols);
   } else {
     union { Vec8<T> v; T e[8]; } u;
 #pragma unroll
@@ -242,165 +245,6 @@ __global__ void __launch_bounds__(512) layernorm_kernel(const NormArgs p) {
     const float2 st = row_stats<G, ACCESS>(v, p.tpr, t, shift, cols, inv_cols, p.eps, join);
     finish_row<T, G, ACCESS, BLOCKS>(p, row, t, shift, v, w, b, st);
   }
-}
-
-// ------------------------------------------------------------------------------- rows by bulk copies
-// A stage holds one row of each of up to three operands for each of the `per`
-// rows that a block works on at once; a row is copied from the 16-byte boundary
-// before its first element, 16 bytes into its place.
-constexpr int kMostStages = 8;
-struct RowRing {
-  uint32_t base, full, empty;   // shared memory; barriers
-  int stages, per, ops, pitch;
-  __device__ __forceinline__ uint32_t at(int stage, int op, int sub) const { return base + uint32_t(((stage * ops + op) * per + sub) * pitch); }
-};
-// One warp starts the copies of a batch's rows into a stage: a lane has one row
-// of one operand (ops * per is at most 32).
-template <int ACCESS, typename T> struct RowCopies {
-  const char* x;   // this lane's operand at row `sub` of batch 0
-  int64_t step;    // bytes from one batch to the next
-  int sub;
-  uint32_t to, bytes;
-  __device__ __forceinline__ RowCopies(const RowRing& r, int64_t cols, const void* const (&rows)[3], const int64_t (&ld)[3]) {
-    const int lane = threadIdx.x & 31, op = lane / r.per;
-    sub = lane - op * r.per;
-    if (op >= r.ops) sub = 1 << 30;
-    const void* from = op == 0 ? rows[0] : op == 1 ? rows[1] : rows[2];
-    const int64_t pitch = (op == 0 ? ld[0] : op == 1 ? ld[1] : ld[2]) * int64_t(sizeof(T));
-    x = static_cast<const char*>(from) + (op < r.ops ? sub * pitch : 0);
-    step = pitch * r.per;
-    bytes = uint32_t(cols * sizeof(T));
-    to = r.at(0, op < r.ops ? op : 0, op < r.ops ? sub : 0) + 16;
-  }
-  __device__ __forceinline__ void operator()(const RowRing& r, int64_t rows, int64_t batch, int stage) const {
-    const int here = int(min(int64_t(r.per), rows - batch * r.per));
-    const uintptr_t from = reinterpret_cast<uintptr_t>(x) + uintptr_t(batch * step), a = from & ~uintptr_t(15);
-    const uint32_t size = ACCESS == kAligned ? bytes : uint32_t(((from + bytes + 15) & ~uintptr_t(15)) - a);
-    const bool mine = sub < here;
-    uint32_t total = uint32_t(r.ops * here) * bytes;
-    if (ACCESS != kAligned) total = __reduce_add_sync(0xffffffffu, mine ? size : 0u);
-    if ((threadIdx.x & 31) == 0) umma::bar_expect(r.full + 8 * stage, total);
-    __syncwarp();
-    if (mine) umma::bulk_load(to + uint32_t(stage * r.ops * r.per * r.pitch), reinterpret_cast<const void*>(a), size, r.full + 8 * stage);
-  }
-};
-__device__ __forceinline__ uint4 load_shared16(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-  return v;
-}
-// Eight elements from shared memory; kScalar: from any element on.
-template <int ACCESS, typename T> __device__ __forceinline__ void take8(Vec8<T>& v, uint32_t at) {
-  if constexpr (sizeof(T) == 4) {
-    if constexpr (ACCESS != kScalar) {
-      const uint4 a = load_shared16(at), b = load_shared16(at + 16);
-      v.a = make_float4(__uint_as_float(a.x), __uint_as_float(a.y), __uint_as_float(a.z), __uint_as_float(a.w));
-      v.b = make_float4(__uint_as_float(b.x), __uint_as_float(b.y), __uint_as_float(b.z), __uint_as_float(b.w));
-    } else {
-      float f[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f[e]) : "r"(at + 4 * e));
-      v.a = make_float4(f[0], f[1], f[2], f[3]);
-      v.b = make_float4(f[4], f[5], f[6], f[7]);
-    }
-  } else if constexpr (ACCESS != kScalar) {
-    v.a = load_shared16(at);
-  } else {
-    const uint32_t skew = at & 15;
-    const uint4 lo = load_shared16(at - skew), hi = load_shared16(at - skew + 16);
-    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-    if (skew & 8) {
-#pragma unroll
-      for (int k = 0; k < 6; k++) w[k] = w[k + 2];
-    }
-    if (skew & 4) {
-#pragma unroll
-      for (int k = 0; k < 5; k++) w[k] = w[k + 1];
-    }
-    const uint32_t bits = (skew & 2) * 8;
-    v.a = make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
-                     __funnelshift_r(w[3], w[4], bits));
-  }
-}
-template <typename T> __device__ __forceinline__ uint32_t skew_of(const T* row) { return uint32_t(reinterpret_cast<uintptr_t>(row) & 15); }
-
-// Many rows: as layernorm_kernel, `per` rows at once.  The first warp starts the
-// copies into a stage when all warps have read it.
-template <typename T, int G, int ACCESS, bool BLOCKS>
-__global__ void __launch_bounds__(512) layernorm_ring_kernel(const NormArgs p, int per, int stages, int pitch) {
-  extern __shared__ __align__(16) uint8_t ring_store[];
-  __shared__ __align__(8) uint64_t bars[2 * kMostStages];
-  __shared__ float2 sums[2][16];
-  const int workers = per * p.tpr, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  RowRing ring{umma::smem_u32(ring_store), umma::smem_u32(bars), umma::smem_u32(bars + kMostStages), stages, per, p.residual ? 2 : 1, pitch};
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < stages; s++) {
-      umma::bar_init(ring.full + 8 * s, 1);
-      umma::bar_init(ring.empty + 8 * s, workers >> 5);
-    }
-    umma::bar_init_fence();
-  }
-  after_previous_kernel();
-  __syncthreads();
-  const RowCopies<ACCESS, T> copies(ring, p.cols, {p.x, p.residual, nullptr}, {p.ldx, p.ldr, 0});
-  auto bring = [&](int64_t batch, int stage) { copies(ring, p.rows, batch, stage); };
-  if (warp == 0)
-    for (int s = 0; s < stages && (blockIdx.x + int64_t(s) * gridDim.x) * per < p.rows; s++) bring(blockIdx.x + int64_t(s) * gridDim.x, s);
-  const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, cols = int(p.cols);
-  const T *x = static_cast<const T*>(p.x), *res = static_cast<const T*>(p.residual);
-  // rows of a thread all start at the same distance from a boundary: gridDim.x * per is a multiple of 8, or each has one
-  const int shift = ACCESS == kShifted ? row_shift(x + (int64_t(blockIdx.x) * per + sub) * p.ldx) : 0;
-  auto at = [&](int g) { return (g * p.tpr + t) * 8 - shift; };
-  RowSums join{sums, p.tpr, sub, 0};
-  Vec8<T> w[G], b[G];
-#pragma unroll
-  for (int g = 0; g < G; g++) {
-    load_columns<ACCESS>(w[g], p.weight, 1.f, at(g), cols);
-    load_columns<ACCESS>(b[g], p.bias, 0.f, at(g), cols);
-  }
-  const float inv_cols = 1.f / float(cols);
-  int stage = 0;
-  uint32_t parity = 0;
-  bool ok = true;
-  for (int64_t batch = blockIdx.x; batch * per < p.rows; batch += gridDim.x) {
-    const int64_t row = batch * per + sub;
-    if (ok) ok = umma::bar_wait(ring.full + 8 * stage, parity);
-    uint64_t v[G][4];
-    if (row < p.rows) {
-      const uint32_t from = ring.at(stage, 0, sub) + 16 + (ACCESS == kAligned ? 0 : skew_of(x + row * p.ldx));
-      const uint32_t more = res ? ring.at(stage, 1, sub) + 16 + (ACCESS == kAligned ? 0 : skew_of(res + row * p.ldr)) : 0;
-#pragma unroll
-      for (int g = 0; g < G; g++) {
-        const int c = at(g);
-        if (c >= cols) continue;
-        Vec8<T> a;
-        take8<ACCESS>(a, from + c * int(sizeof(T)));
-        get_pairs(a, v[g]);
-        if (res) {
-          uint64_t r[4];
-          take8<ACCESS>(a, more + c * int(sizeof(T)));
-          get_pairs(a, r);
-#pragma unroll
-          for (int i = 0; i < 4; i++) v[g][i] = add_pair(v[g][i], r[i]);
-        }
-        mask_pairs<ACCESS>(v[g], c, cols);
-      }
-    }
-    __syncwarp();
-    if (lane == 0) umma::bar_arrive(ring.empty + 8 * stage);
-    if (row < p.rows) {   // the same in all threads of a row
-      float2 st = row_stats<G, ACCESS>(v, p.tpr, t, shift, cols, inv_cols, p.eps, join);
-      if (!ok) st = make_float2(__uint_as_float(0x7fffffffu), __uint_as_float(0x7fffffffu));   // a wait ran out: the outputs say so
-      const int64_t ahead = batch + int64_t(stages) * gridDim.x;
-      if (warp == 0 && ahead * per < p.rows) {
-        if (ok) ok = umma::bar_wait(ring.empty + 8 * stage, parity);
-        if (ok) bring(ahead, stage);
-      }
-      finish_row<T, G, ACCESS, BLOCKS>(p, row, t, shift, v, w, b, st);
-    }
-    if (++stage == stages) { stage = 0; parity ^= 1; }
-  }
-  if (!ok) umma::drain_copies();
 }
 
 // Rows too long for registers: one block per row, which reads it three times
@@ -590,6 +434,86 @@ __global__ void __launch_bounds__(512) layernorm_backward_kernel(const NormBackA
     }
   }
 }
+
+// ------------------------------------------------------------------------------- rows by bulk copies
+// A stage holds one row of each of up to three operands for each of the `per`
+// rows that a block works on at once; a row is copied from the 16-byte boundary
+// before its first element, 16 bytes into its place.
+constexpr int kMostStages = 8;
+struct RowRing {
+  uint32_t base, full, empty;   // shared memory; barriers
+  int stages, per, ops, pitch;
+  __device__ __forceinline__ uint32_t at(int stage, int op, int sub) const { return base + uint32_t(((stage * ops + op) * per + sub) * pitch); }
+};
+// One warp starts the copies of a batch's rows into a stage: a lane has one row
+// of one operand (ops * per is at most 32).
+template <int ACCESS, typename T> struct RowCopies {
+  const char* x;   // this lane's operand at row `sub` of batch 0
+  int64_t step;    // bytes from one batch to the next
+  int sub;
+  uint32_t to, bytes;
+  __device__ __forceinline__ RowCopies(const RowRing& r, int64_t cols, const void* const (&rows)[3], const int64_t (&ld)[3]) {
+    const int lane = threadIdx.x & 31, op = lane / r.per;
+    sub = lane - op * r.per;
+    if (op >= r.ops) sub = 1 << 30;
+    const void* from = op == 0 ? rows[0] : op == 1 ? rows[1] : rows[2];
+    const int64_t pitch = (op == 0 ? ld[0] : op == 1 ? ld[1] : ld[2]) * int64_t(sizeof(T));
+    x = static_cast<const char*>(from) + (op < r.ops ? sub * pitch : 0);
+    step = pitch * r.per;
+    bytes = uint32_t(cols * sizeof(T));
+    to = r.at(0, op < r.ops ? op : 0, op < r.ops ? sub : 0) + 16;
+  }
+  __device__ __forceinline__ void operator()(const RowRing& r, int64_t rows, int64_t batch, int stage) const {
+    const int here = int(min(int64_t(r.per), rows - batch * r.per));
+    const uintptr_t from = reinterpret_cast<uintptr_t>(x) + uintptr_t(batch * step), a = from & ~uintptr_t(15);
+    const uint32_t size = ACCESS == kAligned ? bytes : uint32_t(((from + bytes + 15) & ~uintptr_t(15)) - a);
+    const bool mine = sub < here;
+    uint32_t total = uint32_t(r.ops * here) * bytes;
+    if (ACCESS != kAligned) total = __reduce_add_sync(0xffffffffu, mine ? size : 0u);
+    if ((threadIdx.x & 31) == 0) umma::bar_expect(r.full + 8 * stage, total);
+    __syncwarp();
+    if (mine) umma::bulk_load(to + uint32_t(stage * r.ops * r.per * r.pitch), reinterpret_cast<const void*>(a), size, r.full + 8 * stage);
+  }
+};
+__device__ __forceinline__ uint4 load_shared16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+// Eight elements from shared memory; kScalar: from any element on.
+template <int ACCESS, typename T> __device__ __forceinline__ void take8(Vec8<T>& v, uint32_t at) {
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (ACCESS != kScalar) {
+      const uint4 a = load_shared16(at), b = load_shared16(at + 16);
+      v.a = make_float4(__uint_as_float(a.x), __uint_as_float(a.y), __uint_as_float(a.z), __uint_as_float(a.w));
+      v.b = make_float4(__uint_as_float(b.x), __uint_as_float(b.y), __uint_as_float(b.z), __uint_as_float(b.w));
+    } else {
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f[e]) : "r"(at + 4 * e));
+      v.a = make_float4(f[0], f[1], f[2], f[3]);
+      v.b = make_float4(f[4], f[5], f[6], f[7]);
+    }
+  } else if constexpr (ACCESS != kScalar) {
+    v.a = load_shared16(at);
+  } else {
+    const uint32_t skew = at & 15;
+    const uint4 lo = load_shared16(at - skew), hi = load_shared16(at - skew + 16);
+    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    if (skew & 8) {
+#pragma unroll
+      for (int k = 0; k < 6; k++) w[k] = w[k + 2];
+    }
+    if (skew & 4) {
+#pragma unroll
+      for (int k = 0; k < 5; k++) w[k] = w[k + 1];
+    }
+    const uint32_t bits = (skew & 2) * 8;
+    v.a = make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                     __funnelshift_r(w[3], w[4], bits));
+  }
+}
+template <typename T> __device__ __forceinline__ uint32_t skew_of(const T* row) { return uint32_t(reinterpret_cast<uintptr_t>(row) & 15); }
 
 // Many rows: as layernorm_backward_kernel, rows by bulk copies.  The block's
 // sums over its rows are joined across its `per` threads of a column at the end.
@@ -830,7 +754,10 @@ bool in_registers(int64_t cols, int access, int most) { return groups_of(cols, a
 int64_t round32(int64_t v) { return (v + 31) / 32 * 32; }
 
 // Threads per row (a multiple of 32) and groups of 8 elements per thread, for
-// rows loaded directly: one group, for the latency, where 512 threads hold the row.
+// rows loaded directly, 512 threads per SM.  Few rows: one group, for the latency,
+// where 512 threads hold the row.  Many: two, which needs half as many sums
+// across warps (8192 rows, us, one group / two: 1024 f32 28 / 24, 2048 bf16
+// 36 / 26, 4096 bf16 70 / 50, four 57; 300 rows of 2048 f32 4.4 / 4.9).
 struct RowPlan {
   int tpr, groups, block;
   int64_t blocks, slots;
@@ -838,7 +765,7 @@ struct RowPlan {
 RowPlan row_plan(int64_t rows, int64_t cols, int access) {
   const int64_t groups = groups_of(cols, access);
   RowPlan r;
-  r.groups = 1;
+  r.groups = rows >= 2 * int64_t(sm_count()) && groups > 32 ? 2 : 1;
   while (groups > int64_t(r.groups) * 512) r.groups *= 2;
   r.tpr = int(round32((groups + r.groups - 1) / r.groups));
   const int per = std::max(1, 128 / r.tpr);
@@ -852,30 +779,30 @@ RowPlan row_plan(int64_t rows, int64_t cols, int access) {
   return r;
 }
 
-// The same for rows by bulk copies: up to `most` groups per thread, `workers`
-// threads per block that work, as many stages as its share of shared memory holds.
+// The same for rows by bulk copies: one block per SM, up to `most` groups per
+// thread, as many stages as shared memory holds.
 struct RingPlan {
   int tpr, groups, per, block, stages, pitch;
   size_t smem;
   int64_t blocks;
   bool fits;
 };
-RingPlan ring_plan(int64_t rows, int64_t cols, size_t elem, int ops, int access, int most, int workers, int blocks_per_sm) {
+RingPlan ring_plan(int64_t rows, int64_t cols, size_t elem, int ops, int access, int most) {
+  constexpr int workers = 512;
   RingPlan r{};
   const int64_t groups = groups_of(cols, access);
   if (groups > int64_t(most) * 512) return r;
   r.groups = 1;
   while (r.groups < most && groups > int64_t(r.groups) * 128) r.groups *= 2;   // up to 128 threads with one group each
   r.tpr = int(round32((groups + r.groups - 1) / r.groups));
-  if (r.tpr > workers) blocks_per_sm = 1;
   r.per = std::min(std::max(1, workers / r.tpr), 32 / ops);   // a lane of the copying warp for each row
   r.block = r.per * r.tpr;
   r.pitch = int((cols * int64_t(elem) + 15) / 16 * 16 + 64);
-  const size_t stage = size_t(ops) * r.per * r.pitch, share = size_t(216 * 1024) / blocks_per_sm;
+  const size_t stage = size_t(ops) * r.per * r.pitch, share = size_t(216 * 1024);
   r.stages = int(std::min<size_t>(tgb::kMostStages, share / stage));
   if (r.stages < 2) return r;
   r.smem = r.stages * stage;
-  r.blocks = std::min<int64_t>((rows + r.per - 1) / r.per, int64_t(sm_count()) * blocks_per_sm);
+  r.blocks = std::min<int64_t>((rows + r.per - 1) / r.per, int64_t(sm_count()));
   if (access == tg8::kShifted && r.blocks * r.per < rows) {   // a thread's rows start alike
     const int64_t unit = 8 / (r.per % 8 == 0 ? 8 : r.per % 4 == 0 ? 4 : r.per % 2 == 0 ? 2 : 1);
     r.blocks = std::max(unit, r.blocks / unit * unit);
@@ -900,27 +827,6 @@ template <typename T, bool BLOCKS> tg_status launch_norm(NormArgs p, int access,
   if (!in_registers(p.cols, access, kMost)) {
     launch_kernel(tgb::layernorm_long_kernel<T, BLOCKS>, unsigned(std::min<int64_t>(p.rows, 0x7fffffff)), 512, 0, 0, st, p);
     return check_launch("layernorm");
-  }
-  if (p.rows >= 2 * int64_t(sm_count())) {
-    const RingPlan r = ring_plan(p.rows, p.cols, sizeof(T), p.residual ? 2 : 1, access, kMost, 256, 2);
-    if (r.fits) {
-      p.tpr = r.tpr;
-      tg_status sized = TG_OK;
-      with_mode(access, [&](auto mode) {
-        constexpr int A = decltype(mode)::value;
-        if constexpr (!(BLOCKS && A == tg8::kShifted)) {
-          with_groups(r.groups, [&](auto g) {
-            constexpr int G = decltype(g)::value;
-            if constexpr (G <= kMost) {
-              auto kern = tgb::layernorm_ring_kernel<T, G, A, BLOCKS>;
-              sized = ensure_smem(reinterpret_cast<const void*>(kern), 216 * 1024);
-              if (sized == TG_OK) launch_kernel(kern, unsigned(r.blocks), r.block, r.smem, 0, st, p, r.per, r.stages, r.pitch);
-            }
-          });
-        }
-      });
-      return sized == TG_OK ? check_launch("layernorm") : sized;
-    }
   }
   const RowPlan r = row_plan(p.rows, p.cols, access);
   p.tpr = r.tpr;
@@ -988,7 +894,8 @@ template <typename T> tg_status launch_backward(NormBackArgs p, T* grad_w, T* gr
   if (access == tg8::kShifted && !in_registers(p.cols, access, kMost)) access = tg8::kScalar;
   const bool lng = !in_registers(p.cols, access, kMost);
   RingPlan ring{};
-  if (p.rows >= 2 * int64_t(sm_count())) ring = ring_plan(p.rows, p.cols, sizeof(T), p.grad_h && p.grad_x ? 3 : 2, access, kMost, 512, 1);
+  // by copies from a row per SM on (us, by copies / directly, bf16: 74 x 4096 11.2 / 9.6, 148 x 4096 11.2 / 11.8, 148 x 8192 16 / 21, 2400 x 8192 44 / 61)
+  if (p.rows >= sm_count()) ring = ring_plan(p.rows, p.cols, sizeof(T), p.grad_h && p.grad_x ? 3 : 2, access, kMost);
   RowPlan r{};
   if (lng) p.slots = std::max<int64_t>(1, std::min<int64_t>(p.rows, 64));
   else if (ring.fits) { p.slots = ring.blocks; p.tpr = ring.tpr; }
