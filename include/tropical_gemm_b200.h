@@ -290,8 +290,9 @@ tg_status tg_rows8_column_sum(tg_dtype dtype, tg_dtype out_dtype, int64_t rows, 
  * with a row's mean and rstd = 1 / sqrt(variance + eps), the variance being the
  * mean square of h - mean.  All arithmetic is f32 on the unrounded sum; x,
  * residual, weight, bias, h and y are of type dtype.  residual, weight (ones),
- * bias (zeros), h, mean and rstd may be null, mean and rstd together.  Equal
- * rows of one call give equal bits. */
+ * bias (zeros), h, mean and rstd may be null, mean and rstd together.  Finite
+ * rows whose squared distances from the mean pass f32's range (from about 1e19
+ * on) have rstd 0. */
 tg_status tg_layernorm(tg_dtype dtype, int64_t rows, int64_t cols,
                        const void* x, int64_t ldx, const void* residual, int64_t ldr,
                        const void* weight, const void* bias, float eps,
@@ -324,8 +325,10 @@ tg_status tg_layernorm_backward(tg_dtype dtype, int64_t rows, int64_t cols,
  * and round to nearest even: a float code's precision does not depend on its
  * scale's mantissa, and with a power of two the rounding to 8 bits is the only
  * one.  A block that holds a NaN or an infinity gets scale NaN, so that
- * everything made of it is NaN.  The products take any f32 scales; the product
- * of two scales that meet is taken in f32.
+ * everything made of it is NaN.  The products take any f32 scales; two scales
+ * that meet may be multiplied first, so their product lies within f32's range.
+ * Where all scales of a product are powers of two (or NaN) the tensor core
+ * applies them itself; which way is taken is decided on the device.
  * ------------------------------------------------------------------------ */
 
 /* q, scale = x with a scale per row and block of 128 columns.  qt (cols x
@@ -364,7 +367,9 @@ tg_status tg_blocks8_layernorm(tg_dtype dtype, int64_t rows, int64_t cols,
 /* C[i,j] = sum over blocks b of a_scale(i, b) * b_scale(j, b) * sum over k in b
  * of A[i,k] * B[j,k], + bias[j]: A (m x k) with tall == 1, B (n x k) with
  * b_tall 1 or 128, C (m x n) and bias (n, or null) of type dtype.  Sums are
- * f32: the tensor core's within a block of 128, then added up in order. */
+ * f32, in an order that depends on the sizes and not on the run: the tensor
+ * core's over one block or over as many as keep its error below the output's
+ * rounding, then added up. */
 tg_status tg_blocks8_gemm(tg_dtype dtype, int64_t m, int64_t n, int64_t k,
                           const void* a, int64_t lda, const float* a_scale, int64_t a_scale_row, int64_t a_scale_block,
                           const void* b, int64_t ldb, int b_tall, const float* b_scale, int64_t b_scale_row, int64_t b_scale_block,

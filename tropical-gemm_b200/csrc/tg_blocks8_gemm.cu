@@ -12,7 +12,12 @@ namespace {
 
 // How a product is done, and what it is expected to take (us, on a B200).  The
 // few-token kernel reads 128 rows of B per CTA and block, at the rate of one SM's
-// way from L2: us per launch and per block of 16, 32 and 64 tokens
+// way from L2.  The paired kernel does 256 x 256 in the time that an SM's tensor
+// core needs, but its call is three launches.  Measured (bf16 outputs, us, few / pairs):
+// 333 x 1531 x 1111 5.6 / 16.3, 256 x 4096 x 4096 15.6 / 21.3, 1024 x 1024 x 4096 15.7 / 21.1,
+// 512 x 4096 x 4096 30 / 20.6; the constants are fitted to such pairs and choose the
+// faster of each.
+// us per launch and per block of 16, 32 and 64 tokens
 constexpr double kFewBase[] = {2.3, 2.8, 4.2}, kFewBlock[] = {0.22, 0.245, 0.34};
 // us per call and per block of the paired kernel (its call is three launches)
 constexpr double kPairBase = 9.0, kPairBlock = 0.28, kPairTile = 0.5, kJoin = 2.5;

@@ -4,9 +4,10 @@
 //   C[i,j] = sum_b a_scale(i,b) b_scale(j,b) sum_{k in b} A[i,k] B[j,k] + bias[j]
 //
 // A block is one step of 128 bytes per row: four products of 32 into an
-// accumulator in tensor memory, which the epilogue warps take from there, scale
-// and add to f32 sums in registers while the next block goes into another
-// accumulator.
+// accumulator in tensor memory.  Where all scales are powers of two the tensor
+// core applies them on the way in (pairs of CTAs) and the sum stays there;
+// otherwise the epilogue warps take each block's sums out, scale them and add them
+// to f32 sums in registers while the next block goes into another accumulator.
 #pragma once
 #include "tg_blocks8.cuh"
 #include "tg_rows8_umma.cuh"
@@ -86,10 +87,11 @@ __device__ __forceinline__ bool other_scales(const int* other) { return __syncth
 //
 // With other scales each block goes into an accumulator of its own, of two in
 // turn, which the epilogue scales and adds up: a hand-over of 800 cycles and 500
-// of reads and arithmetic per block of 512, so this is 1.8 times slower
-// (8192^3 bf16: 0.39 and 0.70 ms).
+// of reads and arithmetic per block of 512, so this takes about twice as long
+// (8192^3 bf16: 0.39 and 0.76 ms).
 //
-// What bounds it: power (8192^3 2.8 PFLOP/s; 4096^3 57 us in four rounds of tiles).
+// What bounds it: power (8192^3 2.8 PFLOP/s, operands of zeros 3.8); 4096^3, 56 us, is
+// 256 tiles on 74 pairs, four rounds for 3.46.
 struct PairShape {
   static constexpr int kStages = 6, kStage = 2 * tg8::kOperand, kEpi = 8, kSlots = 4, kThreads = 512;
   static constexpr int kLow = 48, kHigh = 208;   // registers per thread of the first two warpgroups, and of the epilogue's two
@@ -447,6 +449,10 @@ __global__ void __launch_bounds__(256) blocks_bias_kernel(const ProductArgs8 p) 
 // the sum is split over the S CTAs of a cluster (1 to 8), so that all SMs read.
 // Each CTA finishes a share of the tokens: the others write their parts into its
 // shared memory.  Four epilogue warps, one row of B per thread.
+//
+// What bounds it: launch and set-up where the weights are few (1 x 4096 x 4096
+// 5.0 us, their read 2.6), then what an SM takes from memory: one step of 16 KB of
+// weights per 0.22 us and CTA (16 x 8192 x 4096 8.0 us, floor 5.2).
 //
 // A CTA that waits for its cluster must not wait for tensor memory held by one
 // that waits for another cluster: with split > 1 a CTA asks for more than half

@@ -22,6 +22,7 @@ namespace tgb {
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr int kMostTop = 32;   // alternatives: one per lane
 constexpr int kManyRows = 128, kFewRows = 512;   // threads per row and CTA
+constexpr int kSorted = 6;     // of a warp's 32 logits: more than these are cheaper to sort than to insert one by one
 constexpr int kGroups = 4;     // of 8 logits per thread on their way at once
 
 __device__ __forceinline__ float neg_inf() { return __int_as_float(int(0xff800000)); }
@@ -68,6 +69,19 @@ __device__ __forceinline__ float logit_of(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t token_of(uint64_t key) { return ~uint32_t(key); }
 
+// Descending over the lanes.
+template <typename K> __device__ __forceinline__ K sort_lanes(K v, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int d = size / 2; d; d >>= 1) {
+      const K o = __shfl_xor_sync(0xffffffffu, v, d);
+      const bool descending = (lane & size) == 0 || size == 32, low = (lane & d) == 0;
+      v = (descending == low) == (v > o) ? v : o;
+    }
+  return v;
+}
+
 // A warp's best keys so far, sorted, one per lane; 0 is below every key.
 struct Best {
   uint64_t key;
@@ -91,6 +105,15 @@ struct Best {
   }
 };
 
+// The best 32 of a sorted list and of 32 more keys.  A call, for the sake of the
+// loop that it stands in four times (4096 x 65536 with 20 alternatives, inline 267 us).
+__device__ __noinline__ uint64_t merge_keys(uint64_t best, uint64_t keys) {
+  const int lane = threadIdx.x & 31;
+  Best b{best};
+  b.merge(sort_lanes(keys, lane), lane);
+  return b.key;
+}
+
 // A value's place in the order alone: larger for larger values, one zero, NaN on top.
 __device__ __forceinline__ uint32_t rank_of(float x) { return uint32_t(key_of(x, 0) >> 32); }
 __device__ __forceinline__ float value_of_rank(uint32_t r) { return __uint_as_float(r >> 31 ? r ^ 0x80000000u : ~r); }
@@ -100,17 +123,12 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// Descending over the lanes.
-__device__ __forceinline__ uint32_t sort_lanes(uint32_t v, int lane) {
+// The ranks of the lanes' largest logits in descending order; a group that holds a NaN counts for nothing.
+__device__ __forceinline__ uint32_t lane_ranks(const float (&tops)[kGroups], int lane) {
+  float top = neg_inf();
 #pragma unroll
-  for (int size = 2; size <= 32; size *= 2)
-#pragma unroll
-    for (int d = size / 2; d; d >>= 1) {
-      const uint32_t o = __shfl_xor_sync(0xffffffffu, v, d);
-      const bool descending = (lane & size) == 0 || size == 32, low = (lane & d) == 0;
-      v = descending == low ? max(v, o) : min(v, o);
-    }
-  return v;
+  for (int u = 0; u < kGroups; u++) top = fmaxf(top, tops[u]);
+  return sort_lanes(top == neg_inf() ? 0u : rank_of(top), lane);
 }
 
 struct TokenArgs {
@@ -150,8 +168,9 @@ __device__ __forceinline__ void merge_lists(uint64_t (*lists)[kMostTop], int cou
 // warp's own k-th best.
 //
 // Many rows take 128 threads each (4096 x 65536 bf16, us without / with 20
-// alternatives: 512 threads 179 / 446, 256 144 / 266, 128 131 / 235, 64 125 / 236): fewer
-// lists to fill, more rows on an SM.  Few rows take 512, and several CTAs each (one
+// alternatives: 512 threads 179 / 446, 256 144 / 266, 128 131 / 235, 64 125 / 236; now
+// 252, and 1060 where every logit is larger than the one before it, which took 12400
+// before many at once were sorted into the list): fewer lists to fill, more rows on an SM.  Few rows take 512, and several CTAs each (one
 // of 131072, 20 alternatives: 512 threads 11.5, 128 17.5).
 template <typename T, int ACCESS, bool TOP, int THREADS>
 __global__ void __launch_bounds__(THREADS, (TOP ? 768 : 1024) / THREADS) token_logprobs_kernel(const TokenArgs p) {
@@ -177,6 +196,7 @@ __global__ void __launch_bounds__(THREADS, (TOP ? 768 : 1024) / THREADS) token_l
     Best best{0};
     uint64_t least = 0;          // the top-th best key so far
     float bound = neg_inf();     // what is less is passed over
+    bool rising = false;         // many of this warp's last batch came into its list
     auto logits_of = [&](const Vec8<T>& a, int g, float (&v)[8]) {
       a.get(v);
       if (ACCESS != kAligned) {
@@ -198,17 +218,23 @@ __global__ void __launch_bounds__(THREADS, (TOP ? 768 : 1024) / THREADS) token_l
         for (int e = 0; e < 8; e++)
           if (!(v[e] < bound) && (ACCESS == kAligned || (c + e >= 0 && c + e < vocab))) mine |= 1u << e;
       }
-      while (const uint32_t lanes = __ballot_sync(0xffffffffu, mine != 0)) {
+      // each lane offers the first of its eight that would enter the list; a few are taken one
+      // at a time, more are sorted and merged
+      while (__any_sync(0xffffffffu, mine != 0)) {
         const int e = __ffs(mine) - 1;
         float x1 = v[0];
 #pragma unroll
         for (int i = 1; i < 8; i++)
           if (e == i) x1 = v[i];
+        const uint64_t key = mine ? key_of(x1, uint32_t(c + e)) : 0;
+        const uint32_t lanes = __ballot_sync(0xffffffffu, key > least);
         const int from = __ffs(lanes) - 1;
-        const uint64_t next = __shfl_sync(0xffffffffu, key_of(x1, uint32_t(c + e)), from);
-        if (lane == from) mine &= mine - 1;
-        if (next <= least) continue;
-        best.insert(next, lane);
+        const bool many = __popc(lanes) > kSorted;
+        if (key <= least || lane == from || many) mine &= mine - 1;
+        if (!lanes) continue;
+        rising |= many;
+        if (many) best.key = merge_keys(best.key, key);
+        else best.insert(__shfl_sync(0xffffffffu, key, from), lane);
         least = __shfl_sync(0xffffffffu, best.key, p.top - 1);
         if (least) bound = fmaxf(bound, value_of_rank(uint32_t(least >> 32)));   // a NaN is passed over by its key
       }
@@ -266,13 +292,15 @@ __global__ void __launch_bounds__(THREADS, (TOP ? 768 : 1024) / THREADS) token_l
         }
       }
       if constexpr (TOP) {
-        if (batch == 0) {   // no lists yet: the lanes' largest logits; a lane that holds a NaN counts for nothing
-          float lane_top = neg_inf();
-#pragma unroll
-          for (int u = 0; u < kGroups; u++) lane_top = fmaxf(lane_top, tops[u]);
-          tighten(sort_lanes(lane_top == neg_inf() ? 0u : rank_of(lane_top), lane));
+        if (batch == 0) {   // no lists yet: the lanes' largest logits
+          tighten(lane_ranks(tops, lane));
         } else if ((batch & (batch - 1)) == 0) {
           tighten(uint32_t(best.key >> 32));
+        }
+        if (rising) {   // the warp's own bound, as in the first batch
+          rising = false;
+          const uint32_t kth = __shfl_sync(0xffffffffu, lane_ranks(tops, lane), p.top - 1);
+          if (kth) bound = fmaxf(bound, value_of_rank(kth));
         }
 #pragma unroll
         for (int u = 0; u < kGroups; u++)

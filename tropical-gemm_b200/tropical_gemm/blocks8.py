@@ -16,7 +16,9 @@ calls of this module record no graph.
 The quantising calls take powers of two as scales, the least that brings a
 block's largest magnitude to 448 or below, and round to nearest even, so that a
 code is one rounding of its value.  A block that holds a NaN or an infinity has
-scale NaN: what is made of it is NaN.  The products take any float32 scales.
+scale NaN: what is made of it is NaN.  The products take any float32 scales
+(the product of two that meet within float32's range) and are about twice as
+fast where all are powers of two, which is found out on the device.
 
 Tensors are CUDA tensors (inputs float32, float16 or bfloat16) with any leading
 dimensions; rows may be strided, their elements are contiguous (other layouts
@@ -87,7 +89,8 @@ def layernorm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opti
 def matmul(a: Blocks8, b: Blocks8, bias: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """A B^T + bias in `dtype`: a (.., K) tokens in blocks along their rows, b (N, K)
     output channels in blocks along their rows or in tiles, bias (N,) of type
-    `dtype`.  Sums are float32."""
+    `dtype`.  Sums are float32; their order depends on the sizes (a token's bits may
+    depend on how many tokens share the call), not on the run."""
     aq, a_scale = a
     bq, b_scale = b
     return _x().matmul(aq, a_scale, bq, b_scale, bias, dtype)
