@@ -417,7 +417,7 @@ tg_status tg_blocks8_quantize(tg_dtype dtype, int64_t rows, int64_t cols, const 
     scratch_free(scratch, st);
     return s;
   }
-  // From 512 rows on the tile kernel is the faster one along rows alone, too (8192 x 8192 bf16 48 us row by row, 35).
+  // From 512 rows on the tile kernel is the faster one along rows alone, too (8192 x 8192 bf16 48 us row by row, 40).
   if (qt || rows >= 512) return launch_tiles<false>(dtype, p, st);
   const dim3 grid(unsigned((cols + 2047) / 2048), unsigned(rows));
   return with_type8(dtype, [&](auto t) {
