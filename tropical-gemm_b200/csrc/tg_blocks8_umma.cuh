@@ -457,7 +457,8 @@ __global__ void __launch_bounds__(256) blocks_bias_kernel(const ProductArgs8 p) 
 // A CTA that waits for its cluster must not wait for tensor memory held by one
 // that waits for another cluster: with split > 1 a CTA asks for more than half
 // of an SM's shared memory, so no two of these share an SM; it takes at most 256
-// of the 512 columns.
+// of the 512 columns.  Nor must one that waits for the kernel before it hold what
+// that one's CTAs still ask for: tensor memory is taken behind that wait.
 template <int NT> struct FewShape {
   static constexpr int kStage = tg8::kOperand + NT * 128, kThreads = 192;
   static constexpr int kExchange = (NT < 32 ? 32 : NT) * 512;       // parts of this CTA's tokens (shares of 4) from the whole cluster
@@ -501,8 +502,8 @@ __global__ void __launch_bounds__(192) blocks_few_kernel(const __grid_constant__
     }
     umma::bar_init_fence();
   }
-  if (warp == 1) umma::tmem_alloc<1>(umma::smem_u32(&slot), S::kColumns);
   after_previous_kernel();
+  if (warp == 1) umma::tmem_alloc<1>(umma::smem_u32(&slot), S::kColumns);
   umma::fence_before();
   __syncthreads();
   umma::fence_after();
