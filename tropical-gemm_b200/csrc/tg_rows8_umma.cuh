@@ -632,8 +632,8 @@ __global__ void __launch_bounds__(128) tokens_kernel(const __grid_constant__ CUt
     umma::bar_init(done, 1);
     umma::bar_init_fence();
   }
+  after_previous_kernel();   // before tensor memory is taken, which that kernel's CTAs may still ask for
   if (warp == 2) umma::tmem_alloc<1>(umma::smem_u32(&slot), S::kColumns);
-  after_previous_kernel();
   umma::fence_before();
   __syncthreads();
   umma::fence_after();
