@@ -219,3 +219,11 @@ def test_other_streams_and_capture():
             t.fill_(7)
         graph.replay()
         assert all(torch.equal(p, q) for p, q in zip((*r, *grads), (*want, *back)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, cols", [(900, 4097), (900, 4600), (611, 5001), (640, 5120), (450, 5121)])
+def test_many_wide_rows(rows, cols, dtype):
+    """Around the widths of which an SM works on two rows at once, several rows to each."""
+    test_forward(rows, cols, dtype)
+    test_blocks_out(rows, cols, dtype)

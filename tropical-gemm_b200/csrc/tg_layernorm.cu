@@ -201,8 +201,10 @@ __device__ __forceinline__ void finish_row(const NormArgs& p, int64_t row, int t
 // and bias stay in registers (rows that start anywhere: slots is a multiple of
 // 8, so all rows of a slot start at the same distance from a boundary).  The
 // next row is on its way while this one is worked on.
-template <typename T, int G, int ACCESS, bool BLOCKS>
-__global__ void __launch_bounds__(512) layernorm_kernel(const NormArgs p) {
+//
+// MOST threads per block: 512, of which an SM has one, or 320, of which it has two.
+template <typename T, int G, int ACCESS, bool BLOCKS, int MOST>
+__global__ void __launch_bounds__(MOST, MOST == 320 ? 2 : 1) layernorm_kernel(const NormArgs p) {
   __shared__ float2 sums[2][16];
   after_previous_kernel();
   const int sub = threadIdx.x / p.tpr, t = threadIdx.x % p.tpr, per_block = blockDim.x / p.tpr;
@@ -758,11 +760,17 @@ int64_t round32(int64_t v) { return (v + 31) / 32 * 32; }
 // where 512 threads hold the row.  Many: two, which needs half as many sums
 // across warps (8192 rows, us, one group / two: 1024 f32 28 / 24, 2048 bf16
 // 36 / 26, 4096 bf16 70 / 50, four 57; 300 rows of 2048 f32 4.4 / 4.9).
+//
+// Rows of 257 to 320 threads leave many idle at one block per SM; with `narrow`
+// there are two, in 96 registers (8192 rows bf16, us, one block / two: 4608 67 / 45,
+// 5120 70 / 47, 777 f16 rows of 5001 13.1 / 9.4; f32, whose registers spill, 5120 88 / 105;
+// 384 threads in 80 registers 6144 74 / 69, with residual 87 / 88).
 struct RowPlan {
   int tpr, groups, block;
   int64_t blocks, slots;
+  bool two;   // blocks per SM
 };
-RowPlan row_plan(int64_t rows, int64_t cols, int access) {
+RowPlan row_plan(int64_t rows, int64_t cols, int access, bool narrow) {
   const int64_t groups = groups_of(cols, access);
   RowPlan r;
   r.groups = rows >= 2 * int64_t(sm_count()) && groups > 32 ? 2 : 1;
@@ -770,7 +778,8 @@ RowPlan row_plan(int64_t rows, int64_t cols, int access) {
   r.tpr = int(round32((groups + r.groups - 1) / r.groups));
   const int per = std::max(1, 128 / r.tpr);
   r.block = per * r.tpr;
-  r.blocks = std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, int64_t(sm_count()) * std::max(1, 512 / r.block)));
+  r.two = narrow && r.groups == 2 && r.tpr > 256 && r.tpr <= 320;
+  r.blocks = std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, int64_t(sm_count()) * (r.two ? 2 : std::max(1, 512 / r.block))));
   r.slots = r.blocks * per;
   if (access == tg8::kShifted && r.slots < rows) {   // a slot's rows start alike
     r.slots = std::max<int64_t>(8, r.slots / 8 * 8);
@@ -828,7 +837,7 @@ template <typename T, bool BLOCKS> tg_status launch_norm(NormArgs p, int access,
     launch_kernel(tgb::layernorm_long_kernel<T, BLOCKS>, unsigned(std::min<int64_t>(p.rows, 0x7fffffff)), 512, 0, 0, st, p);
     return check_launch("layernorm");
   }
-  const RowPlan r = row_plan(p.rows, p.cols, access);
+  const RowPlan r = row_plan(p.rows, p.cols, access, sizeof(T) == 2);
   p.tpr = r.tpr;
   p.slots = r.slots;
   with_mode(access, [&](auto mode) {
@@ -836,7 +845,11 @@ template <typename T, bool BLOCKS> tg_status launch_norm(NormArgs p, int access,
     if constexpr (!(BLOCKS && A == tg8::kShifted)) {
       with_groups(r.groups, [&](auto g) {
         constexpr int G = decltype(g)::value;
-        if constexpr (G <= kMost) launch_kernel(tgb::layernorm_kernel<T, G, A, BLOCKS>, unsigned(r.blocks), r.block, 0, 0, st, p);
+        auto go = [&](auto kern) { launch_kernel(kern, unsigned(r.blocks), r.block, 0, 0, st, p); };
+        if constexpr (G == 2 && sizeof(T) == 2) {
+          if (r.two) return go(tgb::layernorm_kernel<T, G, A, BLOCKS, 320>);
+        }
+        if constexpr (G <= kMost) go(tgb::layernorm_kernel<T, G, A, BLOCKS, 512>);
       });
     }
   });
@@ -899,7 +912,7 @@ template <typename T> tg_status launch_backward(NormBackArgs p, T* grad_w, T* gr
   RowPlan r{};
   if (lng) p.slots = std::max<int64_t>(1, std::min<int64_t>(p.rows, 64));
   else if (ring.fits) { p.slots = ring.blocks; p.tpr = ring.tpr; }
-  else { r = row_plan(p.rows, p.cols, access); p.slots = r.slots; p.tpr = r.tpr; }
+  else { r = row_plan(p.rows, p.cols, access, false); p.slots = r.slots; p.tpr = r.tpr; }
   void* scratch = nullptr;
   const size_t part = size_t(p.slots) * size_t(p.cols);
   if (grad_w || grad_b) {
