@@ -365,7 +365,7 @@ __device__ __forceinline__ void back_out(const uint64_t (&a)[4], const uint64_t 
 }
 
 // As layernorm_kernel; a thread also keeps its columns' sums of grad * u and of
-// grad over the slot's rows, joined by column_join_kernel in a fixed order.
+// grad over the slot's rows, joined by layernorm_join_kernel in a fixed order.
 template <typename T, int G, int ACCESS>
 __global__ void __launch_bounds__(512) layernorm_backward_kernel(const NormBackArgs p) {
   __shared__ float2 sums[2][16];
