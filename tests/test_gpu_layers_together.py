@@ -298,3 +298,35 @@ def test_the_example():
     lp, h = tp.token_logprobs(head(x), torch.arange(10, device="cuda"))
     (lp.sum() + h.sum()).backward()
     assert all(torch.isfinite(p.grad).all() and p.grad.any() for p in head.parameters())
+
+
+def test_products_behind_one_another_on_streams():
+    """Short sums of many tiles (several thread blocks per SM), clusters and pairs, each kernel started while the one before it ends."""
+    products = []
+    for m, n, k in [(64, 65536, 128), (17, 30000, 256), (300, 1000, 130), (1, 4096, 4096), (2048, 2048, 512), (64, 20000, 128)]:
+        a = blocks8.quantize(torch.randn(m, k, device="cuda").bfloat16())
+        b = blocks8.quantize_tiles(torch.randn(n, k, device="cuda").bfloat16())
+        products.append((a, b, blocks8.matmul(a, b)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got += [(blocks8.matmul(a, b), z) for a, b, z in products]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, z) for x, z in got)
+
+
+def test_the_same_tensor_twice():
+    """x as its own residual: both of its gradients add up."""
+    x = torch.randn(300, 4700, device="cuda", requires_grad=True)
+    w = torch.randn(4700, device="cuda", requires_grad=True)
+    y, h = tp.layernorm(x, w, None, residual=x)
+    g = torch.randn_like(y)
+    gx, gw = torch.autograd.grad((y, h), (x, w), (g, g))
+    xd, wd = (t.detach().double().requires_grad_(True) for t in (x, w))
+    hd = 2 * xd
+    ex, ew = torch.autograd.grad((torch.nn.functional.layer_norm(hd, (4700,), wd, None, 1e-5), hd), (xd, wd), (g.double(), g.double()))
+    # f32 sums in trees of some 32 steps: 32 half steps of 2^-24, relative to the whole
+    assert (gx.double() - ex).norm() <= 32 * 2.0 ** -24 * ex.norm() and (gw.double() - ew).norm() <= 32 * 2.0 ** -24 * ew.norm()
