@@ -304,12 +304,24 @@ tg_status tg_layernorm(tg_dtype dtype, int64_t rows, int64_t cols,
  *   grad_weight = sum over rows of grad * u;  grad_bias = sum over rows of grad
  * All of type dtype except mean and rstd (f32).  grad_h and weight may be
  * null, and each of the three results.  The sums over rows have a fixed order:
- * equal inputs give equal bits. */
+ * equal inputs give equal bits.
+ * A 16-bit h that is the sum x + residual is that sum rounded: u is then off by
+ * half a step of h times rstd, which a row far from zero shows in full.  The
+ * call below takes the sum's parts. */
 tg_status tg_layernorm_backward(tg_dtype dtype, int64_t rows, int64_t cols,
                                 const void* grad, int64_t ldg, const void* grad_h, int64_t ldgh,
                                 const void* weight, const void* h, int64_t ldh,
                                 const float* mean, const float* rstd,
                                 void* grad_x, int64_t ldx, void* grad_weight, void* grad_bias, void* stream);
+
+/* The same with h = x + residual formed in f32 as tg_layernorm formed it, so
+ * that u is that of y; residual may be null (h is x).  grad_x is the gradient
+ * of x and of residual; its leading dimension is ldgx. */
+tg_status tg_layernorm_residual_backward(tg_dtype dtype, int64_t rows, int64_t cols,
+                                         const void* grad, int64_t ldg, const void* grad_h, int64_t ldgh,
+                                         const void* weight, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                                         const float* mean, const float* rstd,
+                                         void* grad_x, int64_t ldgx, void* grad_weight, void* grad_bias, void* stream);
 
 /* --------------------------------------------------------------------------
  * Matrices held in 8-bit floating point (e4m3, as bytes) with a scale for each

@@ -317,25 +317,35 @@ __global__ void __launch_bounds__(512) layernorm_long_kernel(const NormArgs p) {
   }
 }
 
+// u is that of the output only where h is the sum that the forward took its
+// statistics of: a 16-bit h is that sum rounded, which u would show in full
+// (errors of the gradients against 64 bits 1.5 times those of their own rounding,
+// more where a row is far from zero).  With a residual, h is x and the sum is
+// formed again, as the forward did.
 struct NormBackArgs {
   int64_t rows, cols, slots;
-  const void *grad, *grad_h, *weight, *h;
+  const void *grad, *grad_h, *weight, *h, *residual;   // grad_h, weight, residual: or null
   const float *mean, *rstd;
   void* grad_x;
   float *partial_w, *partial_b;   // (slots x cols), or null
-  int64_t ldg, ldgh, ldh, ldx;
+  int64_t ldg, ldgh, ldh, ldr, ldx;
   int tpr;
 };
 
 // The backward's two passes over a group: a = grad * weight and u, and their part
-// in the sums; then grad_x from the row's means.
-template <int ACCESS, typename T>
-__device__ __forceinline__ void back_group(const Vec8<T>& grad, const Vec8<T>& h, const Vec8<T>& w, int c, int cols, uint64_t minus,
-                                           uint64_t rstd, uint64_t (&a)[4], uint64_t (&u)[4], uint64_t (&dw)[4], uint64_t (&db)[4], uint64_t& s,
-                                           uint64_t& su) {
+// in the sums; then grad_x from the row's means.  SUM: h is x + res.
+template <int ACCESS, bool SUM, typename T>
+__device__ __forceinline__ void back_group(const Vec8<T>& grad, const Vec8<T>& h, const Vec8<T>& res, const Vec8<T>& w, int c, int cols,
+                                           uint64_t minus, uint64_t rstd, uint64_t (&a)[4], uint64_t (&u)[4], uint64_t (&dw)[4], uint64_t (&db)[4],
+                                           uint64_t& s, uint64_t& su) {
   uint64_t k[4];
   get_pairs(grad, a);
   get_pairs(h, u);
+  if (SUM) {
+    get_pairs(res, k);
+#pragma unroll
+    for (int i = 0; i < 4; i++) u[i] = add_pair(u[i], k[i]);
+  }
 #pragma unroll
   for (int i = 0; i < 4; i++) u[i] = mul_pair(add_pair(u[i], minus), rstd);
   mask_pairs<ACCESS>(a, c, cols);
@@ -366,7 +376,9 @@ __device__ __forceinline__ void back_out(const uint64_t (&a)[4], const uint64_t 
 
 // As layernorm_kernel; a thread also keeps its columns' sums of grad * u and of
 // grad over the slot's rows, joined by layernorm_join_kernel in a fixed order.
-template <typename T, int G, int ACCESS>
+// SUM, the sum formed again, is a variant of its own: as a branch it took 14 us of
+// 109 from the rows without (8192 x 8192 bf16, by copies).
+template <typename T, int G, int ACCESS, bool SUM>
 __global__ void __launch_bounds__(512) layernorm_backward_kernel(const NormBackArgs p) {
   __shared__ float2 sums[2][16];
   after_previous_kernel();
@@ -375,6 +387,7 @@ __global__ void __launch_bounds__(512) layernorm_backward_kernel(const NormBackA
   const int64_t slot = int64_t(blockIdx.x) * per_block + sub;
   if (slot >= p.slots) return;
   const T *grad = static_cast<const T*>(p.grad), *h = static_cast<const T*>(p.h), *gh = static_cast<const T*>(p.grad_h);
+  const T* res = SUM ? static_cast<const T*>(p.residual) : nullptr;
   const int shift = ACCESS == kShifted ? row_shift(grad + slot * p.ldg) : 0;
   auto at = [&](int g) { return (g * p.tpr + t) * 8 - shift; };
   RowSums join{sums, p.tpr, sub, 0};
@@ -398,7 +411,11 @@ __global__ void __launch_bounds__(512) layernorm_backward_kernel(const NormBackA
   const float inv_cols = 1.f / float(cols);
   for (; row < p.rows; row += p.slots) {
     if (!kAhead) load(row);
-    Vec8<T> ch[G];
+    Vec8<T> ch[G], cr[G];
+    if (SUM) {
+#pragma unroll
+      for (int g = 0; g < G; g++) load_at<ACCESS>(cr[g], res + row * p.ldr, at(g), cols);
+    }
     if (gh && p.grad_x) {
 #pragma unroll
       for (int g = 0; g < G; g++) load_at<ACCESS>(ch[g], gh + row * p.ldgh, at(g), cols);
@@ -407,7 +424,7 @@ __global__ void __launch_bounds__(512) layernorm_backward_kernel(const NormBackA
     const uint64_t rstd = pair_of(ns.y), minus = pair_of(-ns.x);
 #pragma unroll
     for (int g = 0; g < G; g++)
-      if (at(g) < cols) back_group<ACCESS>(ng[g], nh[g], w[g], at(g), cols, minus, rstd, a[g], u[g], dw[g], db[g], s, su);
+      if (at(g) < cols) back_group<ACCESS, SUM>(ng[g], nh[g], cr[g], w[g], at(g), cols, minus, rstd, a[g], u[g], dw[g], db[g], s, su);
     if (kAhead && row + p.slots < p.rows) load(row + p.slots);
     if (!p.grad_x) continue;
     const float2 sums2 = join.two(make_float2(sum_of(s), sum_of(su)));
@@ -438,7 +455,7 @@ __global__ void __launch_bounds__(512) layernorm_backward_kernel(const NormBackA
 }
 
 // ------------------------------------------------------------------------------- rows by bulk copies
-// A stage holds one row of each of up to three operands for each of the `per`
+// A stage holds one row of each of up to four operands for each of the `per`
 // rows that a block works on at once; a row is copied from the 16-byte boundary
 // before its first element, 16 bytes into its place.
 constexpr int kMostStages = 8;
@@ -454,12 +471,12 @@ template <int ACCESS, typename T> struct RowCopies {
   int64_t step;    // bytes from one batch to the next
   int sub;
   uint32_t to, bytes;
-  __device__ __forceinline__ RowCopies(const RowRing& r, int64_t cols, const void* const (&rows)[3], const int64_t (&ld)[3]) {
+  __device__ __forceinline__ RowCopies(const RowRing& r, int64_t cols, const void* const (&rows)[4], const int64_t (&ld)[4]) {
     const int lane = threadIdx.x & 31, op = lane / r.per;
     sub = lane - op * r.per;
     if (op >= r.ops) sub = 1 << 30;
-    const void* from = op == 0 ? rows[0] : op == 1 ? rows[1] : rows[2];
-    const int64_t pitch = (op == 0 ? ld[0] : op == 1 ? ld[1] : ld[2]) * int64_t(sizeof(T));
+    const void* from = op == 0 ? rows[0] : op == 1 ? rows[1] : op == 2 ? rows[2] : rows[3];
+    const int64_t pitch = (op == 0 ? ld[0] : op == 1 ? ld[1] : op == 2 ? ld[2] : ld[3]) * int64_t(sizeof(T));
     x = static_cast<const char*>(from) + (op < r.ops ? sub * pitch : 0);
     step = pitch * r.per;
     bytes = uint32_t(cols * sizeof(T));
@@ -519,14 +536,16 @@ template <typename T> __device__ __forceinline__ uint32_t skew_of(const T* row) 
 
 // Many rows: as layernorm_backward_kernel, rows by bulk copies.  The block's
 // sums over its rows are joined across its `per` threads of a column at the end.
-template <typename T, int G, int ACCESS>
+template <typename T, int G, int ACCESS, bool SUM>
 __global__ void __launch_bounds__(512) layernorm_backward_ring_kernel(const NormBackArgs p, int per, int stages, int pitch) {
   extern __shared__ __align__(16) uint8_t ring_store[];
   __shared__ __align__(8) uint64_t bars[2 * kMostStages];
   __shared__ float2 sums[2][16];
   const int workers = per * p.tpr, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const T *grad = static_cast<const T*>(p.grad), *h = static_cast<const T*>(p.h), *gh = p.grad_x ? static_cast<const T*>(p.grad_h) : nullptr;
-  RowRing ring{umma::smem_u32(ring_store), umma::smem_u32(bars), umma::smem_u32(bars + kMostStages), stages, per, gh ? 3 : 2, pitch};
+  const T* res = SUM ? static_cast<const T*>(p.residual) : nullptr;
+  const int op_res = gh ? 3 : 2;   // its place in a stage
+  RowRing ring{umma::smem_u32(ring_store), umma::smem_u32(bars), umma::smem_u32(bars + kMostStages), stages, per, op_res + (SUM ? 1 : 0), pitch};
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; s++) {
       umma::bar_init(ring.full + 8 * s, 1);
@@ -536,7 +555,7 @@ __global__ void __launch_bounds__(512) layernorm_backward_ring_kernel(const Norm
   }
   after_previous_kernel();
   __syncthreads();
-  const RowCopies<ACCESS, T> copies(ring, p.cols, {grad, h, gh}, {p.ldg, p.ldh, p.ldgh});
+  const RowCopies<ACCESS, T> copies(ring, p.cols, {grad, h, gh || !SUM ? gh : res, res}, {p.ldg, p.ldh, gh || !SUM ? p.ldgh : p.ldr, p.ldr});
   auto bring = [&](int64_t batch, int stage) { copies(ring, p.rows, batch, stage); };
   if (warp == 0)
     for (int s = 0; s < stages && (blockIdx.x + int64_t(s) * gridDim.x) * per < p.rows; s++) bring(blockIdx.x + int64_t(s) * gridDim.x, s);
@@ -564,14 +583,16 @@ __global__ void __launch_bounds__(512) layernorm_backward_ring_kernel(const Norm
       uint64_t a[G][4], u[G][4], s = 0, su = 0;
       const uint32_t from = ring.at(stage, 0, sub) + 16 + (ACCESS == kAligned ? 0 : skew_of(grad + row * p.ldg));
       const uint32_t from_h = ring.at(stage, 1, sub) + 16 + (ACCESS == kAligned ? 0 : skew_of(h + row * p.ldh));
+      const uint32_t from_r = SUM ? ring.at(stage, op_res, sub) + 16 + (ACCESS == kAligned ? 0 : skew_of(res + row * p.ldr)) : 0;
 #pragma unroll
       for (int g = 0; g < G; g++) {
         const int c = at(g);
         if (c >= cols) continue;
-        Vec8<T> vg, vh;
+        Vec8<T> vg, vh, vr;
         take8<ACCESS>(vg, from + c * int(sizeof(T)));
         take8<ACCESS>(vh, from_h + c * int(sizeof(T)));
-        back_group<ACCESS>(vg, vh, w[g], c, cols, minus, rstd, a[g], u[g], dw[g], db[g], s, su);
+        if (SUM) take8<ACCESS>(vr, from_r + c * int(sizeof(T)));
+        back_group<ACCESS, SUM>(vg, vh, vr, w[g], c, cols, minus, rstd, a[g], u[g], dw[g], db[g], s, su);
       }
       if (p.grad_x) {
         float2 sums2 = join.two(make_float2(sum_of(s), sum_of(su)));
@@ -642,12 +663,19 @@ __global__ void __launch_bounds__(512) layernorm_backward_long_kernel(const Norm
     const float mean = p.mean[row], rstd = p.rstd[row];
     const T *grad = static_cast<const T*>(p.grad) + row * p.ldg, *h = static_cast<const T*>(p.h) + row * p.ldh;
     const T* gh = p.grad_h ? static_cast<const T*>(p.grad_h) + row * p.ldgh : nullptr;
+    const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.ldr : nullptr;
     auto load = [&](int64_t c, float (&a)[8], float (&u)[8]) {
       Vec8<T> v;
-      load_any(v, grad, c, p.cols);
-      v.get(a);
       load_any(v, h, c, p.cols);
       v.get(u);
+      if (res) {
+        load_any(v, res, c, p.cols);
+        v.get(a);
+#pragma unroll
+        for (int e = 0; e < 8; e++) u[e] += a[e];
+      }
+      load_any(v, grad, c, p.cols);
+      v.get(a);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const bool in = c + e < p.cols;
@@ -697,10 +725,16 @@ __global__ void __launch_bounds__(128) layernorm_columns_kernel(const NormBackAr
     const float mean = p.mean[row], rstd = p.rstd[row];
     Vec8<T> v;
     float a[8], u[8];
-    load_any(v, static_cast<const T*>(p.grad) + row * p.ldg, c, p.cols);
-    v.get(a);
     load_any(v, static_cast<const T*>(p.h) + row * p.ldh, c, p.cols);
     v.get(u);
+    if (p.residual) {
+      load_any(v, static_cast<const T*>(p.residual) + row * p.ldr, c, p.cols);
+      v.get(a);
+#pragma unroll
+      for (int e = 0; e < 8; e++) u[e] += a[e];
+    }
+    load_any(v, static_cast<const T*>(p.grad) + row * p.ldg, c, p.cols);
+    v.get(a);
 #pragma unroll
     for (int e = 0; e < 8; e++) {
       dw[e] = fmaf(a[e], (u[e] - mean) * rstd, dw[e]);
@@ -908,7 +942,7 @@ template <typename T> tg_status launch_backward(NormBackArgs p, T* grad_w, T* gr
   const bool lng = !in_registers(p.cols, access, kMost);
   RingPlan ring{};
   // by copies from a row per SM on (us, by copies / directly, bf16: 74 x 4096 11.2 / 9.6, 148 x 4096 11.2 / 11.8, 148 x 8192 16 / 21, 2400 x 8192 44 / 61)
-  if (p.rows >= sm_count()) ring = ring_plan(p.rows, p.cols, sizeof(T), p.grad_h && p.grad_x ? 3 : 2, access, kMost);
+  if (p.rows >= sm_count()) ring = ring_plan(p.rows, p.cols, sizeof(T), 2 + (p.grad_h && p.grad_x ? 1 : 0) + (p.residual ? 1 : 0), access, kMost);
   RowPlan r{};
   if (lng) p.slots = std::max<int64_t>(1, std::min<int64_t>(p.rows, 64));
   else if (ring.fits) { p.slots = ring.blocks; p.tpr = ring.tpr; }
@@ -937,8 +971,18 @@ template <typename T> tg_status launch_backward(NormBackArgs p, T* grad_w, T* gr
           if (s == TG_OK) launch_kernel(by_copies, unsigned(ring.blocks), ring.block, ring.smem, 0, st, p, ring.per, ring.stages, ring.pitch);
         }
       };
-      if ((ring.fits ? ring.groups : r.groups) == 1) go(tgb::layernorm_backward_kernel<T, 1, A>, tgb::layernorm_backward_ring_kernel<T, 1, A>);
-      else go(tgb::layernorm_backward_kernel<T, 2, A>, tgb::layernorm_backward_ring_kernel<T, 2, A>);
+      auto with = [&](auto g, auto sum) {
+        constexpr int G = decltype(g)::value;
+        constexpr bool SUM = decltype(sum)::value;
+        go(tgb::layernorm_backward_kernel<T, G, A, SUM>, tgb::layernorm_backward_ring_kernel<T, G, A, SUM>);
+      };
+      const bool one = (ring.fits ? ring.groups : r.groups) == 1;
+      using One = std::integral_constant<int, 1>;
+      using Two = std::integral_constant<int, 2>;
+      if (p.residual && one) with(One{}, std::true_type{});
+      else if (p.residual) with(Two{}, std::true_type{});
+      else if (one) with(One{}, std::false_type{});
+      else with(Two{}, std::false_type{});
     });
   }
   if (scratch && s == TG_OK)
@@ -977,9 +1021,10 @@ tg_status tg_blocks8_layernorm(tg_dtype dtype, int64_t rows, int64_t cols, const
   return norm_forward(dtype, p, static_cast<cudaStream_t>(stream));
 }
 
-tg_status tg_layernorm_backward(tg_dtype dtype, int64_t rows, int64_t cols, const void* grad, int64_t ldg, const void* grad_h,
-                                int64_t ldgh, const void* weight, const void* h, int64_t ldh, const float* mean,
-                                const float* rstd, void* grad_x, int64_t ldx, void* grad_weight, void* grad_bias, void* stream) {
+tg_status tg_layernorm_residual_backward(tg_dtype dtype, int64_t rows, int64_t cols, const void* grad, int64_t ldg, const void* grad_h,
+                                         int64_t ldgh, const void* weight, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                                         const float* mean, const float* rstd, void* grad_x, int64_t ldgx, void* grad_weight, void* grad_bias,
+                                         void* stream) {
   clear_error();
   TG_CHECK(check_type(dtype));
   TG_CHECK(check_shape(rows, cols));
@@ -992,26 +1037,35 @@ tg_status tg_layernorm_backward(tg_dtype dtype, int64_t rows, int64_t cols, cons
     }
     return TG_OK;
   }
-  if (!grad || !h || !mean || !rstd) return fail(TG_ERR_INVALID_ARGUMENT, "null operand");
+  if (!grad || !x || !mean || !rstd) return fail(TG_ERR_INVALID_ARGUMENT, "null operand");
   TG_CHECK(check_pitch("ldg", grad, ldg, cols));
   TG_CHECK(check_pitch("ldgh", grad_h, ldgh, cols));
-  TG_CHECK(check_pitch("ldh", h, ldh, cols));
-  TG_CHECK(check_pitch("ldx", grad_x, ldx, cols));
+  TG_CHECK(check_pitch(residual ? "ldx" : "ldh", x, ldx, cols));
+  TG_CHECK(check_pitch("ldr", residual, ldr, cols));
+  TG_CHECK(check_pitch(residual ? "ldgx" : "ldx", grad_x, ldgx, cols));
   NormBackArgs p{};
   p.rows = rows; p.cols = cols; p.grad = grad; p.ldg = ldg; p.grad_h = grad_h; p.ldgh = ldgh; p.weight = weight;
-  p.h = h; p.ldh = ldh; p.mean = mean; p.rstd = rstd; p.grad_x = grad_x; p.ldx = ldx;
+  p.h = x; p.ldh = ldx; p.residual = residual; p.ldr = ldr; p.mean = mean; p.rstd = rstd; p.grad_x = grad_x; p.ldx = ldgx;
   const size_t e = elem8_size(dtype);
   RowAccess access(cols);
   access.add(grad, ldg, e);
   access.add(grad_h, ldgh, e);
-  access.add(h, ldh, e);
-  access.add(grad_x, ldx, e);
+  access.add(x, ldx, e);
+  access.add(residual, ldr, e);
+  access.add(grad_x, ldgx, e);
   int how = access.get();
   if (how == tg8::kAligned && !aligned(weight, 16)) how = tg8::kScalar;
   return with_type8(dtype, [&](auto t) {
     using T = decltype(t);
     return launch_backward<T>(p, static_cast<T*>(grad_weight), static_cast<T*>(grad_bias), how, st);
   });
+}
+
+tg_status tg_layernorm_backward(tg_dtype dtype, int64_t rows, int64_t cols, const void* grad, int64_t ldg, const void* grad_h,
+                                int64_t ldgh, const void* weight, const void* h, int64_t ldh, const float* mean,
+                                const float* rstd, void* grad_x, int64_t ldx, void* grad_weight, void* grad_bias, void* stream) {
+  return tg_layernorm_residual_backward(dtype, rows, cols, grad, ldg, grad_h, ldgh, weight, h, ldh, nullptr, 0, mean, rstd, grad_x, ldx, grad_weight,
+                                        grad_bias, stream);
 }
 
 }  // extern "C"

@@ -220,26 +220,27 @@ std::tuple<Tensor, Tensor, Tensor> layernorm_blocks8(const Tensor& x, const OptT
 }
 
 std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& grad, const Tensor& h, const Tensor& mean, const Tensor& rstd, const Tensor& weight,
-                                                 const Tensor& grad_h, bool want_x, bool want_weight, bool want_bias) {
+                                                 const Tensor& grad_h, const Tensor& residual, bool want_x, bool want_weight, bool want_bias) {
   const tg_dtype code = type(h.scalar_type(), "h");
   const at::Device dev = grad.device();
-  on(dev, {&h, &mean, &rstd, &weight, &grad_h});
+  on(dev, {&h, &mean, &rstd, &weight, &grad_h, &residual});
   const int64_t k = h.dim() ? h.size(-1) : 0;
   if (k == 0) refuse("h needs at least one column");
   check_like(grad, h, "grad", "h");
   check_like(grad_h, h, "grad_h", "h");
+  check_like(residual, h, "residual", "h");
   check_columns(weight, h, k, "weight");
   check_row_values(mean, h, "mean");
   check_row_values(rstd, h, "rstd");
   c10::cuda::CUDAGuard guard(dev);
-  const Flat gf(grad), hf(h), ghf(grad_h);
+  const Flat gf(grad), hf(h), ghf(grad_h), rf(residual);
   const Tensor w = dense(weight), mu = dense(mean), r = dense(rstd);
   Tensor grad_x, grad_w, grad_b;
   if (want_x) grad_x = make(h.sizes(), h, h.scalar_type());
   if (want_weight) grad_w = make({k}, h, h.scalar_type());
   if (want_bias) grad_b = make({k}, h, h.scalar_type());
-  check(tg_layernorm_backward(code, rows_of(h), k, gf.ptr(), gf.ld, ghf.ptr(), ghf.ld, ptr(w), hf.ptr(), hf.ld, f32(mu), f32(r), ptr(grad_x), k,
-                              ptr(grad_w), ptr(grad_b), stream(dev)));
+  check(tg_layernorm_residual_backward(code, rows_of(h), k, gf.ptr(), gf.ld, ghf.ptr(), ghf.ld, ptr(w), hf.ptr(), hf.ld, rf.ptr(), rf.ld, f32(mu), f32(r),
+                                       ptr(grad_x), k, ptr(grad_w), ptr(grad_b), stream(dev)));
   return {grad_x, grad_w, grad_b};
 }
 
@@ -275,7 +276,9 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                                                 const OptTensor& residual, double eps, bool train) {
     const Norm r = norm(x, or_none(weight), or_none(bias), or_none(residual), eps, train, false);
     if (train) {
-      ctx->save_for_backward({residual ? r.h : x, r.mean, r.rstd, or_none(weight)});
+      // h in 16 bits is the sum rounded: the backward takes its parts
+      const bool parts = residual && x.scalar_type() != at::kFloat;
+      ctx->save_for_backward({residual && !parts ? r.h : x, r.mean, r.rstd, or_none(weight), parts ? *residual : Tensor()});
       ctx->saved_data["needs"] = std::vector<int64_t>{wants(x), wants(or_none(weight)), wants(or_none(bias)), wants(or_none(residual))};
       ctx->set_materialize_grads(false);
     }
@@ -288,7 +291,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const Tensor &grad_y = grads[0], &grad_h = grads[1];
     Tensor grad_x, grad_w, grad_b;
     if (grad_y.defined())
-      std::tie(grad_x, grad_w, grad_b) = norm_backward(grad_y, saved[0], saved[1], saved[2], saved[3], grad_h, needs[0] || needs[3], needs[1], needs[2]);
+      std::tie(grad_x, grad_w, grad_b) = norm_backward(grad_y, saved[0], saved[1], saved[2], saved[3], grad_h, saved[4], needs[0] || needs[3], needs[1], needs[2]);
     else
       grad_x = grad_h;
     const Tensor none;
@@ -451,8 +454,9 @@ std::tuple<Tensor, Tensor> token_logprobs_grad(const Tensor& logits, const Tenso
 PYBIND11_MODULE(_layers_torch, m) {
   m.def("layernorm", &layernorm);
   m.def("layernorm_blocks8", &layernorm_blocks8);
-  m.def("layernorm_backward", [](const Tensor& grad, const Tensor& h, const Tensor& mean, const Tensor& rstd, const OptTensor& weight, const OptTensor& grad_h) {
-    return norm_backward(grad, h, mean, rstd, or_none(weight), or_none(grad_h), true, true, true);
+  m.def("layernorm_backward", [](const Tensor& grad, const Tensor& h, const Tensor& mean, const Tensor& rstd, const OptTensor& weight, const OptTensor& grad_h,
+                                  const OptTensor& residual) {
+    return norm_backward(grad, h, mean, rstd, or_none(weight), or_none(grad_h), or_none(residual), true, true, true);
   });
   m.def("layernorm_grad", &layernorm_grad);
   m.def("quantize", &quantize);

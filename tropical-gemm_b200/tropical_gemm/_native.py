@@ -70,6 +70,7 @@ def lib() -> ctypes.CDLL:
             "tg_rows8_column_sum": [i32, i32, i64, i64, vp, i64, vp, vp],
             "tg_layernorm": [i32, i64, i64, vp, i64, vp, i64, vp, vp, f32, vp, i64, vp, i64, vp, vp, vp],
             "tg_layernorm_backward": [i32, i64, i64, vp, i64, vp, i64, vp, vp, i64, vp, vp, vp, i64, vp, vp, vp],
+            "tg_layernorm_residual_backward": [i32, i64, i64, vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, vp, vp, i64, vp, vp, vp],
             "tg_blocks8_quantize": [i32, i64, i64, vp, i64, vp, i64, vp, i64, i64, vp, i64, vp, i64, i64, vp, vp],
             "tg_blocks8_quantize_tiles": [i32, i64, i64, vp, i64, vp, i64, vp, i64, i64, vp, i64, vp],
             "tg_blocks8_transpose": [i64, i64, vp, i64, vp, i64, vp],

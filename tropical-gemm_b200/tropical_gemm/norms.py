@@ -38,11 +38,17 @@ def layernorm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opti
 
 
 def layernorm_backward(grad: torch.Tensor, h: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight: Optional[torch.Tensor] = None,
-                       grad_h: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                       grad_h: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients of `layernorm` with respect to x (and residual: the same),
     weight and bias, from the gradients of y and of h; all of h's type.  The
-    sums over rows are float32 in a fixed order."""
-    return _x().layernorm_backward(grad, h, mean, rstd, weight, grad_h)
+    sums over rows are float32 in a fixed order.
+
+    With `residual`, `h` is the x that `layernorm` was given beside it, and their
+    sum is formed in float32 as there.  The h that `layernorm` gives is that sum
+    rounded to its type; taken in its place, a 16-bit one puts an error of half a
+    step of h, over the row's spread, into (h - mean) rstd.  A float32 h is the
+    sum itself and needs no parts."""
+    return _x().layernorm_backward(grad, h, mean, rstd, weight, grad_h, residual)
 
 
 __all__ = ["LayerNorm", "layernorm", "layernorm_backward"]

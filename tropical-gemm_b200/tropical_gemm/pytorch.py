@@ -195,8 +195,9 @@ def rmsnorm_linear_rows8(x: torch.Tensor, norm_weight: torch.Tensor, weight, res
 def layernorm(x: torch.Tensor, weight=None, bias=None, residual=None, eps: float = 1e-5):
     """(y, h): h = x + residual, y = (h - mean) / sqrt(variance + eps) * weight + bias
     over the last dimension, with autograd (`norms.layernorm`).  Kept for the
-    backward: h and two float32 values per row.  Gradients cannot be
-    differentiated again.  (A call that is captured into a CUDA graph refuses
+    backward: two float32 values per row and h, or, where h is rounded (16-bit
+    types with a residual), x and residual in its place, neither of which may
+    then be changed before it.  Gradients cannot be differentiated again.  (A call that is captured into a CUDA graph refuses
     leaves whose autograd graph of another stream is still alive; so do the two
     below.)"""
     return _layers.ext().layernorm_grad(x, weight, bias, residual, eps)
