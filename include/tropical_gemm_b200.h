@@ -290,9 +290,10 @@ tg_status tg_rows8_column_sum(tg_dtype dtype, tg_dtype out_dtype, int64_t rows, 
  * with a row's mean and rstd = 1 / sqrt(variance + eps), the variance being the
  * mean square of h - mean.  All arithmetic is f32 on the unrounded sum; x,
  * residual, weight, bias, h and y are of type dtype.  residual, weight (ones),
- * bias (zeros), h, mean and rstd may be null, mean and rstd together.  Finite
- * rows whose squared distances from the mean pass f32's range (from about 1e19
- * on) have rstd 0. */
+ * bias (zeros), h, mean and rstd may be null, mean and rstd together.  Rows of
+ * magnitudes up to 2^126 have finite statistics: where the squares of h - mean
+ * add up to more than f32 holds (distances from about 1e19 / sqrt(cols) on),
+ * rstd is 0, y is the bias, and grad_x is grad_h. */
 tg_status tg_layernorm(tg_dtype dtype, int64_t rows, int64_t cols,
                        const void* x, int64_t ldx, const void* residual, int64_t ldr,
                        const void* weight, const void* bias, float eps,

@@ -110,8 +110,10 @@ template <int ACCESS, typename T> __device__ __forceinline__ void load_columns(V
 
 // Mean and rstd from the row's mean (the sum's, rounded), the sum of h - mean and
 // of its square: what the rounding of the first mean left is taken out again.
+// Squares that pass f32's range say that rstd is 0; the sum beside them may have
+// passed it too, in both directions, and is left out.
 __device__ __forceinline__ float2 finish_stats(float mean, float2 off, float inv_cols, float eps) {
-  const float d = off.x * inv_cols;
+  const float d = off.y == __int_as_float(0x7f800000) ? 0.f : off.x * inv_cols;
   float var = fmaf(off.y, inv_cols, -d * d);
   if (var < 0.f) var = 0.f;   // a NaN stays
   return make_float2(mean + d, rsqrtf(var + eps));   // within two units of the last place
@@ -135,14 +137,15 @@ __device__ __forceinline__ void store_block(const NormArgs& p, int64_t row, int6
 template <int G, int ACCESS>
 __device__ __forceinline__ float2 row_stats(const uint64_t (&v)[G][4], int tpr, int t, int shift, int cols, float inv_cols, float eps, RowSums& join) {
   auto at = [&](int g) { return (g * tpr + t) * 8 - shift; };
-  uint64_t sum = 0;
+  uint64_t sum = 0;   // of h / cols, which stays within f32's range where h does
+  const uint64_t share = pair_of(inv_cols);
 #pragma unroll
   for (int g = 0; g < G; g++) {
     if (at(g) >= cols) continue;
 #pragma unroll
-    for (int i = 0; i < 4; i++) sum = add_pair(sum, v[g][i]);
+    for (int i = 0; i < 4; i++) fma_pair(sum, v[g][i], share);
   }
-  const float rough = join.one(sum_of(sum)) * inv_cols;
+  const float rough = join.one(sum_of(sum));
   const uint64_t minus = pair_of(-rough);
   uint64_t off = 0, square = 0;
 #pragma unroll
@@ -279,9 +282,9 @@ __global__ void __launch_bounds__(512) layernorm_long_kernel(const NormArgs p) {
       float v[8];
       load(c, v);
 #pragma unroll
-      for (int e = 0; e < 8; e++) sum += c + e < p.cols ? v[e] : 0.f;
+      for (int e = 0; e < 8; e++) sum = fmaf(c + e < p.cols ? v[e] : 0.f, inv_cols, sum);
     }
-    const float rough = join.one(sum) * inv_cols;
+    const float rough = join.one(sum);
     float2 off = make_float2(0.f, 0.f);
     for (int64_t i = 0; i < last; i++) {
       const int64_t c = (i * 512 + threadIdx.x) * 8;
