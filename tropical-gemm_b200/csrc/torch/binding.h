@@ -4,6 +4,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -110,8 +111,15 @@ void check(tg_status s) {
   py::module_::import("tropical_gemm._native").attr("check")(int(s));
 }
 
-// Outputs, on like's device: CUDA tensors only, so torch's choice of a backend (0.4 us each) is left out.
-Tensor make(at::IntArrayRef sizes, const Tensor& like, at::ScalarType t) { return Tensor(at::detail::empty_cuda(sizes, t, like.device(), std::nullopt)); }
+// Whether somebody is to see a new tensor: a dispatch mode that watches calls, or
+// the deterministic mode's filling of what is not written.
+bool watched() { return c10::impl::dispatch_mode_enabled() || at::globalContext().deterministicAlgorithms(); }
+// Outputs, on like's device: CUDA tensors only, so torch's choice of a backend
+// (0.4 us each) is left out where nobody watches it.
+Tensor make(at::IntArrayRef sizes, const Tensor& like, at::ScalarType t) {
+  if (watched()) return at::empty(sizes, like.options().dtype(t).requires_grad(false));
+  return Tensor(at::detail::empty_cuda(sizes, t, like.device(), std::nullopt));
+}
 
 at::DimVector with_last(const Tensor& t, int64_t last) {
   at::DimVector v(t.sizes().begin(), t.sizes().end());

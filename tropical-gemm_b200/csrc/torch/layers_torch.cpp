@@ -45,6 +45,7 @@ Tensor make_scales(at::IntArrayRef sizes, const Tensor& like) {
     rows *= sizes[i];
   }
   stride.back() = std::max<int64_t>(rows, 1);
+  if (watched()) return at::empty_strided(size, stride, like.options().dtype(at::kFloat).requires_grad(false));
   return Tensor(at::detail::empty_strided_cuda(size, stride, at::kFloat, like.device()));
 }
 int64_t pitch(const Tensor& q) { return q.size(-1) == 0 ? 0 : (q.size(-1) + 15) / 16 * 16; }   // of make_codes
