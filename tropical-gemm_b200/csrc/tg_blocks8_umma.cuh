@@ -301,9 +301,9 @@ blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       const int64_t row0 = item.m0 + rank * 128 + w * 32, col0 = item.n0 + half * 128;
       const bool parts = p.splits > 1;
       if (!parts) {
-        asm volatile("bar.sync 1, 256;" ::: "memory");   // the last tile's bias is no longer read
+        named_sync(1, 256);   // the last tile's bias is no longer read
         bias[tid] = p.bias && item.n0 + tid < p.n ? to_f32(static_cast<const T*>(p.bias)[item.n0 + tid]) : 0.f;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        named_sync(1, 256);
       }
       float acc[128];
       auto taken = [&](int buf) {   // the next sum may have the accumulator

@@ -36,7 +36,7 @@ struct RowSums {
     if (tpr > 32) {
       const int warps = tpr >> 5, first = sub * warps;
       if ((threadIdx.x & 31) == 0) sums[turn][threadIdx.x >> 5] = s;
-      asm volatile("bar.sync %0, %1;" ::"r"(sub + 1), "r"(tpr) : "memory");
+      named_sync(sub + 1, tpr);
       const float2* from = &sums[turn][first];
       turn ^= 1;
       uint64_t all = pair_of(from[0].x, from[0].y);
@@ -641,15 +641,15 @@ __global__ void __launch_bounds__(512) layernorm_backward_ring_kernel(const Norm
       for (int e = 0; e < 8; e++)
         if (inside<kShifted>(at(g), e, cols)) store[sub * cols + at(g) + e] = ok ? f[e] : __uint_as_float(0x7fffffffu);
     }
-    asm volatile("bar.sync 15, %0;" ::"r"(workers) : "memory");
+    named_sync(15, workers);
     for (int c = threadIdx.x; c < cols; c += workers) {
       float sum = 0.f;
       for (int i = 0; i < per; i++) sum += store[i * cols + c];
       partial[int64_t(blockIdx.x) * p.cols + c] = sum;
     }
-    asm volatile("bar.sync 15, %0;" ::"r"(workers) : "memory");
+    named_sync(15, workers);
   };
-  if (p.partial_w || p.partial_b) asm volatile("bar.sync 15, %0;" ::"r"(workers) : "memory");
+  if (p.partial_w || p.partial_b) named_sync(15, workers);
   join_columns(dw, p.partial_w);
   join_columns(db, p.partial_b);
 }

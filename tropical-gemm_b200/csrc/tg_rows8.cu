@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(G == 1 ? 1024 : 512) rows_kernel(RowArgs p) {
 struct RowJoin {
   float4 (*stats)[16];   // [2][warps of the block]
   int tpr, sub, turn;
-  __device__ __forceinline__ void barrier() const { asm volatile("bar.sync %0, %1;" ::"r"(sub + 1), "r"(tpr) : "memory"); }
+  __device__ __forceinline__ void barrier() const { named_sync(sub + 1, tpr); }
   __device__ __forceinline__ RowStats operator()(RowStats s) {
 #pragma unroll
     for (int d = 16; d; d >>= 1) s.sum += __shfl_xor_sync(0xffffffffu, s.sum, d);

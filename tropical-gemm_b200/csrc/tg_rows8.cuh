@@ -206,6 +206,13 @@ __device__ __forceinline__ void bytes_f32(uint2 w, float (&v)[8]) {
   v[4] = byte_f32<0>(b); v[5] = byte_f32<1>(b); v[6] = byte_f32<2>(b); v[7] = byte_f32<3>(b);
 }
 
+// Barrier `id` of the block's (1 to 15), for `threads` of them in whole warps whose
+// lanes it wants together: a store by one lane before need not have left them so.
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  __syncwarp();
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 // Kernels of these calls are launched with programmatic stream serialisation:
 // a kernel may be set up while the one before it ends, waits here before it
 // touches global memory until that one is complete, and lets the next one be

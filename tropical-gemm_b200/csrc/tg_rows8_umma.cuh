@@ -418,11 +418,11 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         if (++h == item.halves) { h = 0; ch++; }
         float rs = 0.f;
         if (MODE == kForward && p.splits == 1) {
-          asm volatile("bar.sync 1, 256;" ::: "memory");   // the last tile's columns are no longer read
+          named_sync(1, 256);   // the last tile's columns are no longer read
           const bool in = n0 + tid < p.n;
           cols[tid] = in ? p.col_scale[n0 + tid] : 0.f;
           cols[kTile + tid] = in && p.bias ? to_f32(static_cast<const T*>(p.bias)[n0 + tid]) : 0.f;
-          asm volatile("bar.sync 1, 256;" ::: "memory");
+          named_sync(1, 256);
           if (row < p.m) rs = p.row_scale[row];
         }
         if (ok) {   // a whole sum: the limit grows with its length
