@@ -623,7 +623,12 @@ __global__ void __launch_bounds__(512) layernorm_backward_ring_kernel(const Norm
     if (lane == 0) umma::bar_arrive(ring.empty + 8 * stage);
     const int64_t ahead = batch + int64_t(stages) * gridDim.x;
     if (warp == 0 && ahead * per < p.rows) {
+      // Waits may run out in some lanes alone.  Rows off the boundaries add up their
+      // bytes across the warp, so its lanes go on by vote; whole ones have a
+      // __syncwarp there, which lanes that gave up meet in the next turn (a vote here
+      // would take 5 us of 106, 8192 x 8192 bf16).
       if (ok) ok = umma::bar_wait(ring.empty + 8 * stage, parity);
+      if (ACCESS != kAligned) ok = __all_sync(0xffffffffu, ok);
       if (ok) bring(ahead, stage);
     }
     if (++stage == stages) { stage = 0; parity ^= 1; }
