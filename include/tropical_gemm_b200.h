@@ -339,7 +339,7 @@ tg_status tg_layernorm_residual_backward(tg_dtype dtype, int64_t rows, int64_t c
  * scale's mantissa, and with a power of two the rounding to 8 bits is the only
  * one.  A block that holds a NaN or an infinity gets scale NaN, so that
  * everything made of it is NaN.  The products take any f32 scales; two scales
- * that meet may be multiplied first, so their product lies within f32's range.
+ * that meet are multiplied first, so their product lies within f32's range.
  * Where all scales of a product are powers of two (or NaN) the tensor core
  * applies them itself; which way is taken is decided on the device.
  * ------------------------------------------------------------------------ */

@@ -371,7 +371,7 @@ blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 float k[4] = {1.f, 1.f, 1.f, 1.f};
                 if (ROWS) asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(k[0]), "=f"(k[1]), "=f"(k[2]), "=f"(k[3]) : "r"(mine + (c + e) * 4));
 #pragma unroll
-                for (int q = 0; q < 4; q++) acc[c + e + q] = ROWS ? fmaf(__uint_as_float(t[e + q]) * s, k[q], acc[c + e + q]) : fmaf(__uint_as_float(t[e + q]), s, acc[c + e + q]);
+                for (int q = 0; q < 4; q++) acc[c + e + q] = fmaf(__uint_as_float(t[e + q]), ROWS ? s * k[q] : s, acc[c + e + q]);   // the scales first: a sum of 2^24 and one scale may pass f32's range
               }
             }
           }
@@ -606,8 +606,9 @@ __global__ void __launch_bounds__(192) blocks_few_kernel(const __grid_constant__
         for (int j = 0; j < kChunk / 4; j++) {
           uint64_t c0, c1;
           load_pairs(mine + (c + 4 * j) * 4, c0, c1);
-          fma_pair(acc[c / 2 + 2 * j], mul_pair(pair_of(t[4 * j], t[4 * j + 1]), w2), c0);
-          fma_pair(acc[c / 2 + 2 * j + 1], mul_pair(pair_of(t[4 * j + 2], t[4 * j + 3]), w2), c1);
+          // the scales first: a sum of 2^24 and one scale may pass f32's range
+          fma_pair(acc[c / 2 + 2 * j], pair_of(t[4 * j], t[4 * j + 1]), mul_pair(c0, w2));
+          fma_pair(acc[c / 2 + 2 * j + 1], pair_of(t[4 * j + 2], t[4 * j + 3]), mul_pair(c1, w2));
         }
       }
       if (++buf == S::kBufs) { buf = 0; turn ^= 1; }
