@@ -7,6 +7,7 @@ import torch
 
 import tropical_gemm.pytorch as tp
 from tropical_gemm import blocks8, logprobs, norms
+from tropical_gemm.blocks8 import Blocks8
 from _layer_forms import HALF, TINY, TYPES, close, tokens as form
 from test_gpu_layernorm_sums import check as check_gradients
 from test_gpu_logprobs import check as check_tokens, floor
@@ -176,3 +177,43 @@ def test_bias_gradient(rows, n, dtype):
     x, w, b, g = normal(rows, 24, dtype=dtype), normal(n, 24, dtype=dtype), normal(n, dtype=dtype).requires_grad_(True), normal(rows, n, dtype=dtype, seed=1)
     (gb,) = torch.autograd.grad(tp.linear_blocks8(x, w, b), b, g)
     close(gb, g.double().sum(0), 1.01 * HALF[dtype], 64 * F32 * g.double().abs().sum(0) + TINY[dtype])
+
+
+# ------------------------------------------------------------------------------------------ offsets that pass 32 bits
+def test_more_than_two_to_the_31_elements():
+    """Rows far into a tensor are as they are alone.  70000 x 32768, 4.3 GiB; the slice has its own many rows, so that the same kernels take it."""
+    rows, cols, last = 70000, 32768, 2000
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    for i in range(0, rows, 10000):
+        x[i:i + 10000] = normal(10000, cols, dtype=torch.bfloat16, seed=i)
+    tail = x[rows - last:].clone()
+    ids = torch.arange(rows, device="cuda") % cols
+    r, s = logprobs.token_logprobs(x, ids, top=4), logprobs.token_logprobs(tail, ids[rows - last:], top=4)
+    assert all(torch.equal(p[rows - last:], q) for p, q in zip(r, s))
+    one = torch.ones(rows, device="cuda")
+    g = logprobs.token_logprobs_backward(x, ids, r.stats, r.entropy, one, one)[rows - last:].clone()
+    assert torch.equal(g, logprobs.token_logprobs_backward(tail, ids[rows - last:], s.stats, s.entropy, one[:last], one[:last]))
+    del r, g
+    for c in (cols, 4096):   # a row too long for registers, and eight times as many shorter ones
+        v, t = x.view(-1, c), tail.view(-1, c)
+        n = t.size(0)
+        a, b = norms.layernorm(v, residual=v, stats=True), norms.layernorm(t, residual=t, stats=True)
+        assert torch.equal(a.y[-n:], b.y) and torch.equal(a.h[-n:], b.h) and torch.equal(a.rstd[-n:], b.rstd)
+        p = norms.layernorm_backward(v, v, a.mean, a.rstd, None, v, residual=v)[0][-n:].clone()
+        assert torch.equal(p, norms.layernorm_backward(t, t, b.mean, b.rstd, None, t, residual=t)[0])
+        del a, b, p
+    e, f = blocks8.layernorm(x).blocks, blocks8.layernorm(tail).blocks
+    assert torch.equal(e.q[rows - last:].view(torch.uint8), f.q.view(torch.uint8)) and torch.equal(e.scale[rows - last:], f.scale)
+    a, t = blocks8.quantize_both(x)
+    b = blocks8.quantize(tail)
+    assert torch.equal(a.q[rows - last:].view(torch.uint8), b.q.view(torch.uint8)) and torch.equal(a.scale[rows - last:], b.scale)
+    half = rows // 2 // 128 * 128
+    u = blocks8.quantize_both(x[half:])[1]
+    assert torch.equal(t.q[:, half:].contiguous().view(torch.uint8), u.q.contiguous().view(torch.uint8)) and torch.equal(t.scale[:, half // 128:], u.scale)
+    w = blocks8.quantize_tiles(torch.eye(128, cols, device="cuda"))
+    z = blocks8.matmul(a, w)
+    assert torch.equal(z[rows - last:], blocks8.matmul(b, w))
+    turned = blocks8.transpose(Blocks8(a.q, torch.ones(-(-rows // 128), cols // 128, device="cuda")))
+    assert torch.equal(turned.q[-300:, -300:].float(), a.q[-300:, -300:].float().t())
+    d = blocks8.dequantize(a)
+    assert torch.equal(d[rows - last:], blocks8.dequantize(b))
