@@ -13,13 +13,15 @@ namespace {
 // How a product is done, and what it is expected to take (us, on a B200).  The
 // few-token kernel reads 128 rows of B per CTA and block, at the rate of one SM's
 // way from L2.  The paired kernel does 256 x 256 in the time that an SM's tensor
-// core needs, but its call is three launches.  Measured (bf16 outputs, us, few / pairs):
-// 333 x 1531 x 1111 5.6 / 16.3, 256 x 4096 x 4096 15.6 / 21.3, 1024 x 1024 x 4096 15.7 / 21.1,
-// 512 x 4096 x 4096 30 / 20.6; the constants are fitted to such pairs and choose the
-// faster of each.
+// core needs, but its call is two launches (packing the scales and the product),
+// three where a sum is split.  Measured (bf16 outputs, operands in L2, us, few /
+// pairs): 333 x 1531 x 1111 5.6 / 16.3, 256 x 4096 x 4096 15.6 / 21.3,
+// 1024 x 1024 x 4096 15.7 / 21.1, 512 x 4096 x 4096 30 / 20.6; the constants are fitted
+// to such pairs and choose the faster of each.  Operands that come from memory have
+// no term of their own.
 // us per launch and per block of 16, 32 and 64 tokens
 constexpr double kFewBase[] = {2.3, 2.8, 4.2}, kFewBlock[] = {0.22, 0.245, 0.34};
-// us per call and per block of the paired kernel (its call is three launches)
+// us per call (two launches; kJoin is the third) and per block of the paired kernel
 constexpr double kPairBase = 9.0, kPairBlock = 0.28, kPairTile = 0.5, kJoin = 2.5;
 struct Plan {
   int tokens = 0;   // per tile of the few-token kernel, 0: pairs

@@ -88,7 +88,8 @@ __device__ __forceinline__ bool other_scales(const int* other) { return __syncth
 // With other scales each block goes into an accumulator of its own, of two in
 // turn, which the epilogue scales and adds up: a hand-over of 800 cycles and 500
 // of reads and arithmetic per block of 512, so this takes about twice as long
-// (8192^3 bf16: 0.39 and 0.76 ms).
+// (8192^3 bf16: 0.39 and 0.76 ms), and with a scale for each of B's rows, which is
+// read from shared memory and multiplied for each output and block, 1.76 ms.
 //
 // What bounds it: power (8192^3 2.8 PFLOP/s, operands of zeros 3.8); 4096^3, 56 us, is
 // 256 tiles on 74 pairs, four rounds for 3.46.
@@ -242,7 +243,7 @@ blocks_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
               const uint32_t off = at.slot * (S::kStage >> 4), id = idesc | umma::scale_byte(j);
               if (issue) {
 #pragma unroll
-                for (int q = 0; q < 4; q++) umma::mma_f8_scaled<2>(tmem, da0 + (off + q * 2), db0 + (off + q * 2), id, sa, sa + 4, !first || q);
+                for (int q = 0; q < 4; q++) umma::mma_f8_scaled(tmem, da0 + (off + q * 2), db0 + (off + q * 2), id, sa, sa + 4, !first || q);
                 umma::mma_commit<2>(empty(at.slot));
                 if (j + 1 == blocks) umma::mma_commit<2>(scales_empty(sc.slot));
                 if (left == 0) umma::mma_commit<2>(acc_full(0));
@@ -451,8 +452,8 @@ __global__ void __launch_bounds__(256) blocks_bias_kernel(const ProductArgs8 p) 
 // shared memory.  Four epilogue warps, one row of B per thread.
 //
 // What bounds it: launch and set-up where the weights are few (1 x 4096 x 4096
-// 5.0 us, their read 2.6), then what an SM takes from memory: one step of 16 KB of
-// weights per 0.22 us and CTA (16 x 8192 x 4096 8.0 us, floor 5.2).
+// 5.1 us, their read 2.6), then what an SM takes from memory: one step of 16 KB of
+// weights per 0.22 us and CTA (16 x 8192 x 4096 8.1 us, floor 5.2).
 //
 // A CTA that waits for its cluster must not wait for tensor memory held by one
 // that waits for another cluster: with split > 1 a CTA asks for more than half

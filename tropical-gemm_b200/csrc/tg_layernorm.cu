@@ -4,11 +4,14 @@
 //   h = x + residual, u = (h - mean) rstd, y = u weight + bias
 //   grad_x = rstd (a - mean(a) - u mean(a u)) + grad_h,  a = grad weight
 //
-// All are bound by memory: a row is read once, kept in registers between its
-// sums and its output, and written once.  The backward's rows, of three operands
-// beside the columns' sums, come by bulk copies into a ring in shared memory where
-// there are many, which keeps more of them on the way than registers could
-// (8192 x 8192 bf16 104 us, loaded directly 389 with f32 arithmetic one by one).
+// All are bound by memory.  A row that fits registers is read once, kept there
+// between its sums and its output, and written once; a longer one (forward: f32
+// above 8192 columns, 16-bit above 16384; backward: above 8192) is read three times.
+// The backward's rows, of two to four operands beside the columns' sums, come by
+// bulk copies into a ring in shared memory where there are many, which keeps more
+// of them on the way than registers could (8192 x 8192 bf16, us: grad, h and grad_h
+// 106; with h's parts in its place, four operands, 117; three loaded directly 389
+// with f32 arithmetic one by one).
 #include <algorithm>
 #include "tg_blocks8.cuh"
 #include "tg_umma.cuh"
@@ -23,7 +26,7 @@ struct NormArgs {
   float *scale, *mean, *rstd;
   int64_t ldx, ldr, ldh, ldy, ldq, scale_row, scale_block;
   float eps;
-  int tpr;                    // threads per row: 32 .. 512, a power of two
+  int tpr;                    // threads per row: 32 .. 512, a multiple of 32
 };
 
 // Sums over the tpr threads of a row (a multiple of 32), one or two at a time:

@@ -204,15 +204,11 @@ template <int CTAS> __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t 
 // the lanes); the instruction descriptor chooses the byte.
 __host__ __device__ constexpr uint32_t instr_desc_scaled(uint32_t m, uint32_t n) { return (n >> 3) << 17 | 1u << 23 | (m >> 7) << 27; }
 __host__ __device__ constexpr uint32_t scale_byte(uint32_t byte) { return byte << 4 | byte << 29; }
-template <int CTAS>
+// Issued by the leader of a pair of CTAs.
 __device__ __forceinline__ void mma_f8_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, bool accumulate) {
   const uint32_t acc = accumulate;
-  if constexpr (CTAS == 2)
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n}\n"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(sa), "r"(sb) : "memory");
-  else
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n}\n"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(sa), "r"(sb) : "memory");
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n}\n"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(sa), "r"(sb) : "memory");
 }
 // Columns of this warp's 32 lanes from registers.
 __device__ __forceinline__ void tmem_store4(uint32_t addr, const uint32_t (&r)[4]) {

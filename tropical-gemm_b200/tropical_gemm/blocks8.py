@@ -17,8 +17,9 @@ The quantising calls take powers of two as scales, the least that brings a
 block's largest magnitude to 448 or below, and round to nearest even, so that a
 code is one rounding of its value.  A block that holds a NaN or an infinity has
 scale NaN: what is made of it is NaN.  The products take any float32 scales
-(the product of two that meet within float32's range) and are about twice as
-fast where all are powers of two, which is found out on the device.
+(the product of two that meet within float32's range).  Where all are powers of
+two, which is found out on the device, those of many tokens are about twice as
+fast with b in tiles, four times with b in rows.
 
 Tensors are CUDA tensors (inputs float32, float16 or bfloat16) with any leading
 dimensions; rows may be strided, their elements are contiguous (other layouts
